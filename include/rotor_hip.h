@@ -348,6 +348,48 @@ int rt_rope_attention_decode(rt_ctx* ctx, const float* q, const float* k, const 
                              float* v_cache, const float* rope, int H, int Hkv, int hd, int Lmax, const int* pos,
                              void* workspace, size_t workspace_bytes, float* out);
 
+/* ---- KV cache in 4 bits ------------------------------------------------------------
+ * One layer's keys and values for B sequences, 0.56 bytes a value instead of the 4 of the
+ * fp32 cache above (which replaces the fp32 lists of src/rotor/bitnet_model.py:223-228);
+ * head_dim 64 or 128.  Sequence b stands at pos[b] (device int32 [B]): row (b, m) of a call
+ * is its position p = pos[b] + m.  A row whose p lies outside [0, Lmax) has no place in the
+ * cache: it is not written, and its outputs are zeros.
+ *
+ * 64 consecutive dimensions of one head at one position (a group) are held as codes
+ * c = 0..15 and two bf16 numbers z and h, and stand for fp32(z + h (2 c - 15)):
+ *   z = (max + min) / 2 and h = (max - min) / 30, each rounded to fp32, then to bf16,
+ *   c = clamp(rint(((x - z) / h + 15) / 2), 0, 15) in 64 bits; (x - z) / h is 0 where h = 0.
+ * A group that holds a value that is not finite, or whose z or h is not, reads as NaN.
+ * The bytes are opaque; fresh memory needs no initialisation: only positions that were
+ * written take part in anything.  Buffers are 16-byte aligned, pos 4-byte aligned.
+ * Lmax <= 2^20; the same Lmax goes to every call on a cache. */
+
+/* Bytes of a layer's cache: B * Hkv * ceil(Lmax / 64) blocks of 72 * hd bytes (0 for sizes the
+ * calls below refuse). */
+size_t rt_kv4_bytes(int B, int Hkv, int hd, int Lmax);
+
+/* RoPE (rotate-half, rope fp32 [Lmax][hd/2][2], in 64 bits, rounded once) of q [B][M][H][hd]
+ * into q_out (q_out may be q) and of k [B][M][Hkv][hd], then k and v into the cache at every
+ * row's position: rt_rope_kv_append for this cache, in one launch (the KV concat of
+ * src/rotor/transformer.py:250-252).  k and v are not modified. */
+int rt_kv4_append(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache,
+                  float* q_out, int B, int M, int H, int Hkv, int hd, int Lmax, const int* pos);
+
+/* The values held at every row's position, fp32 k and v [B][Hkv][M][hd]
+ * (the reference's cache arrays, src/rotor/transformer.py:255-257). */
+int rt_kv4_read(rt_ctx* ctx, const void* cache, float* k, float* v, int B, int M, int Hkv, int hd, int Lmax,
+                const int* pos);
+
+/* Causal GQA attention (rt_attention for this cache): out [B][M][H][hd] for queries q
+ * [B][M][H][hd] (as rt_kv4_append leaves them) over keys 0..p, scale 1/sqrt(hd)
+ * (src/rotor/transformer.py:260-281 plus the causal mask).  Where B, M and the heads alone do
+ * not fill the GPU, the keys are split and joined in a second launch through `workspace`
+ * (rt_kv4_attention_workspace bytes of device memory, possibly 0, no initialisation; calls that
+ * may run at the same time need workspaces of their own). */
+size_t rt_kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax);
+int rt_kv4_attention(rt_ctx* ctx, const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
+                     int Lmax, const int* pos, void* workspace, size_t workspace_bytes);
+
 /* Final RMSNorm of x fp32 [D] with norm_w, tied bf16 LM head logits [V]
  * (src/rotor/bitnet_model.py:231-235) and greedy argmax (src/rotor/generation.py:42;
  * first index of the maximum).  `best` (device u64, zero before first use) is left

@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <unordered_map>
@@ -1205,6 +1206,70 @@ int rt_lm_head_argmax(rt_ctx* ctx, const uint16_t* emb, const float* x, const fl
     DeviceGuard g(ctx->device);
     RT_HIP(launch_lm_head(emb, x, norm_w, eps, V, D, logits, best, token, pos, advance, next_ids, out_tokens, pos_base,
                           out_cap, next_h, ctx->stream));
+    return RT_OK;
+}
+
+// --- 4-bit KV cache ---------------------------------------------------------------------
+
+static bool kv4_layout_ok(int B, int Hkv, int hd, int Lmax) {
+    return B > 0 && Hkv > 0 && (long long)B * Hkv <= (1 << 24) && (hd == 64 || hd == 128) && Lmax > 0 &&
+           Lmax <= (1 << 20);
+}
+
+static int kv4_check(rt_ctx* ctx, std::initializer_list<const void*> ptrs, const int* pos, int B, int M, int H,
+                     int Hkv, int hd, int Lmax, const char* who) {
+    bool aligned = true;
+    for (const void* p : ptrs) {
+        if (!p) return fail(RT_EINVAL, std::string(who) + ": NULL argument");
+        aligned = aligned && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+    }
+    if (!ctx || !pos) return fail(RT_EINVAL, std::string(who) + ": NULL argument");
+    if (!kv4_layout_ok(B, Hkv, hd, Lmax) || H <= 0 || H % Hkv || H / Hkv > 1024)
+        return fail(RT_EINVAL, std::string(who) + ": unsupported layout (head_dim 64 or 128, H % Hkv == 0, H / Hkv <= "
+                                                  "1024, B * Hkv <= 2^24, Lmax <= 2^20)");
+    if (M <= 0 || M > Lmax) return fail(RT_EINVAL, std::string(who) + ": M out of range");
+    if (!aligned) return fail(RT_EINVAL, std::string(who) + ": buffers must be 16-byte aligned");
+    return RT_OK;
+}
+
+size_t rt_kv4_bytes(int B, int Hkv, int hd, int Lmax) {
+    return kv4_layout_ok(B, Hkv, hd, Lmax) ? kv4_bytes(B, Hkv, hd, Lmax) : 0;
+}
+
+int rt_kv4_append(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache,
+                  float* q_out, int B, int M, int H, int Hkv, int hd, int Lmax, const int* pos) {
+    const int rc = kv4_check(ctx, {q, k, v, rope, cache, q_out}, pos, B, M, H, Hkv, hd, Lmax, "rt_kv4_append");
+    if (rc) return rc;
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_kv4_append(q, k, v, rope, cache, q_out, B, M, H, Hkv, hd, Lmax, pos, ctx->stream));
+    return RT_OK;
+}
+
+int rt_kv4_read(rt_ctx* ctx, const void* cache, float* k, float* v, int B, int M, int Hkv, int hd, int Lmax,
+                const int* pos) {
+    const int rc = kv4_check(ctx, {cache, k, v}, pos, B, M, Hkv, Hkv, hd, Lmax, "rt_kv4_read");
+    if (rc) return rc;
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_kv4_read(cache, k, v, B, M, Hkv, hd, Lmax, pos, ctx->stream));
+    return RT_OK;
+}
+
+size_t rt_kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax) {
+    if (!kv4_layout_ok(B, Hkv, hd, Lmax) || H <= 0 || H % Hkv || H / Hkv > 1024 || M <= 0 || M > Lmax) return 0;
+    return kv4_attention_workspace(B, M, H, Hkv, hd, Lmax);
+}
+
+int rt_kv4_attention(rt_ctx* ctx, const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
+                     int Lmax, const int* pos, void* workspace, size_t workspace_bytes) {
+    const int rc = kv4_check(ctx, {q, cache, out}, pos, B, M, H, Hkv, hd, Lmax, "rt_kv4_attention");
+    if (rc) return rc;
+    const size_t need = kv4_attention_workspace(B, M, H, Hkv, hd, Lmax);
+    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(RT_EINVAL, "rt_kv4_attention: workspace too small (rt_kv4_attention_workspace) or not 16-byte "
+                               "aligned");
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_kv4_attention(q, cache, out, B, M, H, Hkv, hd, Lmax, pos, static_cast<float*>(workspace),
+                                ctx->stream));
     return RT_OK;
 }
 

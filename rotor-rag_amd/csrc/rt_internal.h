@@ -421,6 +421,16 @@ hipError_t launch_attn_partial(const float* q, const float* knew, const float* v
                                const float* rope, int H, int Hkv, int hd, int Lmax, const int* pos, float scale,
                                float* work, hipStream_t s);
 hipError_t launch_attn_combine(const float* work, int H, int hd, int S, float* out, hipStream_t s);
+// 4-bit KV cache (rt_kv4.hip)
+size_t kv4_bytes(int B, int Hkv, int hd, int Lmax);
+size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax);
+hipError_t launch_kv4_append(const float* q, const float* k, const float* v, const float* rope, void* cache,
+                             float* q_out, int B, int M, int H, int Hkv, int hd, int Lmax, const int* pos,
+                             hipStream_t s);
+hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, int Hkv, int hd, int Lmax,
+                           const int* pos, hipStream_t s);
+hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
+                                int Lmax, const int* pos, float* work, hipStream_t s);
 hipError_t launch_lm_head(const uint16_t* E, const float* x, const float* norm_w, float eps, int V, int D,
                           float* logits, unsigned long long* best, int* token, int* pos, int advance,
                           int* next_ids, int* out_tokens, int pos_base, int out_cap, float* next_h, hipStream_t s);

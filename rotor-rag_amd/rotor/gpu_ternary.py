@@ -527,6 +527,99 @@ class HIPTernaryOps:
                                                    ctypes.byref(h)), "rt_plan_create_gate_up")
         return LinearPlan(self, h, ([w_gu], [x, aux, aux2], [a, ssq], [g_out, u_out]))
 
+    # -- KV cache in 4 bits (rt_kv4_*) ---------------------------------------------
+    def kv4_cache(self, n_kv_heads: int, head_dim: int, max_len: int, batch: int = 1):
+        """One layer's 4-bit KV cache for `batch` sequences of up to max_len positions: a uint8
+        device tensor [batch, n_kv_heads, ceil(max_len / 64), 72 * head_dim] (its bytes are
+        opaque and need no initialisation)."""
+        if not self.lib.rt_kv4_bytes(int(batch), int(n_kv_heads), int(head_dim), int(max_len)):
+            raise ValueError("kv4_cache: needs head_dim 64 or 128, batch * n_kv_heads <= 2^24, 1 <= max_len <= 2^20")
+        torch = _torch()
+        return torch.empty((int(batch), int(n_kv_heads), (int(max_len) + 63) // 64, 72 * int(head_dim)),
+                           dtype=torch.uint8, device=self.device)
+
+    def _kv4_check(self, who, cache, pos, max_len):
+        """(B, Hkv, hd, Lmax) of a cache and its positions."""
+        torch = _torch()
+        if (cache.dtype != torch.uint8 or cache.ndim != 4 or not cache.is_contiguous() or cache.device != self.device
+                or cache.shape[3] not in (72 * 64, 72 * 128)):
+            raise ValueError(f"{who}: cache must be a contiguous uint8 [B, Hkv, blocks, 72 * head_dim] tensor on the "
+                             "backend's device (kv4_cache)")
+        B, Hkv, blocks, size = cache.shape
+        Lmax = 64 * blocks if max_len is None else int(max_len)
+        if not 64 * (blocks - 1) < Lmax <= 64 * blocks:
+            raise ValueError(f"{who}: max_len {Lmax} does not fit a cache of {blocks} blocks of 64 positions")
+        if pos.dtype != torch.int32 or tuple(pos.shape) != (B,) or pos.device != self.device or not pos.is_contiguous():
+            raise ValueError(f"{who}: pos must be a contiguous int32 [{B}] tensor on the backend's device")
+        return B, Hkv, size // 72, Lmax
+
+    def _kv4_in(self, x):
+        """float32 device tensor, contiguous and 16-byte aligned (a copy where x is not)."""
+        t = self._dev(x, _torch().float32)
+        return t.clone() if t.data_ptr() % 16 else t
+
+    def _kv4_out(self, who, out, shape):
+        torch = _torch()
+        if out is None:
+            return torch.empty(shape, dtype=torch.float32, device=self.device)
+        if out.dtype != torch.float32 or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != self.device:
+            raise ValueError(f"{who}: the output must be a contiguous float32 {list(shape)} tensor on the backend's device")
+        return out
+
+    def kv4_append(self, q, k, v, cache, rope, pos, max_len=None, q_out=None):
+        """RoPE of q [B, M, H, hd] and k [B, M, Hkv, hd], then k and v into the 4-bit cache at
+        positions pos[b] + m (rt_kv4_append); rope float32 [>= max_len, hd / 2, 2].  Returns the
+        rotated q (q_out, which may be q).  max_len: the cache's positions, where they are fewer
+        than its blocks hold (None: as many as the blocks and rope hold).  Rows outside
+        [0, max_len) are not written; their q is 0."""
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_append", cache, pos, max_len)
+        qt, kt, vt, rt = (self._kv4_in(x) for x in (q, k, v, rope))
+        if max_len is None and rt.ndim == 3:
+            Lmax = min(Lmax, max(rt.shape[0], Lmax - 63))
+        if qt.ndim != 4 or qt.shape[0] != B or qt.shape[3] != hd or qt.shape[2] % Hkv or qt.numel() == 0:
+            raise ValueError(f"kv4_append: q of shape {tuple(qt.shape)} does not fit a cache of {B} sequences, {Hkv} KV "
+                             f"heads of {hd}")
+        M, H = qt.shape[1], qt.shape[2]
+        if tuple(kt.shape) != (B, M, Hkv, hd) or kt.shape != vt.shape:
+            raise ValueError(f"kv4_append: k and v must be {[B, M, Hkv, hd]}")
+        if rt.ndim != 3 or tuple(rt.shape[1:]) != (hd // 2, 2) or rt.shape[0] < Lmax:
+            raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
+        out = self._kv4_out("kv4_append", q_out, qt.shape)
+        self._bind_stream()
+        _hip.check(self.lib.rt_kv4_append(self.ctx, qt.data_ptr(), kt.data_ptr(), vt.data_ptr(), rt.data_ptr(),
+                                          cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr()),
+                   "rt_kv4_append")
+        return out
+
+    def kv4_read(self, cache, pos, length: int, max_len=None):
+        """The values that a 4-bit cache holds at positions pos[b] + (0 .. length - 1): (k, v)
+        float32 [B, Hkv, length, hd]; zeros outside [0, max_len) (rt_kv4_read)."""
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_read", cache, pos, max_len)
+        k, v = (self._kv4_out("kv4_read", None, (B, Hkv, int(length), hd)) for _ in range(2))
+        self._bind_stream()
+        _hip.check(self.lib.rt_kv4_read(self.ctx, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, int(length), Hkv, hd,
+                                        Lmax, pos.data_ptr()), "rt_kv4_read")
+        return k, v
+
+    def kv4_attention(self, q, cache, pos, max_len=None, out=None):
+        """Causal GQA attention of q [B, M, H, hd] (rotated, as kv4_append returns it) at positions
+        pos[b] + m over a 4-bit cache (rt_kv4_attention): float32 [B, M, H, hd]."""
+        torch = _torch()
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", cache, pos, max_len)
+        qt = self._kv4_in(q)
+        if qt.ndim != 4 or qt.shape[0] != B or qt.shape[3] != hd or qt.shape[2] % Hkv or qt.numel() == 0:
+            raise ValueError(f"kv4_attention: q of shape {tuple(qt.shape)} does not fit a cache of {B} sequences, {Hkv} "
+                             f"KV heads of {hd}")
+        M, H = qt.shape[1], qt.shape[2]
+        y = self._kv4_out("kv4_attention", out, qt.shape)
+        need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._bind_stream()
+        _hip.check(self.lib.rt_kv4_attention(self.ctx, qt.data_ptr(), cache.data_ptr(), y.data_ptr(), B, M, H, Hkv, hd,
+                                             Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need),
+                   "rt_kv4_attention")
+        return y
+
     def __del__(self):
         try:
             if getattr(self, "ctx", None):
