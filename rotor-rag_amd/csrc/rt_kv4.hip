@@ -216,14 +216,21 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict
 
 // ---- attention ---------------------------------------------------------------------------
 // The eight levels 2 c - 15 of a dword, exact in fp16: a nibble at bits 4..7 of a half under
-// 0x6400 is 1024 + 16 c, and (1024 + 16 c) / 8 - 143 = 2 c - 15.
-__device__ __forceinline__ v8h kv4_levels(unsigned w) {
+// 0x6400 is 1024 + 16 c, and (1024 + 16 c) / 8 - 143 = 2 c - 15.  Masking and setting the
+// exponent are one v_and_or_b32, which takes one of its two constants from a VGPR: `mask` is
+// kv4_mask()'s.
+__device__ __forceinline__ unsigned kv4_mask() {
+    unsigned m = 0x00F000F0u;
+    asm("" : "+v"(m));
+    return m;
+}
+__device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
     const v2h f = {(_Float16)0.125f, (_Float16)0.125f}, o = {(_Float16)-143.0f, (_Float16)-143.0f};
     v8h r;
     const unsigned n[4] = {w << 4, w, w >> 4, w >> 8};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const v2h x = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (n[i] & 0x00F000F0u) | 0x64006400u), f, o);
+        const v2h x = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (n[i] & mask) | 0x64006400u), f, o);
         r[2 * i] = x[0];
         r[2 * i + 1] = x[1];
     }
@@ -237,296 +244,393 @@ __device__ __forceinline__ v8h kv4_levels(unsigned w) {
 __device__ __forceinline__ void kv4_split(v2f x, v2h& hi, v2h& lo) {
     float a = x[0], b = x[1];
     asm("" : "+v"(a), "+v"(b));
-    x = v2f{a, b};
-    hi = __builtin_convertvector(x, v2h);
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, v2f), v2h);
+    hi = __builtin_convertvector((v2f{a, b}), v2h);
+    float c, d;  // a - hi[0], b - hi[1]: one instruction each, with hi's halves as they lie
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(c) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(hi), "v"(b));
+    lo = __builtin_convertvector((v2f{c, d}), v2h);
 }
 // 2^n as fp32, -126 <= n <= 127
 __device__ __forceinline__ float kv4_pow2(int n) { return __uint_as_float((unsigned)(n + 127) << 23); }
 __device__ __forceinline__ int kv4_exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
 
+// Joins the lanes l, l ^ 16, l ^ 32, l ^ 48 (all four get the result); x in two lane halves only.
+template <typename Op>
+__device__ __forceinline__ float kv4_join32(float x, Op op) {
+    const v2u y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+template <typename Op>
+__device__ __forceinline__ float kv4_join16(float x, Op op) {
+    const v2u y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return kv4_join32(op(__uint_as_float(y[0]), __uint_as_float(y[1])), op);
+}
+struct Kv4Max {
+    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Kv4Sum {
+    __device__ float operator()(float a, float b) const { return a + b; }
+};
+
+// The largest of 16 lanes' x (lanes l ^ 1, l ^ 2, l ^ 4, l ^ 8).
+__device__ __forceinline__ int kv4_rows_max(int x) {
+#pragma unroll
+    for (int w = 1; w < 16; w <<= 1) x = max(x, __shfl_xor(x, w, 64));
+    return x;
+}
+
 struct Kv4AttnArgs {
     const float* q;
     const uint8_t* cache;
     float* out;
-    float* work;
+    float* work;  // S > 1: [unit][split]: O [tile rows][HD], then (reference, sum of weights) [tile rows][2]
     const int* pos;
-    int M, H, Hkv, Lmax, nblk, tiles, S;
+    int M, H, Hkv, Lmax, nblk, tiles, S, bh;  // bh = B * Hkv
     float scale;  // log2(e) / sqrt(HD)
 };
 
-// Rows R = m G + g of KV head kh, 16 a workgroup; lane l works on row l % 16 with the keys of
-// lane group h = l / 16.  The split's blocks go to its 4 waves in turn, an online softmax
-// (base 2) each:
+// The power of two that brings the largest of a row's scaled queries into [2^14, 2^15).
+__device__ __forceinline__ int kv4_query_power(float big) { return min(max(14 - kv4_exponent(big), -113), 126); }
+
+// ---- few rows ------------------------------------------------------------------------------
+// A tile is RT rows (R = m G + g of KV head kh), RT = 4, 8 or 16.  The matrix instructions have 16
+// columns: column i is row i % RT over the key tiles of number i / RT modulo 16 / RT, so that every
+// lane's softmax counts however few the rows (with 16 columns for 4 rows, 12 lanes of 16 worked on
+// nothing: 131072 keys, 20 heads over 5, 44 us); the columns of a row are joined at the end.  Lane l
+// works on column i = l % 16 with the keys of lane group h = l / 16.  The split's blocks go to its
+// 4 waves in turn, an online softmax (base 2) for every column:
 //   D = U Q^T per group of 64 dimensions (U the keys' levels, exact in fp16; Q two fp16 terms,
 //       scaled so that the row's largest is in [2^14, 2^15)),  s = h D + z sum_d q
-//   O^T += U^T W^T  (U the values' levels, W = 2^s h, two fp16 terms, scaled by the largest h so far)
-//   O   += sum_j 2^s z
-// so that all products are exact and all sums fp32.  The waves' results are merged in LDS; with
-// S > 1 the split's go to the workspace: O [16][HD], then (m, l) [16][2].
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(const Kv4AttnArgs a) {
-    constexpr int NG = HD / 64, NT = HD / 16;
+//   w = 2^(s - ref),  O^T += U^T (w h)^T  (U the values' levels, w h two fp16 terms),  O += sum_j w z
+// so that all products are exact and all sums fp32.  ref is the largest score so far plus e - 14,
+// 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a group's h is no less than
+// 2^-29 of it unless it is 0), which keeps w h below 2^15, and w, w z in fp32's range.
+// Every load is issued half a round before its use: the keys of the next block when those of this
+// one are multiplied, its values after this one's.
+template <int HD, int RT>
+__global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
+    constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
     __shared__ float om[4][16][HD + 4];
     __shared__ float ml[4][16][2];
     const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x);
     const int split = w0 % a.S, unit = w0 / a.S, tile = unit % a.tiles, bh = unit / a.tiles;
     const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
-    const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4;
+    const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const unsigned mask = kv4_mask();
     const int pos = a.pos[b];
-    const int R = tile * 16 + i, m = R / G, rows = a.M * G;
-    const int last = R < rows ? kv4_row_pos(pos, m, a.Lmax) : -1;  // keys <= last are this row's
-    int kend = last + 1;
+    const int rows = a.M * G, R = min(tile * RT + i % RT, rows - 1), m = R / G;  // (rows past the end repeat the last)
+    const int last = kv4_row_pos(pos, m, a.Lmax);  // keys <= last are this row's
+    const int kend = __builtin_amdgcn_readfirstlane(kv4_rows_max(last)) + 1;
+    const int all = __builtin_amdgcn_readfirstlane(-kv4_rows_max(-last));
+    const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
+    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * a.S;
+    // Key tile wx = 2 w + x of a block: keys 32 w + 8 x + kl + r of lane group h.  The column's own
+    // tiles are wx = NA q + ca.
+    const int kl = 16 * (h >> 1) + 4 * (h & 1);
+    auto tile_key = [](int wx) { return 32 * (wx >> 1) + 8 * (wx & 1); };
+    v4u kc[4], ks[NG][NQ], vc[2 * NG], vs[NG][NQ];
+    auto load_k = [&](int j) {
+        const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
+        const unsigned* sc = reinterpret_cast<const unsigned*>(blk + 64 * HD);
 #pragma unroll
-    for (int w = 1; w < 16; w <<= 1) kend = max(kend, __shfl_xor(kend, w, 64));
-    kend = __builtin_amdgcn_readfirstlane(kend);
+        for (int wx = 0; wx < 4; ++wx) {
+            const uint8_t* kp = blk + (tile_key(wx) + 16 * (i >> 3) + (i & 7)) * (HD / 2) + h * 8 * NG;
+            if constexpr (NG == 2) kc[wx] = *reinterpret_cast<const v4u*>(kp);
+            else {
+                const v2u x = *reinterpret_cast<const v2u*>(kp);
+                kc[wx][0] = x[0];
+                kc[wx][1] = x[1];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) ks[g][q] = *reinterpret_cast<const v4u*>(sc + g * 64 + tile_key(NA * q + ca) + kl);
+    };
+    auto load_v = [&](int j) {
+        const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
+        const unsigned* sc = reinterpret_cast<const unsigned*>(blk + 64 * HD) + HD;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) vs[g][q] = *reinterpret_cast<const v4u*>(sc + g * 64 + tile_key(NA * q + ca) + kl);
+#pragma unroll
+        for (int u = 0; u < 2 * NG; ++u) vc[u] = *reinterpret_cast<const v4u*>(blk + 32 * HD + ((u * 16 + i) * 4 + h) * 16);
+    };
+    int j = split * 4 + wave;
+    if (j < nb) {
+        load_k(j);
+        load_v(j);
+    }
     // the row's queries: dimensions 64 g + 16 h + 8 e + (0..7)
-    float qx[NG][16], qs[NG], big = 0.0f;
-    const float* qp = a.q + (((size_t)b * a.M + min(m, a.M - 1)) * a.H + (size_t)kh * G + (R < rows ? R % G : 0)) * HD;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const v4f x = *reinterpret_cast<const v4f*>(qp + 64 * g + 16 * h + 4 * e);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                qx[g][4 * e + j] = x[j] * a.scale;
-                big = fmaxf(big, fabsf(qx[g][4 * e + j]));
-            }
-        }
-    big = fmaxf(big, __shfl_xor(big, 16, 64));
-    big = fmaxf(big, __shfl_xor(big, 32, 64));
-    const int qe = min(max(14 - kv4_exponent(big), -113), 126);
-    const float qf = kv4_pow2(qe), qi = kv4_pow2(-qe);
+    float qs[NG], qi;
     v8h qh[NG][2], ql[NG][2];
+    {
+        float qx[NG][16], big = 0.0f;
+        const float* qp = a.q + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        qs[g] = 0.0f;
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const v2f x = {qx[g][e] * qf, qx[g][e + 1] * qf};
-            v2h hi, lo;
-            kv4_split(x, hi, lo);
+            for (int e = 0; e < 4; ++e) {
+                const v4f x = *reinterpret_cast<const v4f*>(qp + 64 * g + 16 * h + 4 * e);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                qh[g][e / 8][e % 8 + j] = hi[j];
-                ql[g][e / 8][e % 8 + j] = lo[j];
-                qs[g] += x[j];
+                for (int c = 0; c < 4; ++c) {
+                    qx[g][4 * e + c] = x[c] * a.scale;
+                    big = fmaxf(big, fabsf(qx[g][4 * e + c]));
+                }
             }
+        const int qe = kv4_query_power(kv4_join16(big, Kv4Max()));
+        const float qf = kv4_pow2(qe);
+        qi = kv4_pow2(-qe);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            qs[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const v2f x = {qx[g][e] * qf, qx[g][e + 1] * qf};
+                v2h hi, lo;
+                kv4_split(x, hi, lo);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    qh[g][e / 8][e % 8 + c] = hi[c];
+                    ql[g][e / 8][e % 8 + c] = lo[c];
+                    qs[g] += x[c];
+                }
+            }
+            qs[g] = kv4_join16(qs[g], Kv4Sum());
         }
-        qs[g] += __shfl_xor(qs[g], 16, 64);
-        qs[g] += __shfl_xor(qs[g], 32, 64);
     }
     v4f o[NT];
-    float zs[NG], mrow = -INFINITY, lrow = 0.0f;
-    int ref[NG];  // exponent of the largest h of the values so far
+    float zs[NG], top = -INFINITY, ref = -INFINITY, lrow = 0.0f, hmax = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = v4f{};
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        zs[g] = 0.0f;
-        ref[g] = -111;
-    }
-    const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
-    const int nb = (kend + kKv4Block - 1) / kKv4Block;
-    for (int j = split * 4 + wave; j < nb; j += 4 * a.S) {
-        const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
-        const unsigned* sc = reinterpret_cast<const unsigned*>(blk + 64 * HD);
-        const int key0 = j * kKv4Block;
-        float s[4][4];
-        // keys of lane group h in tile (w, x): 32 w + 16 (h / 2) + 8 x + 4 (h % 2) + r
-        const int kl = 16 * (h >> 1) + 4 * (h & 1);
+    for (int g = 0; g < NG; ++g) zs[g] = 0.0f;
+    for (; j < nb; j += step) {
+        const int key0 = j * kKv4Block + kl;
+        const bool edge = j * kKv4Block + kKv4Block - 1 > all;  // some row does not see the whole block
+        float s[NQ][4];
 #pragma unroll
-        for (int wx = 0; wx < 4; ++wx) {
-            const int tk = 32 * (wx >> 1) + 8 * (wx & 1);
-            unsigned kw[2 * NG];
-            const unsigned* kp = reinterpret_cast<const unsigned*>(blk + (tk + 16 * (i >> 3) + (i & 7)) * (HD / 2)) + h * 2 * NG;
-            if constexpr (NG == 2) {
-                const v4u x = *reinterpret_cast<const v4u*>(kp);
+        for (int q = 0; q < NQ; ++q) {
+            v4f own[NG];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) kw[e] = x[e];
-            } else {
-                const v2u x = *reinterpret_cast<const v2u*>(kp);
-                kw[0] = x[0];
-                kw[1] = x[1];
-            }
-            v4f dot[NG];
+            for (int c = 0; c < NA; ++c) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                dot[g] = v4f{};
+                for (int g = 0; g < NG; ++g) {
+                    v4f dot{};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const v8h u = kv4_levels(kw[2 * g + e]);
-                    dot[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, qh[g][e], dot[g], 0, 0, 0);
-                    dot[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, ql[g][e], dot[g], 0, 0, 0);
+                    for (int e = 0; e < 2; ++e) {
+                        const v8h u = kv4_levels(kc[NA * q + c][2 * g + e], mask);
+                        dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, qh[g][e], dot, 0, 0, 0);
+                        dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, ql[g][e], dot, 0, 0, 0);
+                    }
+                    if (c == 0) own[g] = dot;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) own[g][r] = ca == c ? dot[r] : own[g][r];
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[wx][r] = 0.0f;
+            for (int r = 0; r < 4; ++r) {
+                float x = kv4_z(ks[0][q][r]) * qs[0];
+                if constexpr (NG == 2) x = fmaf(kv4_z(ks[1][q][r]), qs[1], x);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const v4u x = *reinterpret_cast<const v4u*>(sc + g * 64 + tk + kl);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[wx][r] = fmaf(kv4_h(x[r]), dot[g][r], fmaf(kv4_z(x[r]), qs[g], s[wx][r]));
+                for (int g = 0; g < NG; ++g) x = fmaf(kv4_h(ks[g][q][r]), own[g][r], x);
+                s[q][r] = x;
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[wx][r] = key0 + tk + kl + r <= last ? s[wx][r] * qi : -INFINITY;
         }
-        float mx = mrow;
+        if (j + step < nb) load_k(j + step);
+        if (edge) {
 #pragma unroll
-        for (int wx = 0; wx < 4; ++wx)
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[wx][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mb = mx == -INFINITY ? 0.0f : mx;
-        const float alpha = exp2f(mrow - mb);
-        mrow = mx;
-        lrow *= alpha;
+                for (int r = 0; r < 4; ++r) {
+                    const int key = key0 + tile_key(NA * q + ca) + r;
+                    s[q][r] = key <= last ? s[q][r] : -INFINITY;
+                    if (key >= kend)  // what lies behind the newest key is not read as a number
 #pragma unroll
-        for (int wx = 0; wx < 4; ++wx)
+                        for (int g = 0; g < NG; ++g) vs[g][q][r] = 0u;
+                }
+        }
+        float mx = -INFINITY, hm = 0.0f, zm = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[wx][r] = exp2f(s[wx][r] - mb);  // (-inf: 0)
-                lrow += s[wx][r];
+                mx = fmaxf(mx, s[q][r]);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    hm = fmaxf(hm, kv4_h(vs[g][q][r]));
+                    zm = fmaxf(zm, fabsf(kv4_z(vs[g][q][r])));
+                }
+            }
+        top = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
+        hmax = fmaxf(hmax, kv4_join16(fmaxf(hm, zm * 0x1p-24f), Kv4Max()));
+        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max(kv4_exponent(hmax), -80) - 14);
+        if (__any(now != ref)) {
+            const float alpha = __builtin_amdgcn_exp2f(ref - now);
+            lrow *= alpha;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) zs[g] *= alpha;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n] *= alpha;
+            ref = now;
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[q][r] = __builtin_amdgcn_exp2f(fmaf(s[q][r], qi, -ref));  // (-inf: 0)
+                lrow += s[q][r];
             }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            v4u vs[4];
-            float top = 0.0f;
+            unsigned wh[NQ][2], wl[NQ][2];
 #pragma unroll
-            for (int wx = 0; wx < 4; ++wx) {
-                const int tk = 32 * (wx >> 1) + 8 * (wx & 1) + kl;
-                vs[wx] = *reinterpret_cast<const v4u*>(sc + HD + g * 64 + tk);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    // what lies behind the newest key is not read as a number
-                    if (key0 + tk + r >= kend) vs[wx][r] = 0u;
-                    top = fmaxf(top, kv4_h(vs[wx][r]));
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const int e = __builtin_amdgcn_readfirstlane(max(ref[g], min(kv4_exponent(top), 127)));
-            const float f = kv4_pow2(14 - e), fix = alpha * (ref[g] - e < -126 ? 0.0f : kv4_pow2(ref[g] - e));
-            ref[g] = e;
-            zs[g] *= alpha;
-            v8h wh[2], wl[2];
-#pragma unroll
-            for (int wx = 0; wx < 4; ++wx) {
-                const int tk = 32 * (wx >> 1) + 8 * (wx & 1) + kl;
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     v2h hi, lo;
-                    kv4_split(v2f{s[wx][r] * (kv4_h(vs[wx][r]) * f), s[wx][r + 1] * (kv4_h(vs[wx][r + 1]) * f)}, hi, lo);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const bool see = key0 + tk + r + j <= last;
-                        wh[wx >> 1][4 * (wx & 1) + r + j] = hi[j];
-                        wl[wx >> 1][4 * (wx & 1) + r + j] = lo[j];
-                        zs[g] = fmaf(s[wx][r + j], see ? kv4_z(vs[wx][r + j]) : 0.0f, zs[g]);
-                    }
+                    kv4_split(v2f{s[q][r] * kv4_h(vs[g][q][r]), s[q][r + 1] * kv4_h(vs[g][q][r + 1])}, hi, lo);
+                    wh[q][r / 2] = __builtin_bit_cast(unsigned, hi);
+                    wl[q][r / 2] = __builtin_bit_cast(unsigned, lo);
                 }
+            if (edge) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool see = key0 + tile_key(NA * q + ca) + r <= last;
+                        zs[g] = fmaf(s[q][r], see ? kv4_z(vs[g][q][r]) : 0.0f, zs[g]);
+                    }
+            } else {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) zs[g] = fmaf(s[q][r], kv4_z(vs[g][q][r]), zs[g]);
             }
+            // the weights of the products over tiles 2 w and 2 w + 1: the column's own tile, or zeros
+            v4u th[2], tl[2];
 #pragma unroll
-            for (int u = 2 * g; u < 2 * g + 2; ++u) {
-                const v4u x = *reinterpret_cast<const v4u*>(blk + 32 * HD + ((u * 16 + i) * 4 + h) * 16);
+            for (int wx = 0; wx < 4; ++wx)
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    v4f acc = o[2 * u + v] * fix;
+                for (int c = 0; c < 2; ++c) {
+                    const bool mine = NA == 1 || wx % NA == ca;
+                    th[wx >> 1][2 * (wx & 1) + c] = mine ? wh[wx / NA][c] : 0u;
+                    tl[wx >> 1][2 * (wx & 1) + c] = mine ? wl[wx / NA][c] : 0u;
+                }
+#pragma unroll
+            for (int u = 2 * g; u < 2 * g + 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const v8h lev = kv4_levels(x[2 * v + w]);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, wh[w], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, wl[w], acc, 0, 0, 0);
+                        const v8h lev = kv4_levels(vc[u][2 * v + w], mask);
+                        v4f& acc = o[2 * u + v];
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, th[w]), acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, tl[w]), acc, 0, 0, 0);
                     }
-                    o[2 * u + v] = acc;
-                }
-            }
         }
+        if (j + step < nb) load_v(j + step);
     }
-    // this wave's O[row][dim], row i, dimensions 32 u + 16 v + 4 h + r
-    lrow += __shfl_xor(lrow, 16, 64);
-    lrow += __shfl_xor(lrow, 32, 64);
+    // this wave's O[column][dim], column i, dimensions 32 u + 16 v + 4 h + r
+    lrow = kv4_join16(lrow, Kv4Sum());
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        zs[g] += __shfl_xor(zs[g], 16, 64);
-        zs[g] += __shfl_xor(zs[g], 32, 64);
-        const float back = kv4_pow2(max(ref[g] - 14, -126));
+        zs[g] = kv4_join16(zs[g], Kv4Sum());
 #pragma unroll
-        for (int n = 4 * g; n < 4 * g + 4; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) om[wave][i][n * 16 + 4 * h + r] = fmaf(o[n][r], back, zs[g]);
+        for (int n = 4 * g; n < 4 * g + 4; ++n) *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = o[n] + zs[g];
     }
     if (h == 0) {
-        ml[wave][i][0] = mrow;
+        ml[wave][i][0] = ref;
         ml[wave][i][1] = lrow;
     }
     __syncthreads();
-    const int row = t >> 4, RR = tile * 16 + row;
+    // join the 4 waves' NA columns of a row: 256 / RT threads a row
+    constexpr int TPR = 256 / RT, NP = 4 * NA;
+    const int row = t / TPR, RR = tile * RT + row;
     if (RR >= rows) return;
-    float mm = -INFINITY, den = 0.0f, f[4];
+    float mm = -INFINITY, den = 0.0f, f[NP];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w][row][0]);
+    for (int p = 0; p < NP; ++p) mm = fmaxf(mm, ml[p / NA][p % NA * RT + row][0]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = ml[w][row][0] == -INFINITY ? 0.0f : exp2f(ml[w][row][0] - mm);
-        den += f[w] * ml[w][row][1];
+    for (int p = 0; p < NP; ++p) {
+        const float l = ml[p / NA][p % NA * RT + row][1];
+        f[p] = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[p / NA][p % NA * RT + row][0] - mm);
+        den += f[p] * l;
     }
     float* dst;
     float inv = 1.0f;
     if (a.S > 1) {
-        float* part = a.work + ((size_t)unit * a.S + split) * (16 * (HD + 2));
+        float* part = a.work + ((size_t)unit * a.S + split) * (RT * (HD + 2));
         dst = part + row * HD;
-        if ((t & 15) == 0) {
-            part[16 * HD + 2 * row] = mm;
-            part[16 * HD + 2 * row + 1] = den;
+        if (t % TPR == 0) {
+            part[RT * HD + 2 * row] = mm;
+            part[RT * HD + 2 * row + 1] = den;
         }
     } else {
         dst = a.out + (((size_t)b * a.M + RR / G) * a.H + (size_t)kh * G + RR % G) * HD;
         inv = den;
     }
+    constexpr int W = HD / TPR < 4 ? (HD / TPR < 1 ? 1 : HD / TPR) : 4;  // values a thread writes at once
 #pragma unroll
-    for (int d = (t & 15) * 4; d < HD; d += 64) {
-        v4f x{};
+    for (int d = t % TPR * W; d < HD; d += TPR * W) {
+        float x[W] = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = f[w] == 0.0f ? x[j] : x[j] + f[w] * om[w][row][d + j];
+            for (int c = 0; c < W; ++c) x[c] = fmaf(f[p], om[p / NA][p % NA * RT + row][d + c], x[c]);  // (no weight: 0 * 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = mm == -INFINITY && den == 0.0f ? 0.0f : x[j] / inv;
-        *reinterpret_cast<v4f*>(dst + d) = x;
+        for (int c = 0; c < W; ++c) dst[d + c] = den == 0.0f ? 0.0f : x[c] / inv;
     }
 }
 
-// out from the S partials of every unit: one thread per four values.
+// out from the S partials of every unit (tiles of TR rows).  A row takes HD / 4 lanes, four values
+// each, in sg copies that share its splits (sg = 1 where there are rows enough to fill the GPU).
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4AttnArgs a, int units) {
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int d = (int)(idx % (HD / 4)) * 4, row = (int)(idx / (HD / 4) % 16);
-    const long long unit = idx / (HD / 4) / 16;
-    if (unit >= units) return;
-    const int G = a.H / a.Hkv, tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles), R = tile * 16 + row;
-    if (R >= a.M * G) return;
-    const float* part = a.work + (size_t)unit * a.S * (16 * (HD + 2));
-    float mm = -INFINITY, den = 0.0f;
-    for (int s = 0; s < a.S; ++s) mm = fmaxf(mm, part[(size_t)s * 16 * (HD + 2) + 16 * HD + 2 * row]);
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4AttnArgs a, int TR, int sg) {
+    constexpr int LR = HD / 4, GR = 256 / LR;
+    __shared__ v4f sx[GR][LR];
+    __shared__ float sd[GR];
+    const int t = threadIdx.x, c = t % LR, grp = t / LR;
+    const int G = a.H / a.Hkv, rows = a.M * G;
+    const long long rr = (long long)blockIdx.x * (GR / sg) + grp / sg;  // (unit, row of the tile)
+    const long long unit = rr / TR;
+    const int row = (int)(rr % TR), tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles), R = tile * TR + row;
+    const bool live = bh < a.bh && R < rows;
+    const size_t psz = (size_t)TR * (HD + 2);
+    const float* part = a.work + (live ? (size_t)unit * a.S : 0) * psz;
+    const float* pm = part + (size_t)TR * HD + 2 * (live ? row : 0);
+    float mm = -INFINITY;
+    for (int s = c; s < a.S; s += LR) mm = fmaxf(mm, pm[s * psz]);
+#pragma unroll
+    for (int w = 1; w < LR; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
     v4f x{};
-    for (int s = 0; s < a.S; ++s) {
-        const float* ps = part + (size_t)s * 16 * (HD + 2);
-        const float m = ps[16 * HD + 2 * row], l = ps[16 * HD + 2 * row + 1];
-        if (m == -INFINITY && l == 0.0f) continue;
-        const float f = exp2f(m - mm);
-        const v4f y = *reinterpret_cast<const v4f*>(ps + row * HD + d);
-        den += f * l;
+    float den = 0.0f;
+    for (int s = grp % sg; s < a.S; s += sg) {
+        const float m = pm[s * psz], l = pm[s * psz + 1];
+        const v4f y = *reinterpret_cast<const v4f*>(part + s * psz + (size_t)(live ? row : 0) * HD + 4 * c);
+        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+        den = fmaf(f, l, den);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += f * y[j];
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(f, y[e], x[e]);  // (no weight: 0 * 0)
     }
+    if (sg > 1) {
+        sx[grp][c] = x;
+        if (c == 0) sd[grp] = den;
+        __syncthreads();
+        if (grp % sg) return;
+        for (int k = 1; k < sg; ++k) {
+            x += sx[grp + k][c];
+            den += sd[grp + k];
+        }
+    }
+    if (!live) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = den == 0.0f ? 0.0f : x[j] / den;
-    *reinterpret_cast<v4f*>(a.out + (((size_t)(bh / a.Hkv) * a.M + R / G) * a.H + (size_t)(bh % a.Hkv) * G + R % G) * HD + d) = x;
+    for (int e = 0; e < 4; ++e) x[e] = den == 0.0f ? 0.0f : x[e] / den;
+    *reinterpret_cast<v4f*>(a.out + (((size_t)(bh / a.Hkv) * a.M + R / G) * a.H + (size_t)(bh % a.Hkv) * G + R % G) * HD +
+                            4 * c) = x;
 }
 
 // Workgroups of 256 in one launch: its work items are counted in 32 bits.
@@ -566,26 +670,28 @@ hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, 
 }
 
 namespace {
-// Row tiles of 16, and the splits of the keys that fill the chip (two workgroups a CU) where
+// Row tiles of RT rows, and the splits of the keys that fill the chip (two workgroups a CU) where
 // the units alone do not.
 struct Kv4Shape {
     long long units;
-    int tiles, S;
+    int RT, tiles, S;
 };
 Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     Kv4Shape p;
-    const long long tiles = ((long long)M * (H / Hkv) + 15) / 16;
+    const long long rows = (long long)M * (H / Hkv);
+    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    const long long tiles = (rows + p.RT - 1) / p.RT;
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;
     const int quads = (Lmax + 4 * kKv4Block - 1) / (4 * kKv4Block);
-    p.S = (int)std::max(1ll, std::min<long long>(quads, (512 + p.units - 1) / p.units));
+    p.S = (int)std::max(1ll, std::min<long long>(quads, 512 / p.units));
     return p;
 }
 }  // namespace
 
 size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax) {
     const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
-    return p.S > 1 ? (size_t)p.units * p.S * 16 * (hd + 2) * sizeof(float) : 0;
+    return p.S > 1 ? (size_t)p.units * p.S * p.RT * (hd + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
@@ -593,15 +699,23 @@ hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, i
     const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
     if (p.units * p.S > kMaxGroups) return hipErrorInvalidValue;
     const Kv4AttnArgs a{q, static_cast<const uint8_t*>(cache), out, work, pos, M, H, Hkv, Lmax,
-                        (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, 1.44269504088896341f / sqrtf((float)hd)};
+                        (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv, 1.44269504088896341f / sqrtf((float)hd)};
     auto go = [&](auto kernel, auto combine) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(p.units * p.S)), dim3(256), 0, s, a);
-        if (p.S > 1)
-            hipLaunchKernelGGL(combine, dim3((unsigned)((p.units * 16 * (hd / 4) + 255) / 256)), dim3(256), 0, s, a,
-                               (int)p.units);
+        if (p.S > 1) {
+            const long long all = p.units * p.RT, gr = 1024 / hd;  // rows; rows a workgroup where sg is 1
+            const int sg = all >= 4096 ? 1 : (int)gr;
+            hipLaunchKernelGGL(combine, dim3((unsigned)((all * sg + gr - 1) / gr)), dim3(256), 0, s, a, p.RT, sg);
+        }
     };
-    if (hd == 128) go(kv4_attn_kernel<128>, kv4_combine_kernel<128>);
-    else go(kv4_attn_kernel<64>, kv4_combine_kernel<64>);
+    switch (p.RT + (hd == 128 ? 1 : 0)) {
+        case 4: go(kv4_attn_kernel<64, 4>, kv4_combine_kernel<64>); break;
+        case 5: go(kv4_attn_kernel<128, 4>, kv4_combine_kernel<128>); break;
+        case 8: go(kv4_attn_kernel<64, 8>, kv4_combine_kernel<64>); break;
+        case 9: go(kv4_attn_kernel<128, 8>, kv4_combine_kernel<128>); break;
+        case 16: go(kv4_attn_kernel<64, 16>, kv4_combine_kernel<64>); break;
+        default: go(kv4_attn_kernel<128, 16>, kv4_combine_kernel<128>); break;
+    }
     return hipGetLastError();
 }
 

@@ -538,6 +538,8 @@ class HIPTernaryOps:
         return torch.empty((int(batch), int(n_kv_heads), (int(max_len) + 63) // 64, 72 * int(head_dim)),
                            dtype=torch.uint8, device=self.device)
 
+    # A step of decoding is a few microseconds of GPU work, so these calls look at each tensor once and
+    # touch nothing that is already as the library takes it.
     def _kv4_check(self, who, cache, pos, max_len):
         """(B, Hkv, hd, Lmax) of a cache and its positions."""
         torch = _torch()
@@ -549,21 +551,26 @@ class HIPTernaryOps:
         Lmax = 64 * blocks if max_len is None else int(max_len)
         if not 64 * (blocks - 1) < Lmax <= 64 * blocks:
             raise ValueError(f"{who}: max_len {Lmax} does not fit a cache of {blocks} blocks of 64 positions")
-        if pos.dtype != torch.int32 or tuple(pos.shape) != (B,) or pos.device != self.device or not pos.is_contiguous():
+        if pos.dtype != torch.int32 or pos.shape != (B,) or pos.device != self.device or not pos.is_contiguous():
             raise ValueError(f"{who}: pos must be a contiguous int32 [{B}] tensor on the backend's device")
         return B, Hkv, size // 72, Lmax
 
     def _kv4_in(self, x):
         """float32 device tensor, contiguous and 16-byte aligned (a copy where x is not)."""
-        t = self._dev(x, _torch().float32)
-        return t.clone() if t.data_ptr() % 16 else t
+        torch = _torch()
+        if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.device == self.device
+                and x.is_contiguous()):
+            x = self._dev(x, torch.float32)
+        return x.clone() if x.data_ptr() & 15 else x
 
-    def _kv4_out(self, who, out, shape):
+    def _kv4_out(self, who, out, like):
+        """out, or a new tensor of like's shape."""
         torch = _torch()
         if out is None:
-            return torch.empty(shape, dtype=torch.float32, device=self.device)
-        if out.dtype != torch.float32 or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != self.device:
-            raise ValueError(f"{who}: the output must be a contiguous float32 {list(shape)} tensor on the backend's device")
+            return torch.empty_like(like)
+        if out.dtype != torch.float32 or out.shape != like.shape or not out.is_contiguous() or out.device != self.device:
+            raise ValueError(f"{who}: the output must be a contiguous float32 {list(like.shape)} tensor on the backend's "
+                             "device")
         return out
 
     def kv4_append(self, q, k, v, cache, rope, pos, max_len=None, q_out=None):
@@ -573,32 +580,36 @@ class HIPTernaryOps:
         than its blocks hold (None: as many as the blocks and rope hold).  Rows outside
         [0, max_len) are not written; their q is 0."""
         B, Hkv, hd, Lmax = self._kv4_check("kv4_append", cache, pos, max_len)
-        qt, kt, vt, rt = (self._kv4_in(x) for x in (q, k, v, rope))
-        if max_len is None and rt.ndim == 3:
-            Lmax = min(Lmax, max(rt.shape[0], Lmax - 63))
-        if qt.ndim != 4 or qt.shape[0] != B or qt.shape[3] != hd or qt.shape[2] % Hkv or qt.numel() == 0:
-            raise ValueError(f"kv4_append: q of shape {tuple(qt.shape)} does not fit a cache of {B} sequences, {Hkv} KV "
+        q, k, v, rope = self._kv4_in(q), self._kv4_in(k), self._kv4_in(v), self._kv4_in(rope)
+        if max_len is None and rope.ndim == 3:
+            Lmax = min(Lmax, max(rope.shape[0], Lmax - 63))
+        if q.ndim != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[2] % Hkv or q.numel() == 0:
+            raise ValueError(f"kv4_append: q of shape {tuple(q.shape)} does not fit a cache of {B} sequences, {Hkv} KV "
                              f"heads of {hd}")
-        M, H = qt.shape[1], qt.shape[2]
-        if tuple(kt.shape) != (B, M, Hkv, hd) or kt.shape != vt.shape:
+        M, H = q.shape[1], q.shape[2]
+        if k.shape != (B, M, Hkv, hd) or k.shape != v.shape:
             raise ValueError(f"kv4_append: k and v must be {[B, M, Hkv, hd]}")
-        if rt.ndim != 3 or tuple(rt.shape[1:]) != (hd // 2, 2) or rt.shape[0] < Lmax:
+        if rope.ndim != 3 or rope.shape[1:] != (hd // 2, 2) or rope.shape[0] < Lmax:
             raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
-        out = self._kv4_out("kv4_append", q_out, qt.shape)
+        out = self._kv4_out("kv4_append", q_out, q)
         self._bind_stream()
-        _hip.check(self.lib.rt_kv4_append(self.ctx, qt.data_ptr(), kt.data_ptr(), vt.data_ptr(), rt.data_ptr(),
-                                          cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr()),
-                   "rt_kv4_append")
+        rc = self.lib.rt_kv4_append(self.ctx, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), cache.data_ptr(),
+                                    out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
+        _hip.check(rc, "rt_kv4_append")
         return out
 
     def kv4_read(self, cache, pos, length: int, max_len=None):
         """The values that a 4-bit cache holds at positions pos[b] + (0 .. length - 1): (k, v)
         float32 [B, Hkv, length, hd]; zeros outside [0, max_len) (rt_kv4_read)."""
+        torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_read", cache, pos, max_len)
-        k, v = (self._kv4_out("kv4_read", None, (B, Hkv, int(length), hd)) for _ in range(2))
+        if not 0 < length <= Lmax:
+            raise ValueError(f"kv4_read: length {length} of a cache of {Lmax} positions")
+        k = torch.empty((B, Hkv, length, hd), dtype=torch.float32, device=self.device)
+        v = torch.empty_like(k)
         self._bind_stream()
-        _hip.check(self.lib.rt_kv4_read(self.ctx, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, int(length), Hkv, hd,
-                                        Lmax, pos.data_ptr()), "rt_kv4_read")
+        _hip.check(self.lib.rt_kv4_read(self.ctx, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, length, Hkv, hd, Lmax,
+                                        pos.data_ptr()), "rt_kv4_read")
         return k, v
 
     def kv4_attention(self, q, cache, pos, max_len=None, out=None):
@@ -606,19 +617,19 @@ class HIPTernaryOps:
         pos[b] + m over a 4-bit cache (rt_kv4_attention): float32 [B, M, H, hd]."""
         torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", cache, pos, max_len)
-        qt = self._kv4_in(q)
-        if qt.ndim != 4 or qt.shape[0] != B or qt.shape[3] != hd or qt.shape[2] % Hkv or qt.numel() == 0:
-            raise ValueError(f"kv4_attention: q of shape {tuple(qt.shape)} does not fit a cache of {B} sequences, {Hkv} "
+        q = self._kv4_in(q)
+        if q.ndim != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[2] % Hkv or q.numel() == 0:
+            raise ValueError(f"kv4_attention: q of shape {tuple(q.shape)} does not fit a cache of {B} sequences, {Hkv} "
                              f"KV heads of {hd}")
-        M, H = qt.shape[1], qt.shape[2]
-        y = self._kv4_out("kv4_attention", out, qt.shape)
+        M, H = q.shape[1], q.shape[2]
+        out = self._kv4_out("kv4_attention", out, q)
         need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._bind_stream()
-        _hip.check(self.lib.rt_kv4_attention(self.ctx, qt.data_ptr(), cache.data_ptr(), y.data_ptr(), B, M, H, Hkv, hd,
-                                             Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need),
-                   "rt_kv4_attention")
-        return y
+        rc = self.lib.rt_kv4_attention(self.ctx, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax,
+                                       pos.data_ptr(), ws.data_ptr() if need else None, need)
+        _hip.check(rc, "rt_kv4_attention")
+        return out
 
     def __del__(self):
         try:

@@ -169,6 +169,9 @@ def test_python_refusals(ops):
                  (f(3, 0, 6, 64), f(3, 0, 2, 64), f(3, 0, 2, 64), rope)]:
         with pytest.raises(ValueError, match="kv4_append"):
             ops.kv4_append(*args[:3], cache, args[3], pos)
+    for n in (0, -1, 129):
+        with pytest.raises(ValueError, match="length"):
+            ops.kv4_read(cache, pos, n)
     with pytest.raises(ValueError, match="rope"):
         ops.kv4_append(q, kv, kv, cache, rope[:99], pos, max_len=100)
     with pytest.raises(ValueError, match="output"):
