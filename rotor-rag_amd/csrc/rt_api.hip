@@ -125,6 +125,7 @@ hipError_t prepare_device(int dev) {
     if (done[dev]) return hipSuccess;
     hipError_t e = gemm_prepare_device();
     if (e == hipSuccess) e = model_prepare_device();
+    if (e == hipSuccess) e = kv4_prepare_device();
     if (e == hipSuccess) done[dev] = true;
     return e;
 }

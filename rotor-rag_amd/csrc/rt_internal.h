@@ -422,6 +422,7 @@ hipError_t launch_attn_partial(const float* q, const float* knew, const float* v
                                float* work, hipStream_t s);
 hipError_t launch_attn_combine(const float* work, int H, int hd, int S, float* out, hipStream_t s);
 // 4-bit KV cache (rt_kv4.hip)
+hipError_t kv4_prepare_device();
 size_t kv4_bytes(int B, int Hkv, int hd, int Lmax);
 size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax);
 hipError_t launch_kv4_append(const float* q, const float* k, const float* v, const float* rope, void* cache,

@@ -24,6 +24,7 @@
 //
 // Floating-point contraction is off: what is rounded where is part of the cache's definition.
 #include <algorithm>
+#include <type_traits>
 
 #include "rt_internal.h"
 
@@ -33,6 +34,7 @@ namespace rt {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -224,13 +226,16 @@ __device__ __forceinline__ unsigned kv4_mask() {
     asm("" : "+v"(m));
     return m;
 }
-__device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
+__device__ __forceinline__ v2h kv4_level2(unsigned w, int i, unsigned mask) {  // elements 2 i, 2 i + 1
     const v2h f = {(_Float16)0.125f, (_Float16)0.125f}, o = {(_Float16)-143.0f, (_Float16)-143.0f};
+    const unsigned n = i == 0 ? w << 4 : w >> (4 * i - 4);
+    return __builtin_elementwise_fma(__builtin_bit_cast(v2h, (n & mask) | 0x64006400u), f, o);
+}
+__device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
     v8h r;
-    const unsigned n[4] = {w << 4, w, w >> 4, w >> 8};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const v2h x = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (n[i] & mask) | 0x64006400u), f, o);
+        const v2h x = kv4_level2(w, i, mask);
         r[2 * i] = x[0];
         r[2 * i + 1] = x[1];
     }
@@ -241,14 +246,18 @@ __device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
 // the product that x comes from and its conversion apart: fused (v_fma_mixlo_f16) in one use of
 // hi and not in the other, hi differs by its last bit in one of some ten thousand, and that
 // much of x was lost (5e-6 of a result over 8192 keys).
+__device__ __forceinline__ float kv4_minus_one() {
+    float m = -1.0f;
+    asm("" : "+s"(m));
+    return m;
+}
 __device__ __forceinline__ void kv4_split(v2f x, v2h& hi, v2h& lo) {
     float a = x[0], b = x[1];
     asm("" : "+v"(a), "+v"(b));
     hi = __builtin_convertvector((v2f{a, b}), v2h);
-    float c, d;  // a - hi[0], b - hi[1]: one instruction each, with hi's halves as they lie
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(c) : "v"(hi), "v"(a));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(hi), "v"(b));
-    lo = __builtin_convertvector((v2f{c, d}), v2h);
+    // (- 1.0 as a number that the compiler does not see: a subtraction would convert hi first)
+    const float m = kv4_minus_one();
+    lo = __builtin_convertvector((v2f{fmaf((float)hi[0], m, a), fmaf((float)hi[1], m, b)}), v2h);
 }
 // 2^n as fp32, -126 <= n <= 127
 __device__ __forceinline__ float kv4_pow2(int n) { return __uint_as_float((unsigned)(n + 127) << 23); }
@@ -586,6 +595,383 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     }
 }
 
+// ---- many rows -----------------------------------------------------------------------------
+// A workgroup takes a tile of 256 rows (R = m G + g) of one KV head, 32 for each of its 8 waves, over
+// blocks of 64 keys.  Together the waves turn a block's codes into keys and values once, as two fp16
+// terms each (k 2^a = z 2^a + h 2^a u, the largest of the block in [2^14, 2^15); values with the
+// largest so far), into LDS (64 KiB a block at 128 dimensions, two blocks) in the order of the matrix
+// instructions; each wave then does, on 32x32x16 products with fp32 sums,
+//   S^T = K Q^T and O^T += V^T P^T, each as hi hi + hi lo + lo hi (what is left out is below 2^-22),
+// with an online softmax (base 2) per row, rows on lanes: a lane half holds keys 8 (r / 4) +
+// 4 (l / 32) + r % 4 of its row in register r, which is the value product's operand as it is.
+// The conversion of the next block goes out in pieces of some 12 vector instructions, one under every
+// three products of the second half block.  LDS operands are requested two steps (six products)
+// before their use, the codes of the block after next while this one is worked on.
+// The other way round, codes as exact operands and the scales on the scores as for few rows, does
+// with two products of three but asks the vector units for 18 operations a score instead of 9.
+// A NaN among the values (a group that reads as NaN) becomes 0 in LDS and is put into the sums of
+// the rows that see it afterwards: in a product it would reach every row.
+// The largest of a wave's upper and lower halves (unsigned, each for itself), in an SGPR.
+__device__ __forceinline__ unsigned kv4_wave_max2(unsigned x) {
+    typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+    auto most = [](unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(v2s, a), __builtin_bit_cast(v2s, b)));
+    };
+    x = most(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xF, 0xF, false));  // row_ror 1, 2, 4, 8
+    x = most(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xF, 0xF, false));
+    x = most(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xF, 0xF, false));
+    x = most(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xF, 0xF, false));
+    const v2u y = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = most(y[0], y[1]);
+    const v2u w = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(most(w[0], w[1]));
+}
+
+constexpr int kKv4Tile = 256;
+
+template <int HD>
+__global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a) {
+    constexpr int NG = HD / 64, NU = HD / 32, OCT = HD / 8, TR = kKv4Tile;
+    constexpr int PLANE = OCT * 64, BUF = 4 * PLANE;  // 16-byte units: K hi, K lo, V hi, V lo
+    extern __shared__ __attribute__((aligned(16))) v8h lds_kv4[];  // two blocks of
+    // keys [octet of dimensions][64] and values [4 w + 2 s + l][HD], hi then lo
+    // the last tiles see the most keys: they go out first, of all heads
+    const int w0 = (int)blockIdx.x, split = w0 % a.S, unit0 = w0 / a.S, bh = unit0 % a.bh, tile = a.tiles - 1 - unit0 / a.bh;
+    const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
+    const int t = threadIdx.x, lane = t & 63, c32 = lane & 31, hl = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const unsigned mask = kv4_mask();
+    const int pos = a.pos[b];
+    const int rows = a.M * G, R0 = tile * TR + wave * 32, R = min(R0 + c32, rows - 1), m = R / G;
+    const int last = kv4_row_pos(pos, m, a.Lmax);
+    // keys [0, kend) of the tile's rows, from its first and last row
+    const int m0 = tile * TR / G, m1 = (min(tile * TR + TR, rows) - 1) / G;
+    const long long pe = min((long long)pos + m1, (long long)a.Lmax - 1);
+    const int kend = pe < 0 || (long long)pos + m0 >= a.Lmax ? 0 : (int)pe + 1;
+    int lo_last = last, hi_last = last;  // of the wave's rows
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+        lo_last = min(lo_last, __shfl_xor(lo_last, w, 64));
+        hi_last = max(hi_last, __shfl_xor(hi_last, w, 64));
+    }
+    lo_last = __builtin_amdgcn_readfirstlane(lo_last);
+    hi_last = R0 < rows ? __builtin_amdgcn_readfirstlane(hi_last) : -1;
+    const int nb = (kend + kKv4Block - 1) / kKv4Block;
+    const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
+    // This thread's part of a block.  Keys: of key `lane`, lane group ch = wave % 4, group wave / 4 (64
+    // dimensions: octet wave / 4).  Values: dimensions (u, v, d), (u, d) = vl, over the keys of lane group ch
+    // of half wv (64 dimensions: v = wave / 4), with these keys' scales.  And the scales of key `lane`, from
+    // which every wave finds the block's largest numbers.
+    const int ch = wave & 3, cg = wave >> 2;
+    const int vl = HD == 128 ? lane : lane & 31, wv = HD == 128 ? cg : lane >> 5;
+    const int vkey = 32 * wv + 16 * (ch >> 1) + 4 * (ch & 1);  // first of its keys: + (0..3, 8..11)
+    // (byte offsets in a block, whose address is uniform)
+    const unsigned at_k = (lane * OCT + ch * 2 * NG + cg * NG) * 4,
+                   at_v = 32 * HD + ((vl * 4 + ch) * 4 + wv + (NG == 2 ? 0 : 2 * cg)) * 4,
+                   at_s = 64 * HD + lane * 4, at_vs = 68 * HD + ((vl >> 5) * 64 + vkey) * 4;
+    unsigned kc[NG], vc[NG], ks[NG], vk[NG];
+    v4u vs[2];
+    const uint8_t* blk = head;  // the block that is loaded
+    auto word = [&](unsigned at) __attribute__((always_inline)) { return *reinterpret_cast<const unsigned*>(blk + at); };
+    constexpr int LK = 2 * NG, LV = 2 * NG + 2;  // loads of the keys' and of the values' part
+    auto load_k = [&](int n) __attribute__((always_inline)) {
+        if (n < NG) kc[n] = word(at_k + 4 * n);
+        else ks[n - NG] = word(at_s + 256 * (n - NG));
+    };
+    auto load_v = [&](int n) __attribute__((always_inline)) {
+        if (n < NG) vc[n] = word(at_v + 8 * n);
+        else if (n < 2 * NG) vk[n - NG] = word(at_s + 4 * HD + 256 * (n - NG));
+        else vs[n - 2 * NG] = *reinterpret_cast<const v4u*>(blk + (at_vs + 32 * (n - 2 * NG)));
+    };
+    auto load_ks = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < LK; ++n) load_k(n);
+    };
+    auto load_vs = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < LV; ++n) load_v(n);
+    };
+    // the block's codes -> LDS; what the products over it need to know
+    struct Blk {
+        float c;    // scores' factor but for the row's
+        float fix;  // factor of the sums so far
+        unsigned long long nan[NG];  // keys whose values read as NaN, by group
+    };
+    int ve = -111;  // exponent of the largest value so far
+    float kf = 0.0f, vf = 0.0f;
+    // the block in registers, before its conversion: `more` false: there is none
+    auto prepare = [&](int j, bool more) __attribute__((always_inline)) {
+        const int key0 = j * kKv4Block;
+        Blk n;
+        if (key0 + kKv4Block > kend) {  // what lies behind the newest key is not read as a number
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                if (key0 + lane >= kend) ks[g] = vk[g] = 0u;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (key0 + vkey + 8 * x + r >= kend) vs[x][r] = 0u;
+        }
+        float kmax = 0.0f, vmax = 0.0f;
+        unsigned long long nans = 0ull;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            kmax = fmaxf(kmax, fmaf(15.0f, kv4_h(ks[g]), fabsf(kv4_z(ks[g]))));
+            vmax = fmaxf(vmax, fmaf(15.0f, kv4_h(vk[g]), fabsf(kv4_z(vk[g]))));
+            n.nan[g] = __ballot((vk[g] & 0x7F800000u) == 0x7F800000u);
+            nans |= n.nan[g];
+        }
+        if (nans != 0ull)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if ((vs[x][r] & 0x7F800000u) == 0x7F800000u) vs[x][r] = 0u;
+        // (their exponents' order is that of their upper halves)
+        const unsigned top2 = kv4_wave_max2(__float_as_uint(kmax) >> 16 | (__float_as_uint(vmax) & 0xFFFF0000u));
+        const int ke = min(max((int)(top2 >> 7 & 255u) - 127, -111), 127);
+        const int vn = more ? min(max((int)(top2 >> 23) - 127, ve), 127) : ve;
+        kf = kv4_pow2(14 - ke);
+        vf = kv4_pow2(14 - vn);
+        n.c = kv4_pow2(ke - 14);
+        n.fix = ve - vn < -126 ? 0.0f : kv4_pow2(ve - vn);
+        ve = vn;
+        return n;
+    };
+    // piece k of its conversion: elements 2 (k % 4), .. + 1 of dword k / 4, and a dword's stores with its last
+    v4u chi, clo;
+    auto piece = [&](unsigned w, int k, float z0, float h0, float z1, float h1, v8h* hi_at, v8h* lo_at)
+                     __attribute__((always_inline)) {
+        const v2h u = kv4_level2(w, k % 4, mask);
+        v2h hi, lo;
+        kv4_split(v2f{fmaf((float)u[0], h0, z0), fmaf((float)u[1], h1, z1)}, hi, lo);
+        chi[k % 4] = __builtin_bit_cast(unsigned, hi);
+        clo[k % 4] = __builtin_bit_cast(unsigned, lo);
+        if (k % 4 == 3) {
+            *hi_at = __builtin_bit_cast(v8h, chi);
+            *lo_at = __builtin_bit_cast(v8h, clo);
+        }
+    };
+    auto piece_k = [&](int k, v8h* buf) __attribute__((always_inline)) {
+        // 128 dimensions: octets 8 g + 2 ch + e; 64: octet 2 ch + wave / 4
+        const unsigned own = NG == 2 && cg ? ks[NG - 1] : ks[0];
+        const float z = kv4_z(own) * kf, h = kv4_h(own) * kf;
+        v8h* const at = buf + (NG == 2 ? 8 * cg + 2 * ch + k / 4 : 2 * ch + cg) * 64 + lane;
+        piece(kc[k / 4], k, z, h, z, h, at, at + PLANE);
+    };
+    auto piece_v = [&](int k, v8h* buf) __attribute__((always_inline)) {
+        const unsigned s0 = vs[k % 4 / 2][k % 2 * 2], s1 = vs[k % 4 / 2][k % 2 * 2 + 1];
+        v8h* const at = buf + 2 * PLANE + (4 * wv + ch) * HD + vl / 16 * 32 + 16 * (NG == 2 ? k / 4 : cg) + vl % 16;
+        piece(vc[k / 4], k, kv4_z(s0) * vf, kv4_h(s0) * vf, kv4_z(s1) * vf, kv4_h(s1) * vf, at, at + PLANE);
+    };
+    auto convert = [&](v8h* buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4 * NG; ++k) piece_k(k, buf);
+#pragma unroll
+        for (int k = 0; k < 4 * NG; ++k) piece_v(k, buf);
+    };
+    if (split < nb) {
+        blk = head + (size_t)split * kv4_block_bytes(HD);
+        load_ks();
+        load_vs();
+    }
+    // the row's queries: dimensions 16 s + 8 hl + (0..7) in lane half hl
+    float qi;
+    v8h qh[OCT / 2], ql[OCT / 2];
+    {
+        float qx[OCT / 2][8], big = 0.0f;
+        const float* qp = a.q + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD + 8 * hl;
+#pragma unroll
+        for (int s = 0; s < OCT / 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const v4f x = *reinterpret_cast<const v4f*>(qp + 16 * s + 4 * e);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    qx[s][4 * e + c] = x[c] * a.scale;
+                    big = fmaxf(big, fabsf(qx[s][4 * e + c]));
+                }
+            }
+        const int qe = kv4_query_power(kv4_join32(big, Kv4Max()));
+        const float qf = kv4_pow2(qe);
+        qi = kv4_pow2(-qe);
+#pragma unroll
+        for (int s = 0; s < OCT / 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                v2h hi, lo;
+                kv4_split(v2f{qx[s][e] * qf, qx[s][e + 1] * qf}, hi, lo);
+                qh[s][e] = hi[0];
+                qh[s][e + 1] = hi[1];
+                ql[s][e] = lo[0];
+                ql[s][e + 1] = lo[1];
+            }
+    }
+    v16f o[NU];
+    float top = -INFINITY, lrow = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) o[u] = v16f{};
+    Blk cur{}, next{};
+    // 32 keys (half w of a block): scores, softmax, values.  With NEXT, a piece of the next block's
+    // conversion goes out under every three products.
+    auto multiply = [&](auto w_, auto next_, int j, const v8h* buf, v8h* other) __attribute__((always_inline)) {
+        constexpr int w = decltype(w_)::value;
+        constexpr bool NEXT = decltype(next_)::value;
+        const int key0 = j * kKv4Block + 32 * w;
+        const v8h* const lk = buf + 32 * w + c32 + hl * 64;
+        const v8h* const lv = buf + 2 * PLANE + (4 * w + hl) * HD + c32;
+        constexpr int QS = OCT / 2, VS = 2 * NU, AHEAD = 2;
+        v8h rh[AHEAD + 1], rl[AHEAD + 1];
+        auto fetch = [&](int k) __attribute__((always_inline)) {  // operands of step k: QS of the scores, then VS of the values
+            if (k < QS) {
+                rh[k % (AHEAD + 1)] = lk[2 * k * 64];
+                rl[k % (AHEAD + 1)] = lk[PLANE + 2 * k * 64];
+            } else if (k < QS + VS) {
+                const int u = (k - QS) / 2, x = (k - QS) % 2;
+                rh[k % (AHEAD + 1)] = lv[2 * x * HD + 32 * u];
+                rl[k % (AHEAD + 1)] = lv[PLANE + 2 * x * HD + 32 * u];
+            }
+        };
+        auto spread = [&]() __attribute__((always_inline)) {  // a step's instructions: products, vector work between them
+            if constexpr (NEXT) {
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) fetch(k);
+        v16f s = v16f{};
+#pragma unroll
+        for (int k = 0; k < QS; ++k) {
+            fetch(k + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(rh[k % (AHEAD + 1)], qh[k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(rh[k % (AHEAD + 1)], ql[k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(rl[k % (AHEAD + 1)], qh[k], s, 0, 0, 0);
+            if constexpr (NEXT) piece_k(k, other);
+            else if (k >= QS - LV) load_v(k - (QS - LV));  // (a load holds the wave some 60 cycles: under the products)
+            spread();
+        }
+        const float c = qi * cur.c, fix = w == 0 ? cur.fix : 1.0f;
+        if (key0 + 31 > lo_last)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = key0 + 8 * (r >> 2) + 4 * hl + (r & 3) <= last ? s[r] : -INFINITY;
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        const float now = fmaxf(top, kv4_join32(mx, Kv4Max()) * c);
+        if (__any(now != top) || fix != 1.0f) {
+            const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+            lrow *= alpha;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) o[u] *= alpha * fix;
+            top = now;
+        }
+        const float off = 14.0f - (top == -INFINITY ? 0.0f : top);
+        v8h ph[2], pl[2];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], c, off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], c, off));
+            lrow += p0 + p1;
+            v2h hi, lo;
+            kv4_split(v2f{p0, p1}, hi, lo);
+            ph[r >> 3][r & 7] = hi[0];
+            ph[r >> 3][(r & 7) + 1] = hi[1];
+            pl[r >> 3][r & 7] = lo[0];
+            pl[r >> 3][(r & 7) + 1] = lo[1];
+        }
+#pragma unroll
+        for (int k = QS; k < QS + VS; ++k) {
+            fetch(k + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            const int u = (k - QS) / 2, x = (k - QS) % 2;
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rh[k % (AHEAD + 1)], ph[x], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rh[k % (AHEAD + 1)], pl[x], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rl[k % (AHEAD + 1)], ph[x], o[u], 0, 0, 0);
+            if constexpr (NEXT) piece_v(k - QS, other);
+            if (NEXT && k >= QS + VS - LK) load_k(k - (QS + VS - LK));
+            spread();
+        }
+    };
+    using Half0 = std::integral_constant<int, 0>;
+    using Half1 = std::integral_constant<int, 1>;
+    // The registers hold the keys' part of block j + S when block j is begun; its values' part follows.
+    // Behind the last block the last one is loaded, and converted into a buffer that is not read.
+    auto block_at = [&](int j) __attribute__((always_inline)) { return head + (size_t)min(j, nb - 1) * kv4_block_bytes(HD); };
+    if (split < nb) {
+        cur = prepare(split, true);
+        convert(lds_kv4);
+        blk = block_at(split + a.S);
+        load_ks();
+    }
+    __syncthreads();
+    int side = 0;
+    for (int j = split; j < nb; j += a.S, side ^= 1) {
+        v8h *const buf = lds_kv4 + side * BUF, *const other = lds_kv4 + (side ^ 1) * BUF;
+        const bool more = j + a.S < nb;
+        blk = block_at(j + a.S);
+        if (j * kKv4Block <= hi_last || cur.fix != 1.0f) {
+            // of a SIMD's two waves one goes first in the first half, the other in the second
+            if (wave < 4) __builtin_amdgcn_s_setprio(1);
+            multiply(Half0{}, std::false_type{}, j, buf, other);
+            if (wave < 4) __builtin_amdgcn_s_setprio(0);
+            else __builtin_amdgcn_s_setprio(1);
+            next = prepare(j + a.S, more);
+            blk = block_at(j + 2 * a.S);
+            multiply(Half1{}, std::true_type{}, j, buf, other);
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                for (unsigned long long nans = cur.nan[g]; nans != 0ull; nans &= nans - 1) {  // (rare)
+                    const bool see = j * kKv4Block + (int)__builtin_ctzll(nans) <= last;
+#pragma unroll
+                    for (int u = 2 * g; u < 2 * g + 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[u][r] = see ? __builtin_nanf("") : o[u][r];
+                }
+        } else {  // none of the wave's rows sees the block
+            load_vs();
+            next = prepare(j + a.S, more);
+            convert(other);
+            blk = block_at(j + 2 * a.S);
+            load_ks();
+        }
+        __syncthreads();
+        cur = next;
+    }
+    // O[row][dim]: dimensions 32 u + 8 (r / 4) + 4 hl + r % 4 of the lane's row
+    lrow = kv4_join32(lrow, Kv4Sum());
+    if (R0 + c32 >= rows) return;
+    const float back = kv4_pow2(max(ve - 14, -126));
+    float inv = 1.0f;
+    float* dst;
+    if (a.S > 1) {
+        float* part = a.work + ((size_t)((size_t)bh * a.tiles + tile) * a.S + split) * (TR * (HD + 2));
+        dst = part + (wave * 32 + c32) * HD;
+        if (hl == 0) {
+            part[TR * HD + 2 * (wave * 32 + c32)] = top;
+            part[TR * HD + 2 * (wave * 32 + c32) + 1] = lrow;
+        }
+    } else {
+        dst = a.out + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD;
+        inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            v4f x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[u][r + e] * inv * back;
+            *reinterpret_cast<v4f*>(dst + 32 * u + 2 * r + 4 * hl) = x;
+        }
+}
+
 // out from the S partials of every unit (tiles of TR rows).  A row takes HD / 4 lanes, four values
 // each, in sg copies that share its splits (sg = 1 where there are rows enough to fill the GPU).
 template <int HD>
@@ -636,6 +1022,11 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4AttnArgs a, i
 // Workgroups of 256 in one launch: its work items are counted in 32 bits.
 constexpr long long kMaxGroups = 0xFFFFFFFFll / 256;
 
+hipError_t kv4_prepare_device() {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<128>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, 1024 * 128);
+}
+
 size_t kv4_bytes(int B, int Hkv, int hd, int Lmax) {
     return (size_t)B * Hkv * ((Lmax + kKv4Block - 1) / kKv4Block) * kv4_block_bytes(hd);
 }
@@ -679,13 +1070,29 @@ struct Kv4Shape {
 Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     Kv4Shape p;
     const long long rows = (long long)M * (H / Hkv);
-    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 32 ? 16 : kKv4Tile;
     const long long tiles = (rows + p.RT - 1) / p.RT;
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;
-    const int quads = (Lmax + 4 * kKv4Block - 1) / (4 * kKv4Block);
-    p.S = (int)std::max(1ll, std::min<long long>(quads, 512 / p.units));
+    const int blocks = (Lmax + kKv4Block - 1) / kKv4Block, most = p.RT == kKv4Tile ? blocks : (blocks + 3) / 4;
+    p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
     return p;
+}
+template <int HD>
+hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.units * p.S)), block(256);
+    switch (p.RT) {
+        case 4: hipLaunchKernelGGL((kv4_attn_kernel<HD, 4>), grid, block, 0, s, a); break;
+        case 8: hipLaunchKernelGGL((kv4_attn_kernel<HD, 8>), grid, block, 0, s, a); break;
+        case 16: hipLaunchKernelGGL((kv4_attn_kernel<HD, 16>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL(kv4_prefill_kernel<HD>, grid, dim3(512), 1024 * HD, s, a); break;
+    }
+    if (p.S > 1) {
+        const long long all = p.units * p.RT, gr = 1024 / HD;  // rows; rows a workgroup where sg is 1
+        const int sg = all >= 4096 ? 1 : (int)gr;
+        hipLaunchKernelGGL(kv4_combine_kernel<HD>, dim3((unsigned)((all * sg + gr - 1) / gr)), block, 0, s, a, p.RT, sg);
+    }
+    return hipGetLastError();
 }
 }  // namespace
 
@@ -700,23 +1107,7 @@ hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, i
     if (p.units * p.S > kMaxGroups) return hipErrorInvalidValue;
     const Kv4AttnArgs a{q, static_cast<const uint8_t*>(cache), out, work, pos, M, H, Hkv, Lmax,
                         (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv, 1.44269504088896341f / sqrtf((float)hd)};
-    auto go = [&](auto kernel, auto combine) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(p.units * p.S)), dim3(256), 0, s, a);
-        if (p.S > 1) {
-            const long long all = p.units * p.RT, gr = 1024 / hd;  // rows; rows a workgroup where sg is 1
-            const int sg = all >= 4096 ? 1 : (int)gr;
-            hipLaunchKernelGGL(combine, dim3((unsigned)((all * sg + gr - 1) / gr)), dim3(256), 0, s, a, p.RT, sg);
-        }
-    };
-    switch (p.RT + (hd == 128 ? 1 : 0)) {
-        case 4: go(kv4_attn_kernel<64, 4>, kv4_combine_kernel<64>); break;
-        case 5: go(kv4_attn_kernel<128, 4>, kv4_combine_kernel<128>); break;
-        case 8: go(kv4_attn_kernel<64, 8>, kv4_combine_kernel<64>); break;
-        case 9: go(kv4_attn_kernel<128, 8>, kv4_combine_kernel<128>); break;
-        case 16: go(kv4_attn_kernel<64, 16>, kv4_combine_kernel<64>); break;
-        default: go(kv4_attn_kernel<128, 16>, kv4_combine_kernel<128>); break;
-    }
-    return hipGetLastError();
+    return hd == 128 ? run_kv4_attention<128>(a, p, s) : run_kv4_attention<64>(a, p, s);
 }
 
 }  // namespace rt
