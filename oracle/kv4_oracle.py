@@ -49,11 +49,11 @@ def rope(x, table, p):
     return np.concatenate([a * c - b * s, b * c + a * s], -1).astype(np.float32)
 
 
-def attention(q, K, V, pos):
+def attention(q, K, V, pos, Lmax=None):
     """q fp32 [B, M, H, hd], K and V [B, Hkv, L, hd], pos [B] -> float64 [B, M, H, hd]: keys 0..pos + m;
-    rows outside [0, L) are zeros."""
+    rows outside [0, Lmax) (None: L) are zeros."""
     B, M, H, hd = q.shape
-    Hkv, L = K.shape[1], K.shape[2]
+    Hkv, L = K.shape[1], K.shape[2] if Lmax is None else Lmax
     out = np.zeros((B, M, H, hd))
     for b in range(B):
         for m in range(M):
@@ -68,21 +68,23 @@ def attention(q, K, V, pos):
     return out
 
 
-def attention_bound(q, c, z, h, pos):
+def attention_bound(q, c, z, h, pos, Lmax=None):
     """How far the device's attention may be from attention(), elementwise (same shape), for keys and
     values given as (codes, z, h) pairs c = (ck, cv), .. [B, Hkv, L, ..].
 
-    One fp32 rounding is e = 2^-24.  A score: q times its factor (1 e), in two fp16 terms (2^-22 = 4 e),
-    2 x 64 products summed in fp32 in any order (128 e of the sum of magnitudes) and joined with z's
-    sums (63 additions, 3 more): at most 200 e of A = sum h |q u| + |z| |q|; then the difference to the
-    maximum, both of at most A in base 2, and the exponential: 2 e A log2(e) ln 2 + 4 e.  So a weight is off by
-    d = 2 (204 A + 4) e relative to the weights' mean error.  A sum over n keys: the products' two terms
-    (4 e), w's rounding and factors (4 e), 2 n additions, and as many for z; the rescalings of up to n / 64
-    blocks (2 each) and joins: at most (2 n + n / 16 + 40) e of sum p (h |u| + |z|), and the sum of weights
-    n e more."""
+    One fp32 rounding is e = 2^-24.  A score, with A = sum h |q u| + |z| |q| over its dimensions.  Few rows:
+    q times its factor (1 e), in two fp16 terms (2^-22 = 4 e), 2 x 64 products summed in fp32 in any order
+    (128 e of the sum of magnitudes, with levels c - 8 of no more than twice |u|, 2 x 128), joined with z's
+    sums (63 additions, 5 more): at most 330 e of A.  Many rows: q and k in two fp16 terms each (4 e
+    each and 4 e for the product left out, k's sum 1 e), 3 x 128 products summed: at most 400 e.  Then the
+    difference to the maximum, both of at most A in base 2, and the exponential: 2 e A log2(e) ln 2 + 4 e.  So a
+    weight is off by d = 2 (404 A + 4) e relative to the weights' mean error.  A sum over n keys: the
+    products' terms (12 e), the weight's rounding and factors (4 e), 3 n additions, and as many for z;
+    the rescalings of up to n / 32 half blocks (2 each) and joins: at most (3 n + n / 16 + 50) e of
+    sum p (h |u| + |z|), and the sum of weights n e more."""
     B, M, H, hd = q.shape
     (ck, cv), (zk, zv), (hk, hv) = c, z, h
-    Hkv, L = ck.shape[1], ck.shape[2]
+    Hkv, L = ck.shape[1], ck.shape[2] if Lmax is None else Lmax
     rep = lambda x: np.repeat(x, 64, -1)  # noqa: E731
     uk, uv = np.abs(2 * ck - 15) * rep(hk) + np.abs(rep(zk)), np.abs(2 * cv - 15) * rep(hv) + np.abs(rep(zv))
     K = rep(zk) + rep(hk) * (2 * ck - 15)
@@ -99,5 +101,5 @@ def attention_bound(q, c, z, h, pos):
                 A = (uk[b, j, :p + 1] @ np.abs(x)).max()
                 s = K[b, j, :p + 1] @ x
                 w = np.exp(s - s.max())
-                out[b, m, n] = (2 * (204 * A + 4) + 3 * (p + 1) + (p + 1) / 16 + 40) * e * (w @ uv[b, j, :p + 1] / w.sum())
+                out[b, m, n] = (2 * (404 * A + 4) + 4 * (p + 1) + (p + 1) / 16 + 50) * e * (w @ uv[b, j, :p + 1] / w.sum())
     return out

@@ -221,8 +221,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict
 // 0x6400 is 1024 + 16 c, and (1024 + 16 c) / 8 - 143 = 2 c - 15.  Masking and setting the
 // exponent are one v_and_or_b32, which takes one of its two constants from a VGPR: `mask` is
 // kv4_mask()'s.
-__device__ __forceinline__ unsigned kv4_mask() {
-    unsigned m = 0x00F000F0u;
+__device__ __forceinline__ unsigned kv4_mask(unsigned m = 0x00F000F0u) {
     asm("" : "+v"(m));
     return m;
 }
@@ -230,6 +229,22 @@ __device__ __forceinline__ v2h kv4_level2(unsigned w, int i, unsigned mask) {  /
     const v2h f = {(_Float16)0.125f, (_Float16)0.125f}, o = {(_Float16)-143.0f, (_Float16)-143.0f};
     const unsigned n = i == 0 ? w << 4 : w >> (4 * i - 4);
     return __builtin_elementwise_fma(__builtin_bit_cast(v2h, (n & mask) | 0x64006400u), f, o);
+}
+// c - 8 for the eight codes of a dword, elements 2, 3, 6 and 7 16 (c - 8): nine instructions instead of
+// eleven.  (As fp16 subnormals, c 2^-24, five would do, and the matrix instructions take them, but align
+// products by the exponents they would have if normal: results were off by 2^-18.)
+__device__ __forceinline__ v8h kv4_codes(unsigned w, unsigned mask, unsigned mask0) {
+    const v2h o = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o16 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const unsigned v = w >> 8;
+    const v2h x[4] = {__builtin_bit_cast(v2h, (w & mask0) | 0x64006400u) + o, __builtin_bit_cast(v2h, (w & mask) | 0x64006400u) + o16,
+                      __builtin_bit_cast(v2h, (v & mask0) | 0x64006400u) + o, __builtin_bit_cast(v2h, (v & mask) | 0x64006400u) + o16};
+    v8h r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[2 * i] = x[i][0];
+        r[2 * i + 1] = x[i][1];
+    }
+    return r;
 }
 __device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
     v8h r;
@@ -281,13 +296,6 @@ struct Kv4Sum {
     __device__ float operator()(float a, float b) const { return a + b; }
 };
 
-// The largest of 16 lanes' x (lanes l ^ 1, l ^ 2, l ^ 4, l ^ 8).
-__device__ __forceinline__ int kv4_rows_max(int x) {
-#pragma unroll
-    for (int w = 1; w < 16; w <<= 1) x = max(x, __shfl_xor(x, w, 64));
-    return x;
-}
-
 struct Kv4AttnArgs {
     const float* q;
     const uint8_t* cache;
@@ -297,6 +305,16 @@ struct Kv4AttnArgs {
     int M, H, Hkv, Lmax, nblk, tiles, S, bh;  // bh = B * Hkv
     float scale;  // log2(e) / sqrt(HD)
 };
+
+// What rows m0..m1 of a sequence at pos see: keys [0, kend) some of them, keys [0, all] each of them
+// (rows outside the cache see none).
+struct Kv4Range {
+    int kend, all;
+};
+__device__ __forceinline__ Kv4Range kv4_range(int pos, int m0, int m1, int Lmax) {
+    const long long p0 = (long long)pos + m0, p1 = (long long)pos + m1;
+    return {p1 < 0 || p0 >= Lmax ? 0 : (int)min(p1, (long long)Lmax - 1) + 1, p0 < 0 || p1 >= Lmax ? -1 : (int)p0};
+}
 
 // The power of two that brings the largest of a row's scaled queries into [2^14, 2^15).
 __device__ __forceinline__ int kv4_query_power(float big) { return min(max(14 - kv4_exponent(big), -113), 126); }
@@ -308,9 +326,10 @@ __device__ __forceinline__ int kv4_query_power(float big) { return min(max(14 - 
 // nothing: 131072 keys, 20 heads over 5, 44 us); the columns of a row are joined at the end.  Lane l
 // works on column i = l % 16 with the keys of lane group h = l / 16.  The split's blocks go to its
 // 4 waves in turn, an online softmax (base 2) for every column:
-//   D = U Q^T per group of 64 dimensions (U the keys' levels, exact in fp16; Q two fp16 terms,
-//       scaled so that the row's largest is in [2^14, 2^15)),  s = h D + z sum_d q
-//   w = 2^(s - ref),  O^T += U^T (w h)^T  (U the values' levels, w h two fp16 terms),  O += sum_j w z
+//   D = C Q^T per group of 64 dimensions (C the keys' codes less 8, exact in fp16; Q two fp16 terms,
+//       scaled so that the row's largest is in [2^14, 2^15)),  s = 2 h D + (z + h) sum_d q
+//   w = 2^(s - ref),  O^T += U^T (w h)^T  (U the values' levels 2 c - 15: uncentred, the sums over many
+//       keys would cancel; w h two fp16 terms),  O += sum_j w z
 // so that all products are exact and all sums fp32.  ref is the largest score so far plus e - 14,
 // 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a group's h is no less than
 // 2^-29 of it unless it is 0), which keeps w h below 2^15, and w, w z in fp32's range.
@@ -326,12 +345,20 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const unsigned mask = kv4_mask();
-    const int pos = a.pos[b];
+    const unsigned mask = kv4_mask(), mask0 = kv4_mask(0x000F000Fu);
     const int rows = a.M * G, R = min(tile * RT + i % RT, rows - 1), m = R / G;  // (rows past the end repeat the last)
+    // the row's queries, dimensions 64 g + 16 h + 8 e + (0..7): requested before the first block, since loads
+    // return in order
+    v4f qx[NG][4];
+    const float* qp = a.q + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qx[g][e] = *reinterpret_cast<const v4f*>(qp + 64 * g + 16 * h + 4 * e);
+    const int pos = a.pos[b];
     const int last = kv4_row_pos(pos, m, a.Lmax);  // keys <= last are this row's
-    const int kend = __builtin_amdgcn_readfirstlane(kv4_rows_max(last)) + 1;
-    const int all = __builtin_amdgcn_readfirstlane(-kv4_rows_max(-last));
+    const Kv4Range range = kv4_range(pos, tile * RT / G, (min(tile * RT + RT, rows) - 1) / G, a.Lmax);
+    const int kend = range.kend, all = range.all;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
     const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * a.S;
     // Key tile wx = 2 w + x of a block: keys 32 w + 8 x + kl + r of lane group h.  The column's own
@@ -339,12 +366,14 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const int kl = 16 * (h >> 1) + 4 * (h & 1);
     auto tile_key = [](int wx) { return 32 * (wx >> 1) + 8 * (wx & 1); };
     v4u kc[4], ks[NG][NQ], vc[2 * NG], vs[NG][NQ];
+    // (byte offsets in a block, whose address is uniform)
+    const unsigned at_k = (16 * (i >> 3) + (i & 7)) * (HD / 2) + h * 8 * NG, at_v = 32 * HD + (i * 4 + h) * 16,
+                   at_s = 64 * HD + (tile_key(ca) + kl) * 4;
     auto load_k = [&](int j) {
         const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
-        const unsigned* sc = reinterpret_cast<const unsigned*>(blk + 64 * HD);
 #pragma unroll
         for (int wx = 0; wx < 4; ++wx) {
-            const uint8_t* kp = blk + (tile_key(wx) + 16 * (i >> 3) + (i & 7)) * (HD / 2) + h * 8 * NG;
+            const uint8_t* kp = blk + (at_k + tile_key(wx) * (HD / 2));
             if constexpr (NG == 2) kc[wx] = *reinterpret_cast<const v4u*>(kp);
             else {
                 const v2u x = *reinterpret_cast<const v2u*>(kp);
@@ -355,51 +384,49 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) ks[g][q] = *reinterpret_cast<const v4u*>(sc + g * 64 + tile_key(NA * q + ca) + kl);
+            for (int q = 0; q < NQ; ++q) ks[g][q] = *reinterpret_cast<const v4u*>(blk + (at_s + (g * 64 + tile_key(NA * q)) * 4));
     };
     auto load_v = [&](int j) {
         const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
-        const unsigned* sc = reinterpret_cast<const unsigned*>(blk + 64 * HD) + HD;
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) vs[g][q] = *reinterpret_cast<const v4u*>(sc + g * 64 + tile_key(NA * q + ca) + kl);
+            for (int q = 0; q < NQ; ++q)
+                vs[g][q] = *reinterpret_cast<const v4u*>(blk + (at_s + 4 * HD + (g * 64 + tile_key(NA * q)) * 4));
 #pragma unroll
-        for (int u = 0; u < 2 * NG; ++u) vc[u] = *reinterpret_cast<const v4u*>(blk + 32 * HD + ((u * 16 + i) * 4 + h) * 16);
+        for (int u = 0; u < 2 * NG; ++u) vc[u] = *reinterpret_cast<const v4u*>(blk + (at_v + u * 1024));
     };
     int j = split * 4 + wave;
     if (j < nb) {
         load_k(j);
         load_v(j);
     }
-    // the row's queries: dimensions 64 g + 16 h + 8 e + (0..7)
     float qs[NG], qi;
     v8h qh[NG][2], ql[NG][2];
     {
-        float qx[NG][16], big = 0.0f;
-        const float* qp = a.q + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD;
+        float big = 0.0f;
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const v4f x = *reinterpret_cast<const v4f*>(qp + 64 * g + 16 * h + 4 * e);
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    qx[g][4 * e + c] = x[c] * a.scale;
-                    big = fmaxf(big, fabsf(qx[g][4 * e + c]));
+                    qx[g][e][c] *= a.scale;
+                    big = fmaxf(big, fabsf(qx[g][e][c]));
                 }
-            }
         const int qe = kv4_query_power(kv4_join16(big, Kv4Max()));
         const float qf = kv4_pow2(qe);
-        qi = kv4_pow2(-qe);
+        qi = kv4_pow2(1 - qe);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             qs[g] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const v2f x = {qx[g][e] * qf, qx[g][e + 1] * qf};
+                // (every other pair meets codes that are 16 times as large)
+                const v2f x = {qx[g][e / 4][e % 4] * qf, qx[g][e / 4][e % 4 + 1] * qf};
+                const float part = e & 2 ? 0.0625f : 1.0f;
                 v2h hi, lo;
-                kv4_split(x, hi, lo);
+                kv4_split(x * part, hi, lo);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     qh[g][e / 8][e % 8 + c] = hi[c];
@@ -407,7 +434,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
                     qs[g] += x[c];
                 }
             }
-            qs[g] = kv4_join16(qs[g], Kv4Sum());
+            qs[g] = kv4_join16(qs[g], Kv4Sum()) * 0.5f;
         }
     }
     v4f o[NT];
@@ -430,7 +457,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
                     v4f dot{};
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const v8h u = kv4_levels(kc[NA * q + c][2 * g + e], mask);
+                        const v8h u = kv4_codes(kc[NA * q + c][2 * g + e], mask, mask0);
                         dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, qh[g][e], dot, 0, 0, 0);
                         dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, ql[g][e], dot, 0, 0, 0);
                     }
@@ -442,10 +469,12 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = kv4_z(ks[0][q][r]) * qs[0];
-                if constexpr (NG == 2) x = fmaf(kv4_z(ks[1][q][r]), qs[1], x);
+                float x = 0.0f;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) x = fmaf(kv4_h(ks[g][q][r]), own[g][r], x);
+                for (int g = 0; g < NG; ++g) {
+                    const float kh = kv4_h(ks[g][q][r]);
+                    x = fmaf(kh, own[g][r], fmaf(kv4_z(ks[g][q][r]) + kh, qs[g], x));
+                }
                 s[q][r] = x;
             }
         }
@@ -644,18 +673,10 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
     const int pos = a.pos[b];
     const int rows = a.M * G, R0 = tile * TR + wave * 32, R = min(R0 + c32, rows - 1), m = R / G;
     const int last = kv4_row_pos(pos, m, a.Lmax);
-    // keys [0, kend) of the tile's rows, from its first and last row
-    const int m0 = tile * TR / G, m1 = (min(tile * TR + TR, rows) - 1) / G;
-    const long long pe = min((long long)pos + m1, (long long)a.Lmax - 1);
-    const int kend = pe < 0 || (long long)pos + m0 >= a.Lmax ? 0 : (int)pe + 1;
-    int lo_last = last, hi_last = last;  // of the wave's rows
-#pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-        lo_last = min(lo_last, __shfl_xor(lo_last, w, 64));
-        hi_last = max(hi_last, __shfl_xor(hi_last, w, 64));
-    }
-    lo_last = __builtin_amdgcn_readfirstlane(lo_last);
-    hi_last = R0 < rows ? __builtin_amdgcn_readfirstlane(hi_last) : -1;
+    const int kend = kv4_range(pos, tile * TR / G, (min(tile * TR + TR, rows) - 1) / G, a.Lmax).kend;
+    // what the wave's rows see
+    const Kv4Range mine = kv4_range(pos, min(R0, rows - 1) / G, (min(R0 + 32, rows) - 1) / G, a.Lmax);
+    const int lo_last = mine.all, hi_last = R0 < rows ? mine.kend - 1 : -1;
     const int nb = (kend + kKv4Block - 1) / kKv4Block;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
     // This thread's part of a block.  Keys: of key `lane`, lane group ch = wave % 4, group wave / 4 (64
@@ -776,17 +797,34 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         load_ks();
         load_vs();
     }
+    // A wave's rows pass through its part of LDS, queries here and results at the end, so that memory is read
+    // and written in whole lines (lane by lane, 32 rows at once, took 10000 and 9000 cycles): 16-byte unit c
+    // of row r lies at unit c ^ (r % 16).  Coalesced, instruction n takes rows n RPI + lane / UPR, unit lane % UPR.
+    constexpr int UPR = HD / 4, RPI = 64 / UPR;
+    v4f* const own = reinterpret_cast<v4f*>(lds_kv4) + wave * 32 * UPR;
+    auto in_lds = [&](int r, int c) __attribute__((always_inline)) { return own + r * UPR + (c ^ (r & 15)); };
+    const int mw = R0 / G;
+    const float inv_g = 1.0f / (float)G;
+    auto row_at = [&](int r) __attribute__((always_inline)) {  // (row R0 + r of this KV head) * HD
+        const int x = min(R0 + r, rows - 1) - mw * G, dm = (int)(((float)x + 0.5f) * inv_g);
+        return (((size_t)b * a.M + mw + dm) * a.H + (size_t)kh * G + (x - dm * G)) * HD;
+    };
     // the row's queries: dimensions 16 s + 8 hl + (0..7) in lane half hl
     float qi;
     v8h qh[OCT / 2], ql[OCT / 2];
     {
+        if (R0 < rows)
+#pragma unroll
+            for (int n = 0; n < 32 / RPI; ++n) {
+                const int r = n * RPI + lane / UPR;
+                *in_lds(r, lane % UPR) = *reinterpret_cast<const v4f*>(a.q + row_at(r) + lane % UPR * 4);
+            }
         float qx[OCT / 2][8], big = 0.0f;
-        const float* qp = a.q + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD + 8 * hl;
 #pragma unroll
         for (int s = 0; s < OCT / 2; ++s)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const v4f x = *reinterpret_cast<const v4f*>(qp + 16 * s + 4 * e);
+                const v4f x = *in_lds(c32, 4 * s + 2 * hl + e);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     qx[s][4 * e + c] = x[c] * a.scale;
@@ -903,6 +941,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
     // The registers hold the keys' part of block j + S when block j is begun; its values' part follows.
     // Behind the last block the last one is loaded, and converted into a buffer that is not read.
     auto block_at = [&](int j) __attribute__((always_inline)) { return head + (size_t)min(j, nb - 1) * kv4_block_bytes(HD); };
+    __syncthreads();  // (the waves' parts for the queries are the first block's)
     if (split < nb) {
         cur = prepare(split, true);
         convert(lds_kv4);
@@ -946,20 +985,12 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
     }
     // O[row][dim]: dimensions 32 u + 8 (r / 4) + 4 hl + r % 4 of the lane's row
     lrow = kv4_join32(lrow, Kv4Sum());
-    if (R0 + c32 >= rows) return;
-    const float back = kv4_pow2(max(ve - 14, -126));
-    float inv = 1.0f;
-    float* dst;
-    if (a.S > 1) {
-        float* part = a.work + ((size_t)((size_t)bh * a.tiles + tile) * a.S + split) * (TR * (HD + 2));
-        dst = part + (wave * 32 + c32) * HD;
-        if (hl == 0) {
-            part[TR * HD + 2 * (wave * 32 + c32)] = top;
-            part[TR * HD + 2 * (wave * 32 + c32) + 1] = lrow;
-        }
-    } else {
-        dst = a.out + (((size_t)b * a.M + m) * a.H + (size_t)kh * G + R % G) * HD;
-        inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
+    if (R0 >= rows) return;
+    const float back = kv4_pow2(max(ve - 14, -126)), inv = a.S > 1 ? 1.0f : lrow == 0.0f ? 0.0f : 1.0f / lrow;
+    float* const part = a.work + ((size_t)((size_t)bh * a.tiles + tile) * a.S + split) * (TR * (HD + 2));
+    if (a.S > 1 && hl == 0) {
+        part[TR * HD + 2 * (wave * 32 + c32)] = top;
+        part[TR * HD + 2 * (wave * 32 + c32) + 1] = lrow;
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -968,47 +999,71 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
             v4f x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = o[u][r + e] * inv * back;
-            *reinterpret_cast<v4f*>(dst + 32 * u + 2 * r + 4 * hl) = x;
+            *in_lds(c32, 8 * u + r / 2 + hl) = x;
         }
+#pragma unroll
+    for (int n = 0; n < 32 / RPI; ++n) {
+        const int r = n * RPI + lane / UPR;
+        float* const dst = a.S > 1 ? part + (wave * 32 + r) * HD : a.out + row_at(r);
+        const v4f x = *in_lds(r, lane % UPR);
+        if (R0 + r < rows) *reinterpret_cast<v4f*>(dst + lane % UPR * 4) = x;
+    }
 }
 
 // out from the S partials of every unit (tiles of TR rows).  A row takes HD / 4 lanes, four values
-// each, in sg copies that share its splits (sg = 1 where there are rows enough to fill the GPU).
+// each, in sg copies that share its splits: 1 where there are rows enough to fill the GPU, else all
+// of the workgroup's (1024 threads where there are many splits, so that each lane has few loads, all
+// in flight at once).
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4AttnArgs a, int TR, int sg) {
-    constexpr int LR = HD / 4, GR = 256 / LR;
-    __shared__ v4f sx[GR][LR];
-    __shared__ float sd[GR];
+__global__ void __launch_bounds__(1024) kv4_combine_kernel(const Kv4AttnArgs a, int TR, int sg) {
+    constexpr int LR = HD / 4, AT = 4;
+    __shared__ v4f sx[1024];
+    __shared__ float sd[1024 / LR];
     const int t = threadIdx.x, c = t % LR, grp = t / LR;
-    const int G = a.H / a.Hkv, rows = a.M * G;
-    const long long rr = (long long)blockIdx.x * (GR / sg) + grp / sg;  // (unit, row of the tile)
-    const long long unit = rr / TR;
-    const int row = (int)(rr % TR), tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles), R = tile * TR + row;
-    const bool live = bh < a.bh && R < rows;
+    const int G = a.H / a.Hkv, rows = a.M * G, most = min(TR, rows);  // (a tile's rows that can be live)
+    const long long rr = (long long)blockIdx.x * ((int)blockDim.x / LR / sg) + grp / sg;  // (unit, row of the tile)
+    const long long unit = rr / most;
+    const int row = (int)(rr % most), tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles), R = tile * TR + row;
+    const bool live = unit < (long long)a.bh * a.tiles && R < rows;
     const size_t psz = (size_t)TR * (HD + 2);
     const float* part = a.work + (live ? (size_t)unit * a.S : 0) * psz;
-    const float* pm = part + (size_t)TR * HD + 2 * (live ? row : 0);
+    const float *pm = part + (size_t)TR * HD + 2 * (live ? row : 0), *po = part + (size_t)(live ? row : 0) * HD + 4 * c;
     float mm = -INFINITY;
     for (int s = c; s < a.S; s += LR) mm = fmaxf(mm, pm[s * psz]);
-#pragma unroll
-    for (int w = 1; w < LR; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
     v4f x{};
     float den = 0.0f;
-    for (int s = grp % sg; s < a.S; s += sg) {
-        const float m = pm[s * psz], l = pm[s * psz + 1];
-        const v4f y = *reinterpret_cast<const v4f*>(part + s * psz + (size_t)(live ? row : 0) * HD + 4 * c);
-        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
-        den = fmaf(f, l, den);
+    bool first = true;
+    for (int s0 = grp % sg; s0 < a.S || first; s0 += AT * sg) {
+        v4f y[AT];
+        float m[AT], l[AT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf(f, y[e], x[e]);  // (no weight: 0 * 0)
+        for (int k = 0; k < AT; ++k) {
+            const int s = s0 + k * sg;
+            const bool in = s < a.S;
+            m[k] = in ? pm[s * psz] : 0.0f;
+            l[k] = in ? pm[s * psz + 1] : 0.0f;
+            y[k] = in ? *reinterpret_cast<const v4f*>(po + s * psz) : v4f{};
+        }
+        if (first) {  // (the first loads are on their way meanwhile)
+#pragma unroll
+            for (int w = 1; w < LR; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
+            first = false;
+        }
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+            const float f = l[k] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mm);
+            den = fmaf(f, l[k], den);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(f, y[k][e], x[e]);  // (no weight: 0 * 0)
+        }
     }
     if (sg > 1) {
-        sx[grp][c] = x;
+        sx[t] = x;
         if (c == 0) sd[grp] = den;
         __syncthreads();
         if (grp % sg) return;
         for (int k = 1; k < sg; ++k) {
-            x += sx[grp + k][c];
+            x += sx[t + k * LR];
             den += sd[grp + k];
         }
     }
@@ -1061,20 +1116,31 @@ hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, 
 }
 
 namespace {
-// Row tiles of RT rows, and the splits of the keys that fill the chip (two workgroups a CU) where
-// the units alone do not.
+// Which kernel, and how many splits of the keys.  The host does not know the positions: a call is taken
+// to stand half way into its cache.  (Times: 20 heads of 128 over 5, the launches back to back.)
 struct Kv4Shape {
     long long units;
     int RT, tiles, S;
 };
 Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     Kv4Shape p;
-    const long long rows = (long long)M * (H / Hkv);
-    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 32 ? 16 : kKv4Tile;
+    const long long rows = (long long)M * (H / Hkv), big = (long long)B * Hkv * ((rows + kKv4Tile - 1) / kKv4Tile);
+    const int blocks = (Lmax + kKv4Block - 1) / kKv4Block;
+    // A tile of 256 rows costs some 30 us a launch before its first product pays (its queries and results
+    // pass through one workgroup a CU), and then 22 ns a block of 64 keys against 50 in tiles of 16 rows: 512
+    // tokens from an empty cache (180 blocks of tiles) 28 against 23 us, 1024 (680) 49 / 48, 128 after 8192
+    // (1290) 59 / 78, 8 sequences of 512 after 512 (3900) 126 / 187.
+    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : big * blocks < 1300 ? 16 : kKv4Tile;
     const long long tiles = (rows + p.RT - 1) / p.RT;
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;
-    const int blocks = (Lmax + kKv4Block - 1) / kKv4Block, most = p.RT == kKv4Tile ? blocks : (blocks + 3) / 4;
+    // A split's results pass through memory and a second launch (3 to 16 us), so there is none where a
+    // wave has 5 blocks or fewer without (8 sequences of 12 heads over 777 keys 7.8 us, in 4 splits 9.7), and
+    // a tile of 256 rows keeps 8 blocks a split (128 tokens after 8192: 16 splits 59 us, 24 64).  Else as many
+    // as two workgroups a CU take in one round, the big tiles, one a CU, in two: one token over 1538 keys
+    // in 8 / 4 / 1 splits 10.6 / 12.4 / 17.5 us, over 131072 in 200 / 102 / 50 36.7 / 30.8 / 34.2; 2048 of 8192
+    // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495.
+    const int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : (blocks + 3) / 4;
     p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
     return p;
 }
@@ -1088,9 +1154,10 @@ hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_
         default: hipLaunchKernelGGL(kv4_prefill_kernel<HD>, grid, dim3(512), 1024 * HD, s, a); break;
     }
     if (p.S > 1) {
-        const long long all = p.units * p.RT, gr = 1024 / HD;  // rows; rows a workgroup where sg is 1
-        const int sg = all >= 4096 ? 1 : (int)gr;
-        hipLaunchKernelGGL(kv4_combine_kernel<HD>, dim3((unsigned)((all * sg + gr - 1) / gr)), block, 0, s, a, p.RT, sg);
+        const long long all = p.units * std::min<long long>(p.RT, (long long)a.M * (a.H / a.Hkv));  // rows
+        const int threads = p.S > 16 && all < 4096 ? 1024 : 256, gr = threads / (HD / 4), sg = all >= 4096 ? 1 : gr;
+        hipLaunchKernelGGL(kv4_combine_kernel<HD>, dim3((unsigned)((all * sg + gr - 1) / gr)), dim3(threads), 0, s, a, p.RT,
+                           sg);
     }
     return hipGetLastError();
 }

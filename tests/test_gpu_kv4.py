@@ -197,10 +197,8 @@ def _check(hip, q, cache, pairs, pos, Lmax):
     y = out.cpu().numpy()
     K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
     with np.errstate(all="ignore"):
-        # positions that were never written cannot be asked for
-        pad = [np.pad(x, ((0, 0), (0, 0), (0, Lmax - x.shape[2]), (0, 0))) for x in (K, V)]
-        want = K4.attention(q, *pad, pos)
-        bound = K4.attention_bound(q, *pairs, pos)
+        want = K4.attention(q, K, V, pos, Lmax)
+        bound = K4.attention_bound(q, *pairs, pos, Lmax)
     off = np.abs(y - want)
     assert (off <= bound + 1e-37).all(), f"off by {np.max(off / (bound + 1e-37)):.3g} bounds"
     # roundings are as often up as down: the whole is far nearer than the sum of the worst cases
@@ -234,6 +232,23 @@ ATTENDS = [
 ]
 
 
+# The same rows over caches so long that they are taken in tiles of 256 (a call is taken to stand half
+# way into its cache: 1300 blocks of such tiles and more)
+ATTENDS += [
+    (1, 33, 4, 4, 64, 21000, [0], 33),
+    (1, 64, 20, 5, 128, 16700, [64], 128),
+    (1, 100, 20, 5, 128, 16700, [0], 100),
+    (2, 77, 14, 2, 64, 10600, [0, 301], 378),
+    (1, 130, 3, 3, 128, 28000, [70], 200),
+    (1, 300, 2, 2, 64, 21000, [211], 511),
+    (1, 129, 7, 1, 64, 21000, [3], 132),
+    (2, 90, 4, 2, 128, 21000, [-50, 40], 130),   # rows in front of the cache
+    (2, 40, 8, 2, 64, 21000, [-100, 30000], 1),  # nothing but rows outside it
+    (1, 70, 2, 1, 64, 83250, [83210], 83250),    # rows behind it
+    (3, 9, 1, 1, 128, 28000, [5, 0, 64], 73),    # nine rows
+]
+
+
 @pytest.mark.parametrize("B,M,H,Hkv,hd,Lmax,pos,n", ATTENDS)
 def test_attention(hip, B, M, H, Hkv, hd, Lmax, pos, n):
     cache, pairs = _filled(hip, B * 100 + M, B, H, Hkv, hd, Lmax, n)
@@ -244,23 +259,23 @@ def test_attention(hip, B, M, H, Hkv, hd, Lmax, pos, n):
             assert 0 <= pos[b] + m < Lmax or (y[b, m] == 0).all()
 
 
-@pytest.mark.parametrize("M", [1, 3, 70])
+@pytest.mark.parametrize("M,Lmax", [(1, 300), (1, 4000), (3, 300), (70, 300), (70, 21000)])
 @pytest.mark.parametrize("qs,ks,vs", [(1e-30, 1, 1), (20, 1, 1), (1, 1e-20, 1), (1e-15, 1e15, 1), (1, 1, 1e-25), (1, 1, 1e25),
                                       (0, 1, 1), (1, 0, 0)])
-def test_attention_scales(hip, M, qs, ks, vs):
+def test_attention_scales(hip, M, Lmax, qs, ks, vs):
     """Queries, keys and values of any size, zero among them."""
-    B, H, Hkv, hd, Lmax, n = 1, 8, 2, 128, 300, 290
+    B, H, Hkv, hd, n = 1, 8, 2, 128, 290
     q, k, v = _inputs(M, B, n, H, Hkv, hd)
     f = np.float32
     cache, pairs = _filled(hip, 5, B, H, Hkv, hd, Lmax, n, k=k * f(ks), v=v * f(vs))
     _check(hip, q[:, :M] * f(qs), cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M", [1, 40])
-def test_attention_values_of_very_different_sizes(hip, M):
+@pytest.mark.parametrize("M,Lmax", [(1, 700), (1, 2000), (40, 700), (40, 83300)])
+def test_attention_values_of_very_different_sizes(hip, M, Lmax):
     """The weights' fp16 terms are scaled by the largest step of the values seen: outliers, early and late, that
     weigh little do not take the others' bits."""
-    B, H, Hkv, hd, Lmax, n = 1, 4, 1, 64, 700, 700
+    B, H, Hkv, hd, n = 1, 4, 1, 64, 700
     q, k, v = _inputs(11, B, n, H, Hkv, hd)
     v *= np.exp2(np.random.default_rng(2).integers(-8, 9, (B, n, 1, 1))).astype(np.float32)
     v[:, [3, 400, 650]] *= 1000
@@ -268,25 +283,25 @@ def test_attention_values_of_very_different_sizes(hip, M):
     _check(hip, q[:, :M], cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M", [1, 24])
-def test_attention_long_and_even(hip, M):
+@pytest.mark.parametrize("M,Lmax", [(1, 8192), (24, 8192), (24, 42000)])
+def test_attention_long_and_even(hip, M, Lmax):
     """8192 keys that weigh about the same: the result is a small difference of large sums.  In 64 bits against
     fp32 sums of numbers with random signs: each of 2 x 8192 terms (magnitude at most 3 of the values' deviation)
     is off by 2^-24 of a running sum no larger than that of the result's own order times 8192; the relative error's
     deviation is below 2^-24 x sqrt(2 x 8192) = 8e-6 even if every rounding were a full half step of the largest
     running sum, and rounding errors of that size are rarer: 2e-6 is asked for (the plain fp32 form has 1e-6)."""
-    B, H, Hkv, hd, Lmax = 1, 8, 2, 128, 8192
-    q, k, v = _inputs(4, B, Lmax, H, Hkv, hd)
-    cache, pairs = _filled(hip, 5, B, H, Hkv, hd, Lmax, Lmax, k=0.05 * k, v=v)
-    y, want = _check(hip, q[:, :M], cache, pairs, [Lmax - M], Lmax)
+    B, H, Hkv, hd, n = 1, 8, 2, 128, 8192
+    q, k, v = _inputs(4, B, n, H, Hkv, hd)
+    cache, pairs = _filled(hip, 5, B, H, Hkv, hd, Lmax, n, k=np.float32(0.05) * k, v=v)
+    y, want = _check(hip, q[:, :M], cache, pairs, [n - M], Lmax)
     assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("M", [1, 9, 80])
-def test_attention_nan(hip, M):
+@pytest.mark.parametrize("M,Lmax", [(1, 200), (1, 3000), (9, 200), (80, 200), (80, 21000)])
+def test_attention_nan(hip, M, Lmax):
     """A NaN that a row sees makes that row NaN (a value's: in its group of 64 dimensions); one that it does not
     see leaves every bit of it."""
-    B, H, Hkv, hd, Lmax, n = 2, 4, 2, 128, 200, 180
+    B, H, Hkv, hd, n = 2, 4, 2, 128, 180
     q, k, v = _inputs(M, B, n, H, Hkv, hd)
     q = q[:, :M]
     pos = [n - M, 60]
@@ -305,13 +320,14 @@ def test_attention_nan(hip, M):
     assert _same(y, want)
 
 
-def test_attention_nan_query(hip):
-    B, M, H, Hkv, hd, Lmax, n = 1, 20, 4, 2, 64, 100, 90
+@pytest.mark.parametrize("Lmax", [100, 42000])
+def test_attention_nan_query(hip, Lmax):
+    B, M, H, Hkv, hd, n = 1, 20, 4, 2, 64, 90
     cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, n)
     q, _, _ = _inputs(6, B, M, H, Hkv, hd)
-    clean = hip.kv4_attention(*_cuda(q), cache, _pos([70])).cpu().numpy()
+    clean = hip.kv4_attention(*_cuda(q), cache, _pos([70]), max_len=Lmax).cpu().numpy()
     q[0, 3, 1, 5], q[0, 7, 2, 9] = np.nan, np.inf
-    y = hip.kv4_attention(*_cuda(q), cache, _pos([70])).cpu().numpy()
+    y = hip.kv4_attention(*_cuda(q), cache, _pos([70]), max_len=Lmax).cpu().numpy()
     want = clean.copy()
     want[0, 3, 1] = want[0, 7, 2] = np.nan
     assert _same(y, want)
@@ -366,13 +382,13 @@ def test_past_four_gigabytes(hip):
     assert torch.linalg.norm(both[-1] - alone[0]) <= 2e-5 * torch.linalg.norm(alone)
 
 
-@pytest.mark.parametrize("M", [1, 20])
-def test_graph_and_streams(hip, M):
+@pytest.mark.parametrize("M,Lmax", [(1, 400), (1, 5000), (20, 400), (20, 42000)])
+def test_graph_and_streams(hip, M, Lmax):
     """A step (append, attention, read) captured on a stream of its own and replayed with moving positions, with
     eager work between the replays."""
     import torch
 
-    B, H, Hkv, hd, Lmax, n = 2, 8, 2, 128, 400, 200
+    B, H, Hkv, hd, n = 2, 8, 2, 128, 200
     cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, n)
     mine = cache.clone()
     (rope,) = _cuda(_rope(Lmax, hd))
@@ -433,6 +449,6 @@ def test_prompt_then_steps(hip):
                 held[0][b, :, p], held[1][b, :, p] = K4.held(K4.rope(k[b, m], table, p)), K4.held(v[b, m])
         want = K4.attention(rq, *held, pos)
         # (at most 156 keys: the derived bound's factor, on magnitudes that are at most 5 here)
-        assert np.abs(y - want).max() <= (2 * (204 * 60 + 4) + 3 * 156 + 50) * 2.0 ** -24 * 5
+        assert np.abs(y - want).max() <= (2 * (404 * 60 + 4) + 4 * 156 + 60) * 2.0 ** -24 * 5
         assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want)
         pos += M

@@ -68,6 +68,7 @@ def test_workspace_sizes(lib):
     """Nothing for calls that fill the GPU by themselves, something for one token, 0 for refused sizes."""
     assert lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 131072) > 0
     assert lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 64) == 0
+    assert lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 640) == 0  # few keys a wave as it is
     assert lib.rt_kv4_attention_workspace(64, 512, 20, 5, 128, 4096) == 0
     for bad in [(1, 1, 21, 5, 128, 64), (1, 65, 20, 5, 128, 64), (1, 0, 20, 5, 128, 64), (1, 1, 20, 5, 32, 64),
                 (1, 1, 0, 5, 128, 64), (1, 1, 1025, 1, 64, 64)]:
@@ -121,10 +122,10 @@ def test_refusals(lib, call, bufs):
 
 
 def test_attention_refuses_small_workspaces(lib):
-    need = lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 640)
+    need = lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 4096)
     assert need > 0
     for bad in [dict(ws=None, ws_bytes=0), dict(ws_bytes=need - 1), dict(ws=ODD, ws_bytes=need)]:
-        assert _attend(lib, **bad) == RT_EINVAL
+        assert _attend(lib, Lmax=4096, **bad) == RT_EINVAL
         assert "workspace" in lib.rt_last_error().decode()
 
 
