@@ -53,19 +53,47 @@ __device__ __forceinline__ unsigned bf16_bits(float x) {  // x finite or infinit
 __device__ __forceinline__ float kv4_z(unsigned s) { return __uint_as_float(s & 0xFFFF0000u); }
 __device__ __forceinline__ float kv4_h(unsigned s) { return __uint_as_float(s << 16); }
 
-// z and h of a group from its extremes, as the cache's dword, in 64 bits up to the roundings:
-// a code next to a border must not hang on the order of fp32 operations.  A group with a
-// value that is not finite, or whose z or h is not, reads as NaN.
+// z and h of a group from its extremes, as the cache's dword.  By definition in 64 bits up to the
+// roundings, so that nothing hangs on the order of fp32 operations.  z in fp32 is the same number; h
+// in fp32 is within 2^-22 of it, so its bf16 is the same unless it lies next to a border: those (one
+// group in 4000) and very small ones take the division.  A group with a value that is not finite, or
+// whose z or h is not, reads as NaN.
 __device__ __forceinline__ unsigned kv4_scale(float lo, float hi, bool finite) {
-    const double a = 0.5 * (double)lo, b = 0.5 * (double)hi;
-    const unsigned z = bf16_bits((float)(b + a)), h = bf16_bits((float)((b - a) / 15.0));
+    float fz = 0.5f * hi + 0.5f * lo, fh = (0.5f * hi - 0.5f * lo) * (1.0f / 15.0f);
+    const unsigned low = __float_as_uint(fh) & 0xFFFFu;
+    if (low - 0x7FF0u <= 0x20u || !(fabsf(fh) >= 0x1p-90f) || !(fabsf(fh) <= 0x1p100f)) {
+        const double a = 0.5 * (double)lo, b = 0.5 * (double)hi;
+        fz = (float)(b + a);
+        fh = (float)((b - a) / 15.0);
+    }
+    const unsigned z = bf16_bits(fz), h = bf16_bits(fh);
     const bool ok = finite && (z & 0x7F80u) != 0x7F80u && (h & 0x7F80u) != 0x7F80u;
     return ok ? z << 16 | h : 0x7FC00000u;
 }
-__device__ __forceinline__ unsigned kv4_code(float x, unsigned s) {
-    const double z = (double)kv4_z(s), h = (double)kv4_h(s);
-    const double t = h == 0.0 ? 0.0 : ((double)x - z) / h;
-    return (unsigned)(int)fmin(fmax(rint((t + 15.0) * 0.5), 0.0), 15.0);
+// The codes of eight values.  In fp32, ((x - z) / h + 15) / 2 is off by less than 2^-18: only where it
+// lies within 2^-16 of a border (or is no number: h = 0, or too small for its reciprocal) is the
+// definition's 64-bit form needed, one element in 30000.
+__device__ __forceinline__ unsigned kv4_encode(const float (&x)[8], unsigned s) {
+    const float z = kv4_z(s), h = kv4_h(s), inv = 1.0f / h;
+    float c[8];
+    bool close = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float y = ((x[e] - z) * inv + 15.0f) * 0.5f;
+        c[e] = rintf(y);
+        close = close || !(fabsf(y - c[e]) <= 0.5f - 0x1p-16f);
+    }
+    if (close) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double t = h == 0.0f ? 0.0 : ((double)x[e] - (double)z) / (double)h;
+            c[e] = (float)rint((t + 15.0) * 0.5);
+        }
+    }
+    unsigned w = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (unsigned)(int)fminf(fmaxf(c[e], 0.0f), 15.0f) << kv4_shift(e);
+    return w;
 }
 
 // A row (b, m) stands at position pos[b] + m; rows outside [0, Lmax) have no place in the cache.
@@ -99,8 +127,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
         const long long row = hr / H;
         if (row >= (long long)B * M) return;
         const int b = (int)(row / M), m = (int)(row % M), p = kv4_row_pos(pos_p[b], m, Lmax);
-        const v4f x1 = *reinterpret_cast<const v4f*>(q + hr * HD + i);
-        const v4f x2 = *reinterpret_cast<const v4f*>(q + hr * HD + HALF + i);
+        const v4f x1 = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(q + hr * HD + i));
+        const v4f x2 = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(q + hr * HD + HALF + i));
         v4f y1{}, y2{};
         if (p >= 0) {
             const v4f cs0 = *reinterpret_cast<const v4f*>(rope + ((size_t)p * HALF + i) * 2);
@@ -126,8 +154,15 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
     const bool is_v = t >= 128;
     const int o = t % TPR;  // dimensions 8 o .. 8 o + 7
     unsigned* const sc = reinterpret_cast<unsigned*>(blk + 64 * HD) + (is_v ? HD : 0);
-    for (int r = (t & 127) / TPR; r < kKv4Rows; r += 128 / TPR) {
-        const int p = p0 + r;
+    // V's dword of thread (dimension, l): positions 4 l + (0..3, 8..11) of the 16; what it holds is asked for
+    // now, for the positions that are not this call's
+    const int dim = min(t >> 1, HD - 1), vl = t & 1;
+    unsigned* const vat = reinterpret_cast<unsigned*>(blk + 32 * HD) +
+                          ((dim / 32 * 16 + dim % 16) * 4 + p0 % 32 / 16 * 2 + vl) * 4 + dim % 32 / 16 * 2 + p0 % kKv4Block / 32;
+    const unsigned old = pos > p0 || end < first + kKv4Rows ? *vat : 0u;
+    for (int r0 = 0; r0 < kKv4Rows; r0 += 128 / TPR) {
+        if (p0 + r0 >= end || p0 + r0 + 128 / TPR <= pos) continue;  // (uniform) none of these rows
+        const int r = r0 + (t & 127) / TPR, p = p0 + r;
         const bool in = p >= pos && p < end;
         float x[8];
         const float* src = (is_v ? v : k) + ((size_t)b * M + (in ? p - pos : 0)) * Hkv * HD + (size_t)kh * HD;
@@ -159,9 +194,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
         }
         const unsigned long long bad = __ballot(!fin);
         const unsigned s = kv4_scale(lo, hi, ((bad >> (lane & 56)) & 0xFFull) == 0ull);
-        unsigned word = 0u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word |= kv4_code(x[e], s) << kv4_shift(e);
+        const unsigned word = kv4_encode(x, s);
         const int P = p % kKv4Block;
         if (is_v) codes[r][o] = word;
         if (in) {
@@ -170,50 +203,81 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
         }
     }
     __syncthreads();
-    // thread (dimension, l): the dword of positions 4 l + (0..3, 8..11) of the 16
     if (t >= 2 * HD) return;
-    const int dim = t >> 1, l = t & 1, w = p0 % kKv4Block / 32, s2 = p0 % 32 / 16;
-    unsigned word = 0u, mask = 0u;
+    unsigned word = 0u, keep = 0xFFFFFFFFu;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int r = 8 * (e >> 2) + 4 * l + (e & 3), p = p0 + r;
+        const int r = 8 * (e >> 2) + 4 * vl + (e & 3), p = p0 + r;
         if (p >= pos && p < end) {
             word |= ((codes[r][dim / 8] >> kv4_shift(dim % 8)) & 15u) << kv4_shift(e);
-            mask |= 15u << kv4_shift(e);
+            keep &= ~(15u << kv4_shift(e));
         }
     }
-    if (mask == 0u) return;
-    unsigned* const at = reinterpret_cast<unsigned*>(blk + 32 * HD) +
-                         ((dim / 32 * 16 + dim % 16) * 4 + 2 * s2 + l) * 4 + dim % 32 / 16 * 2 + w;
-    *at = mask == 0xFFFFFFFFu ? word : (*at & ~mask) | word;
+    if (keep != 0xFFFFFFFFu) *vat = (old & keep) | word;
 }
 
 // ---- read --------------------------------------------------------------------------------
-// Rows (b, m) of K and V as fp32 [B][Hkv][M][HD]; one thread per 8 dimensions of a position
-// of K, and per dimension and position of V.
+// Rows (b, m) of K and V as fp32 [B][Hkv][M][HD].  A workgroup takes the rows of one block of 64
+// positions of one head (blocks in front of the cache and behind it too: zeros).  A thread has 4
+// dimensions of 8 positions (4 at 64 dimensions), so that every store instruction writes whole rows:
+// with a position and a dimension a thread it was stores of 4 bytes, 4 x 32768 positions (5 heads of
+// 128) 440 us.
 template <int HD>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ cache, float* __restrict__ k,
-                                                       float* __restrict__ v, int B, int M, int Hkv, int Lmax, int nblk,
-                                                       const int* __restrict__ pos_p) {
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;  // (b, kv head, m, dimension)
-    const int d = (int)(idx % HD);
-    const long long row = idx / HD;
-    const int m = (int)(row % M), bh = (int)(row / M);
-    if (bh >= B * Hkv) return;
-    const int p = kv4_row_pos(pos_p[bh / Hkv], m, Lmax);
-    float kx = 0.0f, vx = 0.0f;
-    if (p >= 0) {
-        const uint8_t* blk = cache + ((size_t)bh * nblk + p / kKv4Block) * kv4_block_bytes(HD);
-        const unsigned *w = reinterpret_cast<const unsigned*>(blk), *sc = w + 16 * HD;
-        const int P = p % kKv4Block;
-        const unsigned kw = w[P * (HD / 8) + (d % 64 / 16) * (HD / 32) + d / 64 * 2 + d % 16 / 8];
-        const unsigned vw = w[8 * HD + ((d / 32 * 16 + d % 16) * 4 + P % 32 / 16 * 2 + P % 8 / 4) * 4 + d % 32 / 16 * 2 + P / 32];
-        const unsigned ks = sc[d / 64 * 64 + P], vs = sc[HD + d / 64 * 64 + P];
-        kx = kv4_z(ks) + kv4_h(ks) * (float)(2 * (int)((kw >> kv4_shift(d % 8)) & 15u) - 15);
-        vx = kv4_z(vs) + kv4_h(vs) * (float)(2 * (int)((vw >> kv4_shift(P % 16 / 8 * 4 + P % 4)) & 15u) - 15);
+                                                       float* __restrict__ v, int M, int Hkv, int Lmax, int nblk,
+                                                       int chunks, const int* __restrict__ pos_p) {
+    constexpr int LR = HD / 4, N = 64 * LR / 256;  // lanes a row, positions a thread
+    const int chunk = blockIdx.x % chunks, bh = blockIdx.x / chunks, t = threadIdx.x;
+    const int pos = pos_p[bh / Hkv], grp = t / LR, d = t % LR * 4, g = d / 64;
+    const long long j = (pos >> 6) + (long long)chunk;  // (rounds down)
+    if (j * kKv4Block >= (long long)pos + M) return;
+    const bool in = j >= 0 && j < nblk;
+    const uint8_t* blk = cache + ((size_t)bh * nblk + (in ? j : 0)) * kv4_block_bytes(HD);
+    const unsigned *w = reinterpret_cast<const unsigned*>(blk), *sc = w + 16 * HD + g * 64;
+    // K: positions N grp + n.  V: the N positions from number first_v on of the eight of dword (w, s, l) = octet
+    const int octet = grp * N / 8, first_v = grp * N % 8, vbase = 32 * (octet >> 2) + 16 * (octet >> 1 & 1) + 4 * (octet & 1);
+    // rows of this call: number m, -1 for none
+    auto row = [&](int P) {
+        const long long m = j * kKv4Block + P - pos;
+        return m >= 0 && m < M ? (int)m : -1;
+    };
+    unsigned kw[N], ks[N], vw[4], vs[N];
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int P = N * grp + n, e = first_v + n, Pv = vbase + 8 * (e >> 2) + (e & 3);
+        const bool kin = in && row(P) >= 0, vin = in && row(Pv) >= 0;
+        kw[n] = kin ? w[P * (HD / 8) + d % 64 / 16 * (HD / 32) + g * 2 + d % 16 / 8] : 0u;
+        ks[n] = kin ? sc[P] : 0u;
+        vs[n] = vin ? sc[HD + Pv] : 0u;
+        any = any || vin;
     }
-    k[idx] = kx;
-    v[idx] = vx;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        vw[c] = any ? w[8 * HD + ((d / 32 * 16 + (d + c) % 16) * 4 + (octet & 3)) * 4 + d % 32 / 16 * 2 + (octet >> 2)] : 0u;
+    const size_t base = (size_t)bh * M * HD + d;
+    auto put = [&](float* out, int P, const v4f& x) {
+        const int m = row(P);
+        const long long p = j * kKv4Block + P;
+        if (m >= 0) __builtin_nontemporal_store(p >= 0 && p < Lmax ? x : v4f{}, reinterpret_cast<v4f*>(out + base + (size_t)m * HD));
+    };
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v4f x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            x[c] = kv4_z(ks[n]) + kv4_h(ks[n]) * (float)(2 * (int)((kw[n] >> kv4_shift(d % 8 + c)) & 15u) - 15);
+        put(k, N * grp + n, x);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int e = first_v + n;
+        v4f x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            x[c] = kv4_z(vs[n]) + kv4_h(vs[n]) * (float)(2 * (int)((vw[c] >> kv4_shift(e)) & 15u) - 15);
+        put(v, vbase + 8 * (e >> 2) + (e & 3), x);
+    }
 }
 
 // ---- attention ---------------------------------------------------------------------------
@@ -1104,11 +1168,12 @@ hipError_t launch_kv4_append(const float* q, const float* k, const float* v, con
 hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, int Hkv, int hd, int Lmax,
                            const int* pos, hipStream_t s) {
     const int nblk = (Lmax + kKv4Block - 1) / kKv4Block;
-    const long long n = ((long long)B * Hkv * M * hd + 255) / 256;
+    const int chunks = (M + kKv4Block - 2) / kKv4Block + 1;
+    const long long n = (long long)B * Hkv * chunks;
     if (n > kMaxGroups) return hipErrorInvalidValue;
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, s, static_cast<const uint8_t*>(cache), k, v, B, M,
-                           Hkv, Lmax, nblk, pos);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, s, static_cast<const uint8_t*>(cache), k, v, M, Hkv,
+                           Lmax, nblk, chunks, pos);
     };
     if (hd == 128) go(kv4_read_kernel<128>);
     else go(kv4_read_kernel<64>);

@@ -20,8 +20,9 @@ Layer semantics of this build (the benchmark configuration, BitNet b1.58 structu
 The reference differs (no RoPE, no mask, SiLU gate, sub-norm after o_proj; see its
 src/rotor/transformer.py:206-341); logits are therefore not comparable with it, only
 the per-linear arithmetic is.  Every ternary linear runs in the HIP library; attention,
-RoPE, norms and the LM head are HIP kernels of the same library.  The model runs on the
-GPU only: ``use_gpu=False`` raises.
+RoPE, norms and the LM head are HIP kernels of the same library.  The KV cache is fp32, or
+4-bit with ``kv_cache_bits=4`` in the config (load_bitnet_model takes it too).  The model runs on
+the GPU only: ``use_gpu=False`` raises.
 """
 from __future__ import annotations
 
@@ -56,7 +57,8 @@ class KVCache:
     (src/rotor/bitnet_model.py:223-228 builds it from src/rotor/transformer.py:250-257):
     ``len(cache)`` is the number of layers and ``cache[i]`` is ``{'k': K, 'v': V}``, float32
     arrays ``[1, n_kv_heads, length, head_dim]`` copied from the device on access (keys
-    after RoPE, as this model attends with them).  ``cache.length`` is the number of
+    after RoPE, as this model attends with them; with kv_cache_bits 4, the values that the 4-bit
+    cache holds).  ``cache.length`` is the number of
     cached tokens.
 
     The cache memory belongs to the model and holds one sequence at a time: a forward that
@@ -105,6 +107,12 @@ class BitNetModel:
         self.eps = float(config.get("rms_norm_eps", 1e-6))
         self.max_seq_len = int(config.get("max_seq_len", 2048))
         self.max_tokens = int(config.get("max_batch_tokens", 512))
+        # 32: the KV cache in fp32; 4: in 4 bits (rt_kv4_*), 0.56 bytes a value instead of 4
+        self.kv_cache_bits = int(config.get("kv_cache_bits", 32))
+        if self.kv_cache_bits not in (4, 32):
+            raise ValueError(f"kv_cache_bits {self.kv_cache_bits}: 32 or 4")
+        if self.kv_cache_bits == 4 and (self.head_dim not in (64, 128) or not 0 < self.max_seq_len <= 1 << 20):
+            raise ValueError("a 4-bit KV cache needs a head_dim of 64 or 128 and max_seq_len <= 2^20")
         self.use_gpu = True
         from .gpu_layers import get_gpu, last_error
 
@@ -225,6 +233,7 @@ class _DeviceModel:
         D, F, H, Hkv, hd = model.d_model, model.d_ff, model.n_heads, model.n_kv_heads, model.head_dim
         self.D, self.F, self.H, self.Hkv, self.hd = D, F, H, Hkv, hd
         self.Lmax = model.max_seq_len
+        self.kv4 = model.kv_cache_bits == 4
         if H * hd != D or H % Hkv:
             raise ValueError("unsupported head layout")
         self.layers = []
@@ -240,8 +249,11 @@ class _DeviceModel:
                     d[name] = hip.upload_device(wb, K, scale)
                 else:
                     d[name] = hip.upload(np.asarray(wb), K, scale)
-            d["kc"] = torch.zeros((Hkv, hd, self.Lmax), dtype=torch.float32, device=dev)
-            d["vc"] = torch.zeros((Hkv, self.Lmax, hd), dtype=torch.float32, device=dev)
+            if self.kv4:
+                d["k4"] = hip.kv4_cache(Hkv, hd, self.Lmax)
+            else:
+                d["kc"] = torch.zeros((Hkv, hd, self.Lmax), dtype=torch.float32, device=dev)
+                d["vc"] = torch.zeros((Hkv, self.Lmax, hd), dtype=torch.float32, device=dev)
             self.layers.append(d)
         self.emb = emb.to(dev)
         self.final_norm = final_norm.to(dev)
@@ -312,6 +324,10 @@ class _DeviceModel:
         st["gu_pair"] = []     # per layer (M > 64): the gate/up GEMM writes relu(g)^2 * u into am
         st["ossq"] = torch.empty(H * hd // 32, dtype=torch.float64, device=dev)
         hip, eps = self.hip, self.m.eps
+        if self.kv4:
+            n = _hip.load().rt_kv4_attention_workspace(1, M, H, Hkv, hd, self.Lmax)
+            st["ws4"] = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        attn_in_prologue = self.attn_in_prologue and not self.kv4
         chain = M == 1 and self.ssq_chain
         for li, L in enumerate(self.layers):
             st["attn_fused"].append(False)
@@ -324,14 +340,14 @@ class _DeviceModel:
                                                     eps=eps, ys=qkv_ys))
                 else:
                     st["qkv"].append(hip.plan_fused(qkv_w, _hip.SRC_RMSNORM, h, L["input_norm"], eps=eps, ys=qkv_ys))
-                if self.attn_in_qkv and L["attn_sub_norm"] is not None and self.attn_in_prologue:
+                if self.attn_in_qkv and L["attn_sub_norm"] is not None and attn_in_prologue:
                     st["attn_fused"][li] = self._attach_attention(st["qkv"][li], L)
                 if st["attn_fused"][li] and self.attn_combine_in_qkv and self.Lmax <= 640:
                     st["attn_comb"][li] = self._attach_combine(st["qkv"][li], o, st["ossq"])
                 if st["attn_comb"][li]:
                     st["o_plan"].append(hip.plan_fused([L["o_proj"]], _hip.SRC_RMSNORM_SSQ, o, L["attn_sub_norm"],
                                                        st["ossq"], eps=eps, ys=[h], residuals=[h]))
-                elif L["attn_sub_norm"] is not None and self.attn_in_prologue:
+                elif L["attn_sub_norm"] is not None and attn_in_prologue:
                     st["o_plan"].append(hip.plan_fused([L["o_proj"]], _hip.SRC_ATTN_NORM, self.attn_ws,
                                                        L["attn_sub_norm"], eps=eps, ys=[h], residuals=[h],
                                                        attn_head_dim=self.hd, attn_max_len=self.Lmax))
@@ -457,7 +473,13 @@ class _DeviceModel:
             else:
                 hip.act_rmsnorm_quantize(h, L["input_norm"], self.act_d, eps)
                 st["qkv"][li].gemv()
-            if M == 1:
+            if self.kv4:
+                self._attend_kv4(st, L, M)
+                if tb is not None and M == 1:
+                    tb["attn"][li].copy_(o[0])
+                elif self.trace is not None:
+                    self.trace.setdefault("attn", []).append(o.clone())
+            elif M == 1:
                 combine_here = False
                 if not st["attn_fused"][li]:
                     # RoPE + KV append + split attention in one launch (else they ran in the
@@ -510,12 +532,27 @@ class _DeviceModel:
                                   next_h.data_ptr() if next_h is not None else None), "rt_lm_head_argmax")
         return st
 
+    def _attend_kv4(self, st, L, M):
+        """RoPE, the new keys and values into layer L's 4-bit cache, attention over it into st["o"]."""
+        lib, ctx, chk = _hip.load(), self.hip.ctx, _hip.check
+        q, ws = st["q"].data_ptr(), st["ws4"]
+        chk(lib.rt_kv4_append(ctx, q, st["k"].data_ptr(), st["v"].data_ptr(), self.rope.data_ptr(), L["k4"].data_ptr(), q,
+                              1, M, self.H, self.Hkv, self.hd, self.Lmax, self.pos.data_ptr()), "rt_kv4_append")
+        chk(lib.rt_kv4_attention(ctx, q, L["k4"].data_ptr(), st["o"].data_ptr(), 1, M, self.H, self.Hkv, self.hd, self.Lmax,
+                                 self.pos.data_ptr(), ws.data_ptr() if ws is not None else None,
+                                 ws.numel() if ws is not None else 0), "rt_kv4_attention")
+
     def layer_cache(self, li, length, epoch):
         """Layer li's cached K and V of the current sequence's first `length` tokens, as
         float32 [1, Hkv, length, hd] host arrays."""
         if epoch != self.epoch:
             raise ValueError("stale KV cache: the model's device cache now holds a newer sequence")
         L = self.layers[li]
+        if self.kv4:
+            import torch
+
+            k, v = self.hip.kv4_read(L["k4"], torch.zeros(1, dtype=torch.int32, device=self.device), length, self.Lmax)
+            return {"k": k.cpu().numpy(), "v": v.cpu().numpy()}
         k = L["kc"][:, :, :length].transpose(1, 2)  # the device keeps keys [Hkv, hd, Lmax]
         v = L["vc"][:, :length, :]
         return {"k": k.cpu().numpy()[None], "v": v.cpu().numpy()[None]}
@@ -696,11 +733,12 @@ def config_from_hf(cfg: Dict) -> Dict:
     }
 
 
-def load_bitnet_model(model_dir: str, use_gpu: bool = False) -> BitNetModel:
-    """src/rotor/bitnet_model.py:349-394: config.json + model.safetensors -> BitNetModel."""
+def load_bitnet_model(model_dir: str, use_gpu: bool = False, kv_cache_bits: int = 32) -> BitNetModel:
+    """src/rotor/bitnet_model.py:349-394: config.json + model.safetensors -> BitNetModel.
+    kv_cache_bits 4 keeps the KV cache in 4 bits (a 7.1th of the memory)."""
     model_dir = Path(model_dir)
     with open(model_dir / "config.json") as f:
         cfg = json.load(f)
-    model = BitNetModel(config_from_hf(cfg), use_gpu=use_gpu)
+    model = BitNetModel(dict(config_from_hf(cfg), kv_cache_bits=kv_cache_bits), use_gpu=use_gpu)
     model.load_weights_from_safetensors(str(model_dir / "model.safetensors"))
     return model

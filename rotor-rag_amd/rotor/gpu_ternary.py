@@ -555,6 +555,14 @@ class HIPTernaryOps:
             raise ValueError(f"{who}: pos must be a contiguous int32 [{B}] tensor on the backend's device")
         return B, Hkv, size // 72, Lmax
 
+    def _kv4_run(self, name, fn, *args):
+        """fn(ctx, *args) on the current stream (taken as the number it is: making a Stream object of it
+        costs as much as a small launch)."""
+        rc = self.lib.rt_ctx_set_stream(self.ctx, _torch()._C._cuda_getCurrentRawStream(self.device_index))
+        rc = rc or fn(self.ctx, *args)
+        if rc:
+            _hip.check(rc, name)
+
     def _kv4_in(self, x):
         """float32 device tensor, contiguous and 16-byte aligned (a copy where x is not)."""
         torch = _torch()
@@ -592,10 +600,8 @@ class HIPTernaryOps:
         if rope.ndim != 3 or rope.shape[1:] != (hd // 2, 2) or rope.shape[0] < Lmax:
             raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
         out = self._kv4_out("kv4_append", q_out, q)
-        self._bind_stream()
-        rc = self.lib.rt_kv4_append(self.ctx, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), cache.data_ptr(),
-                                    out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
-        _hip.check(rc, "rt_kv4_append")
+        self._kv4_run("rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
+                      cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
         return out
 
     def kv4_read(self, cache, pos, length: int, max_len=None):
@@ -607,9 +613,8 @@ class HIPTernaryOps:
             raise ValueError(f"kv4_read: length {length} of a cache of {Lmax} positions")
         k = torch.empty((B, Hkv, length, hd), dtype=torch.float32, device=self.device)
         v = torch.empty_like(k)
-        self._bind_stream()
-        _hip.check(self.lib.rt_kv4_read(self.ctx, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, length, Hkv, hd, Lmax,
-                                        pos.data_ptr()), "rt_kv4_read")
+        self._kv4_run("rt_kv4_read", self.lib.rt_kv4_read, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, length, Hkv, hd,
+                      Lmax, pos.data_ptr())
         return k, v
 
     def kv4_attention(self, q, cache, pos, max_len=None, out=None):
@@ -625,10 +630,8 @@ class HIPTernaryOps:
         out = self._kv4_out("kv4_attention", out, q)
         need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._bind_stream()
-        rc = self.lib.rt_kv4_attention(self.ctx, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax,
-                                       pos.data_ptr(), ws.data_ptr() if need else None, need)
-        _hip.check(rc, "rt_kv4_attention")
+        self._kv4_run("rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
+                      Hkv, hd, Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need)
         return out
 
     def __del__(self):
