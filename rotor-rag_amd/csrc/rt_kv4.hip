@@ -364,9 +364,10 @@ struct Kv4AttnArgs {
     const float* q;
     const uint8_t* cache;
     float* out;
-    float* work;  // S > 1: [unit][split]: O [tile rows][HD], then (reference, sum of weights) [tile rows][2]
+    float* work;  // [unit][split] (S = 0: [workgroup]): O [tile rows][HD], (reference, sum of weights) [tile rows][2]
     const int* pos;
-    int M, H, Hkv, Lmax, nblk, tiles, S, bh;  // bh = B * Hkv
+    int M, H, Hkv, Lmax, nblk, tiles, S, bh;  // bh = B * Hkv.  S = 0: splits by length (kv4_piece)
+    int* heads;                               // S = 0: (pieces, first) of every head
     float scale;  // log2(e) / sqrt(HD)
 };
 
@@ -378,6 +379,47 @@ struct Kv4Range {
 __device__ __forceinline__ Kv4Range kv4_range(int pos, int m0, int m1, int Lmax) {
     const long long p0 = (long long)pos + m0, p1 = (long long)pos + m1;
     return {p1 < 0 || p0 >= Lmax ? 0 : (int)min(p1, (long long)Lmax - 1) + 1, p0 < 0 || p1 >= Lmax ? -1 : (int)p0};
+}
+
+// Splits by length, for a batch of up to 64 sequences (one tile a unit): with the same number for each, the
+// longest decides the launch.  A sequence of n blocks is cut into pieces of at most q of them, q a multiple of
+// 4 (a block a wave) for which the pieces of all heads fit the kKv4Slots workgroups that the chip holds at
+// once; workgroup w takes pieces in the order (sequence, head, piece).  Every wave works this out for itself,
+// lane b for sequence b, and the first piece of a head tells the join where its partials are.
+constexpr int kKv4Slots = 512;
+struct Kv4Piece {
+    int b, head, piece, n, first;  // n pieces a head of sequence b; first: the workgroup of this head's first
+};
+__device__ __forceinline__ int kv4_wave_scan(int x) {  // inclusive, over the lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+// The piece of workgroup w; n = 0: none.
+__device__ __forceinline__ Kv4Piece kv4_piece(const Kv4AttnArgs& a, int w, int lane) {
+    const int B = a.bh / a.Hkv;
+    const int nb = lane < B ? (kv4_range(a.pos[lane], 0, a.M - 1, a.Lmax).kend + kKv4Block - 1) / kKv4Block : 0;
+    const long long all = (long long)__builtin_amdgcn_readlane(kv4_wave_scan(nb), 63) * a.Hkv;
+    int q = max(4, (int)(all / (kKv4Slots - a.bh / 4) + 3) & ~3), n, incl;
+    for (;; q += max(4, q / 16 & ~3)) {  // (ends at the latest with a piece a head: bh <= kKv4Slots)
+        n = lane < B ? max(1, (int)(((float)(nb + q - 1) + 0.25f) * (1.0f / (float)q))) : 0;
+        incl = kv4_wave_scan(n);
+        if (__builtin_amdgcn_readlane(incl, 63) * a.Hkv <= kKv4Slots) break;
+    }
+    const unsigned long long here = __ballot(w < incl * a.Hkv);
+    if (here == 0ull) return Kv4Piece{0, 0, 0, 0, 0};
+    Kv4Piece p;
+    p.b = (int)__builtin_ctzll(here);
+    p.n = __builtin_amdgcn_readlane(n, p.b);
+    const int start = (__builtin_amdgcn_readlane(incl, p.b) - p.n) * a.Hkv;
+    p.head = (w - start) / p.n;
+    p.piece = w - start - p.head * p.n;
+    p.first = start + p.head * p.n;
+    return p;
 }
 
 // The power of two that brings the largest of a row's scaled queries into [2^14, 2^15).
@@ -404,10 +446,29 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
     __shared__ float om[4][16][HD + 4];
     __shared__ float ml[4][16][2];
-    const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    const int split = w0 % a.S, unit = w0 / a.S, tile = unit % a.tiles, bh = unit / a.tiles;
-    const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
+    int split, S, tile, bh, slot;  // slot: the partial's in the workspace
+    if (a.S == 0) {
+        const Kv4Piece p = kv4_piece(a, (int)blockIdx.x, lane);
+        if (p.n == 0) return;
+        split = p.piece;
+        S = p.n;
+        tile = 0;
+        bh = p.b * a.Hkv + p.head;
+        slot = p.first + p.piece;
+        if (split == 0 && t == 0) {
+            a.heads[2 * bh] = S;
+            a.heads[2 * bh + 1] = p.first;
+        }
+    } else {
+        const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x), unit = w0 / a.S;
+        split = w0 % a.S;
+        S = a.S;
+        tile = unit % a.tiles;
+        bh = unit / a.tiles;
+        slot = w0;
+    }
+    const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned mask = kv4_mask(), mask0 = kv4_mask(0x000F000Fu);
     const int rows = a.M * G, R = min(tile * RT + i % RT, rows - 1), m = R / G;  // (rows past the end repeat the last)
@@ -424,7 +485,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const Kv4Range range = kv4_range(pos, tile * RT / G, (min(tile * RT + RT, rows) - 1) / G, a.Lmax);
     const int kend = range.kend, all = range.all;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
-    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * a.S;
+    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * S;
     // Key tile wx = 2 w + x of a block: keys 32 w + 8 x + kl + r of lane group h.  The column's own
     // tiles are wx = NA q + ca.
     const int kl = 16 * (h >> 1) + 4 * (h & 1);
@@ -664,8 +725,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     }
     float* dst;
     float inv = 1.0f;
-    if (a.S > 1) {
-        float* part = a.work + ((size_t)unit * a.S + split) * (RT * (HD + 2));
+    if (S > 1) {
+        float* part = a.work + (size_t)slot * (RT * (HD + 2));
         dst = part + row * HD;
         if (t % TPR == 0) {
             part[RT * HD + 2 * row] = mm;
@@ -1090,20 +1151,26 @@ __global__ void __launch_bounds__(1024) kv4_combine_kernel(const Kv4AttnArgs a, 
     const int row = (int)(rr % most), tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles), R = tile * TR + row;
     const bool live = unit < (long long)a.bh * a.tiles && R < rows;
     const size_t psz = (size_t)TR * (HD + 2);
-    const float* part = a.work + (live ? (size_t)unit * a.S : 0) * psz;
+    int S = a.S;
+    size_t slot = (size_t)unit * S;
+    if (S == 0) {
+        S = a.heads[live ? 2 * bh : 0];
+        slot = (size_t)a.heads[live ? 2 * bh + 1 : 1];
+    }
+    const float* part = a.work + (live ? slot : 0) * psz;
     const float *pm = part + (size_t)TR * HD + 2 * (live ? row : 0), *po = part + (size_t)(live ? row : 0) * HD + 4 * c;
     float mm = -INFINITY;
-    for (int s = c; s < a.S; s += LR) mm = fmaxf(mm, pm[s * psz]);
+    for (int s = c; s < S; s += LR) mm = fmaxf(mm, pm[s * psz]);
     v4f x{};
     float den = 0.0f;
     bool first = true;
-    for (int s0 = grp % sg; s0 < a.S || first; s0 += AT * sg) {
+    for (int s0 = grp % sg; s0 < S || first; s0 += AT * sg) {
         v4f y[AT];
         float m[AT], l[AT];
 #pragma unroll
         for (int k = 0; k < AT; ++k) {
             const int s = s0 + k * sg;
-            const bool in = s < a.S;
+            const bool in = s < S;
             m[k] = in ? pm[s * psz] : 0.0f;
             l[k] = in ? pm[s * psz + 1] : 0.0f;
             y[k] = in ? *reinterpret_cast<const v4f*>(po + s * psz) : v4f{};
@@ -1131,7 +1198,7 @@ __global__ void __launch_bounds__(1024) kv4_combine_kernel(const Kv4AttnArgs a, 
             den += sd[grp + k];
         }
     }
-    if (!live) return;
+    if (!live || S == 1) return;  // (in one piece: written already)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = den == 0.0f ? 0.0f : x[e] / den;
     *reinterpret_cast<v4f*>(a.out + (((size_t)(bh / a.Hkv) * a.M + R / G) * a.H + (size_t)(bh % a.Hkv) * G + R % G) * HD +
@@ -1184,8 +1251,8 @@ namespace {
 // Which kernel, and how many splits of the keys.  The host does not know the positions: a call is taken
 // to stand half way into its cache.  (Times: 20 heads of 128 over 5, the launches back to back.)
 struct Kv4Shape {
-    long long units;
-    int RT, tiles, S;
+    long long units, groups;  // groups: workgroups of the attention launch, and partials
+    int RT, tiles, S;         // S = 0: by length (kv4_piece)
 };
 Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     Kv4Shape p;
@@ -1207,20 +1274,29 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495.
     const int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : (blocks + 3) / 4;
     p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
+    p.groups = p.units * p.S;
+    // A batch: splits by length.  Sequences of 100 to 4096 keys, 32 / 8 / 48 of them: 25.6 / 14.6 / 31.9 us,
+    // with the best equal number of splits 27.4 / 16.3 / 35.0; 4 of 100 to 32768 23.7 / 41; 50 of 100 to 1500
+    // (250 heads, few keys) 21.8 / 17.5, so not there; 32 of 4096 each 30.7 / 29.8.
+    if (B > 1 && B <= 64 && tiles == 1 && p.RT != kKv4Tile && p.units <= kKv4Slots / 2 &&
+        blocks > (p.units <= kKv4Slots / 4 ? 20 : 31)) {
+        p.S = 0;
+        p.groups = kKv4Slots;
+    }
     return p;
 }
 template <int HD>
 hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.units * p.S)), block(256);
+    const dim3 grid((unsigned)p.groups), block(256);
     switch (p.RT) {
         case 4: hipLaunchKernelGGL((kv4_attn_kernel<HD, 4>), grid, block, 0, s, a); break;
         case 8: hipLaunchKernelGGL((kv4_attn_kernel<HD, 8>), grid, block, 0, s, a); break;
         case 16: hipLaunchKernelGGL((kv4_attn_kernel<HD, 16>), grid, block, 0, s, a); break;
         default: hipLaunchKernelGGL(kv4_prefill_kernel<HD>, grid, dim3(512), 1024 * HD, s, a); break;
     }
-    if (p.S > 1) {
+    if (p.S != 1) {
         const long long all = p.units * std::min<long long>(p.RT, (long long)a.M * (a.H / a.Hkv));  // rows
-        const int threads = p.S > 16 && all < 4096 ? 1024 : 256, gr = threads / (HD / 4), sg = all >= 4096 ? 1 : gr;
+        const int threads = (p.S == 0 ? p.groups / p.units : p.S) > 16 && all < 4096 ? 1024 : 256, gr = threads / (HD / 4), sg = all >= 4096 ? 1 : gr;
         hipLaunchKernelGGL(kv4_combine_kernel<HD>, dim3((unsigned)((all * sg + gr - 1) / gr)), dim3(threads), 0, s, a, p.RT,
                            sg);
     }
@@ -1230,15 +1306,16 @@ hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_
 
 size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax) {
     const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
-    return p.S > 1 ? (size_t)p.units * p.S * p.RT * (hd + 2) * sizeof(float) : 0;
+    return p.S == 1 ? 0 : (size_t)p.groups * p.RT * (hd + 2) * sizeof(float) + (p.S == 0 ? (size_t)p.units * 8 : 0);
 }
 
 hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                                 int Lmax, const int* pos, float* work, hipStream_t s) {
     const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
-    if (p.units * p.S > kMaxGroups) return hipErrorInvalidValue;
+    if (p.groups > kMaxGroups) return hipErrorInvalidValue;
     const Kv4AttnArgs a{q, static_cast<const uint8_t*>(cache), out, work, pos, M, H, Hkv, Lmax,
-                        (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv, 1.44269504088896341f / sqrtf((float)hd)};
+                        (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv,
+                        reinterpret_cast<int*>(work + (p.S == 0 ? (size_t)p.groups * p.RT * (hd + 2) : 0)), 1.44269504088896341f / sqrtf((float)hd)};
     return hd == 128 ? run_kv4_attention<128>(a, p, s) : run_kv4_attention<64>(a, p, s);
 }
 

@@ -229,6 +229,12 @@ ATTENDS = [
     (3, 2, 4, 2, 64, 64, [-1, 63, 2147483647], 64),  # rows outside the cache
     (2, 90, 4, 2, 128, 100, [-50, 40], 100),
     (2, 40, 8, 2, 64, 100, [-100, 200], 100),         # nothing but such rows
+    # batches whose splits go by length: sequences of none to many blocks, 64 of them, 16 rows a tile
+    (5, 1, 20, 5, 128, 3000, [2999, 0, 1200, 64, -1], 3000),
+    (3, 4, 8, 2, 64, 2000, [1996, 1, 1990], 2000),
+    (64, 1, 4, 2, 64, 2048, [(i * 997) % 2048 for i in range(64)], 2048),
+    (2, 2, 3, 3, 128, 1500, [-2, 5000], 1500),
+    (7, 1, 2, 1, 128, 1400, [1399] * 6 + [3], 1400),
 ]
 
 
