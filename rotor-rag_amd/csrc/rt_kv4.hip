@@ -1271,7 +1271,8 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
     // a tile of 256 rows keeps 8 blocks a split (128 tokens after 8192: 16 splits 59 us, 24 64).  Else as many
     // as two workgroups a CU take in one round, the big tiles, one a CU, in two: one token over 1538 keys
     // in 8 / 4 / 1 splits 10.6 / 12.4 / 17.5 us, over 131072 in 200 / 102 / 50 36.7 / 30.8 / 34.2; 2048 of 8192
-    // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495.
+    // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495 (in equal runs of blocks over 256 workgroups, a unit
+    // cut where a run ends, 417 too: the clock gives way to the matrix cores' power).
     const int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : (blocks + 3) / 4;
     p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
     p.groups = p.units * p.S;
