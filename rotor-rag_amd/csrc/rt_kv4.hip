@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         load_vs();
     }
     // A wave's rows pass through its part of LDS, queries here and results at the end, so that memory is read
-    // and written in whole lines (lane by lane, 32 rows at once, took 10000 and 9000 cycles): 16-byte unit c
+    // and written in whole lines (lane by lane, 32 rows at once, the launch took some 1000 cycles more): 16-byte unit c
     // of row r lies at unit c ^ (r % 16).  Coalesced, instruction n takes rows n RPI + lane / UPR, unit lane % UPR.
     constexpr int UPR = HD / 4, RPI = 64 / UPR;
     v4f* const own = reinterpret_cast<v4f*>(lds_kv4) + wave * 32 * UPR;
@@ -1254,15 +1254,20 @@ struct Kv4Shape {
     long long units, groups;  // groups: workgroups of the attention launch, and partials
     int RT, tiles, S;         // S = 0: by length (kv4_piece)
 };
-Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int Lmax) {
+Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     Kv4Shape p;
-    const long long rows = (long long)M * (H / Hkv), big = (long long)B * Hkv * ((rows + kKv4Tile - 1) / kKv4Tile);
+    const long long rows = (long long)M * (H / Hkv), t16 = (rows + 15) / 16, big = (rows + kKv4Tile - 1) / kKv4Tile;
     const int blocks = (Lmax + kKv4Block - 1) / kKv4Block;
-    // A tile of 256 rows costs some 30 us a launch before its first product pays (its queries and results
-    // pass through one workgroup a CU), and then 22 ns a block of 64 keys against 50 in tiles of 16 rows: 512
-    // tokens from an empty cache (180 blocks of tiles) 28 against 23 us, 1024 (680) 49 / 48, 128 after 8192
-    // (1290) 59 / 78, 8 sequences of 512 after 512 (3900) 126 / 187.
-    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : big * blocks < 1300 ? 16 : kKv4Tile;
+    // 256 rows in one tile or in 16 of 16 rows.  A big tile costs some 24 us a launch before it pays (its
+    // queries and results pass through one workgroup a CU) and its conversion of every block however few its
+    // rows, a small one each block's codes again.  Per block of 64 keys at 128 dimensions, a big tile 10 ns
+    // and 0.75 for every 16 rows in it, a small one 2.6; at 64, 8.5 and 0.4 against 1.3.  In tiles of 16 /
+    // 256 rows, us, 20 heads over 5: 16 sequences of 5 tokens at 4000 41 / 88, of 16 79 / 91, of 32 117 / 100,
+    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 22 / 42, 128 after 8192 61 / 56;
+    // 32 tokens with 16 heads over one at 4095 19 / 40; 16 heads of 64 over 8, 2048 after 6144 264 / 208,
+    // 1024 after 3000 78 / 77.
+    const double gain = (hd == 128 ? 1.85 * t16 - 10.0 * big : 0.9 * t16 - 8.5 * big) * B * Hkv * (Lmax - M / 2) / kKv4Block;
+    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : gain < 24000.0 ? 16 : kKv4Tile;
     const long long tiles = (rows + p.RT - 1) / p.RT;
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;
@@ -1306,14 +1311,14 @@ hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_
 }  // namespace
 
 size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax) {
-    const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
+    const Kv4Shape p = kv4_shape(B, M, H, Hkv, hd, Lmax);
     return p.S == 1 ? 0 : (size_t)p.groups * p.RT * (hd + 2) * sizeof(float) + (p.S == 0 ? (size_t)p.units * 8 : 0);
 }
 
 hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                                 int Lmax, const int* pos, float* work, hipStream_t s) {
-    const Kv4Shape p = kv4_shape(B, M, H, Hkv, Lmax);
-    if (p.groups > kMaxGroups) return hipErrorInvalidValue;
+    const Kv4Shape p = kv4_shape(B, M, H, Hkv, hd, Lmax);
+    if (p.groups > (p.RT == kKv4Tile ? kMaxGroups / 2 : kMaxGroups)) return hipErrorInvalidValue;
     const Kv4AttnArgs a{q, static_cast<const uint8_t*>(cache), out, work, pos, M, H, Hkv, Lmax,
                         (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv,
                         reinterpret_cast<int*>(work + (p.S == 0 ? (size_t)p.groups * p.RT * (hd + 2) : 0)), 1.44269504088896341f / sqrtf((float)hd)};

@@ -238,8 +238,8 @@ ATTENDS = [
 ]
 
 
-# The same rows over caches so long that they are taken in tiles of 256 (a call is taken to stand half
-# way into its cache: 1300 blocks of such tiles and more)
+# The same rows over long caches (a call is taken to stand at the end of its cache, and takes tiles of 256
+# rows where their keys are many)
 ATTENDS += [
     (1, 33, 4, 4, 64, 21000, [0], 33),
     (1, 64, 20, 5, 128, 16700, [64], 128),
@@ -252,6 +252,17 @@ ATTENDS += [
     (2, 40, 8, 2, 64, 21000, [-100, 30000], 1),  # nothing but rows outside it
     (1, 70, 2, 1, 64, 83250, [83210], 83250),    # rows behind it
     (3, 9, 1, 1, 128, 28000, [5, 0, 64], 73),    # nine rows
+    # (... and rows enough for such tiles to pay)
+    (2, 77, 14, 2, 64, 76000, [0, 301], 378),
+    (1, 130, 3, 3, 128, 78000, [70], 200),
+    (1, 250, 6, 6, 64, 44000, [261], 511),
+    (1, 129, 7, 1, 64, 90000, [3], 132),
+    (2, 90, 4, 2, 128, 32000, [-50, 40], 130),
+    (2, 64, 8, 2, 64, 66000, [-100, 70000], 1),
+    (1, 64, 4, 1, 128, 83250, [83210], 83250),
+    # many sequences of few rows: tiles of 16
+    (40, 5, 8, 2, 64, 700, [(i * 97) % 690 for i in range(40)], 700),
+    (130, 3, 20, 5, 128, 300, [(i * 31) % 298 for i in range(130)], 300),
 ]
 
 
@@ -265,7 +276,7 @@ def test_attention(hip, B, M, H, Hkv, hd, Lmax, pos, n):
             assert 0 <= pos[b] + m < Lmax or (y[b, m] == 0).all()
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 300), (1, 4000), (3, 300), (70, 300), (70, 21000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 300), (1, 4000), (3, 300), (70, 300), (70, 21000), (70, 58000)])
 @pytest.mark.parametrize("qs,ks,vs", [(1e-30, 1, 1), (20, 1, 1), (1, 1e-20, 1), (1e-15, 1e15, 1), (1, 1, 1e-25), (1, 1, 1e25),
                                       (0, 1, 1), (1, 0, 0)])
 def test_attention_scales(hip, M, Lmax, qs, ks, vs):
@@ -277,7 +288,7 @@ def test_attention_scales(hip, M, Lmax, qs, ks, vs):
     _check(hip, q[:, :M] * f(qs), cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 700), (1, 2000), (40, 700), (40, 83300)])
+@pytest.mark.parametrize("M,Lmax", [(1, 700), (1, 2000), (40, 700), (40, 83300), (64, 262000)])
 def test_attention_values_of_very_different_sizes(hip, M, Lmax):
     """The weights' fp16 terms are scaled by the largest step of the values seen: outliers, early and late, that
     weigh little do not take the others' bits."""
@@ -289,7 +300,7 @@ def test_attention_values_of_very_different_sizes(hip, M, Lmax):
     _check(hip, q[:, :M], cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 8192), (24, 8192), (24, 42000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 8192), (24, 8192), (24, 42000), (64, 42000)])
 def test_attention_long_and_even(hip, M, Lmax):
     """8192 keys that weigh about the same: the result is a small difference of large sums.  In 64 bits against
     fp32 sums of numbers with random signs: each of 2 x 8192 terms (magnitude at most 3 of the values' deviation)
@@ -303,7 +314,7 @@ def test_attention_long_and_even(hip, M, Lmax):
     assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 200), (1, 3000), (9, 200), (80, 200), (80, 21000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 200), (1, 3000), (9, 200), (80, 200), (80, 21000), (80, 46000)])
 def test_attention_nan(hip, M, Lmax):
     """A NaN that a row sees makes that row NaN (a value's: in its group of 64 dimensions); one that it does not
     see leaves every bit of it."""
@@ -326,9 +337,9 @@ def test_attention_nan(hip, M, Lmax):
     assert _same(y, want)
 
 
-@pytest.mark.parametrize("Lmax", [100, 42000])
-def test_attention_nan_query(hip, Lmax):
-    B, M, H, Hkv, hd, n = 1, 20, 4, 2, 64, 90
+@pytest.mark.parametrize("M,Lmax", [(20, 100), (20, 42000), (128, 132000)])
+def test_attention_nan_query(hip, M, Lmax):
+    B, H, Hkv, hd, n = 1, 4, 2, 64, 70 + M
     cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, n)
     q, _, _ = _inputs(6, B, M, H, Hkv, hd)
     clean = hip.kv4_attention(*_cuda(q), cache, _pos([70]), max_len=Lmax).cpu().numpy()
@@ -388,7 +399,7 @@ def test_past_four_gigabytes(hip):
     assert torch.linalg.norm(both[-1] - alone[0]) <= 2e-5 * torch.linalg.norm(alone)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 400), (1, 5000), (20, 400), (20, 42000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 400), (1, 5000), (20, 400), (20, 42000), (64, 42000)])
 def test_graph_and_streams(hip, M, Lmax):
     """A step (append, attention, read) captured on a stream of its own and replayed with moving positions, with
     eager work between the replays."""
