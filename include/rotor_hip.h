@@ -371,7 +371,8 @@ size_t rt_kv4_bytes(int B, int Hkv, int hd, int Lmax);
 /* RoPE (rotate-half, rope fp32 [Lmax][hd/2][2], in 64 bits, rounded once) of q [B][M][H][hd]
  * into q_out (q_out may be q) and of k [B][M][Hkv][hd], then k and v into the cache at every
  * row's position: rt_rope_kv_append for this cache, in one launch (the KV concat of
- * src/rotor/transformer.py:250-252).  k and v are not modified. */
+ * src/rotor/transformer.py:250-252).  k and v are not modified; but for q_out = q, no two
+ * buffers overlap. */
 int rt_kv4_append(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache,
                   float* q_out, int B, int M, int H, int Hkv, int hd, int Lmax, const int* pos);
 
@@ -382,7 +383,7 @@ int rt_kv4_read(rt_ctx* ctx, const void* cache, float* k, float* v, int B, int M
 
 /* Causal GQA attention (rt_attention for this cache): out [B][M][H][hd] for queries q
  * [B][M][H][hd] (as rt_kv4_append leaves them) over keys 0..p, scale 1/sqrt(hd)
- * (src/rotor/transformer.py:260-281 plus the causal mask).  Where B, M and the heads alone do
+ * (src/rotor/transformer.py:260-281 plus the causal mask); out may be q.  Where B, M and the heads alone do
  * not fill the GPU, the keys are split and joined in a second launch through `workspace`
  * (rt_kv4_attention_workspace bytes of device memory, possibly 0, no initialisation; calls that
  * may run at the same time need workspaces of their own). */

@@ -18,6 +18,7 @@ PyTorch supplies device memory and the stream; the compute is the HIP library.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import numpy as np
 
@@ -571,22 +572,27 @@ class HIPTernaryOps:
             x = self._dev(x, torch.float32)
         return x.clone() if x.data_ptr() & 15 else x
 
-    def _kv4_out(self, who, out, like):
-        """out, or a new tensor of like's shape."""
+    def _kv4_out(self, who, out, like, *others):
+        """out, or a new tensor of like's shape; out may be like, and lies in none of the others."""
         torch = _torch()
         if out is None:
             return torch.empty_like(like)
         if out.dtype != torch.float32 or out.shape != like.shape or not out.is_contiguous() or out.device != self.device:
             raise ValueError(f"{who}: the output must be a contiguous float32 {list(like.shape)} tensor on the backend's "
                              "device")
+        at, end = out.data_ptr(), out.data_ptr() + 4 * out.numel()
+        for x in (like, *others):
+            if x.data_ptr() < end and at < x.data_ptr() + x.numel() * x.element_size() and not (x is like and x.data_ptr() == at):
+                raise ValueError(f"{who}: the output must not share memory with the other arguments (but may be q)")
         return out
 
     def kv4_append(self, q, k, v, cache, rope, pos, max_len=None, q_out=None):
         """RoPE of q [B, M, H, hd] and k [B, M, Hkv, hd], then k and v into the 4-bit cache at
         positions pos[b] + m (rt_kv4_append); rope float32 [>= max_len, hd / 2, 2].  Returns the
         rotated q (q_out, which may be q).  max_len: the cache's positions, where they are fewer
-        than its blocks hold (None: as many as the blocks and rope hold).  Rows outside
-        [0, max_len) are not written; their q is 0."""
+        than its blocks hold (None: as many as the blocks and rope hold; kv4_read and
+        kv4_attention do not see rope, and take what the blocks hold).  Rows outside [0, max_len)
+        are not written; their q is 0.  For inference: gradients do not pass."""
         B, Hkv, hd, Lmax = self._kv4_check("kv4_append", cache, pos, max_len)
         q, k, v, rope = self._kv4_in(q), self._kv4_in(k), self._kv4_in(v), self._kv4_in(rope)
         if max_len is None and rope.ndim == 3:
@@ -599,7 +605,7 @@ class HIPTernaryOps:
             raise ValueError(f"kv4_append: k and v must be {[B, M, Hkv, hd]}")
         if rope.ndim != 3 or rope.shape[1:] != (hd // 2, 2) or rope.shape[0] < Lmax:
             raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
-        out = self._kv4_out("kv4_append", q_out, q)
+        out = self._kv4_out("kv4_append", q_out, q, k, v, rope, cache)
         self._kv4_run("rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
                       cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
         return out
@@ -609,6 +615,7 @@ class HIPTernaryOps:
         float32 [B, Hkv, length, hd]; zeros outside [0, max_len) (rt_kv4_read)."""
         torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_read", cache, pos, max_len)
+        length = operator.index(length)
         if not 0 < length <= Lmax:
             raise ValueError(f"kv4_read: length {length} of a cache of {Lmax} positions")
         k = torch.empty((B, Hkv, length, hd), dtype=torch.float32, device=self.device)
@@ -619,7 +626,8 @@ class HIPTernaryOps:
 
     def kv4_attention(self, q, cache, pos, max_len=None, out=None):
         """Causal GQA attention of q [B, M, H, hd] (rotated, as kv4_append returns it) at positions
-        pos[b] + m over a 4-bit cache (rt_kv4_attention): float32 [B, M, H, hd]."""
+        pos[b] + m over a 4-bit cache (rt_kv4_attention): float32 [B, M, H, hd] (out, which may be
+        q).  Rows outside [0, max_len) are 0.  For inference: gradients do not pass."""
         torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", cache, pos, max_len)
         q = self._kv4_in(q)
@@ -627,7 +635,7 @@ class HIPTernaryOps:
             raise ValueError(f"kv4_attention: q of shape {tuple(q.shape)} does not fit a cache of {B} sequences, {Hkv} "
                              f"KV heads of {hd}")
         M, H = q.shape[1], q.shape[2]
-        out = self._kv4_out("kv4_attention", out, q)
+        out = self._kv4_out("kv4_attention", out, q, cache)
         need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._kv4_run("rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,

@@ -369,6 +369,17 @@ def test_strided_and_odd_inputs(hip):
     assert torch.equal(q, y)
 
 
+@pytest.mark.parametrize("B,M,H,Hkv,hd,Lmax", [(2, 1, 20, 5, 128, 300), (1, 1, 20, 5, 128, 4000), (2, 45, 8, 2, 64, 300),
+                                               (2, 64, 8, 2, 128, 20000)])
+def test_attention_in_place(hip, B, M, H, Hkv, hd, Lmax):
+    cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, 200)
+    (q,) = _cuda(_inputs(6, B, M, H, Hkv, hd)[0])
+    pos = _pos([200 - M, 120][:B])
+    want = hip.kv4_attention(q, cache, pos, max_len=Lmax)
+    assert hip.kv4_attention(q, cache, pos, max_len=Lmax, out=q) is q
+    assert (q == want).all()
+
+
 def test_past_four_gigabytes(hip):
     """The last sequence of a cache of more than 2^32 bytes."""
     import torch

@@ -183,3 +183,14 @@ def test_python_refusals(ops):
     for out in (f(3, 4, 6, 32), q.double(), q.transpose(1, 2)):
         with pytest.raises(ValueError, match="output"):
             ops.kv4_attention(q, cache, pos, out=out)
+    # outputs in another argument's memory (q itself may be one)
+    both = f(4, 4, 6, 64)
+    for call in (lambda: ops.kv4_append(both[1:], kv, kv, cache, rope, pos, q_out=both[:3]),
+                 lambda: ops.kv4_append(q, both.view(-1)[:kv.numel()].view(kv.shape), kv, cache, rope, pos, q_out=both[:3]),
+                 lambda: ops.kv4_append(q, kv, both.view(-1)[-kv.numel():].view(kv.shape), cache, rope, pos, q_out=both[1:]),
+                 lambda: ops.kv4_attention(both[:3], cache, pos, out=both[1:]),
+                 lambda: ops.kv4_attention(q, cache, pos, out=cache.view(-1)[:4 * q.numel()].view(torch.float32).view(q.shape))):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    with pytest.raises(TypeError):
+        ops.kv4_read(cache, pos, 2.5)
