@@ -460,6 +460,13 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
             a.heads[2 * bh] = S;
             a.heads[2 * bh + 1] = p.first;
         }
+    } else if (a.S == 1) {
+        // the last tiles, which see the most keys, of all heads first (from an empty cache, 20 heads over 5, 640 /
+        // 1024 / 1400 tokens 24 / 40 / 63 us; head by head from the first tile on 30 / 48 / 79; 512 23 / 22)
+        split = slot = 0;
+        S = 1;
+        tile = a.tiles - 1 - (int)blockIdx.x / a.bh;
+        bh = (int)blockIdx.x % a.bh;
     } else {
         const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x), unit = w0 / a.S;
         split = w0 % a.S;
@@ -1262,10 +1269,10 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     // queries and results pass through one workgroup a CU) and its conversion of every block however few its
     // rows, a small one each block's codes again.  Per block of 64 keys at 128 dimensions, a big tile 10 ns
     // and 0.75 for every 16 rows in it, a small one 2.6; at 64, 8.5 and 0.4 against 1.3.  In tiles of 16 /
-    // 256 rows, us, 20 heads over 5: 16 sequences of 5 tokens at 4000 41 / 88, of 16 79 / 91, of 32 117 / 100,
-    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 22 / 42, 128 after 8192 61 / 56;
-    // 32 tokens with 16 heads over one at 4095 19 / 40; 16 heads of 64 over 8, 2048 after 6144 264 / 208,
-    // 1024 after 3000 78 / 77.
+    // 256 rows, us, 20 heads over 5: 16 sequences of 5 tokens at 4000 41 / 88, of 16 79 / 91, of 32 128 / 109,
+    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 23 / 42, 1400 63 / 70, 2000 108 / 93, 128
+    // after 8192 62 / 56; 32 tokens with 16 heads over one at 4095 19 / 40; 16 heads of 64 over 8, 2048 after
+    // 6144 240 / 195, 1024 after 3000 68 / 72.
     const double gain = (hd == 128 ? 1.85 * t16 - 10.0 * big : 0.9 * t16 - 8.5 * big) * B * Hkv * (Lmax - M / 2) / kKv4Block;
     p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : gain < 24000.0 ? 16 : kKv4Tile;
     const long long tiles = (rows + p.RT - 1) / p.RT;
