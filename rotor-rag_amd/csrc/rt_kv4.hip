@@ -461,12 +461,15 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
             a.heads[2 * bh + 1] = p.first;
         }
     } else if (a.S == 1) {
-        // the last tiles, which see the most keys, of all heads first (from an empty cache, 20 heads over 5, 640 /
-        // 1024 / 1400 tokens 24 / 40 / 63 us; head by head from the first tile on 30 / 48 / 79; 512 23 / 22)
+        // the last tiles, which see the most keys, of all heads first, and a CU's second workgroup of the short
+        // ones, the longer its first is (from an empty cache, 20 heads over 5, 512 / 640 / 1024 / 1400 tokens
+        // 20.9 / 25.4 / 39.7 / 63.4 us; the second in the same order 23.1 / 23.7 / 39.6 / 62.9; head by head from
+        // the first tile on 22.4 / 30.5 / 47.6 / 78.6)
+        const int w = (int)blockIdx.x, w0 = w >> 8 == 1 && (int)gridDim.x >= 512 ? w ^ 255 : w;
         split = slot = 0;
         S = 1;
-        tile = a.tiles - 1 - (int)blockIdx.x / a.bh;
-        bh = (int)blockIdx.x % a.bh;
+        tile = a.tiles - 1 - w0 / a.bh;
+        bh = w0 % a.bh;
     } else {
         const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x), unit = w0 / a.S;
         split = w0 % a.S;
@@ -1270,7 +1273,7 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     // rows, a small one each block's codes again.  Per block of 64 keys at 128 dimensions, a big tile 10 ns
     // and 0.75 for every 16 rows in it, a small one 2.6; at 64, 8.5 and 0.4 against 1.3.  In tiles of 16 /
     // 256 rows, us, 20 heads over 5: 16 sequences of 5 tokens at 4000 41 / 88, of 16 79 / 91, of 32 128 / 109,
-    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 23 / 42, 1400 63 / 70, 2000 108 / 93, 128
+    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 21 / 42, 1400 63 / 70, 2000 108 / 93, 128
     // after 8192 62 / 56; 32 tokens with 16 heads over one at 4095 19 / 40; 16 heads of 64 over 8, 2048 after
     // 6144 240 / 195, 1024 after 3000 68 / 72.
     const double gain = (hd == 128 ? 1.85 * t16 - 10.0 * big : 0.9 * t16 - 8.5 * big) * B * Hkv * (Lmax - M / 2) / kKv4Block;
