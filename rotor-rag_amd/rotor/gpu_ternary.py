@@ -539,45 +539,52 @@ class HIPTernaryOps:
         return torch.empty((int(batch), int(n_kv_heads), (int(max_len) + 63) // 64, 72 * int(head_dim)),
                            dtype=torch.uint8, device=self.device)
 
-    # A step of decoding is a few microseconds of GPU work, so these calls look at each tensor once and
-    # touch nothing that is already as the library takes it.
-    def _kv4_check(self, who, cache, pos, max_len):
+    # A step of decoding is a few microseconds of GPU work, so these calls look at each tensor once, touch
+    # nothing that is already as the library takes it, and compare devices by their numbers.
+    def _kv4_check(self, who, torch, cache, pos, max_len):
         """(B, Hkv, hd, Lmax) of a cache and its positions."""
-        torch = _torch()
-        if (cache.dtype != torch.uint8 or cache.ndim != 4 or not cache.is_contiguous() or cache.device != self.device
-                or cache.shape[3] not in (72 * 64, 72 * 128)):
+        shape = cache.shape
+        if (cache.dtype is not torch.uint8 or len(shape) != 4 or not cache.is_contiguous()
+                or cache.get_device() != self.device_index or shape[3] not in (72 * 64, 72 * 128)):
             raise ValueError(f"{who}: cache must be a contiguous uint8 [B, Hkv, blocks, 72 * head_dim] tensor on the "
                              "backend's device (kv4_cache)")
-        B, Hkv, blocks, size = cache.shape
+        B, Hkv, blocks, size = shape
         Lmax = 64 * blocks if max_len is None else int(max_len)
         if not 64 * (blocks - 1) < Lmax <= 64 * blocks:
             raise ValueError(f"{who}: max_len {Lmax} does not fit a cache of {blocks} blocks of 64 positions")
-        if pos.dtype != torch.int32 or pos.shape != (B,) or pos.device != self.device or not pos.is_contiguous():
+        if (pos.dtype is not torch.int32 or pos.shape != (B,) or pos.get_device() != self.device_index
+                or not pos.is_contiguous()):
             raise ValueError(f"{who}: pos must be a contiguous int32 [{B}] tensor on the backend's device")
         return B, Hkv, size // 72, Lmax
 
-    def _kv4_run(self, name, fn, *args):
+    def _kv4_rows(self, who, q, B, Hkv, hd):
+        """(M, H) of q [B, M, H, hd]."""
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != B or shape[3] != hd or shape[2] % max(Hkv, 1) or 0 in shape:
+            raise ValueError(f"{who}: q of shape {tuple(shape)} does not fit a cache of {B} sequences, {Hkv} KV heads of {hd}")
+        return shape[1], shape[2]
+
+    def _kv4_run(self, torch, name, fn, *args):
         """fn(ctx, *args) on the current stream (taken as the number it is: making a Stream object of it
         costs as much as a small launch)."""
-        rc = self.lib.rt_ctx_set_stream(self.ctx, _torch()._C._cuda_getCurrentRawStream(self.device_index))
+        rc = self.lib.rt_ctx_set_stream(self.ctx, torch._C._cuda_getCurrentRawStream(self.device_index))
         rc = rc or fn(self.ctx, *args)
         if rc:
             _hip.check(rc, name)
 
-    def _kv4_in(self, x):
+    def _kv4_in(self, torch, x):
         """float32 device tensor, contiguous and 16-byte aligned (a copy where x is not)."""
-        torch = _torch()
-        if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.device == self.device
+        if not (isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.get_device() == self.device_index
                 and x.is_contiguous()):
             x = self._dev(x, torch.float32)
         return x.clone() if x.data_ptr() & 15 else x
 
-    def _kv4_out(self, who, out, like, *others):
+    def _kv4_out(self, who, torch, out, like, *others):
         """out, or a new tensor of like's shape; out may be like, and lies in none of the others."""
-        torch = _torch()
         if out is None:
             return torch.empty_like(like)
-        if out.dtype != torch.float32 or out.shape != like.shape or not out.is_contiguous() or out.device != self.device:
+        if (out.dtype is not torch.float32 or out.shape != like.shape or not out.is_contiguous()
+                or out.get_device() != self.device_index):
             raise ValueError(f"{who}: the output must be a contiguous float32 {list(like.shape)} tensor on the backend's "
                              "device")
         at, end = out.data_ptr(), out.data_ptr() + 4 * out.numel()
@@ -593,20 +600,19 @@ class HIPTernaryOps:
         than its blocks hold (None: as many as the blocks and rope hold; kv4_read and
         kv4_attention do not see rope, and take what the blocks hold).  Rows outside [0, max_len)
         are not written; their q is 0.  For inference: gradients do not pass."""
-        B, Hkv, hd, Lmax = self._kv4_check("kv4_append", cache, pos, max_len)
-        q, k, v, rope = self._kv4_in(q), self._kv4_in(k), self._kv4_in(v), self._kv4_in(rope)
-        if max_len is None and rope.ndim == 3:
-            Lmax = min(Lmax, max(rope.shape[0], Lmax - 63))
-        if q.ndim != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[2] % Hkv or q.numel() == 0:
-            raise ValueError(f"kv4_append: q of shape {tuple(q.shape)} does not fit a cache of {B} sequences, {Hkv} KV "
-                             f"heads of {hd}")
-        M, H = q.shape[1], q.shape[2]
-        if k.shape != (B, M, Hkv, hd) or k.shape != v.shape:
+        torch = _torch()
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_append", torch, cache, pos, max_len)
+        q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
+        table = rope.shape
+        if max_len is None and len(table) == 3:
+            Lmax = min(Lmax, max(table[0], Lmax - 63))
+        M, H = self._kv4_rows("kv4_append", q, B, Hkv, hd)
+        if k.shape != (B, M, Hkv, hd) or v.shape != (B, M, Hkv, hd):
             raise ValueError(f"kv4_append: k and v must be {[B, M, Hkv, hd]}")
-        if rope.ndim != 3 or rope.shape[1:] != (hd // 2, 2) or rope.shape[0] < Lmax:
+        if len(table) != 3 or table[1:] != (hd // 2, 2) or table[0] < Lmax:
             raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
-        out = self._kv4_out("kv4_append", q_out, q, k, v, rope, cache)
-        self._kv4_run("rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
+        out = self._kv4_out("kv4_append", torch, q_out, q, k, v, rope, cache)
+        self._kv4_run(torch, "rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
                       cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
         return out
 
@@ -614,13 +620,13 @@ class HIPTernaryOps:
         """The values that a 4-bit cache holds at positions pos[b] + (0 .. length - 1): (k, v)
         float32 [B, Hkv, length, hd]; zeros outside [0, max_len) (rt_kv4_read)."""
         torch = _torch()
-        B, Hkv, hd, Lmax = self._kv4_check("kv4_read", cache, pos, max_len)
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_read", torch, cache, pos, max_len)
         length = operator.index(length)
         if not 0 < length <= Lmax:
             raise ValueError(f"kv4_read: length {length} of a cache of {Lmax} positions")
         k = torch.empty((B, Hkv, length, hd), dtype=torch.float32, device=self.device)
         v = torch.empty_like(k)
-        self._kv4_run("rt_kv4_read", self.lib.rt_kv4_read, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, length, Hkv, hd,
+        self._kv4_run(torch, "rt_kv4_read", self.lib.rt_kv4_read, cache.data_ptr(), k.data_ptr(), v.data_ptr(), B, length, Hkv, hd,
                       Lmax, pos.data_ptr())
         return k, v
 
@@ -629,16 +635,13 @@ class HIPTernaryOps:
         pos[b] + m over a 4-bit cache (rt_kv4_attention): float32 [B, M, H, hd] (out, which may be
         q).  Rows outside [0, max_len) are 0.  For inference: gradients do not pass."""
         torch = _torch()
-        B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", cache, pos, max_len)
-        q = self._kv4_in(q)
-        if q.ndim != 4 or q.shape[0] != B or q.shape[3] != hd or q.shape[2] % Hkv or q.numel() == 0:
-            raise ValueError(f"kv4_attention: q of shape {tuple(q.shape)} does not fit a cache of {B} sequences, {Hkv} "
-                             f"KV heads of {hd}")
-        M, H = q.shape[1], q.shape[2]
-        out = self._kv4_out("kv4_attention", out, q, cache)
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", torch, cache, pos, max_len)
+        q = self._kv4_in(torch, q)
+        M, H = self._kv4_rows("kv4_attention", q, B, Hkv, hd)
+        out = self._kv4_out("kv4_attention", torch, out, q, cache)
         need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._kv4_run("rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
+        self._kv4_run(torch, "rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
                       Hkv, hd, Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need)
         return out
 

@@ -136,7 +136,7 @@ def ops(lib):
     from rotor.gpu_ternary import HIPTernaryOps
 
     o = HIPTernaryOps.__new__(HIPTernaryOps)
-    o.lib, o.device, o.ctx = lib, torch.device("cpu"), None
+    o.lib, o.device, o.device_index, o.ctx = lib, torch.device("cpu"), -1, None
     return o
 
 
