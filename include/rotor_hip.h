@@ -391,6 +391,13 @@ size_t rt_kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax
 int rt_kv4_attention(rt_ctx* ctx, const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                      int Lmax, const int* pos, void* workspace, size_t workspace_bytes);
 
+/* One token a sequence: rt_kv4_append and rt_kv4_attention in one launch (one more where the keys
+ * are split), with the same results bit for bit.  q, k and v [B][heads][hd] as they come from the
+ * projections; the rotated q is not kept.  H / Hkv <= 16; out may be q, no other buffers overlap;
+ * workspace: rt_kv4_attention_workspace(B, 1, ...) bytes. */
+int rt_kv4_step(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
+                int B, int H, int Hkv, int hd, int Lmax, const int* pos, void* workspace, size_t workspace_bytes);
+
 /* Final RMSNorm of x fp32 [D] with norm_w, tied bf16 LM head logits [V]
  * (src/rotor/bitnet_model.py:231-235) and greedy argmax (src/rotor/generation.py:42;
  * first index of the maximum).  `best` (device u64, zero before first use) is left

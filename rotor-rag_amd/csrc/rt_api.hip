@@ -1260,17 +1260,37 @@ size_t rt_kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax
     return kv4_attention_workspace(B, M, H, Hkv, hd, Lmax);
 }
 
+static int kv4_check_workspace(const void* workspace, size_t bytes, size_t need, const char* who) {
+    if (need && (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(RT_EINVAL, std::string(who) + ": workspace too small (rt_kv4_attention_workspace) or not 16-byte "
+                                                  "aligned");
+    return RT_OK;
+}
+
 int rt_kv4_attention(rt_ctx* ctx, const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                      int Lmax, const int* pos, void* workspace, size_t workspace_bytes) {
-    const int rc = kv4_check(ctx, {q, cache, out}, pos, B, M, H, Hkv, hd, Lmax, "rt_kv4_attention");
+    int rc = kv4_check(ctx, {q, cache, out}, pos, B, M, H, Hkv, hd, Lmax, "rt_kv4_attention");
+    if (!rc)
+        rc = kv4_check_workspace(workspace, workspace_bytes, kv4_attention_workspace(B, M, H, Hkv, hd, Lmax),
+                                 "rt_kv4_attention");
     if (rc) return rc;
-    const size_t need = kv4_attention_workspace(B, M, H, Hkv, hd, Lmax);
-    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
-        return fail(RT_EINVAL, "rt_kv4_attention: workspace too small (rt_kv4_attention_workspace) or not 16-byte "
-                               "aligned");
     DeviceGuard g(ctx->device);
     RT_HIP(launch_kv4_attention(q, cache, out, B, M, H, Hkv, hd, Lmax, pos, static_cast<float*>(workspace),
                                 ctx->stream));
+    return RT_OK;
+}
+
+int rt_kv4_step(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
+                int B, int H, int Hkv, int hd, int Lmax, const int* pos, void* workspace, size_t workspace_bytes) {
+    int rc = kv4_check(ctx, {q, k, v, rope, cache, out}, pos, B, 1, H, Hkv, hd, Lmax, "rt_kv4_step");
+    if (!rc && H / Hkv > 16) rc = fail(RT_EINVAL, "rt_kv4_step: unsupported layout (H / Hkv <= 16)");
+    if (!rc)
+        rc = kv4_check_workspace(workspace, workspace_bytes, kv4_attention_workspace(B, 1, H, Hkv, hd, Lmax),
+                                 "rt_kv4_step");
+    if (rc) return rc;
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_kv4_step(q, k, v, rope, cache, out, B, H, Hkv, hd, Lmax, pos, static_cast<float*>(workspace),
+                           ctx->stream));
     return RT_OK;
 }
 

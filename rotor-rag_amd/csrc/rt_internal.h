@@ -432,6 +432,8 @@ hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, 
                            const int* pos, hipStream_t s);
 hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                                 int Lmax, const int* pos, float* work, hipStream_t s);
+hipError_t launch_kv4_step(const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
+                           int B, int H, int Hkv, int hd, int Lmax, const int* pos, float* work, hipStream_t s);
 hipError_t launch_lm_head(const uint16_t* E, const float* x, const float* norm_w, float eps, int V, int D,
                           float* logits, unsigned long long* best, int* token, int* pos, int advance,
                           int* next_ids, int* out_tokens, int pos_base, int out_cap, float* next_h, hipStream_t s);

@@ -96,6 +96,50 @@ __device__ __forceinline__ unsigned kv4_encode(const float (&x)[8], unsigned s) 
     return w;
 }
 
+// Scale dword (s) and codes of a group whose 64 numbers eight neighbour lanes hold, eight each.
+__device__ __forceinline__ unsigned kv4_group(const float (&x)[8], int lane, unsigned& s) {
+    float lo = x[0], hi = x[0];
+    bool fin = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+        fin = fin && fabsf(x[e]) <= 3.402823466e38f;
+    }
+#pragma unroll
+    for (int w = 1; w < 8; w <<= 1) {
+        lo = fminf(lo, __shfl_xor(lo, w, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, w, 64));
+    }
+    const unsigned long long bad = __ballot(!fin);
+    s = kv4_scale(lo, hi, ((bad >> (lane & 56)) & 0xFFull) == 0ull);
+    return kv4_encode(x, s);
+}
+// Dimensions 8 o .. 8 o + 7 of a key at p, rotated (src: the head's row).
+template <int HD>
+__device__ __forceinline__ void kv4_rotate(float (&x)[8], const float* src, const float* rope, int p, int o) {
+    constexpr int HALF = HD / 2;
+    const bool up = 8 * o >= HALF;
+    const int i = (8 * o) % HALF;
+    const float* other = src + (up ? i : i + HALF);
+    const float* cs = rope + ((size_t)p * HALF + i) * 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const double a = x[e], d = other[e], c = cs[2 * e], s = cs[2 * e + 1];
+        x[e] = up ? (float)(a * c + d * s) : (float)(a * c - d * s);
+    }
+}
+// Where a block keeps the codes of 8 dimensions of a key, and the eight values' dword of a dimension
+// (positions 16 x + 4 vl + (0..3, 8..11)) at p.
+template <int HD>
+__device__ __forceinline__ int kv4_key_word(int p, int o) {
+    return p % kKv4Block * (HD / 8) + (o % 8 / 2) * (HD / 32) + o / 8 * 2 + o % 2;
+}
+template <int HD>
+__device__ __forceinline__ int kv4_value_word(int p, int vl, int dim) {
+    return 8 * HD + ((dim / 32 * 16 + dim % 16) * 4 + p % 32 / 16 * 2 + vl) * 4 + dim % 32 / 16 * 2 + p % kKv4Block / 32;
+}
+
 // A row (b, m) stands at position pos[b] + m; rows outside [0, Lmax) have no place in the cache.
 __device__ __forceinline__ int kv4_row_pos(int pos, int m, int Lmax) {
     const long long p = (long long)pos + m;
@@ -157,8 +201,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
     // V's dword of thread (dimension, l): positions 4 l + (0..3, 8..11) of the 16; what it holds is asked for
     // now, for the positions that are not this call's
     const int dim = min(t >> 1, HD - 1), vl = t & 1;
-    unsigned* const vat = reinterpret_cast<unsigned*>(blk + 32 * HD) +
-                          ((dim / 32 * 16 + dim % 16) * 4 + p0 % 32 / 16 * 2 + vl) * 4 + dim % 32 / 16 * 2 + p0 % kKv4Block / 32;
+    unsigned* const vat = reinterpret_cast<unsigned*>(blk) + kv4_value_word<HD>(p0, vl, dim);
     const unsigned old = pos > p0 || end < first + kKv4Rows ? *vat : 0u;
     for (int r0 = 0; r0 < kKv4Rows; r0 += 128 / TPR) {
         if (p0 + r0 >= end || p0 + r0 + 128 / TPR <= pos) continue;  // (uniform) none of these rows
@@ -168,37 +211,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const float* q, const f
         const float* src = (is_v ? v : k) + ((size_t)b * M + (in ? p - pos : 0)) * Hkv * HD + (size_t)kh * HD;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = src[8 * o + e];
-        if (!is_v) {
-            const bool up = 8 * o >= HALF;
-            const int i = (8 * o) % HALF;
-            const float* other = src + (up ? i : i + HALF);
-            const float* cs = rope + ((size_t)(in ? p : 0) * HALF + i) * 2;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const double a = x[e], d = other[e], c = cs[2 * e], s = cs[2 * e + 1];
-                x[e] = up ? (float)(a * c + d * s) : (float)(a * c - d * s);
-            }
-        }
-        float lo = x[0], hi = x[0];
-        bool fin = true;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
-            fin = fin && fabsf(x[e]) <= 3.402823466e38f;
-        }
-#pragma unroll
-        for (int w = 1; w < 8; w <<= 1) {
-            lo = fminf(lo, __shfl_xor(lo, w, 64));
-            hi = fmaxf(hi, __shfl_xor(hi, w, 64));
-        }
-        const unsigned long long bad = __ballot(!fin);
-        const unsigned s = kv4_scale(lo, hi, ((bad >> (lane & 56)) & 0xFFull) == 0ull);
-        const unsigned word = kv4_encode(x, s);
+        if (!is_v) kv4_rotate<HD>(x, src, rope, in ? p : 0, o);
+        unsigned s;
+        const unsigned word = kv4_group(x, lane, s);
         const int P = p % kKv4Block;
         if (is_v) codes[r][o] = word;
         if (in) {
-            if (!is_v) reinterpret_cast<unsigned*>(blk)[P * TPR + (o % 8 / 2) * (HD / 32) + o / 8 * 2 + o % 2] = word;
+            if (!is_v) reinterpret_cast<unsigned*>(blk)[kv4_key_word<HD>(p, o)] = word;
             if (o % 8 == 0) sc[o / 8 * 64 + P] = s;
         }
     }
@@ -369,6 +388,9 @@ struct Kv4AttnArgs {
     int M, H, Hkv, Lmax, nblk, tiles, S, bh;  // bh = B * Hkv.  S = 0: splits by length (kv4_piece)
     int* heads;                               // S = 0: (pieces, first) of every head
     float scale;  // log2(e) / sqrt(HD)
+    // a decode step (M = 1; q not rotated): the new row's key and value, the angles, the cache to write to
+    const float *k, *v, *rope;
+    uint8_t* put;
 };
 
 // What rows m0..m1 of a sequence at pos see: keys [0, kend) some of them, keys [0, all] each of them
@@ -425,6 +447,57 @@ __device__ __forceinline__ Kv4Piece kv4_piece(const Kv4AttnArgs& a, int w, int l
 // The power of two that brings the largest of a row's scaled queries into [2^14, 2^15).
 __device__ __forceinline__ int kv4_query_power(float big) { return min(max(14 - kv4_exponent(big), -113), 126); }
 
+// The one new row of a head (k, v: its HD numbers) into its block at p, by one wave, as kv4_append_kernel
+// writes it.
+template <int HD>
+__device__ __forceinline__ void kv4_put_row(const float* k, const float* v, const float* rope, uint8_t* blk, int p, int lane) {
+    constexpr int TPR = HD / 8;  // lanes [0, TPR) take the key, the next TPR the value, the rest the value again
+    const bool is_v = lane >= TPR;
+    const int o = lane % TPR, r = p % 16, vl = r >> 2 & 1, sh = kv4_shift(r >> 3 << 2 | (r & 3));
+    unsigned *const words = reinterpret_cast<unsigned*>(blk), *at[HD / 64], old[HD / 64];
+#pragma unroll
+    for (int n = 0; n < HD / 64; ++n) {
+        at[n] = words + kv4_value_word<HD>(p, vl, 64 * n + lane);
+        old[n] = *at[n];
+    }
+    float x[8];
+    const float* src = is_v ? v : k;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = src[8 * o + e];
+    if (!is_v) kv4_rotate<HD>(x, src, rope, p, o);
+    unsigned s;
+    const unsigned word = kv4_group(x, lane, s);
+    if (!is_v) words[kv4_key_word<HD>(p, o)] = word;
+    if (lane < 2 * TPR && o % 8 == 0) words[16 * HD + (is_v ? HD : 0) + o / 8 * 64 + p % kKv4Block] = s;
+#pragma unroll
+    for (int n = 0; n < HD / 64; ++n) {
+        const unsigned w = (unsigned)__shfl((int)word, TPR + 8 * n + lane / 8, 64);
+        *at[n] = (old[n] & ~(15u << sh)) | ((w >> kv4_shift(lane % 8)) & 15u) << sh;
+    }
+    __threadfence_block();  // the wave's loads of the block come after
+}
+// Rotates queries that lie as the few-rows kernel holds them, with the products and roundings of
+// kv4_append_kernel.
+template <int HD>
+__device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4f* cs, int h) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const double co = cs[2 * e + c / 2][2 * (c % 2)], si = cs[2 * e + c / 2][2 * (c % 2) + 1];
+            if constexpr (HD == 128) {  // pairs (i, i + 64): both in this lane
+                const double a = qx[0][e][c], b = qx[1][e][c];
+                qx[0][e][c] = (float)(a * co - b * si);
+                qx[1][e][c] = (float)(b * co + a * si);
+            } else {  // (i, i + 32): lane groups h and h + 2
+                const unsigned u = __float_as_uint(qx[0][e][c]);
+                const v2u y = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+                const double a = __uint_as_float(y[0]), b = __uint_as_float(y[1]);
+                qx[0][e][c] = h < 2 ? (float)(a * co - b * si) : (float)(b * co + a * si);
+            }
+        }
+}
+
 // ---- few rows ------------------------------------------------------------------------------
 // A tile is RT rows (R = m G + g of KV head kh), RT = 4, 8 or 16.  The matrix instructions have 16
 // columns: column i is row i % RT over the key tiles of number i / RT modulo 16 / RT, so that every
@@ -441,7 +514,9 @@ __device__ __forceinline__ int kv4_query_power(float big) { return min(max(14 - 
 // 2^-29 of it unless it is 0), which keeps w h below 2^15, and w, w z in fp32's range.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.
-template <int HD, int RT>
+// STEP (one token, G <= 16 so that a head is one tile): append and attention in one launch.  Every
+// workgroup rotates its queries; the wave whose block the token lies in writes it there first.
+template <int HD, int RT, bool STEP>
 __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
     __shared__ float om[4][16][HD + 4];
@@ -496,6 +571,17 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const int kend = range.kend, all = range.all;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
     const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * S;
+    int j = split * 4 + wave;
+    v4f cs[STEP ? 8 : 1];  // cos, sin of pairs 16 (h % (HD / 32)) + (0..15)
+    if constexpr (STEP) {
+        const float* at = a.rope + ((size_t)max(last, 0) * (HD / 2) + h % (HD / 32) * 16) * 2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cs[e] = *reinterpret_cast<const v4f*>(at + 4 * e);
+        const int p = __builtin_amdgcn_readfirstlane(last);
+        if (p >= 0 && p / kKv4Block % step == j)
+            kv4_put_row<HD>(a.k + (size_t)bh * HD, a.v + (size_t)bh * HD, a.rope,
+                            a.put + ((size_t)bh * a.nblk + p / kKv4Block) * kv4_block_bytes(HD), p, lane);
+    }
     // Key tile wx = 2 w + x of a block: keys 32 w + 8 x + kl + r of lane group h.  The column's own
     // tiles are wx = NA q + ca.
     const int kl = 16 * (h >> 1) + 4 * (h & 1);
@@ -531,11 +617,12 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 #pragma unroll
         for (int u = 0; u < 2 * NG; ++u) vc[u] = *reinterpret_cast<const v4u*>(blk + (at_v + u * 1024));
     };
-    int j = split * 4 + wave;
+    if constexpr (STEP && RT == 16) kv4_rotate_query<HD>(qx, cs, h);  // (no registers for both)
     if (j < nb) {
         load_k(j);
         load_v(j);
     }
+    if constexpr (STEP && RT != 16) kv4_rotate_query<HD>(qx, cs, h);
     float qs[NG], qi;
     v8h qh[NG][2], ql[NG][2];
     {
@@ -1301,15 +1388,18 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     }
     return p;
 }
+template <int HD, bool STEP>
+void run_kv4_few(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {
+    const dim3 grid((unsigned)p.groups), block(256);
+    if (p.RT == 4) hipLaunchKernelGGL((kv4_attn_kernel<HD, 4, STEP>), grid, block, 0, s, a);
+    else if (p.RT == 8) hipLaunchKernelGGL((kv4_attn_kernel<HD, 8, STEP>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((kv4_attn_kernel<HD, 16, STEP>), grid, block, 0, s, a);
+}
 template <int HD>
 hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {
-    const dim3 grid((unsigned)p.groups), block(256);
-    switch (p.RT) {
-        case 4: hipLaunchKernelGGL((kv4_attn_kernel<HD, 4>), grid, block, 0, s, a); break;
-        case 8: hipLaunchKernelGGL((kv4_attn_kernel<HD, 8>), grid, block, 0, s, a); break;
-        case 16: hipLaunchKernelGGL((kv4_attn_kernel<HD, 16>), grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL(kv4_prefill_kernel<HD>, grid, dim3(512), 1024 * HD, s, a); break;
-    }
+    if (a.put) run_kv4_few<HD, true>(a, p, s);
+    else if (p.RT != kKv4Tile) run_kv4_few<HD, false>(a, p, s);
+    else hipLaunchKernelGGL(kv4_prefill_kernel<HD>, dim3((unsigned)p.groups), dim3(512), 1024 * HD, s, a);
     if (p.S != 1) {
         const long long all = p.units * std::min<long long>(p.RT, (long long)a.M * (a.H / a.Hkv));  // rows
         const int threads = (p.S == 0 ? p.groups / p.units : p.S) > 16 && all < 4096 ? 1024 : 256, gr = threads / (HD / 4), sg = all >= 4096 ? 1 : gr;
@@ -1325,14 +1415,52 @@ size_t kv4_attention_workspace(int B, int M, int H, int Hkv, int hd, int Lmax) {
     return p.S == 1 ? 0 : (size_t)p.groups * p.RT * (hd + 2) * sizeof(float) + (p.S == 0 ? (size_t)p.units * 8 : 0);
 }
 
+namespace {
+hipError_t launch_kv4(Kv4AttnArgs a, int B, int hd, hipStream_t s) {
+    const Kv4Shape p = kv4_shape(B, a.M, a.H, a.Hkv, hd, a.Lmax);
+    if (p.groups > (p.RT == kKv4Tile ? kMaxGroups / 2 : kMaxGroups)) return hipErrorInvalidValue;
+    a.nblk = (a.Lmax + kKv4Block - 1) / kKv4Block;
+    a.tiles = p.tiles;
+    a.S = p.S;
+    a.bh = B * a.Hkv;
+    a.heads = reinterpret_cast<int*>(a.work + (p.S == 0 ? (size_t)p.groups * p.RT * (hd + 2) : 0));
+    a.scale = 1.44269504088896341f / sqrtf((float)hd);
+    return hd == 128 ? run_kv4_attention<128>(a, p, s) : run_kv4_attention<64>(a, p, s);
+}
+}  // namespace
+
 hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, int B, int M, int H, int Hkv, int hd,
                                 int Lmax, const int* pos, float* work, hipStream_t s) {
-    const Kv4Shape p = kv4_shape(B, M, H, Hkv, hd, Lmax);
-    if (p.groups > (p.RT == kKv4Tile ? kMaxGroups / 2 : kMaxGroups)) return hipErrorInvalidValue;
-    const Kv4AttnArgs a{q, static_cast<const uint8_t*>(cache), out, work, pos, M, H, Hkv, Lmax,
-                        (Lmax + kKv4Block - 1) / kKv4Block, p.tiles, p.S, B * Hkv,
-                        reinterpret_cast<int*>(work + (p.S == 0 ? (size_t)p.groups * p.RT * (hd + 2) : 0)), 1.44269504088896341f / sqrtf((float)hd)};
-    return hd == 128 ? run_kv4_attention<128>(a, p, s) : run_kv4_attention<64>(a, p, s);
+    Kv4AttnArgs a{};
+    a.q = q;
+    a.cache = static_cast<const uint8_t*>(cache);
+    a.out = out;
+    a.work = work;
+    a.pos = pos;
+    a.M = M;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.Lmax = Lmax;
+    return launch_kv4(a, B, hd, s);
+}
+
+// One token a sequence: append and attention (H / Hkv <= 16: a head is one tile, and its new row one wave's).
+hipError_t launch_kv4_step(const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
+                           int B, int H, int Hkv, int hd, int Lmax, const int* pos, float* work, hipStream_t s) {
+    Kv4AttnArgs a{};
+    a.q = q;
+    a.cache = a.put = static_cast<uint8_t*>(cache);
+    a.out = out;
+    a.work = work;
+    a.pos = pos;
+    a.M = 1;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.Lmax = Lmax;
+    a.k = k;
+    a.v = v;
+    a.rope = rope;
+    return launch_kv4(a, B, hd, s);
 }
 
 }  // namespace rt

@@ -86,6 +86,7 @@ SIGNATURES = {
     "rt_kv4_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "rt_kv4_attention_workspace": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I]),
     "rt_kv4_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, ctypes.c_size_t]),
+    "rt_kv4_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, ctypes.c_size_t]),
     "rt_lm_head_argmax": (_I, [_P, _P, _P, _P, _F, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P]),
 }
 

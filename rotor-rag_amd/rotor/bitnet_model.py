@@ -535,12 +535,14 @@ class _DeviceModel:
     def _attend_kv4(self, st, L, M):
         """RoPE, the new keys and values into layer L's 4-bit cache, attention over it into st["o"]."""
         lib, ctx, chk = _hip.load(), self.hip.ctx, _hip.check
-        q, ws = st["q"].data_ptr(), st["ws4"]
-        chk(lib.rt_kv4_append(ctx, q, st["k"].data_ptr(), st["v"].data_ptr(), self.rope.data_ptr(), L["k4"].data_ptr(), q,
-                              1, M, self.H, self.Hkv, self.hd, self.Lmax, self.pos.data_ptr()), "rt_kv4_append")
-        chk(lib.rt_kv4_attention(ctx, q, L["k4"].data_ptr(), st["o"].data_ptr(), 1, M, self.H, self.Hkv, self.hd, self.Lmax,
-                                 self.pos.data_ptr(), ws.data_ptr() if ws is not None else None,
-                                 ws.numel() if ws is not None else 0), "rt_kv4_attention")
+        q, k, v, o, cache, rope, pos = (x.data_ptr() for x in (st["q"], st["k"], st["v"], st["o"], L["k4"], self.rope, self.pos))
+        sizes, ws = (self.H, self.Hkv, self.hd, self.Lmax, pos), st["ws4"]
+        ws = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
+        if M == 1 and self.H // self.Hkv <= 16:
+            chk(lib.rt_kv4_step(ctx, q, k, v, rope, cache, o, 1, *sizes, *ws), "rt_kv4_step")
+            return
+        chk(lib.rt_kv4_append(ctx, q, k, v, rope, cache, q, 1, M, *sizes), "rt_kv4_append")
+        chk(lib.rt_kv4_attention(ctx, q, cache, o, 1, M, *sizes, *ws), "rt_kv4_attention")
 
     def layer_cache(self, li, length, epoch):
         """Layer li's cached K and V of the current sequence's first `length` tokens, as

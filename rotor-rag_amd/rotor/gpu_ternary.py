@@ -564,6 +564,22 @@ class HIPTernaryOps:
             raise ValueError(f"{who}: q of shape {tuple(shape)} does not fit a cache of {B} sequences, {Hkv} KV heads of {hd}")
         return shape[1], shape[2]
 
+    def _kv4_new(self, who, q, k, v, rope, B, Hkv, hd, Lmax, max_len):
+        """(Lmax, M, H) of new rows and their angles."""
+        table = rope.shape
+        if max_len is None and len(table) == 3:
+            Lmax = min(Lmax, max(table[0], Lmax - 63))
+        M, H = self._kv4_rows(who, q, B, Hkv, hd)
+        if k.shape != (B, M, Hkv, hd) or v.shape != (B, M, Hkv, hd):
+            raise ValueError(f"{who}: k and v must be {[B, M, Hkv, hd]}")
+        if len(table) != 3 or table[1:] != (hd // 2, 2) or table[0] < Lmax:
+            raise ValueError(f"{who}: rope must be [>= {Lmax}, {hd // 2}, 2]")
+        return Lmax, M, H
+
+    def _kv4_workspace(self, torch, B, M, H, Hkv, hd, Lmax):
+        need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
+        return need, torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+
     def _kv4_run(self, torch, name, fn, *args):
         """fn(ctx, *args) on the current stream (taken as the number it is: making a Stream object of it
         costs as much as a small launch)."""
@@ -603,17 +619,26 @@ class HIPTernaryOps:
         torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_append", torch, cache, pos, max_len)
         q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
-        table = rope.shape
-        if max_len is None and len(table) == 3:
-            Lmax = min(Lmax, max(table[0], Lmax - 63))
-        M, H = self._kv4_rows("kv4_append", q, B, Hkv, hd)
-        if k.shape != (B, M, Hkv, hd) or v.shape != (B, M, Hkv, hd):
-            raise ValueError(f"kv4_append: k and v must be {[B, M, Hkv, hd]}")
-        if len(table) != 3 or table[1:] != (hd // 2, 2) or table[0] < Lmax:
-            raise ValueError(f"kv4_append: rope must be [>= {Lmax}, {hd // 2}, 2]")
+        Lmax, M, H = self._kv4_new("kv4_append", q, k, v, rope, B, Hkv, hd, Lmax, max_len)
         out = self._kv4_out("kv4_append", torch, q_out, q, k, v, rope, cache)
         self._kv4_run(torch, "rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
                       cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
+        return out
+
+    def kv4_step(self, q, k, v, cache, rope, pos, max_len=None, out=None):
+        """A decoding step (q [B, 1, H, hd], k and v [B, 1, Hkv, hd], H / Hkv <= 16): kv4_append and
+        kv4_attention of its q in one launch (rt_kv4_step), with the same results; out may be q."""
+        torch = _torch()
+        B, Hkv, hd, Lmax = self._kv4_check("kv4_step", torch, cache, pos, max_len)
+        q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
+        Lmax, M, H = self._kv4_new("kv4_step", q, k, v, rope, B, Hkv, hd, Lmax, max_len)
+        if M != 1 or H > 16 * Hkv:
+            raise ValueError("kv4_step: takes one token a sequence, and H / Hkv <= 16")
+        out = self._kv4_out("kv4_step", torch, out, q, k, v, rope, cache)
+        need, ws = self._kv4_workspace(torch, B, 1, H, Hkv, hd, Lmax)
+        self._kv4_run(torch, "rt_kv4_step", self.lib.rt_kv4_step, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
+                      cache.data_ptr(), out.data_ptr(), B, H, Hkv, hd, Lmax, pos.data_ptr(),
+                      ws.data_ptr() if need else None, need)
         return out
 
     def kv4_read(self, cache, pos, length: int, max_len=None):
@@ -639,8 +664,7 @@ class HIPTernaryOps:
         q = self._kv4_in(torch, q)
         M, H = self._kv4_rows("kv4_attention", q, B, Hkv, hd)
         out = self._kv4_out("kv4_attention", torch, out, q, cache)
-        need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        need, ws = self._kv4_workspace(torch, B, M, H, Hkv, hd, Lmax)
         self._kv4_run(torch, "rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
                       Hkv, hd, Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need)
         return out

@@ -380,6 +380,43 @@ def test_attention_in_place(hip, B, M, H, Hkv, hd, Lmax):
     assert (q == want).all()
 
 
+# (B, H, Hkv, hd, Lmax, positions): the token in a block's first and last place, outside the cache, in each wave's
+# part and each split; 4, 8 and 16 rows a head, part of them; splits by length
+STEPS = [
+    (1, 20, 5, 128, 640, [0]), (1, 20, 5, 128, 640, [63]), (1, 20, 5, 128, 640, [64]), (1, 20, 5, 128, 640, [639]),
+    (1, 20, 5, 128, 4000, [1537]), (1, 20, 5, 128, 4000, [70]), (2, 3, 3, 64, 130, [129, 31]),
+    (4, 12, 12, 64, 777, [776, 5, 128, 400]), (3, 16, 1, 128, 300, [299, 0, 150]), (2, 16, 1, 64, 1500, [299, 1499]),
+    (2, 14, 2, 64, 200, [100, 197]), (2, 14, 2, 128, 2000, [100, 1997]), (1, 30, 2, 128, 2000, [1000]),
+    (3, 4, 2, 64, 64, [-1, 63, 2147483647]), (5, 20, 5, 128, 3000, [2999, 0, 1200, 64, -1]),
+    (64, 4, 2, 64, 2048, [(i * 997) % 2048 for i in range(64)]), (2, 5, 1, 128, 64, [-2, 64]),
+]
+
+
+@pytest.mark.parametrize("B,H,Hkv,hd,Lmax,pos", STEPS)
+def test_step(hip, B, H, Hkv, hd, Lmax, pos):
+    """One launch for both: the same bytes in the cache, the same outputs, over several steps."""
+    import torch
+
+    cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, Lmax)
+    mine = cache.clone()
+    (rope,) = _cuda(_rope(Lmax, hd))
+    at = _pos(pos)
+    for i in range(3):
+        q, k, v = _cuda(*_inputs(20 + i, B, 1, H, Hkv, hd))
+        if i == 1:  # a group that reads as NaN
+            k[0, 0, 0, 1] = float("nan")
+            v[-1, 0, -1, -1] = float("inf")
+        keep = [x.clone() for x in (q, k, v)]
+        y = hip.kv4_step(q, k, v, mine, rope, at, max_len=Lmax)
+        assert all(torch.equal(a.view(torch.int32), b.view(torch.int32)) for a, b in zip(keep, (q, k, v)))
+        want = hip.kv4_attention(hip.kv4_append(q, k, v, cache, rope, at, max_len=Lmax), cache, at, max_len=Lmax)
+        assert torch.equal(mine, cache)
+        assert _same(y.cpu().numpy(), want.cpu().numpy())
+        assert hip.kv4_step(q, k, v, mine, rope, at, max_len=Lmax, out=q) is q
+        assert _same(q.cpu().numpy(), want.cpu().numpy()) and torch.equal(mine, cache)
+        at = at + 1
+
+
 def test_past_four_gigabytes(hip):
     """The last sequence of a cache of more than 2^32 bytes."""
     import torch
@@ -426,6 +463,12 @@ def test_graph_and_streams(hip, M, Lmax):
     def step(c):
         r = hip.kv4_append(q, k, v, c, rope, pos, max_len=Lmax)
         return [r, hip.kv4_attention(r, c, pos, max_len=Lmax), *hip.kv4_read(c, pos, M, max_len=Lmax)]
+
+    if M == 1:
+        two = step
+
+        def step(c):
+            return [*two(c), hip.kv4_step(q, k, v, c, rope, pos, max_len=Lmax)]
 
     step(mine.clone())  # (first launches)
     torch.cuda.synchronize()

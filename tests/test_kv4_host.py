@@ -98,15 +98,22 @@ def _attend(lib, ctx=P, q=P, cache=P, out=P, pos=P, ws=P, ws_bytes=1 << 30, **kw
                                 ws_bytes)
 
 
+def _step(lib, ctx=P, q=P, k=P, v=P, rope=P, cache=P, out=P, pos=P, ws=P, ws_bytes=1 << 30, **kw):
+    a = {**GOOD, **kw}
+    return lib.rt_kv4_step(ctx, q, k, v, rope, cache, out, a["B"], a["H"], a["Hkv"], a["hd"], a["Lmax"], pos, ws, ws_bytes)
+
+
 BAD_SIZES = [dict(B=0), dict(B=-1), dict(M=0), dict(M=641), dict(Hkv=0), dict(Hkv=-5), dict(hd=32), dict(hd=256),
              dict(hd=0), dict(Lmax=0), dict(Lmax=(1 << 20) + 1), dict(B=1 << 22), dict(B=1 << 30, Hkv=4)]
 
 
 @pytest.mark.parametrize("call,bufs", [(_append, ["ctx", "q", "k", "v", "rope", "cache", "q_out", "pos"]),
                                        (_read, ["ctx", "cache", "k", "v", "pos"]),
-                                       (_attend, ["ctx", "q", "cache", "out", "pos"])])
+                                       (_attend, ["ctx", "q", "cache", "out", "pos"]),
+                                       (_step, ["ctx", "q", "k", "v", "rope", "cache", "out", "pos"])])
 def test_refusals(lib, call, bufs):
-    who = {"_append": "rt_kv4_append", "_read": "rt_kv4_read", "_attend": "rt_kv4_attention"}[call.__name__]
+    who = {"_append": "rt_kv4_append", "_read": "rt_kv4_read", "_attend": "rt_kv4_attention",
+           "_step": "rt_kv4_step"}[call.__name__]
     for name in bufs:
         assert call(lib, **{name: None}) == RT_EINVAL
         assert who in lib.rt_last_error().decode() and "NULL" in lib.rt_last_error().decode()
@@ -114,19 +121,24 @@ def test_refusals(lib, call, bufs):
             assert call(lib, **{name: ODD}) == RT_EINVAL
             assert who in lib.rt_last_error().decode() and "aligned" in lib.rt_last_error().decode()
     for bad in BAD_SIZES:
+        if call is _step and "M" in bad:
+            continue
         assert call(lib, **bad) == RT_EINVAL, bad
         assert who in lib.rt_last_error().decode()
     if call is not _read:
         for bad in [dict(H=0), dict(H=21), dict(H=-20), dict(H=1025, Hkv=1)]:
             assert call(lib, **bad) == RT_EINVAL, bad
+    if call is _step:
+        assert call(lib, H=17, Hkv=1) == RT_EINVAL and "H / Hkv" in lib.rt_last_error().decode()
 
 
 def test_attention_refuses_small_workspaces(lib):
     need = lib.rt_kv4_attention_workspace(1, 1, 20, 5, 128, 4096)
     assert need > 0
     for bad in [dict(ws=None, ws_bytes=0), dict(ws_bytes=need - 1), dict(ws=ODD, ws_bytes=need)]:
-        assert _attend(lib, Lmax=4096, **bad) == RT_EINVAL
-        assert "workspace" in lib.rt_last_error().decode()
+        for call in (_attend, _step):
+            assert call(lib, Lmax=4096, **bad) == RT_EINVAL
+            assert "workspace" in lib.rt_last_error().decode()
 
 
 @pytest.fixture()
@@ -170,6 +182,11 @@ def test_python_refusals(ops):
                  (f(3, 0, 6, 64), f(3, 0, 2, 64), f(3, 0, 2, 64), rope)]:
         with pytest.raises(ValueError, match="kv4_append"):
             ops.kv4_append(*args[:3], cache, args[3], pos)
+    one, kv1 = q[:, :1].contiguous(), kv[:, :1].contiguous()
+    for args in [(q, kv, kv, rope), (one[..., :32], kv1, kv1, rope), (one, kv, kv1, rope), (one, kv1, kv1, rope[:64]),
+                 (f(3, 1, 34, 64), kv1, kv1, rope)]:
+        with pytest.raises(ValueError, match="kv4_step"):
+            ops.kv4_step(*args[:3], cache, args[3], pos)
     for n in (0, -1, 129):
         with pytest.raises(ValueError, match="length"):
             ops.kv4_read(cache, pos, n)
@@ -188,6 +205,7 @@ def test_python_refusals(ops):
     for call in (lambda: ops.kv4_append(both[1:], kv, kv, cache, rope, pos, q_out=both[:3]),
                  lambda: ops.kv4_append(q, both.view(-1)[:kv.numel()].view(kv.shape), kv, cache, rope, pos, q_out=both[:3]),
                  lambda: ops.kv4_append(q, kv, both.view(-1)[-kv.numel():].view(kv.shape), cache, rope, pos, q_out=both[1:]),
+                 lambda: ops.kv4_step(one, kv1, kv1, cache, rope, pos, out=rope.view(-1)[:one.numel()].view(one.shape)),
                  lambda: ops.kv4_attention(both[:3], cache, pos, out=both[1:]),
                  lambda: ops.kv4_attention(q, cache, pos, out=cache.view(-1)[:4 * q.numel()].view(torch.float32).view(q.shape))):
         with pytest.raises(ValueError, match="share memory"):
