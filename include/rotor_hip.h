@@ -73,7 +73,8 @@ const char* rt_last_error(void);
  * 106 = 105 without rt_plan_set_row_stats and RT_SRC_RMSNORM_STATS (measured slower than each
  * decode prologue reducing its own row), + rt_attention_decode_combine,
  * rt_plan_attention_combine and rt_lm_head_argmax's next_h; 107 = 106 + rt_plan_set_output_ssq;
- * 108 = 107 + rt_plan_create_act_gate_up. */
+ * 108 = 107 + rt_plan_create_act_gate_up; the rt_kv4_* calls came to 108 later and change none
+ * of its others. */
 int rt_version(void);
 
 /* Number of visible HIP devices (0 when none); RT_OK even when 0. */
@@ -360,6 +361,8 @@ int rt_rope_attention_decode(rt_ctx* ctx, const float* q, const float* k, const 
  *   z = (max + min) / 2 and h = (max - min) / 30, each rounded to fp32, then to bf16,
  *   c = clamp(rint(((x - z) / h + 15) / 2), 0, 15) in 64 bits; (x - z) / h is 0 where h = 0.
  * A group that holds a value that is not finite, or whose z or h is not, reads as NaN.
+ * rt_kv4_attention and rt_kv4_step take keys and values up to 2^96 in magnitude (their
+ * intermediate sums are fp32); append and read take every fp32 number.
  * The bytes are opaque; fresh memory needs no initialisation: only positions that were
  * written take part in anything.  Buffers are 16-byte aligned, pos 4-byte aligned.
  * Lmax <= 2^20; the same Lmax goes to every call on a cache. */

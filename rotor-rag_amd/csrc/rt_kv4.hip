@@ -1345,8 +1345,9 @@ hipError_t launch_kv4_read(const void* cache, float* k, float* v, int B, int M, 
 }
 
 namespace {
-// Which kernel, and how many splits of the keys.  The host does not know the positions: a call is taken
-// to stand half way into its cache.  (Times: 20 heads of 128 over 5, the launches back to back.)
+// Which kernel, and how many splits of the keys.  The host does not know the positions: the tile is chosen
+// as for a call at its cache's end, the splits as half way into it.  (Times: 20 heads of 128 over 5, the
+// launches back to back.)
 struct Kv4Shape {
     long long units, groups;  // groups: workgroups of the attention launch, and partials
     int RT, tiles, S;         // S = 0: by length (kv4_piece)
