@@ -73,7 +73,9 @@ def test_attention_and_cache(models, name):
                 want = K4.attention(q, c["k"], c["v"], [0])
                 assert np.linalg.norm(got.reshape(want.shape) - want) <= 2e-6 * np.linalg.norm(want)
             M, got = rows[-1]
-            q = model._dev._state(1)["q"].cpu().numpy().reshape(1, 1, H, hd)
+            # (one token's queries are rotated in the attention's launch and not kept)
+            table = model._dev.rope.cpu().numpy().reshape(-1, hd // 2, 2)
+            q = K4.rope(model._dev._state(1)["q"].cpu().numpy().reshape(H, hd), table, cache.length - 1)[None, None]
             c = cache[n - 1]
             assert c["k"].shape == c["v"].shape == (1, Hkv, cache.length, hd)
             want = K4.attention(q, c["k"], c["v"], [cache.length - 1])
