@@ -365,7 +365,8 @@ int rt_rope_attention_decode(rt_ctx* ctx, const float* q, const float* k, const 
  * intermediate sums are fp32); append and read take every fp32 number.
  * The bytes are opaque; fresh memory needs no initialisation: only positions that were
  * written take part in anything.  Buffers are 16-byte aligned, pos 4-byte aligned.
- * Lmax <= 2^20; the same Lmax goes to every call on a cache. */
+ * B * Hkv <= 2^24, H / Hkv <= 1024, 1 <= M <= Lmax <= 2^20; the same Lmax goes to every call
+ * on a cache. */
 
 /* Bytes of a layer's cache: B * Hkv * ceil(Lmax / 64) blocks of 72 * hd bytes (0 for sizes the
  * calls below refuse). */

@@ -504,7 +504,7 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // lane's softmax counts however few the rows (with 16 columns for 4 rows, 12 lanes of 16 worked on
 // nothing: 131072 keys, 20 heads over 5, 44 us); the columns of a row are joined at the end.  Lane l
 // works on column i = l % 16 with the keys of lane group h = l / 16.  The split's blocks go to its
-// 4 waves in turn, an online softmax (base 2) for every column:
+// NW waves in turn, an online softmax (base 2) for every column:
 //   D = C Q^T per group of 64 dimensions (C the keys' codes less 8, exact in fp16; Q two fp16 terms,
 //       scaled so that the row's largest is in [2^14, 2^15)),  s = 2 h D + (z + h) sum_d q
 //   w = 2^(s - ref),  O^T += U^T (w h)^T  (U the values' levels 2 c - 15: uncentred, the sums over many
@@ -516,11 +516,11 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // one are multiplied, its values after this one's.
 // STEP (one token, G <= 16 so that a head is one tile): append and attention in one launch.  Every
 // workgroup rotates its queries; the wave whose block the token lies in writes it there first.
-template <int HD, int RT, bool STEP>
-__global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
+template <int HD, int RT, bool STEP, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
-    __shared__ float om[4][16][HD + 4];
-    __shared__ float ml[4][16][2];
+    __shared__ float om[NW][16][HD + 4];
+    __shared__ float ml[NW][16][2];
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
     int split, S, tile, bh, slot;  // slot: the partial's in the workspace
     if (a.S == 0) {
@@ -570,8 +570,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const Kv4Range range = kv4_range(pos, tile * RT / G, (min(tile * RT + RT, rows) - 1) / G, a.Lmax);
     const int kend = range.kend, all = range.all;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
-    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = 4 * S;
-    int j = split * 4 + wave;
+    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = NW * S;
+    int j = split * NW + wave;
     v4f cs[STEP ? 8 : 1];  // cos, sin of pairs 16 (h % (HD / 32)) + (0..15)
     if constexpr (STEP) {
         const float* at = a.rope + ((size_t)max(last, 0) * (HD / 2) + h % (HD / 32) * 16) * 2;
@@ -807,8 +807,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
         ml[wave][i][1] = lrow;
     }
     __syncthreads();
-    // join the 4 waves' NA columns of a row: 256 / RT threads a row
-    constexpr int TPR = 256 / RT, NP = 4 * NA;
+    // join the waves' NA columns of a row: 64 NW / RT threads a row
+    constexpr int TPR = 64 * NW / RT, NP = NW * NA;
     const int row = t / TPR, RR = tile * RT + row;
     if (RR >= rows) return;
     float mm = -INFINITY, den = 0.0f, f[NP];
@@ -1351,6 +1351,7 @@ namespace {
 struct Kv4Shape {
     long long units, groups;  // groups: workgroups of the attention launch, and partials
     int RT, tiles, S;         // S = 0: by length (kv4_piece)
+    int NW;                   // waves a workgroup (tiles of up to 16 rows)
 };
 Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     Kv4Shape p;
@@ -1379,22 +1380,29 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     const int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : (blocks + 3) / 4;
     p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
     p.groups = p.units * p.S;
+    // A workgroup's keys over eight waves instead of four, where it has a CU to itself and more than two rounds:
+    // 16 tokens at 620 (100) 13.1 / 13.7 us (8.9 / 7.9), 200 at 900 18.7 / 20.1, 3 x 77 at up to 1001 (14 heads of
+    // 64 over 2) 9.9 / 11.0, 16 tokens there at 500 (300) 7.5 / 8.1 (6.9 / 6.8).  Four or eight rows a tile, one
+    // token at 1279 (639, 450) 13.3 / 13.7 (10.2 / 10.1, 9.3 / 8.4): not there.
+    p.NW = p.RT == 16 && p.S == 1 && p.units <= 256 && blocks > 12 ? 8 : 4;
     // A batch: splits by length.  Sequences of 100 to 4096 keys, 32 / 8 / 48 of them: 25.6 / 14.6 / 31.9 us,
     // with the best equal number of splits 27.4 / 16.3 / 35.0; 4 of 100 to 32768 23.7 / 41; 50 of 100 to 1500
     // (250 heads, few keys) 21.8 / 17.5, so not there; 32 of 4096 each 30.7 / 29.8.
     if (B > 1 && B <= 64 && tiles == 1 && p.RT != kKv4Tile && p.units <= kKv4Slots / 2 &&
         blocks > (p.units <= kKv4Slots / 4 ? 20 : 31)) {
         p.S = 0;
+        p.NW = 4;
         p.groups = kKv4Slots;
     }
     return p;
 }
 template <int HD, bool STEP>
 void run_kv4_few(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {
-    const dim3 grid((unsigned)p.groups), block(256);
-    if (p.RT == 4) hipLaunchKernelGGL((kv4_attn_kernel<HD, 4, STEP>), grid, block, 0, s, a);
-    else if (p.RT == 8) hipLaunchKernelGGL((kv4_attn_kernel<HD, 8, STEP>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv4_attn_kernel<HD, 16, STEP>), grid, block, 0, s, a);
+    const dim3 grid((unsigned)p.groups), block(64 * p.NW);
+    if (p.RT == 4) hipLaunchKernelGGL((kv4_attn_kernel<HD, 4, STEP, 4>), grid, block, 0, s, a);
+    else if (p.RT == 8) hipLaunchKernelGGL((kv4_attn_kernel<HD, 8, STEP, 4>), grid, block, 0, s, a);
+    else if (p.NW == 4) hipLaunchKernelGGL((kv4_attn_kernel<HD, 16, STEP, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((kv4_attn_kernel<HD, 16, STEP, 8>), grid, block, 0, s, a);
 }
 template <int HD>
 hipError_t run_kv4_attention(const Kv4AttnArgs& a, const Kv4Shape& p, hipStream_t s) {

@@ -260,6 +260,10 @@ ATTENDS += [
     (2, 90, 4, 2, 128, 32000, [-50, 40], 130),
     (2, 64, 8, 2, 64, 66000, [-100, 70000], 1),
     (1, 64, 4, 1, 128, 83250, [83210], 83250),
+    # eight waves a workgroup: blocks for some, all or none of them
+    (1, 16, 20, 5, 128, 900, [884], 900),
+    (2, 30, 14, 2, 64, 1000, [0, 700], 730),
+    (1, 3, 16, 2, 128, 833, [447], 450),
     # many sequences of few rows: tiles of 16
     (40, 5, 8, 2, 64, 700, [(i * 97) % 690 for i in range(40)], 700),
     (130, 3, 20, 5, 128, 300, [(i * 31) % 298 for i in range(130)], 300),
@@ -386,7 +390,7 @@ STEPS = [
     (1, 20, 5, 128, 640, [0]), (1, 20, 5, 128, 640, [63]), (1, 20, 5, 128, 640, [64]), (1, 20, 5, 128, 640, [639]),
     (1, 20, 5, 128, 4000, [1537]), (1, 20, 5, 128, 4000, [70]), (2, 3, 3, 64, 130, [129, 31]),
     (4, 12, 12, 64, 777, [776, 5, 128, 400]), (3, 16, 1, 128, 300, [299, 0, 150]), (2, 16, 1, 64, 1500, [299, 1499]),
-    (2, 14, 2, 64, 200, [100, 197]), (2, 14, 2, 128, 2000, [100, 1997]), (1, 30, 2, 128, 2000, [1000]),
+    (2, 14, 2, 64, 200, [100, 197]), (2, 14, 2, 128, 2000, [100, 1997]), (1, 30, 2, 128, 2000, [1000]), (1, 16, 1, 128, 1200, [1150]), (3, 24, 2, 64, 1100, [-3, 1099, 200]),
     (3, 4, 2, 64, 64, [-1, 63, 2147483647]), (5, 20, 5, 128, 3000, [2999, 0, 1200, 64, -1]),
     (64, 4, 2, 64, 2048, [(i * 997) % 2048 for i in range(64)]), (2, 5, 1, 128, 64, [-2, 64]),
 ]
