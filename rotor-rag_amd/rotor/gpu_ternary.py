@@ -18,6 +18,7 @@ PyTorch supplies device memory and the stream; the compute is the HIP library.
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 
 import numpy as np
@@ -30,6 +31,11 @@ def _torch():
     import torch
 
     return torch
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace_bytes(B, M, H, Hkv, hd, Lmax):
+    return _hip.load().rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
 
 
 class DeviceTernaryWeights:
@@ -577,7 +583,7 @@ class HIPTernaryOps:
         return Lmax, M, H
 
     def _kv4_workspace(self, torch, B, M, H, Hkv, hd, Lmax):
-        need = self.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
+        need = _kv4_workspace_bytes(B, M, H, Hkv, hd, Lmax)
         return need, torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
 
     def _kv4_run(self, torch, name, fn, *args):
