@@ -372,6 +372,17 @@ __device__ __forceinline__ float kv4_join16(float x, Op op) {
     const v2u y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return kv4_join32(op(__uint_as_float(y[0]), __uint_as_float(y[1])), op);
 }
+// The largest of a wave's numbers, in an SGPR.
+__device__ __forceinline__ unsigned kv4_wave_max(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xF, 0xF, false));  // row_ror 1, 2, 4, 8
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xF, 0xF, false));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xF, 0xF, false));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xF, 0xF, false));
+    const v2u y = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(y[0], y[1]);
+    const v2u w = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(max(w[0], w[1]));
+}
 struct Kv4Max {
     __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
@@ -513,13 +524,16 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a group's h is no less than
 // 2^-29 of it unless it is 0), which keeps w h below 2^15, and w, w z in fp32's range.
 // Every load is issued half a round before its use: the keys of the next block when those of this
-// one are multiplied, its values after this one's.
+// one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
+// and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
+// instructions a block and more registers than there are: 512 / 1024 tokens from an empty cache, 20 heads
+// over 5, 20.2 / 40.4 us, so 17.6 / 34.9; 64 sequences of 4 tokens at 500 17.3, so 13.8).
 // STEP (one token, G <= 16 so that a head is one tile): append and attention in one launch.  Every
 // workgroup rotates its queries; the wave whose block the token lies in writes it there first.
 template <int HD, int RT, bool STEP, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
-    __shared__ float om[NW][16][HD + 4];
+    __shared__ __attribute__((aligned(16))) float om[NW][16][HD + 4];  // (in the loop, each wave's scales of a block)
     __shared__ float ml[NW][16][2];
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
     int split, S, tile, bh, slot;  // slot: the partial's in the workspace
@@ -586,10 +600,11 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     // tiles are wx = NA q + ca.
     const int kl = 16 * (h >> 1) + 4 * (h & 1);
     auto tile_key = [](int wx) { return 32 * (wx >> 1) + 8 * (wx & 1); };
-    v4u kc[4], ks[NG][NQ], vc[2 * NG], vs[NG][NQ];
+    v4u kc[4], vc[2 * NG];
+    unsigned ks[NG], vs[NG];  // scales of key `lane`
     // (byte offsets in a block, whose address is uniform)
     const unsigned at_k = (16 * (i >> 3) + (i & 7)) * (HD / 2) + h * 8 * NG, at_v = 32 * HD + (i * 4 + h) * 16,
-                   at_s = 64 * HD + (tile_key(ca) + kl) * 4;
+                   at_s = 64 * HD + lane * 4;
     auto load_k = [&](int j) {
         const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
 #pragma unroll
@@ -602,23 +617,23 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 kc[wx][1] = x[1];
             }
         }
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) ks[g][q] = *reinterpret_cast<const v4u*>(blk + (at_s + (g * 64 + tile_key(NA * q)) * 4));
     };
     auto load_v = [&](int j) {
         const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-                vs[g][q] = *reinterpret_cast<const v4u*>(blk + (at_s + 4 * HD + (g * 64 + tile_key(NA * q)) * 4));
-#pragma unroll
         for (int u = 0; u < 2 * NG; ++u) vc[u] = *reinterpret_cast<const v4u*>(blk + (at_v + u * 1024));
+    };
+    auto load_s = [&](int j) {
+        const uint8_t* blk = head + (size_t)j * kv4_block_bytes(HD);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            ks[g] = *reinterpret_cast<const unsigned*>(blk + (at_s + 256 * g));
+            vs[g] = *reinterpret_cast<const unsigned*>(blk + (at_s + 4 * HD + 256 * g));
+        }
     };
     if constexpr (STEP && RT == 16) kv4_rotate_query<HD>(qx, cs, h);  // (no registers for both)
     if (j < nb) {
+        load_s(j);
         load_k(j);
         load_v(j);
     }
@@ -660,7 +675,12 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         }
     }
     v4f o[NT];
-    float zs[NG], top = -INFINITY, ref = -INFINITY, lrow = 0.0f, hmax = 0.0f;
+    float zs[NG], top = -INFINITY, ref = -INFINITY, lrow = 0.0f;
+    unsigned hmax = 0u;
+    // the block's scales as numbers: h and z + h of the keys, h and z of the values, [64 keys] each, by group
+    float* const scales = &om[wave][0][0];
+    const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
+    auto scale = [&](int kind, int g, int q) { return own_scales[(64 * (4 * g + kind) + tile_key(NA * q)) / 4]; };
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = v4f{};
 #pragma unroll
@@ -668,6 +688,21 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     for (; j < nb; j += step) {
         const int key0 = j * kKv4Block + kl;
         const bool edge = j * kKv4Block + kKv4Block - 1 > all;  // some row does not see the whole block
+        {
+            const bool behind = j * kKv4Block + lane >= kend;  // what lies behind the newest key is not read as a number
+            float big = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float vh = behind ? 0.0f : kv4_h(vs[g]), vz = behind ? 0.0f : kv4_z(vs[g]);
+                scales[64 * (4 * g) + lane] = kv4_h(ks[g]);
+                scales[64 * (4 * g + 1) + lane] = kv4_z(ks[g]) + kv4_h(ks[g]);
+                scales[64 * (4 * g + 2) + lane] = vh;
+                scales[64 * (4 * g + 3) + lane] = vz;
+                big = fmaxf(big, fmaxf(vh, fabsf(vz) * 0x1p-24f));
+            }
+            hmax = max(hmax, kv4_wave_max(__float_as_uint(big)));
+        }
+        if (j + step < nb) load_s(j + step);
         float s[NQ][4];
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
@@ -690,14 +725,12 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x = 0.0f;
+            for (int r = 0; r < 4; ++r) s[q][r] = 0.0f;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float kh = kv4_h(ks[g][q][r]);
-                    x = fmaf(kh, own[g][r], fmaf(kv4_z(ks[g][q][r]) + kh, qs[g], x));
-                }
-                s[q][r] = x;
+            for (int g = 0; g < NG; ++g) {
+                const v4f kh = scale(0, g, q), kz = scale(1, g, q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[q][r] = fmaf(kh[r], own[g][r], fmaf(kz[r], qs[g], s[q][r]));
             }
         }
         if (j + step < nb) load_k(j + step);
@@ -708,26 +741,15 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 for (int r = 0; r < 4; ++r) {
                     const int key = key0 + tile_key(NA * q + ca) + r;
                     s[q][r] = key <= last ? s[q][r] : -INFINITY;
-                    if (key >= kend)  // what lies behind the newest key is not read as a number
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) vs[g][q][r] = 0u;
                 }
         }
-        float mx = -INFINITY, hm = 0.0f, zm = 0.0f;
+        float mx = -INFINITY;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                mx = fmaxf(mx, s[q][r]);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    hm = fmaxf(hm, kv4_h(vs[g][q][r]));
-                    zm = fmaxf(zm, fabsf(kv4_z(vs[g][q][r])));
-                }
-            }
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][r]);
         top = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
-        hmax = fmaxf(hmax, kv4_join16(fmaxf(hm, zm * 0x1p-24f), Kv4Max()));
-        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max(kv4_exponent(hmax), -80) - 14);
+        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max((int)(hmax >> 23) - 127, -80) - 14);
         if (__any(now != ref)) {
             const float alpha = __builtin_amdgcn_exp2f(ref - now);
             lrow *= alpha;
@@ -748,27 +770,25 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         for (int g = 0; g < NG; ++g) {
             unsigned wh[NQ][2], wl[NQ][2];
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
+            for (int q = 0; q < NQ; ++q) {
+                const v4f vh = scale(2, g, q), vz = scale(3, g, q);
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     v2h hi, lo;
-                    kv4_split(v2f{s[q][r] * kv4_h(vs[g][q][r]), s[q][r + 1] * kv4_h(vs[g][q][r + 1])}, hi, lo);
+                    kv4_split(v2f{s[q][r] * vh[r], s[q][r + 1] * vh[r + 1]}, hi, lo);
                     wh[q][r / 2] = __builtin_bit_cast(unsigned, hi);
                     wl[q][r / 2] = __builtin_bit_cast(unsigned, lo);
                 }
-            if (edge) {
-#pragma unroll
-                for (int q = 0; q < NQ; ++q)
+                if (edge) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool see = key0 + tile_key(NA * q + ca) + r <= last;
-                        zs[g] = fmaf(s[q][r], see ? kv4_z(vs[g][q][r]) : 0.0f, zs[g]);
+                        zs[g] = fmaf(s[q][r], see ? vz[r] : 0.0f, zs[g]);
                     }
-            } else {
+                } else {
 #pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) zs[g] = fmaf(s[q][r], kv4_z(vs[g][q][r]), zs[g]);
+                    for (int r = 0; r < 4; ++r) zs[g] = fmaf(s[q][r], vz[r], zs[g]);
+                }
             }
             // the weights of the products over tiles 2 w and 2 w + 1: the column's own tile, or zeros
             v4u th[2], tl[2];
