@@ -1377,16 +1377,17 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     Kv4Shape p;
     const long long rows = (long long)M * (H / Hkv), t16 = (rows + 15) / 16, big = (rows + kKv4Tile - 1) / kKv4Tile;
     const int blocks = (Lmax + kKv4Block - 1) / kKv4Block;
-    // 256 rows in one tile or in 16 of 16 rows.  A big tile costs some 24 us a launch before it pays (its
-    // queries and results pass through one workgroup a CU) and its conversion of every block however few its
-    // rows, a small one each block's codes again.  Per block of 64 keys at 128 dimensions, a big tile 10 ns
-    // and 0.75 for every 16 rows in it, a small one 2.6; at 64, 8.5 and 0.4 against 1.3.  In tiles of 16 /
-    // 256 rows, us, 20 heads over 5: 16 sequences of 5 tokens at 4000 41 / 88, of 16 79 / 91, of 32 128 / 109,
-    // 4 of 48 52 / 54, of 64 73 / 53; 512 tokens from an empty cache 21 / 42, 1400 63 / 70, 2000 108 / 93, 128
-    // after 8192 62 / 56; 32 tokens with 16 heads over one at 4095 19 / 40; 16 heads of 64 over 8, 2048 after
-    // 6144 240 / 195, 1024 after 3000 68 / 72.
-    const double gain = (hd == 128 ? 1.85 * t16 - 10.0 * big : 0.9 * t16 - 8.5 * big) * B * Hkv * (Lmax - M / 2) / kKv4Block;
-    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : gain < 24000.0 ? 16 : kKv4Tile;
+    // 256 rows in one tile or in 16 of 16 rows.  A big tile's launch costs more before it pays (its queries and
+    // results pass through one workgroup a CU) and its conversion of every block however few its rows, a small
+    // one each block's codes again.  Per block of 64 keys at 128 dimensions, a big tile takes 9.3 ns and 0.75 for
+    // every 16 rows in it, a small one 1.8; at 64, 6.5 and 0.32 against 0.82.  In tiles of 16 / 256 rows, us, 20
+    // heads over 5: 16 sequences of 24 tokens at 4000 71 / 102, of 48 128 / 130, of 64 152 / 145, 4 of 64 61 / 53,
+    // of 96 63 / 88; 1400 tokens from an empty cache 54 / 69, 2000 92 / 93, 512 after 1500 48 / 52, after 2500
+    // 68 / 61, 128 after 8192 53 / 56, 192 75 / 66; 32 heads over 8, 700 after 700 57 / 67, 300 after 4000 95 / 105,
+    // 1000 after 1000 100 / 102; 16 heads of 64 over 8, 2000 after 2000 90 / 98, 2048 after 6144 198 / 195, two of
+    // those 383 / 362.
+    const double gain = (hd == 128 ? 1.05 * t16 - 9.3 * big : 0.5 * t16 - 6.5 * big) * B * Hkv * (Lmax - M / 2) / kKv4Block;
+    p.RT = rows <= 4 ? 4 : rows <= 8 ? 8 : gain < (hd == 128 ? 11500.0 : 18000.0) ? 16 : kKv4Tile;
     const long long tiles = (rows + p.RT - 1) / p.RT;
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;

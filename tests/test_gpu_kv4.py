@@ -253,13 +253,15 @@ ATTENDS += [
     (1, 70, 2, 1, 64, 83250, [83210], 83250),    # rows behind it
     (3, 9, 1, 1, 128, 28000, [5, 0, 64], 73),    # nine rows
     # (... and rows enough for such tiles to pay)
-    (2, 77, 14, 2, 64, 76000, [0, 301], 378),
-    (1, 130, 3, 3, 128, 78000, [70], 200),
-    (1, 250, 6, 6, 64, 44000, [261], 511),
-    (1, 129, 7, 1, 64, 90000, [3], 132),
-    (2, 90, 4, 2, 128, 32000, [-50, 40], 130),
-    (2, 64, 8, 2, 64, 66000, [-100, 70000], 1),
-    (1, 64, 4, 1, 128, 83250, [83210], 83250),
+    (1, 64, 20, 5, 128, 20000, [64], 128),
+    (1, 100, 20, 5, 128, 20000, [0], 100),
+    (2, 73, 14, 2, 64, 98000, [0, 301], 374),
+    (1, 200, 3, 3, 128, 57000, [70], 270),
+    (1, 250, 6, 6, 64, 130000, [261], 511),
+    (1, 127, 16, 2, 64, 98000, [3], 130),
+    (2, 90, 4, 2, 128, 57000, [-50, 40], 130),
+    (2, 64, 32, 8, 64, 50000, [-100, 70000], 1),
+    (1, 64, 12, 3, 128, 33000, [32960], 33000),
     # eight waves a workgroup: blocks for some, all or none of them
     (1, 16, 20, 5, 128, 900, [884], 900),
     (2, 30, 14, 2, 64, 1000, [0, 700], 730),
@@ -280,7 +282,7 @@ def test_attention(hip, B, M, H, Hkv, hd, Lmax, pos, n):
             assert 0 <= pos[b] + m < Lmax or (y[b, m] == 0).all()
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 300), (1, 4000), (3, 300), (70, 300), (70, 21000), (70, 58000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 300), (1, 4000), (3, 300), (70, 300), (70, 21000), (64, 50000)])
 @pytest.mark.parametrize("qs,ks,vs", [(1e-30, 1, 1), (20, 1, 1), (1, 1e-20, 1), (1e-15, 1e15, 1), (1, 1, 1e-25), (1, 1, 1e25),
                                       (0, 1, 1), (1, 0, 0)])
 def test_attention_scales(hip, M, Lmax, qs, ks, vs):
@@ -292,7 +294,7 @@ def test_attention_scales(hip, M, Lmax, qs, ks, vs):
     _check(hip, q[:, :M] * f(qs), cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 700), (1, 2000), (40, 700), (40, 83300), (64, 262000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 700), (1, 2000), (40, 700), (40, 83300), (64, 800000)])
 def test_attention_values_of_very_different_sizes(hip, M, Lmax):
     """The weights' fp16 terms are scaled by the largest step of the values seen: outliers, early and late, that
     weigh little do not take the others' bits."""
@@ -304,7 +306,7 @@ def test_attention_values_of_very_different_sizes(hip, M, Lmax):
     _check(hip, q[:, :M], cache, pairs, [n - M], Lmax)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 8192), (24, 8192), (24, 42000), (64, 42000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 8192), (24, 8192), (24, 42000), (64, 50000)])
 def test_attention_long_and_even(hip, M, Lmax):
     """8192 keys that weigh about the same: the result is a small difference of large sums.  In 64 bits against
     fp32 sums of numbers with random signs: each of 2 x 8192 terms (magnitude at most 3 of the values' deviation)
@@ -318,7 +320,7 @@ def test_attention_long_and_even(hip, M, Lmax):
     assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("M,Lmax", [(1, 200), (1, 3000), (9, 200), (80, 200), (80, 21000), (80, 46000)])
+@pytest.mark.parametrize("M,Lmax", [(1, 200), (1, 3000), (9, 200), (80, 200), (80, 21000), (110, 35000)])
 def test_attention_nan(hip, M, Lmax):
     """A NaN that a row sees makes that row NaN (a value's: in its group of 64 dimensions); one that it does not
     see leaves every bit of it."""
@@ -341,7 +343,7 @@ def test_attention_nan(hip, M, Lmax):
     assert _same(y, want)
 
 
-@pytest.mark.parametrize("M,Lmax", [(20, 100), (20, 42000), (128, 132000)])
+@pytest.mark.parametrize("M,Lmax", [(20, 100), (20, 42000), (128, 400000)])
 def test_attention_nan_query(hip, M, Lmax):
     B, H, Hkv, hd, n = 1, 4, 2, 64, 70 + M
     cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, n)
@@ -374,7 +376,7 @@ def test_strided_and_odd_inputs(hip):
 
 
 @pytest.mark.parametrize("B,M,H,Hkv,hd,Lmax", [(2, 1, 20, 5, 128, 300), (1, 1, 20, 5, 128, 4000), (2, 45, 8, 2, 64, 300),
-                                               (2, 64, 8, 2, 128, 20000)])
+                                               (2, 64, 8, 2, 128, 26000)])
 def test_attention_in_place(hip, B, M, H, Hkv, hd, Lmax):
     cache, _ = _filled(hip, 5, B, H, Hkv, hd, Lmax, 200)
     (q,) = _cuda(_inputs(6, B, M, H, Hkv, hd)[0])
