@@ -1398,14 +1398,21 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     // in 8 / 4 / 1 splits 10.6 / 12.4 / 17.5 us, over 131072 in 200 / 102 / 50 36.7 / 30.8 / 34.2; 2048 of 8192
     // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495 (in equal runs of blocks over 256 workgroups, a unit
     // cut where a run ends, 417 too: the clock gives way to the matrix cores' power).
-    const int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : (blocks + 3) / 4;
-    p.S = (int)std::max(1ll, std::min<long long>(most, 512 / p.units));
+    const int fours = (blocks + 3) / 4;
+    int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : fours, wide = 512;
+    // Tiles of 16 rows: a workgroup's keys over eight waves instead of four, one workgroup a CU, but where every
+    // wave of four takes one block at most, or two in a short cache.  In four / eight, us: 16 tokens at 620 (100)
+    // 12.2 / 10.6 (7.3 / 7.9), at 2400 (3800, 8000) 11.8 / 13.7 (14.5 / 14.0, 20.3 / 17.8), 64 at 2400 19.9 / 18.9,
+    // 160 at 1300 (8000) 25.8 / 17.1 (69.6 / 62.2), 3 x 77 at 900 (14 heads of 64 over 2) 9.9 / 9.2.  Four or
+    // eight rows a tile, one token at 1279 (639, 450) 13.7 / 13.3 (10.1 / 10.2, 8.4 / 9.3): not there.
+    p.NW = 4;
+    if (p.RT == 16 && p.units <= 256 && blocks > 8 && (blocks <= 20 || p.units * fours > 256)) {
+        p.NW = 8;
+        most = blocks <= 20 ? 1 : (blocks + 7) / 8;
+        wide = 256;
+    }
+    p.S = (int)std::max(1ll, std::min<long long>(most, wide / p.units));
     p.groups = p.units * p.S;
-    // A workgroup's keys over eight waves instead of four, where it has a CU to itself and more than two rounds:
-    // 16 tokens at 620 (100) 13.1 / 13.7 us (8.9 / 7.9), 200 at 900 18.7 / 20.1, 3 x 77 at up to 1001 (14 heads of
-    // 64 over 2) 9.9 / 11.0, 16 tokens there at 500 (300) 7.5 / 8.1 (6.9 / 6.8).  Four or eight rows a tile, one
-    // token at 1279 (639, 450) 13.3 / 13.7 (10.2 / 10.1, 9.3 / 8.4): not there.
-    p.NW = p.RT == 16 && p.S == 1 && p.units <= 256 && blocks > 12 ? 8 : 4;
     // A batch: splits by length.  Sequences of 100 to 4096 keys, 32 / 8 / 48 of them: 25.6 / 14.6 / 31.9 us,
     // with the best equal number of splits 27.4 / 16.3 / 35.0; 4 of 100 to 32768 23.7 / 41; 50 of 100 to 1500
     // (250 heads, few keys) 21.8 / 17.5, so not there; 32 of 4096 each 30.7 / 29.8.

@@ -266,6 +266,8 @@ ATTENDS += [
     (1, 16, 20, 5, 128, 900, [884], 900),
     (2, 30, 14, 2, 64, 1000, [0, 700], 730),
     (1, 3, 16, 2, 128, 833, [447], 450),
+    (1, 64, 20, 5, 128, 2600, [2500], 2564),  # ... in splits
+    (2, 30, 14, 2, 64, 1500, [0, 1300], 1330),
     # many sequences of few rows: tiles of 16
     (40, 5, 8, 2, 64, 700, [(i * 97) % 690 for i in range(40)], 700),
     (130, 3, 20, 5, 128, 300, [(i * 31) % 298 for i in range(130)], 300),
