@@ -79,8 +79,9 @@ def attention_bound(q, c, z, h, pos, Lmax=None):
     each and 4 e for the product left out, k's sum 1 e), 3 x 128 products summed: at most 400 e.  Then the
     difference to the maximum, both of at most A in base 2, and the exponential: 2 e A log2(e) ln 2 + 4 e.  So a
     weight is off by d = 2 (404 A + 4) e relative to the weights' mean error.  A sum over n keys: the
-    products' terms (12 e), the weight's rounding and factors (4 e), 3 n additions, and as many for z;
-    the rescalings of up to n / 32 half blocks (2 each) and joins: at most (3 n + n / 16 + 50) e of
+    products' terms (12 e), the weight's rounding and factors (4 e), the rescalings of up to n / 32 half
+    blocks (2 each) and joins, and the additions: many rows 3 n; few rows 2 n of 2 h (c - 8), of no more
+    than twice h |u|, and n of z + h, of no more than h |u| + |z|.  At most (5 n + n / 16 + 50) e of
     sum p (h |u| + |z|), and the sum of weights n e more."""
     B, M, H, hd = q.shape
     (ck, cv), (zk, zv), (hk, hv) = c, z, h
@@ -101,5 +102,5 @@ def attention_bound(q, c, z, h, pos, Lmax=None):
                 A = (uk[b, j, :p + 1] @ np.abs(x)).max()
                 s = K[b, j, :p + 1] @ x
                 w = np.exp(s - s.max())
-                out[b, m, n] = (2 * (404 * A + 4) + 4 * (p + 1) + (p + 1) / 16 + 50) * e * (w @ uv[b, j, :p + 1] / w.sum())
+                out[b, m, n] = (2 * (404 * A + 4) + 6 * (p + 1) + (p + 1) / 16 + 50) * e * (w @ uv[b, j, :p + 1] / w.sum())
     return out

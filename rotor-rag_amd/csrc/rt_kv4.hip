@@ -329,17 +329,6 @@ __device__ __forceinline__ v8h kv4_codes(unsigned w, unsigned mask, unsigned mas
     }
     return r;
 }
-__device__ __forceinline__ v8h kv4_levels(unsigned w, unsigned mask) {
-    v8h r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const v2h x = kv4_level2(w, i, mask);
-        r[2 * i] = x[0];
-        r[2 * i + 1] = x[1];
-    }
-    return r;
-}
-
 // x (|x| < 2^15) as two fp16 terms: the error is at most 2^-22 |x| or 2^-25.  The empty asm keeps
 // the product that x comes from and its conversion apart: fused (v_fma_mixlo_f16) in one use of
 // hi and not in the other, hi differs by its last bit in one of some ten thousand, and that
@@ -518,11 +507,12 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // NW waves in turn, an online softmax (base 2) for every column:
 //   D = C Q^T per group of 64 dimensions (C the keys' codes less 8, exact in fp16; Q two fp16 terms,
 //       scaled so that the row's largest is in [2^14, 2^15)),  s = 2 h D + (z + h) sum_d q
-//   w = 2^(s - ref),  O^T += U^T (w h)^T  (U the values' levels 2 c - 15: uncentred, the sums over many
-//       keys would cancel; w h two fp16 terms),  O += sum_j w z
-// so that all products are exact and all sums fp32.  ref is the largest score so far plus e - 14,
-// 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a group's h is no less than
-// 2^-29 of it unless it is 0), which keeps w h below 2^15, and w, w z in fp32's range.
+//   w = 2^(s - ref),  O^T += C^T (2 w h)^T  (C the values' codes less 8; 2 w h two fp16 terms),
+//       O += sum_j w (z + h)
+// so that all products are exact and all sums fp32.  (With c in place of c - 8 the two sums would cancel over
+// many keys; with the levels 2 c - 15 themselves a dword takes eleven instructions instead of nine.)  ref is the
+// largest score so far plus e - 13, 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a
+// group's h is no less than 2^-29 of it unless it is 0), which keeps 2 w h below 2^15, and w, w z in fp32's range.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
@@ -677,7 +667,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     v4f o[NT];
     float zs[NG], top = -INFINITY, ref = -INFINITY, lrow = 0.0f;
     unsigned hmax = 0u;
-    // the block's scales as numbers: h and z + h of the keys, h and z of the values, [64 keys] each, by group
+    // the block's scales as numbers: h and z + h of the keys, 2 h and z + h of the values, [64 keys] each, by group
     float* const scales = &om[wave][0][0];
     const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
     auto scale = [&](int kind, int g, int q) { return own_scales[(64 * (4 * g + kind) + tile_key(NA * q)) / 4]; };
@@ -696,8 +686,8 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 const float vh = behind ? 0.0f : kv4_h(vs[g]), vz = behind ? 0.0f : kv4_z(vs[g]);
                 scales[64 * (4 * g) + lane] = kv4_h(ks[g]);
                 scales[64 * (4 * g + 1) + lane] = kv4_z(ks[g]) + kv4_h(ks[g]);
-                scales[64 * (4 * g + 2) + lane] = vh;
-                scales[64 * (4 * g + 3) + lane] = vz;
+                scales[64 * (4 * g + 2) + lane] = vh * (lane & 2 ? 0.125f : 2.0f);  // (codes 2, 3, 6, 7 come 16 times as large)
+                scales[64 * (4 * g + 3) + lane] = vz + vh;
                 big = fmaxf(big, fmaxf(vh, fabsf(vz) * 0x1p-24f));
             }
             hmax = max(hmax, kv4_wave_max(__float_as_uint(big)));
@@ -749,7 +739,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][r]);
         top = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
-        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max((int)(hmax >> 23) - 127, -80) - 14);
+        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max((int)(hmax >> 23) - 127, -80) - 13);
         if (__any(now != ref)) {
             const float alpha = __builtin_amdgcn_exp2f(ref - now);
             lrow *= alpha;
@@ -806,7 +796,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const v8h lev = kv4_levels(vc[u][2 * v + w], mask);
+                        const v8h lev = kv4_codes(vc[u][2 * v + w], mask, mask0);
                         v4f& acc = o[2 * u + v];
                         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, th[w]), acc, 0, 0, 0);
                         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, tl[w]), acc, 0, 0, 0);
