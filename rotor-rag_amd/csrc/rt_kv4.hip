@@ -1249,8 +1249,8 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
 template <int HD>
 __global__ void __launch_bounds__(1024) kv4_combine_kernel(const Kv4AttnArgs a, int TR, int sg) {
     constexpr int LR = HD / 4, AT = 4;
-    __shared__ v4f sx[1024];
-    __shared__ float sd[1024 / LR];
+    __shared__ v4f sx[16 * LR];
+    __shared__ float sd[16];
     const int t = threadIdx.x, c = t % LR, grp = t / LR;
     const int G = a.H / a.Hkv, rows = a.M * G, most = min(TR, rows);  // (a tile's rows that can be live)
     const long long rr = (long long)blockIdx.x * ((int)blockDim.x / LR / sg) + grp / sg;  // (unit, row of the tile)
@@ -1295,14 +1295,23 @@ __global__ void __launch_bounds__(1024) kv4_combine_kernel(const Kv4AttnArgs a, 
             for (int e = 0; e < 4; ++e) x[e] = fmaf(f, y[k][e], x[e]);  // (no weight: 0 * 0)
         }
     }
-    if (sg > 1) {
-        sx[t] = x;
-        if (c == 0) sd[grp] = den;
+    if (sg > 1) {  // (one row a workgroup: lanes c, c + LR, .. of every wave, then the waves)
+#pragma unroll
+        for (int w = LR; w < 64; w <<= 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], w, 64);
+            den += __shfl_xor(den, w, 64);
+        }
+        const int waves = (int)blockDim.x / 64;
+        if ((t & 63) < LR) {
+            sx[t / 64 * LR + c] = x;
+            if (c == 0) sd[t / 64] = den;
+        }
         __syncthreads();
-        if (grp % sg) return;
-        for (int k = 1; k < sg; ++k) {
-            x += sx[t + k * LR];
-            den += sd[grp + k];
+        if (t >= LR) return;
+        for (int k = 1; k < waves; ++k) {
+            x += sx[k * LR + c];
+            den += sd[k];
         }
     }
     if (!live || S == 1) return;  // (in one piece: written already)
