@@ -541,9 +541,9 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         }
     } else if (a.S == 1) {
         // the last tiles, which see the most keys, of all heads first, and a CU's second workgroup of the short
-        // ones, the longer its first is (from an empty cache, 20 heads over 5, 512 / 640 / 1024 / 1400 tokens
-        // 20.9 / 25.4 / 39.7 / 63.4 us; the second in the same order 23.1 / 23.7 / 39.6 / 62.9; head by head from
-        // the first tile on 22.4 / 30.5 / 47.6 / 78.6)
+        // ones, the longer its first is (from an empty cache, 20 heads over 5, 512 / 640 / 1024 / 1400 tokens; the
+        // kernel as it was then: 20.9 / 25.4 / 39.7 / 63.4 us; the second in the same order 23.1 / 23.7 / 39.6 /
+        // 62.9; head by head from the first tile on 22.4 / 30.5 / 47.6 / 78.6)
         const int w = (int)blockIdx.x, w0 = w >> 8 == 1 && (int)gridDim.x >= 512 ? w ^ 255 : w;
         split = slot = 0;
         S = 1;
@@ -1391,12 +1391,12 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     p.tiles = (int)std::min(tiles, 0x7FFFFFFFll);
     p.units = (long long)B * Hkv * tiles;
     // A split's results pass through memory and a second launch (3 to 16 us), so there is none where a
-    // wave has 5 blocks or fewer without (8 sequences of 12 heads over 777 keys 7.8 us, in 4 splits 9.7), and
-    // a tile of 256 rows keeps 8 blocks a split (128 tokens after 8192: 16 splits 59 us, 24 64).  Else as many
+    // wave has 5 blocks or fewer without (8 sequences of 12 heads over 777 keys 7.9 us, in 4 splits 9.6), and
+    // a tile of 256 rows keeps 8 blocks a split (128 tokens after 8192: 16 splits 57 us, 24 62).  Else as many
     // as two workgroups a CU take in one round, the big tiles, one a CU, in two: one token over 1538 keys
-    // in 8 / 4 / 1 splits 10.6 / 12.4 / 17.5 us, over 131072 in 200 / 102 / 50 36.7 / 30.8 / 34.2; 2048 of 8192
-    // tokens in 1 / 2 / 3 / 5 splits 513 / 520 / 417 / 495 (in equal runs of blocks over 256 workgroups, a unit
-    // cut where a run ends, 417 too: the clock gives way to the matrix cores' power).
+    // in 8 / 4 / 1 splits 10.6 / 12.4 / 17.7 us, over 131072 in 200 / 102 / 50 35.9 / 30.7 / 33.2; 2048 of 8192
+    // tokens in 1 / 2 / 3 / 5 splits 507 / 504 / 405 / 476 (in equal runs of blocks over 256 workgroups, a unit
+    // cut where a run ends, as long as in 3: the clock gives way to the matrix cores' power).
     const int fours = (blocks + 3) / 4;
     int most = p.RT == kKv4Tile ? blocks / 8 : blocks <= 20 ? 1 : fours, wide = 512;
     // Tiles of 16 rows: a workgroup's keys over eight waves instead of four, one workgroup a CU, but where every
@@ -1412,9 +1412,9 @@ Kv4Shape kv4_shape(int B, int M, int H, int Hkv, int hd, int Lmax) {
     }
     p.S = (int)std::max(1ll, std::min<long long>(most, wide / p.units));
     p.groups = p.units * p.S;
-    // A batch: splits by length.  Sequences of 100 to 4096 keys, 32 / 8 / 48 of them: 25.6 / 14.6 / 31.9 us,
-    // with the best equal number of splits 27.4 / 16.3 / 35.0; 4 of 100 to 32768 23.7 / 41; 50 of 100 to 1500
-    // (250 heads, few keys) 21.8 / 17.5, so not there; 32 of 4096 each 30.7 / 29.8.
+    // A batch: splits by length.  Sequences of 100 to 4096 keys, 32 / 8 / 48 of them: 24.0 / 14.3 / 30.3 us,
+    // with the best equal number of splits 25.5 / 14.6 / 33.3; 4 of 100 to 32768 22.6 / 28.3; 50 of 100 to 1500
+    // (250 heads, few keys) 20.2 / 17.1, so not there; 32 of 4096 each 30.0 / 28.6.
     if (B > 1 && B <= 64 && tiles == 1 && p.RT != kKv4Tile && p.units <= kKv4Slots / 2 &&
         blocks > (p.units <= kKv4Slots / 4 ? 20 : 31)) {
         p.S = 0;
