@@ -338,13 +338,16 @@ __device__ __forceinline__ float kv4_minus_one() {
     asm("" : "+s"(m));
     return m;
 }
-__device__ __forceinline__ void kv4_split(v2f x, v2h& hi, v2h& lo) {
-    float a = x[0], b = x[1];
+__device__ __forceinline__ void kv4_split(float& a, float& b, v2h& hi, v2h& lo) {  // (a and b as they were)
     asm("" : "+v"(a), "+v"(b));
     hi = __builtin_convertvector((v2f{a, b}), v2h);
     // (- 1.0 as a number that the compiler does not see: a subtraction would convert hi first)
     const float m = kv4_minus_one();
     lo = __builtin_convertvector((v2f{fmaf((float)hi[0], m, a), fmaf((float)hi[1], m, b)}), v2h);
+}
+__device__ __forceinline__ void kv4_split(v2f x, v2h& hi, v2h& lo) {
+    float a = x[0], b = x[1];
+    kv4_split(a, b, hi, lo);
 }
 // 2^n as fp32, -126 <= n <= 127
 __device__ __forceinline__ float kv4_pow2(int n) { return __uint_as_float((unsigned)(n + 127) << 23); }
@@ -1146,10 +1149,10 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         v8h ph[2], pl[2];
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], c, off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], c, off));
-            lrow += p0 + p1;
+            float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], c, off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], c, off));
             v2h hi, lo;
-            kv4_split(v2f{p0, p1}, hi, lo);
+            kv4_split(p0, p1, hi, lo);
+            lrow += p0 + p1;
             ph[r >> 3][r & 7] = hi[0];
             ph[r >> 3][(r & 7) + 1] = hi[1];
             pl[r >> 3][r & 7] = lo[0];
