@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict
 }
 
 // ---- attention ---------------------------------------------------------------------------
-// The eight levels 2 c - 15 of a dword, exact in fp16: a nibble at bits 4..7 of a half under
+// The levels 2 c - 15 of two of a dword's codes, exact in fp16: a nibble at bits 4..7 of a half under
 // 0x6400 is 1024 + 16 c, and (1024 + 16 c) / 8 - 143 = 2 c - 15.  Masking and setting the
 // exponent are one v_and_or_b32, which takes one of its two constants from a VGPR: `mask` is
 // kv4_mask()'s.
