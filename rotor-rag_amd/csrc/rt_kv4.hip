@@ -816,7 +816,9 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         for (int n = 4 * g; n < 4 * g + 4; ++n) *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = o[n] + zs[g];
     }
     if (h == 0) {
-        ml[wave][i][0] = ref;
+        // (a column that saw blocks but none of their keys has a reference that stands for no score: among the
+        // others' it would be the largest where all scores are far below zero, and leave them no weight)
+        ml[wave][i][0] = lrow == 0.0f ? -INFINITY : ref;
         ml[wave][i][1] = lrow;
     }
     __syncthreads();

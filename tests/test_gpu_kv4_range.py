@@ -1,0 +1,101 @@
+"""Attention over the 4-bit KV cache where numbers span many binades: scores far below zero.  Against the 64-bit
+oracle and its bound."""
+import numpy as np
+import pytest
+
+import test_gpu_kv4 as G
+from oracle import kv4_oracle as K4
+
+pytestmark = pytest.mark.gpu
+
+F = np.float32
+
+
+def _check(hip, q, cache, pairs, pos, Lmax, y=None):
+    """Every element within the bound; the whole, row by row, within a quarter of it (roundings are as often up as
+    down)."""
+    import torch
+
+    if y is None:
+        out = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax)
+        assert torch.equal(out, hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax))
+        y = out.cpu().numpy()
+    K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
+    want = K4.attention(q, K, V, pos, Lmax)
+    bound = K4.attention_bound(q, *pairs, pos, Lmax) + 1e-37
+    off = np.abs(y - want)
+    assert np.isfinite(y).all()
+    assert (off <= bound).all(), f"off by {np.max(off / bound):.3g} bounds"
+    rows = lambda x: np.linalg.norm(x.reshape(-1, 64), axis=-1)  # noqa: E731
+    assert (rows(off) <= 0.25 * rows(bound)).all(), f"a row is off by {np.max(rows(off) / rows(bound)):.3g} bounds"
+    return y, want
+
+
+# (B, M, H, Hkv, hd, Lmax, positions of row 0, written positions)
+FEW = [
+    # tiles of 4 rows: one block, part of one, splits; queries of one head
+    (1, 1, 20, 5, 128, 640, [0], 1),
+    (1, 1, 20, 5, 128, 640, [70], 71),
+    (1, 1, 20, 5, 128, 2048, [1537], 1538),
+    (1, 4, 2, 2, 64, 300, [62], 66),
+    # of 8, across a block's border, and in splits
+    (1, 2, 20, 5, 128, 640, [63], 65),
+    (1, 4, 8, 4, 64, 2000, [700], 704),
+    # of 16, with four waves and with eight
+    (1, 4, 20, 5, 128, 640, [62], 66),
+    (2, 30, 14, 2, 64, 200, [0, 100], 130),
+    (1, 16, 20, 5, 128, 900, [60], 76),
+    (2, 30, 14, 2, 64, 1500, [0, 800], 830),
+    # splits by length
+    (5, 1, 20, 5, 128, 3000, [1500, 0, 1200, 64, -1], 1501),
+    (3, 4, 8, 2, 64, 2000, [1996, 1, 1990], 2000),
+]
+MANY = [
+    (1, 64, 20, 5, 128, 20000, [64], 128),
+    (1, 100, 20, 5, 128, 20000, [0], 100),
+    (2, 73, 14, 2, 64, 98000, [0, 301], 374),
+    (1, 200, 3, 3, 128, 57000, [70], 270),
+    (2, 90, 4, 2, 128, 57000, [-50, 40], 130),
+]
+
+
+def _far(seed, B, M, n, H, Hkv, hd, nats):
+    """Queries and keys whose scores all lie about `nats` below zero, and values."""
+    q, _, _ = G._inputs(seed, B, M, H, Hkv, hd)
+    _, k, v = G._inputs(seed + 1, B, n, H, Hkv, hd)
+    side = F(np.sqrt(nats / np.sqrt(hd)))  # q . k = -side^2 hd = -nats sqrt(hd)
+    return q * F(0.3) + side, k * F(0.3) - side, v
+
+
+@pytest.mark.parametrize("nats", [100, 300])
+@pytest.mark.parametrize("case", FEW + MANY)
+def test_scores_far_below_zero(hip, case, nats):
+    """A softmax does not hang on a common offset of its scores."""
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, k, v = _far(B * 100 + M, B, M, n, H, Hkv, hd, nats)
+    cache, pairs = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
+    _check(hip, q, cache, pairs, pos, Lmax)
+
+
+def _step(hip, q, k, v, cache, pos, Lmax):
+    """kv4_step of the rows at pos (angles 0), over a cache that holds them already."""
+    import torch
+
+    B, hd = q.shape[0], q.shape[-1]
+    table = np.zeros((Lmax, hd // 2, 2), F)
+    table[..., 0] = 1
+    at = np.clip(pos, 0, k.shape[1] - 1)
+    new = [np.stack([x[b, at[b]] for b in range(B)])[:, None] for x in (k, v)]
+    copy = cache.clone()
+    y = hip.kv4_step(*G._cuda(q, *new), copy, *G._cuda(table), G._pos(pos), max_len=Lmax)
+    assert torch.equal(copy, cache)
+    return y.cpu().numpy()
+
+
+@pytest.mark.parametrize("nats", [100, 300])
+@pytest.mark.parametrize("case", [c for c in FEW if c[1] == 1])
+def test_step_scores_far_below_zero(hip, case, nats):
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, k, v = _far(B * 100 + M, B, M, n, H, Hkv, hd, nats)
+    cache, pairs = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
+    _check(hip, q, cache, pairs, pos, Lmax, y=_step(hip, q, k, v, cache, pos, Lmax))
