@@ -510,12 +510,14 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // NW waves in turn, an online softmax (base 2) for every column:
 //   D = C Q^T per group of 64 dimensions (C the keys' codes less 8, exact in fp16; Q two fp16 terms,
 //       scaled so that the row's largest is in [2^14, 2^15)),  s = 2 h D + (z + h) sum_d q
-//   w = 2^(s - ref),  O^T += C^T (2 w h)^T  (C the values' codes less 8; 2 w h two fp16 terms),
+//   w = 2^(s - top),  O^T += f C^T (2 w h)^T  (C the values' codes less 8; 2 w h f two fp16 terms),
 //       O += sum_j w (z + h)
 // so that all products are exact and all sums fp32.  (With c in place of c - 8 the two sums would cancel over
-// many keys; with the levels 2 c - 15 themselves a dword takes eleven instructions instead of nine.)  ref is the
-// largest score so far plus e - 13, 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a
-// group's h is no less than 2^-29 of it unless it is 0), which keeps 2 w h below 2^15, and w, w z in fp32's range.
+// many keys; with the levels 2 c - 15 themselves a dword takes eleven instructions instead of nine.)  top is the
+// largest score so far, and f = 2^(13 - e), 2^e the largest h of the values so far (or 2^-24 of the largest |z|: a
+// group's h is no less than 2^-29 of it unless it is 0), which keeps 2 w h f below 2^15.  f is no part of what the
+// join sees, nor of the scores' reference: there (top + e - 13, so that one factor served both) it fell to
+// rounding beside scores of 2^25 and more, and the references of waves whose values were 2^126 apart did not meet.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
@@ -668,9 +670,10 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         }
     }
     v4f o[NT];
-    float zs[NG], top = -INFINITY, ref = -INFINITY, lrow = 0.0f;
+    float zs[NG], top = -INFINITY, lrow = 0.0f;
     unsigned hmax = 0u;
-    // the block's scales as numbers: h and z + h of the keys, 2 h and z + h of the values, [64 keys] each, by group
+    int ve = -110;  // e above
+    // the block's scales as numbers: h and z + h of the keys, 2 h f and z + h of the values, [64 keys] each, by group
     float* const scales = &om[wave][0][0];
     const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
     auto scale = [&](int kind, int g, int q) { return own_scales[(64 * (4 * g + kind) + tile_key(NA * q)) / 4]; };
@@ -681,6 +684,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     for (; j < nb; j += step) {
         const int key0 = j * kKv4Block + kl;
         const bool edge = j * kKv4Block + kKv4Block - 1 > all;  // some row does not see the whole block
+        float vh2[NG];
         {
             const bool behind = j * kKv4Block + lane >= kend;  // what lies behind the newest key is not read as a number
             float big = 0.0f;
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
                 const float vh = behind ? 0.0f : kv4_h(vs[g]), vz = behind ? 0.0f : kv4_z(vs[g]);
                 scales[64 * (4 * g) + lane] = kv4_h(ks[g]);
                 scales[64 * (4 * g + 1) + lane] = kv4_z(ks[g]) + kv4_h(ks[g]);
-                scales[64 * (4 * g + 2) + lane] = vh * (lane & 2 ? 0.125f : 2.0f);  // (codes 2, 3, 6, 7 come 16 times as large)
+                vh2[g] = vh * (lane & 2 ? 0.125f : 2.0f);  // (codes 2, 3, 6, 7 come 16 times as large)
                 scales[64 * (4 * g + 3) + lane] = vz + vh;
                 big = fmaxf(big, fmaxf(vh, fabsf(vz) * 0x1p-24f));
             }
@@ -741,17 +745,23 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][r]);
-        top = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
-        const float now = (top == -INFINITY ? 0.0f : top) + (float)(max((int)(hmax >> 23) - 127, -80) - 13);
-        if (__any(now != ref)) {
-            const float alpha = __builtin_amdgcn_exp2f(ref - now);
+        const float now = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
+        const int vn = max((int)(hmax >> 23) - 127, -110);
+        const float f = kv4_pow2(13 - vn);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) scales[64 * (4 * g + 2) + lane] = vh2[g] * f;
+        if (__any(now != top) || vn != ve) {
+            const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+            const float fix = alpha * (ve - vn < -126 ? 0.0f : kv4_pow2(ve - vn));
             lrow *= alpha;
 #pragma unroll
             for (int g = 0; g < NG; ++g) zs[g] *= alpha;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[n] *= alpha;
-            ref = now;
+            for (int n = 0; n < NT; ++n) o[n] *= fix;
+            top = now;
+            ve = vn;
         }
+        const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -809,16 +819,20 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     }
     // this wave's O[column][dim], column i, dimensions 32 u + 16 v + 4 h + r
     lrow = kv4_join16(lrow, Kv4Sum());
+    const float back = kv4_pow2(ve - 13);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         zs[g] = kv4_join16(zs[g], Kv4Sum());
 #pragma unroll
-        for (int n = 4 * g; n < 4 * g + 4; ++n) *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = o[n] + zs[g];
+        for (int n = 4 * g; n < 4 * g + 4; ++n) {
+            v4f x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(o[n][r], back, zs[g]);
+            *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = x;
+        }
     }
     if (h == 0) {
-        // (a column that saw blocks but none of their keys has a reference that stands for no score: among the
-        // others' it would be the largest where all scores are far below zero, and leave them no weight)
-        ml[wave][i][0] = lrow == 0.0f ? -INFINITY : ref;
+        ml[wave][i][0] = top;  // (of a column that saw blocks but none of their keys: -inf, as of one that saw none)
         ml[wave][i][1] = lrow;
     }
     __syncthreads();

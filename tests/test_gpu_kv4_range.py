@@ -1,5 +1,4 @@
-"""Attention over the 4-bit KV cache where numbers span many binades: scores far below zero.  Against the 64-bit
-oracle and its bound."""
+"""Attention over the 4-bit KV cache where numbers span many binades, against the 64-bit oracle and its bound."""
 import numpy as np
 import pytest
 
@@ -18,6 +17,7 @@ def _check(hip, q, cache, pairs, pos, Lmax, y=None):
 
     if y is None:
         out = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax)
+        assert torch.isfinite(out).all()
         assert torch.equal(out, hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax))
         y = out.cpu().numpy()
     K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
@@ -99,3 +99,47 @@ def test_step_scores_far_below_zero(hip, case, nats):
     q, k, v = _far(B * 100 + M, B, M, n, H, Hkv, hd, nats)
     cache, pairs = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
     _check(hip, q, cache, pairs, pos, Lmax, y=_step(hip, q, k, v, cache, pos, Lmax))
+
+
+def _parts(case):
+    """Queries, keys and values of a case and, for each sequence, a key in its middle: the last rows see it, the
+    first do not (one token: it does)."""
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, _, _ = G._inputs(B * 7 + M, B, M, H, Hkv, hd)
+    _, k, v = G._inputs(B * 100 + M, B, n, H, Hkv, hd)
+    at = [p + M // 2 if M > 1 else p // 2 for p in pos]
+    return q, k, v, [(b, p) for b, p in enumerate(at) if 0 <= p < n]
+
+
+def _attend(hip, case, q, k, v):
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    with np.errstate(over="ignore"):
+        cache, pairs = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
+    y, _ = _check(hip, q, cache, pairs, pos, Lmax)
+    if M == 1:
+        assert np.array_equal(_step(hip, q, k, v, cache, pos, Lmax), y)
+    return y, cache
+
+
+@pytest.mark.parametrize("case", FEW + MANY)
+def test_blocks_of_values_far_apart(hip, case):
+    """Every other block of 64 positions holds values of 2^90, the rest of 2^-60: their waves and splits meet in
+    the join."""
+    q, k, v, _ = _parts(case)
+    even = (np.arange(v.shape[1]) // 64 % 2 == 0)[None, :, None, None]
+    _attend(hip, case, q, k, np.where(even, np.ldexp(v, 90), np.ldexp(v, -60)))
+
+
+@pytest.mark.parametrize("d", [20, 22, 23, 24, 25, 26, 30, 60])
+@pytest.mark.parametrize("case", FEW)
+def test_large_scores(hip, case, d):
+    """Scores of some 2^d: one key has all the weight."""
+    q, k, v, _ = _parts(case)
+    _attend(hip, case, q, np.ldexp(k, d - 1), v)
+
+
+@pytest.mark.parametrize("d", [-115, 90])
+@pytest.mark.parametrize("case", FEW + MANY)
+def test_values_of_any_size(hip, case, d):
+    q, k, v, _ = _parts(case)
+    _attend(hip, case, q, k, np.ldexp(v, d))
