@@ -1098,7 +1098,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
             }
     }
     v16f o[NU];
-    float top = -INFINITY, lrow = 0.0f;
+    float top = -INFINITY, off = 14.0f, lrow = 0.0f;
 #pragma unroll
     for (int u = 0; u < NU; ++u) o[u] = v16f{};
     Blk cur{}, next{};
@@ -1155,13 +1155,16 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         const float now = fmaxf(top, kv4_join32(mx, Kv4Max()) * c);
         if (__any(now != top) || fix != 1.0f) {
-            const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+            // weights are 2^(s + off), up to 2^14 (beside a score of 2^25 and more the 14 may round to 16, an
+            // infinity in fp16)
+            const float ref = now == -INFINITY ? 0.0f : now, old = off;
+            off = (14.0f - ref) + ref < 15.0f ? 14.0f - ref : -ref;
+            const float alpha = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(off - old);
             lrow *= alpha;
 #pragma unroll
             for (int u = 0; u < NU; ++u) o[u] *= alpha * fix;
             top = now;
         }
-        const float off = 14.0f - (top == -INFINITY ? 0.0f : top);
         v8h ph[2], pl[2];
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
@@ -1240,7 +1243,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
     const float back = kv4_pow2(max(ve - 14, -126)), inv = a.S > 1 ? 1.0f : lrow == 0.0f ? 0.0f : 1.0f / lrow;
     float* const part = a.work + ((size_t)((size_t)bh * a.tiles + tile) * a.S + split) * (TR * (HD + 2));
     if (a.S > 1 && hl == 0) {
-        part[TR * HD + 2 * (wave * 32 + c32)] = top;
+        part[TR * HD + 2 * (wave * 32 + c32)] = lrow == 0.0f ? -INFINITY : -off;
         part[TR * HD + 2 * (wave * 32 + c32) + 1] = lrow;
     }
 #pragma unroll

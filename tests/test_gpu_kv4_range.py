@@ -131,7 +131,7 @@ def test_blocks_of_values_far_apart(hip, case):
 
 
 @pytest.mark.parametrize("d", [20, 22, 23, 24, 25, 26, 30, 60])
-@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("case", FEW + MANY)
 def test_large_scores(hip, case, d):
     """Scores of some 2^d: one key has all the weight."""
     q, k, v, _ = _parts(case)
