@@ -1146,7 +1146,8 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
             else if (k >= QS - LV) load_v(k - (QS - LV));  // (a load holds the wave some 60 cycles: under the products)
             spread();
         }
-        const float c = qi * cur.c, fix = w == 0 ? cur.fix : 1.0f;
+        // (queries of 0 over small keys: the product of the factors falls to 0, and -inf times 0 is NaN)
+        const float c = fmaxf(qi * cur.c, 0x1p-126f), fix = w == 0 ? cur.fix : 1.0f;
         if (key0 + 31 > lo_last)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = key0 + 8 * (r >> 2) + 4 * hl + (r & 3) <= last ? s[r] : -INFINITY;

@@ -143,3 +143,11 @@ def test_large_scores(hip, case, d):
 def test_values_of_any_size(hip, case, d):
     q, k, v, _ = _parts(case)
     _attend(hip, case, q, k, np.ldexp(v, d))
+
+
+@pytest.mark.parametrize("kd", [-2000, -60, -20])
+@pytest.mark.parametrize("case", FEW + MANY)
+def test_zero_queries(hip, case, kd):
+    """Queries of 0, over keys of 0 or small ones: the mean of the values."""
+    q, k, v, _ = _parts(case)
+    _attend(hip, case, 0 * q, np.ldexp(k, kd), v)
