@@ -518,52 +518,25 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // group's h is no less than 2^-29 of it unless it is 0), which keeps 2 w h f below 2^15.  f is no part of what the
 // join sees, nor of the scores' reference: there (top + e - 13, so that one factor served both) it fell to
 // rounding beside scores of 2^25 and more, and the references of waves whose values were 2^126 apart did not meet.
+// One f for the wave is enough where the steps of its keys' values lie within 2^9 of each other (a row's best key
+// then has 2 w h f >= 2^6, and the second fp16 term ends at 2^-25).  From the first block on where they do not,
+// or where they are below 2^-80, every column and group of 64 dimensions takes an f of its own, by the largest
+// w h that the column has seen (FAR below; a key that it does not see has w = 0): one product a weight and one
+// maximum more, and no loads ahead.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
 // instructions a block and more registers than there are: 512 / 1024 tokens from an empty cache, 20 heads
 // over 5, 20.2 / 40.4 us, so 17.6 / 34.9; 64 sequences of 4 tokens at 500 17.3, so 13.8).
-// STEP (one token, G <= 16 so that a head is one tile): append and attention in one launch.  Every
-// workgroup rotates its queries; the wave whose block the token lies in writes it there first.
-template <int HD, int RT, bool STEP, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
+// A wave's part of a tile of RT rows: blocks j, j + step, .. of head bh.  Column i = lane % 16 (its row, over its key
+// tiles) leaves its sums o (dimensions 32 u + 16 v + 4 h + r of o[2 u + v][r]), its largest score and its sum of
+// weights.  scales: room for 4 HD floats of the wave's own.  ANY: steps may lie far apart from the first block on.
+template <int HD, int RT, bool STEP, bool ANY>
+__device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile, int j, int step, float* scales, int lane,
+                                         v4f (&o)[HD / 16], float& top, float& lrow) {
     constexpr int NG = HD / 64, NT = HD / 16, NA = 16 / RT, NQ = 4 / NA;  // NQ key tiles of 4 a block are a column's
-    __shared__ __attribute__((aligned(16))) float om[NW][16][HD + 4];  // (in the loop, each wave's scales of a block)
-    __shared__ float ml[NW][16][2];
-    const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4, ca = i / RT;
-    int split, S, tile, bh, slot;  // slot: the partial's in the workspace
-    if (a.S == 0) {
-        const Kv4Piece p = kv4_piece(a, (int)blockIdx.x, lane);
-        if (p.n == 0) return;
-        split = p.piece;
-        S = p.n;
-        tile = 0;
-        bh = p.b * a.Hkv + p.head;
-        slot = p.first + p.piece;
-        if (split == 0 && t == 0) {
-            a.heads[2 * bh] = S;
-            a.heads[2 * bh + 1] = p.first;
-        }
-    } else if (a.S == 1) {
-        // the last tiles, which see the most keys, of all heads first, and a CU's second workgroup of the short
-        // ones, the longer its first is (from an empty cache, 20 heads over 5, 512 / 640 / 1024 / 1400 tokens; the
-        // kernel as it was then: 20.9 / 25.4 / 39.7 / 63.4 us; the second in the same order 23.1 / 23.7 / 39.6 /
-        // 62.9; head by head from the first tile on 22.4 / 30.5 / 47.6 / 78.6)
-        const int w = (int)blockIdx.x, w0 = w >> 8 == 1 && (int)gridDim.x >= 512 ? w ^ 255 : w;
-        split = slot = 0;
-        S = 1;
-        tile = a.tiles - 1 - w0 / a.bh;
-        bh = w0 % a.bh;
-    } else {
-        const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x), unit = w0 / a.S;
-        split = w0 % a.S;
-        S = a.S;
-        tile = unit % a.tiles;
-        bh = unit / a.tiles;
-        slot = w0;
-    }
+    const int i = lane & 15, h = lane >> 4, ca = i / RT;
     const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned mask = kv4_mask(), mask0 = kv4_mask(0x000F000Fu);
     const int rows = a.M * G, R = min(tile * RT + i % RT, rows - 1), m = R / G;  // (rows past the end repeat the last)
     // the row's queries, dimensions 64 g + 16 h + 8 e + (0..7): requested before the first block, since loads
@@ -579,8 +552,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
     const Kv4Range range = kv4_range(pos, tile * RT / G, (min(tile * RT + RT, rows) - 1) / G, a.Lmax);
     const int kend = range.kend, all = range.all;
     const uint8_t* const head = a.cache + (size_t)bh * a.nblk * kv4_block_bytes(HD);
-    const int nb = (kend + kKv4Block - 1) / kKv4Block, step = NW * S;
-    int j = split * NW + wave;
+    const int nb = (kend + kKv4Block - 1) / kKv4Block;
     v4f cs[STEP ? 8 : 1];  // cos, sin of pairs 16 (h % (HD / 32)) + (0..15)
     if constexpr (STEP) {
         const float* at = a.rope + ((size_t)max(last, 0) * (HD / 2) + h % (HD / 32) * 16) * 2;
@@ -627,7 +599,9 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
         }
     };
     if constexpr (STEP && RT == 16) kv4_rotate_query<HD>(qx, cs, h);  // (no registers for both)
-    if (j < nb) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) ks[g] = vs[g] = 0u;
+    if (!ANY && j < nb) {
         load_s(j);
         load_k(j);
         load_v(j);
@@ -669,168 +643,268 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
             qs[g] = kv4_join16(qs[g], Kv4Sum()) * 0.5f;
         }
     }
-    v4f o[NT];
-    float zs[NG], top = -INFINITY, lrow = 0.0f;
-    unsigned hmax = 0u;
-    int ve = -110;  // e above
+    float zs[NG];
+    top = -INFINITY;
+    lrow = 0.0f;
+    unsigned vmax = 0u;                      // 2^e's number, as bits
+    float vmin = INFINITY;                   // the smallest step that the lane has met
+    int ve = -110, vn = ve;                  // e of the sums, and with the next block
+    bool far = ANY;
+    int fe[NG];                              // FAR: the columns' f = 2^fe, and
+    float seen[NG];                          // the largest 2 w h
+    // block j's values' scales, which are loaded: h and z + h as numbers (what lies behind the newest key is not read as
+    // one: no step, and where the middle is NaN no row sees it), and with them vmax and vmin (but for groups that
+    // read as NaN)
+    float vh[NG], vzh[NG];
+    auto measure = [&](int j) __attribute__((always_inline)) {
+        const bool behind = j * kKv4Block + lane >= kend;
+        float big = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float z = behind ? __builtin_nanf("") : kv4_z(vs[g]);
+            vh[g] = behind ? 0.0f : kv4_h(vs[g]);
+            vzh[g] = z + vh[g];
+            big = fmaxf(big, fmaxf(vh[g], fabsf(z) * 0x1p-24f));
+            vmin = fminf(vmin, fmaf(z, 0.0f, vh[g]));
+        }
+        vmax = max(vmax, kv4_wave_max(__float_as_uint(big)));
+        vn = max((int)(vmax >> 23) - 127, -110);
+        far = __any(vmin < kv4_pow2(max(vn - 8, -80)));
+    };
     // the block's scales as numbers: h and z + h of the keys, 2 h f and z + h of the values, [64 keys] each, by group
-    float* const scales = &om[wave][0][0];
     const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
     auto scale = [&](int kind, int g, int q) { return own_scales[(64 * (4 * g + kind) + tile_key(NA * q)) / 4]; };
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = v4f{};
 #pragma unroll
     for (int g = 0; g < NG; ++g) zs[g] = 0.0f;
-    for (; j < nb; j += step) {
-        const int key0 = j * kKv4Block + kl;
-        const bool edge = j * kKv4Block + kKv4Block - 1 > all;  // some row does not see the whole block
-        float vh2[NG];
-        {
-            const bool behind = j * kKv4Block + lane >= kend;  // what lies behind the newest key is not read as a number
-            float big = 0.0f;
+    const float two = lane & 2 ? 0.125f : 2.0f;  // (codes 2, 3, 6, 7 come 16 times as large)
+    auto walk = [&](auto far_) __attribute__((always_inline)) {
+        constexpr bool FAR = decltype(far_)::value;
+        for (; j < nb && (FAR || __builtin_expect(!far, 1)); j += step) {
+            if constexpr (FAR) {
+                load_s(j);
+                load_k(j);
+                load_v(j);
+            }
+            const int key0 = j * kKv4Block + kl;
+            const bool edge = j * kKv4Block + kKv4Block - 1 > all;  // some row does not see the whole block
+            if constexpr (FAR) measure(j);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float vh = behind ? 0.0f : kv4_h(vs[g]), vz = behind ? 0.0f : kv4_z(vs[g]);
                 scales[64 * (4 * g) + lane] = kv4_h(ks[g]);
                 scales[64 * (4 * g + 1) + lane] = kv4_z(ks[g]) + kv4_h(ks[g]);
-                vh2[g] = vh * (lane & 2 ? 0.125f : 2.0f);  // (codes 2, 3, 6, 7 come 16 times as large)
-                scales[64 * (4 * g + 3) + lane] = vz + vh;
-                big = fmaxf(big, fmaxf(vh, fabsf(vz) * 0x1p-24f));
+                scales[64 * (4 * g + 2) + lane] = vh[g] * (two * (FAR ? 1.0f : kv4_pow2(13 - vn)));
+                scales[64 * (4 * g + 3) + lane] = vzh[g];
             }
-            hmax = max(hmax, kv4_wave_max(__float_as_uint(big)));
-        }
-        if (j + step < nb) load_s(j + step);
-        float s[NQ][4];
+            if (!FAR && j + step < nb) load_s(j + step);
+            float s[NQ][4];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            v4f own[NG];
+            for (int q = 0; q < NQ; ++q) {
+                v4f own[NG];
 #pragma unroll
-            for (int c = 0; c < NA; ++c) {
+                for (int c = 0; c < NA; ++c) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        v4f dot{};
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const v8h u = kv4_codes(kc[NA * q + c][2 * g + e], mask, mask0);
+                            dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, qh[g][e], dot, 0, 0, 0);
+                            dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, ql[g][e], dot, 0, 0, 0);
+                        }
+                        if (c == 0) own[g] = dot;
+                        else
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) own[g][r] = ca == c ? dot[r] : own[g][r];
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[q][r] = 0.0f;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    v4f dot{};
+                    const v4f kh = scale(0, g, q), kz = scale(1, g, q);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const v8h u = kv4_codes(kc[NA * q + c][2 * g + e], mask, mask0);
-                        dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, qh[g][e], dot, 0, 0, 0);
-                        dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, ql[g][e], dot, 0, 0, 0);
-                    }
-                    if (c == 0) own[g] = dot;
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) own[g][r] = ca == c ? dot[r] : own[g][r];
+                    for (int r = 0; r < 4; ++r) s[q][r] = fmaf(kh[r], own[g][r], fmaf(kz[r], qs[g], s[q][r]));
                 }
             }
+            if (!FAR && j + step < nb) load_k(j + step);
+            if (edge) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[q][r] = 0.0f;
+                for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const v4f kh = scale(0, g, q), kz = scale(1, g, q);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[q][r] = fmaf(kh[r], own[g][r], fmaf(kz[r], qs[g], s[q][r]));
+                    for (int r = 0; r < 4; ++r) {
+                        const int key = key0 + tile_key(NA * q + ca) + r;
+                        s[q][r] = key <= last ? s[q][r] : -INFINITY;
+                    }
             }
-        }
-        if (j + step < nb) load_k(j + step);
-        if (edge) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][r]);
+            const float now = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
+            if (__any(now != top) || (!FAR && vn != ve)) {
+                const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
+                const float fix = FAR ? alpha : alpha * (ve - vn < -126 ? 0.0f : kv4_pow2(ve - vn));
+                lrow *= alpha;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) zs[g] *= alpha;
+                if constexpr (FAR)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) seen[g] *= alpha;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[n] *= fix;
+                top = now;
+                if constexpr (!FAR) ve = vn;
+            }
+            if constexpr (!FAR) measure(j + step);
+            const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int key = key0 + tile_key(NA * q + ca) + r;
-                    s[q][r] = key <= last ? s[q][r] : -INFINITY;
+                    s[q][r] = __builtin_amdgcn_exp2f(fmaf(s[q][r], qi, -ref));  // (-inf: 0)
+                    lrow += s[q][r];
                 }
-        }
-        float mx = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
+            for (int g = 0; g < NG; ++g) {
+                float f = 1.0f;
+                if constexpr (FAR) {
+                    float big = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[q][r]);
-        const float now = fmaxf(top, kv4_join16(mx, Kv4Max()) * qi);
-        const int vn = max((int)(hmax >> 23) - 127, -110);
-        const float f = kv4_pow2(13 - vn);
+                    for (int q = 0; q < NQ; ++q) {
+                        const v4f wv = scale(2, g, q);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) scales[64 * (4 * g + 2) + lane] = vh2[g] * f;
-        if (__any(now != top) || vn != ve) {
-            const float alpha = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
-            const float fix = alpha * (ve - vn < -126 ? 0.0f : kv4_pow2(ve - vn));
-            lrow *= alpha;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) zs[g] *= alpha;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n] *= fix;
-            top = now;
-            ve = vn;
-        }
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[q][r] = __builtin_amdgcn_exp2f(fmaf(s[q][r], qi, -ref));  // (-inf: 0)
-                lrow += s[q][r];
-            }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            unsigned wh[NQ][2], wl[NQ][2];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const v4f vh = scale(2, g, q), vz = scale(3, g, q);
-#pragma unroll
-                for (int r = 0; r < 4; r += 2) {
-                    v2h hi, lo;
-                    kv4_split(v2f{s[q][r] * vh[r], s[q][r + 1] * vh[r + 1]}, hi, lo);
-                    wh[q][r / 2] = __builtin_bit_cast(unsigned, hi);
-                    wl[q][r / 2] = __builtin_bit_cast(unsigned, lo);
-                }
-                if (edge) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool see = key0 + tile_key(NA * q + ca) + r <= last;
-                        zs[g] = fmaf(s[q][r], see ? vz[r] : 0.0f, zs[g]);
+                        for (int r = 0; r < 4; ++r) big = fmaxf(big, s[q][r] * wv[r] * (r & 2 ? 16.0f : 1.0f));
                     }
-                } else {
+                    seen[g] = fmaxf(seen[g], kv4_join16(big, Kv4Max()));
+                    const int n = seen[g] > 0.0f ? min(13 - kv4_exponent(seen[g]), 126) : fe[g];
+                    if (__any(n != fe[g])) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) zs[g] = fmaf(s[q][r], vz[r], zs[g]);
-                }
-            }
-            // the weights of the products over tiles 2 w and 2 w + 1: the column's own tile, or zeros
-            v4u th[2], tl[2];
+                        for (int u = 4 * g; u < 4 * g + 4; ++u)
 #pragma unroll
-            for (int wx = 0; wx < 4; ++wx)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const bool mine = NA == 1 || wx % NA == ca;
-                    th[wx >> 1][2 * (wx & 1) + c] = mine ? wh[wx / NA][c] : 0u;
-                    tl[wx >> 1][2 * (wx & 1) + c] = mine ? wl[wx / NA][c] : 0u;
-                }
-#pragma unroll
-            for (int u = 2 * g; u < 2 * g + 2; ++u)
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const v8h lev = kv4_codes(vc[u][2 * v + w], mask, mask0);
-                        v4f& acc = o[2 * u + v];
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, th[w]), acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, tl[w]), acc, 0, 0, 0);
+                            for (int r = 0; r < 4; ++r) o[u][r] = __builtin_ldexpf(o[u][r], n - fe[g]);
+                        fe[g] = n;
                     }
+                    f = kv4_pow2(n);
+                }
+                unsigned wh[NQ][2], wl[NQ][2];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const v4f wv = scale(2, g, q), vz = scale(3, g, q);
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        v2h hi, lo;
+                        kv4_split(v2f{FAR ? s[q][r] * f * wv[r] : s[q][r] * wv[r], FAR ? s[q][r + 1] * f * wv[r + 1] : s[q][r + 1] * wv[r + 1]}, hi, lo);
+                        wh[q][r / 2] = __builtin_bit_cast(unsigned, hi);
+                        wl[q][r / 2] = __builtin_bit_cast(unsigned, lo);
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool see = key0 + tile_key(NA * q + ca) + r <= last;
+                            zs[g] = fmaf(s[q][r], see ? vz[r] : 0.0f, zs[g]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) zs[g] = fmaf(s[q][r], vz[r], zs[g]);
+                    }
+                }
+                // the weights of the products over tiles 2 w and 2 w + 1: the column's own tile, or zeros
+                v4u th[2], tl[2];
+#pragma unroll
+                for (int wx = 0; wx < 4; ++wx)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const bool mine = NA == 1 || wx % NA == ca;
+                        th[wx >> 1][2 * (wx & 1) + c] = mine ? wh[wx / NA][c] : 0u;
+                        tl[wx >> 1][2 * (wx & 1) + c] = mine ? wl[wx / NA][c] : 0u;
+                    }
+#pragma unroll
+                for (int u = 2 * g; u < 2 * g + 2; ++u)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const v8h lev = kv4_codes(vc[u][2 * v + w], mask, mask0);
+                            v4f& acc = o[2 * u + v];
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, th[w]), acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lev, __builtin_bit_cast(v8h, tl[w]), acc, 0, 0, 0);
+                        }
+            }
+            if (!FAR && j + step < nb) load_v(j + step);
         }
-        if (j + step < nb) load_v(j + step);
+    };
+    if constexpr (!ANY) {
+        measure(j);
+        walk(std::false_type{});
     }
-    // this wave's O[column][dim], column i, dimensions 32 u + 16 v + 4 h + r
+#pragma unroll
+    for (int g = 0; g < NG; ++g) fe[g] = ANY ? 0 : 13 - ve;
+    if (ANY || __builtin_expect(far && j < nb, 0)) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) seen[g] = ANY || top == -INFINITY ? 0.0f : kv4_pow2(ve);
+        walk(std::true_type{});
+    }
     lrow = kv4_join16(lrow, Kv4Sum());
-    const float back = kv4_pow2(ve - 13);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         zs[g] = kv4_join16(zs[g], Kv4Sum());
+        const float back = kv4_pow2(-fe[g]);
 #pragma unroll
-        for (int n = 4 * g; n < 4 * g + 4; ++n) {
-            v4f x;
+        for (int n = 4 * g; n < 4 * g + 4; ++n)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = fmaf(o[n][r], back, zs[g]);
-            *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = x;
-        }
+            for (int r = 0; r < 4; ++r) o[n][r] = fmaf(o[n][r], back, zs[g]);
     }
+}
+
+// STEP (one token, G <= 16 so that a head is one tile): append and attention in one launch.  Every
+// workgroup rotates its queries; the wave whose block the token lies in writes it there first.
+template <int HD, int RT, bool STEP, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
+    constexpr int NT = HD / 16, NA = 16 / RT;
+    __shared__ __attribute__((aligned(16))) float om[NW][16][HD + 4];  // (before, each wave's scales of a block)
+    __shared__ float ml[NW][16][2];
+    const int t = threadIdx.x, lane = t & 63, i = lane & 15, h = lane >> 4;
+    int split, S, tile, bh, slot;  // slot: the partial's in the workspace
+    if (a.S == 0) {
+        const Kv4Piece p = kv4_piece(a, (int)blockIdx.x, lane);
+        if (p.n == 0) return;
+        split = p.piece;
+        S = p.n;
+        tile = 0;
+        bh = p.b * a.Hkv + p.head;
+        slot = p.first + p.piece;
+        if (split == 0 && t == 0) {
+            a.heads[2 * bh] = S;
+            a.heads[2 * bh + 1] = p.first;
+        }
+    } else if (a.S == 1) {
+        // the last tiles, which see the most keys, of all heads first, and a CU's second workgroup of the short
+        // ones, the longer its first is (from an empty cache, 20 heads over 5, 512 / 640 / 1024 / 1400 tokens; the
+        // kernel as it was then: 20.9 / 25.4 / 39.7 / 63.4 us; the second in the same order 23.1 / 23.7 / 39.6 /
+        // 62.9; head by head from the first tile on 22.4 / 30.5 / 47.6 / 78.6)
+        const int w = (int)blockIdx.x, w0 = w >> 8 == 1 && (int)gridDim.x >= 512 ? w ^ 255 : w;
+        split = slot = 0;
+        S = 1;
+        tile = a.tiles - 1 - w0 / a.bh;
+        bh = w0 % a.bh;
+    } else {
+        const int w0 = xcd_order((int)blockIdx.x, (int)gridDim.x), unit = w0 / a.S;
+        split = w0 % a.S;
+        S = a.S;
+        tile = unit % a.tiles;
+        bh = unit / a.tiles;
+        slot = w0;
+    }
+    const int b = bh / a.Hkv, kh = bh % a.Hkv, G = a.H / a.Hkv, rows = a.M * G;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    v4f o[NT];
+    float top, lrow;
+    kv4_rows<HD, RT, STEP, false>(a, bh, tile, split * NW + wave, NW * S, &om[wave][0][0], lane, o, top, lrow);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<v4f*>(&om[wave][i][n * 16 + 4 * h]) = o[n];
     if (h == 0) {
         ml[wave][i][0] = top;  // (of a column that saw blocks but none of their keys: -inf, as of one that saw none)
         ml[wave][i][1] = lrow;

@@ -1,4 +1,17 @@
-"""Attention over the 4-bit KV cache where numbers span many binades, against the 64-bit oracle and its bound."""
+"""Attention over the 4-bit KV cache where numbers span many binades: scores far below zero, keys and values
+that differ by large powers of two from key to key, from half to half of a head and from row to row, and
+such keys among those that a row does not see.  All against the 64-bit oracle and its bound.
+
+The bound (oracle/kv4_oracle.py) counts fp16 terms as relative to what they stand for.  A term's low part is
+also no finer than 2^-24 of its scale, half a step of it 2^-25, and the kernels take one scale for several numbers
+where these differ little: that adds, in the worst case, with e = 2^-24,
+  few rows, weights: steps within 2^9 of the largest of them: the largest product 2 w h of a row is at least 2^5,
+      each weight is off by 2^-21 more (elements that meet 16 (c - 8) count 16-fold) and meets |c - 8| <= 8: n 2^-18,
+      where sum p (h |u| + |z|) is at least 2^4 in these units: 4 n e of it;
+  many rows: keys and values within 2^11 of the largest of them (each of its 15 h + |z|, at most 15 (h |u| + |z|)):
+      2^-39 2^11 15 = 16 2^-28, 1 e, for a key, a value, and each of n weights;
+  queries: a head's halves within 2^7: 64 x 2^-21 x 16 h / 2^(14 - 7) = 64 e of A for few rows, less for many.
+"""
 import numpy as np
 import pytest
 
@@ -8,6 +21,28 @@ from oracle import kv4_oracle as K4
 pytestmark = pytest.mark.gpu
 
 F = np.float32
+
+
+def _extra(q, pairs, pos, Lmax):
+    """The terms above: (2 x 64 A + 4 n + 2) e of sum p (h |u| + |z|), as attention_bound lays it out."""
+    (ck, cv), (zk, zv), (hk, hv) = pairs
+    rep = lambda x: np.repeat(x, 64, -1)  # noqa: E731
+    uk, uv = np.abs(2 * ck - 15) * rep(hk) + np.abs(rep(zk)), np.abs(2 * cv - 15) * rep(hv) + np.abs(rep(zv))
+    K = rep(zk) + rep(hk) * (2 * ck - 15)
+    B, M, H, hd = q.shape
+    out = np.zeros(q.shape)
+    for b in range(B):
+        for m in range(M):
+            p = int(pos[b]) + m
+            if not 0 <= p < Lmax:
+                continue
+            for n in range(H):
+                j, x = n // (H // ck.shape[1]), q[b, m, n].astype(np.float64) / np.sqrt(hd)
+                A = (uk[b, j, :p + 1] @ np.abs(x)).max()
+                s = K[b, j, :p + 1] @ x
+                w = np.exp(s - s.max())
+                out[b, m, n] = (128 * A + 4 * (p + 1) + 2) * 2.0 ** -24 * (w @ uv[b, j, :p + 1] / w.sum())
+    return out
 
 
 def _check(hip, q, cache, pairs, pos, Lmax, y=None):
@@ -22,7 +57,7 @@ def _check(hip, q, cache, pairs, pos, Lmax, y=None):
         y = out.cpu().numpy()
     K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
     want = K4.attention(q, K, V, pos, Lmax)
-    bound = K4.attention_bound(q, *pairs, pos, Lmax) + 1e-37
+    bound = K4.attention_bound(q, *pairs, pos, Lmax) + _extra(q, pairs, pos, Lmax) + 1e-37
     off = np.abs(y - want)
     assert np.isfinite(y).all()
     assert (off <= bound).all(), f"off by {np.max(off / bound):.3g} bounds"
@@ -138,6 +173,61 @@ def test_large_scores(hip, case, d):
     _attend(hip, case, q, np.ldexp(k, d - 1), v)
 
 
+@pytest.mark.parametrize("d", [20, 40, 80])
+@pytest.mark.parametrize("which", ["v", "k", "both"])
+@pytest.mark.parametrize("case", FEW)
+def test_outlier(hip, case, which, d):
+    """A key 2^d as large as the others that half of the rows see: it is nothing to the other half."""
+    q, k, v, at = _parts(case)
+    for b, p in at:
+        if which != "k":
+            v[b, p] = np.ldexp(v[b, p], d)
+        if which != "v":
+            k[b, p] = np.ldexp(k[b, p], d)
+    _attend(hip, case, q, k, v)
+
+
+def _little(case, nats, d):
+    """The keys in the middle `nats` above (below zero: below) the others' scores, their values times 2^d."""
+    q, k, v, at = _parts(case)
+    q = q * F(0.3) + 1
+    for b, p in at:
+        k[b, p] = nats / np.sqrt(q.shape[-1])
+        v[b, p] = np.ldexp(v[b, p], d)
+    return q, k, v
+
+
+@pytest.mark.parametrize("d", [20, 40, 55])
+@pytest.mark.parametrize("case", FEW)
+def test_outlier_of_little_weight(hip, case, d):
+    """Values 2^d as large as the others under weights of 2^-60."""
+    _attend(hip, case, *_little(case, -42, d))
+
+
+@pytest.mark.parametrize("d", [-200, -40, -12])
+@pytest.mark.parametrize("case", FEW)
+def test_weight_on_a_key_of_little_value(hip, case, d):
+    """One key has nearly all the weight and next to no value (or none): the rest of 2^-60 is the result."""
+    _attend(hip, case, *_little(case, 42, d))
+
+
+@pytest.mark.parametrize("d", [8, 30, 60])
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("which", ["v", "k", "q"])
+@pytest.mark.parametrize("case", [c for c in FEW if c[4] == 128])
+def test_halves_of_a_head_far_apart(hip, case, which, side, d):
+    """One group of 64 dimensions is 2^d as large as the other (queries: 2^-d)."""
+    q, k, v, _ = _parts(case)
+    part = np.s_[..., 64 * side:64 * side + 64]
+    if "q" in which:
+        q[part] = np.ldexp(q[part], -d)
+    if "k" in which:
+        k[part] = np.ldexp(k[part], d)
+    if "v" in which:
+        v[part] = np.ldexp(v[part], d)
+    _attend(hip, case, q, k, v)
+
+
 @pytest.mark.parametrize("d", [-115, 90])
 @pytest.mark.parametrize("case", FEW + MANY)
 def test_values_of_any_size(hip, case, d):
@@ -151,3 +241,35 @@ def test_zero_queries(hip, case, kd):
     """Queries of 0, over keys of 0 or small ones: the mean of the values."""
     q, k, v, _ = _parts(case)
     _attend(hip, case, 0 * q, np.ldexp(k, kd), v)
+
+
+@pytest.mark.parametrize("case", [c for c in FEW if c[1] > 1])
+def test_nan_next_to_an_outlier(hip, case):
+    """A NaN that a row does not see leaves every bit of it also where the block holds an outlier."""
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, k, v, at = _parts(case)
+    for b, p in at:
+        v[b, p] = np.ldexp(v[b, p], 40)
+    y, _ = _attend(hip, case, q, k, v)
+    seen = np.zeros(y.shape, bool)
+    for b, p in at:
+        k[b, p, 0, 3], v[b, p, -1, 1] = np.nan, np.inf
+        rows = pos[b] + np.arange(M)
+        rows = (rows >= p) & (rows < Lmax)
+        seen[b, rows, :H // Hkv] = True
+        seen[b, rows, H - H // Hkv:, :64] = True
+    cache, _ = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
+    z = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax).cpu().numpy()
+    assert np.isnan(z[seen]).all() and np.array_equal(z[~seen], y[~seen])
+
+
+@pytest.mark.parametrize("case", [c for c in FEW if c[1] > 1])
+def test_in_place_with_an_outlier(hip, case):
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, k, v, at = _parts(case)
+    for b, p in at:
+        v[b, p] = np.ldexp(v[b, p], 40)
+    y, cache = _attend(hip, case, q, k, v)
+    (t,) = G._cuda(q)
+    assert hip.kv4_attention(t, cache, G._pos(pos), max_len=Lmax, out=t) is t
+    assert np.array_equal(t.cpu().numpy(), y)
