@@ -378,6 +378,9 @@ __device__ __forceinline__ unsigned kv4_wave_max(unsigned x) {
 struct Kv4Max {
     __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
+struct Kv4Min {
+    __device__ float operator()(float a, float b) const { return fminf(a, b); }
+};
 struct Kv4Sum {
     __device__ float operator()(float a, float b) const { return a + b; }
 };
@@ -528,6 +531,7 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
 // instructions a block and more registers than there are: 512 / 1024 tokens from an empty cache, 20 heads
 // over 5, 20.2 / 40.4 us, so 17.6 / 34.9; 64 sequences of 4 tokens at 500 17.3, so 13.8).
+
 // A wave's part of a tile of RT rows: blocks j, j + step, .. of head bh.  Column i = lane % 16 (its row, over its key
 // tiles) leaves its sums o (dimensions 32 u + 16 v + 4 h + r of o[2 u + v][r]), its largest score and its sum of
 // weights.  scales: room for 4 HD floats of the wave's own.  ANY: steps may lie far apart from the first block on.
@@ -965,6 +969,10 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
 // with two products of three but asks the vector units for 18 operations a score instead of 9.
 // A NaN among the values (a group that reads as NaN) becomes 0 in LDS and is put into the sums of
 // the rows that see it afterwards: in a product it would reach every row.
+// A key's fp16 terms end at 2^-39 of the block's largest key, a value's at 2^-39 of the largest value so far, a weight's
+// at 2^-39 of 1.  That is below fp32's roundings where these (15 h + |z| of their groups, keys of 0 aside) lie within
+// 2^11 of each other.  A split whose keys or values do not, or are below 2^-97, whether its rows see them or not, goes
+// through the form for few rows, two tiles of 16 a wave, which scales by what a column sees.
 // The largest of a wave's upper and lower halves (unsigned, each for itself), in an SGPR.
 __device__ __forceinline__ unsigned kv4_wave_max2(unsigned x) {
     typedef unsigned short v2s __attribute__((ext_vector_type(2)));
@@ -983,10 +991,45 @@ __device__ __forceinline__ unsigned kv4_wave_max2(unsigned x) {
 
 constexpr int kKv4Tile = 256;
 
+// A tile of 256 rows in the form for few rows: two tiles of 16 a wave, over the same blocks.
+template <int HD>
+__device__ __forceinline__ void kv4_far_tile(Kv4AttnArgs a, int w0, int wave, int lane, float* scales) {
+    // (what follows from these is worked out here again, and not held through the loop for tiles whose numbers lie near)
+    asm("" : "+s"(a.H), "+s"(a.Hkv), "+s"(a.M), "+s"(w0), "+s"(wave), "+v"(lane));
+    const int split = w0 % a.S, unit = w0 / a.S, bh = unit % a.bh, tile = a.tiles - 1 - unit / a.bh;
+    const int G = a.H / a.Hkv, rows = a.M * G, i = lane & 15;
+    float* const part = a.work + ((size_t)((size_t)bh * a.tiles + tile) * a.S + split) * (kKv4Tile * (HD + 2));
+#pragma unroll 1
+    for (int sub = 2 * wave; sub < 2 * wave + 2; ++sub) {
+        const int tile16 = tile * (kKv4Tile / 16) + sub, R = tile16 * 16 + i;
+        if (tile16 * 16 >= rows) break;
+        v4f x[HD / 16];
+        float top, sum;
+        kv4_rows<HD, 16, false, true>(a, bh, tile16, split, a.S, scales, lane, x, top, sum);
+        if (R >= rows) continue;
+        float* dst = part + (sub * 16 + i) * HD;
+        float over = 1.0f;
+        if (a.S > 1) {
+            part[kKv4Tile * HD + 2 * (sub * 16 + i)] = top;
+            part[kKv4Tile * HD + 2 * (sub * 16 + i) + 1] = sum;
+        } else {
+            dst = a.out + (((size_t)(bh / a.Hkv) * a.M + R / G) * a.H + (size_t)(bh % a.Hkv) * G + R % G) * HD;
+            over = sum;
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[n][r] = sum == 0.0f ? 0.0f : x[n][r] / over;
+            *reinterpret_cast<v4f*>(dst + 16 * n + (lane >> 4) * 4) = x[n];
+        }
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a) {
     constexpr int NG = HD / 64, NU = HD / 32, OCT = HD / 8, TR = kKv4Tile;
     constexpr int PLANE = OCT * 64, BUF = 4 * PLANE;  // 16-byte units: K hi, K lo, V hi, V lo
+    __shared__ v2u span[8];  // of every eighth block, one wave's: `near`
     extern __shared__ __attribute__((aligned(16))) v8h lds_kv4[];  // two blocks of
     // keys [octet of dimensions][64] and values [4 w + 2 s + l][HD], hi then lo
     // the last tiles see the most keys: they go out first, of all heads
@@ -1122,6 +1165,35 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         load_ks();
         load_vs();
     }
+    // The largest 15 h + |z| of the keys (lower half) and values (upper half) of every eighth block, and the smallest's
+    // complement (keys of 0 aside), the upper halves of the fp32 bits.  (In the loop, block by block, the same took 2 %
+    // of the launch, however it was spread.)
+    float kmax = 0.0f, kmin = INFINITY, vmax = 0.0f, vmin = INFINITY;
+    for (int j0 = split + wave * a.S; j0 < nb; j0 += 32 * a.S) {
+        unsigned sc[4][2 * NG];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int g = 0; g < 2 * NG; ++g)
+                sc[c][g] = *reinterpret_cast<const unsigned*>(head + (size_t)min(j0 + 8 * c * a.S, nb - 1) * kv4_block_bytes(HD) + (at_s + 256 * g));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const bool in = min(j0 + 8 * c * a.S, nb - 1) * kKv4Block + lane < kend;
+#pragma unroll
+            for (int g = 0; g < 2 * NG; ++g) {
+                const float x = in ? fmaf(15.0f, kv4_h(sc[c][g]), fabsf(kv4_z(sc[c][g]))) : __builtin_nanf("");
+                if (g < NG) {
+                    kmax = fmaxf(kmax, x);
+                    kmin = x == 0.0f ? kmin : fminf(kmin, x);
+                } else {
+                    vmax = fmaxf(vmax, x);
+                    vmin = fminf(vmin, x);
+                }
+            }
+        }
+    }
+    const v2u near = {kv4_wave_max2(__float_as_uint(kmax) >> 16 | (__float_as_uint(vmax) & 0xFFFF0000u)),
+                      kv4_wave_max2(~(__float_as_uint(kmin) >> 16 | (__float_as_uint(vmin) & 0xFFFF0000u)))};
     // A wave's rows pass through its part of LDS, queries here and results at the end, so that memory is read
     // and written in whole lines (lane by lane, 32 rows at once, the launch took some 1000 cycles more): 16-byte unit c
     // of row r lies at unit c ^ (r % 16).  Coalesced, instruction n takes rows n RPI + lane / UPR, unit lane % UPR.
@@ -1270,7 +1342,17 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
     // The registers hold the keys' part of block j + S when block j is begun; its values' part follows.
     // Behind the last block the last one is loaded, and converted into a buffer that is not read.
     auto block_at = [&](int j) __attribute__((always_inline)) { return head + (size_t)min(j, nb - 1) * kv4_block_bytes(HD); };
+    if (lane == 0) span[wave] = near;
     __syncthreads();  // (the waves' parts for the queries are the first block's)
+    {
+        const v2u x = span[lane & 7];
+        const unsigned hi = kv4_wave_max2(x[0]), lo = ~kv4_wave_max2(x[1]);  // exponents of keys: bits 7.., of values: bits 23..
+        const int kn = hi >> 7 & 255u, kl = lo >> 7 & 255u, vn = hi >> 23 & 255u, vl = lo >> 23 & 255u;
+        if (__builtin_expect(kl < max(kn - 10, 30) || (vn != 0 && vl < max(vn - 10, 30)), 0)) {
+            kv4_far_tile<HD>(a, (int)blockIdx.x, wave, lane, reinterpret_cast<float*>(own));
+            return;
+        }
+    }
     if (split < nb) {
         cur = prepare(split, true);
         convert(lds_kv4);

@@ -45,6 +45,12 @@ def _extra(q, pairs, pos, Lmax):
     return out
 
 
+def _bounds(q, pairs, pos, Lmax):
+    """The result in 64 bits, and how far from it an element may be."""
+    K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
+    return K4.attention(q, K, V, pos, Lmax), K4.attention_bound(q, *pairs, pos, Lmax) + _extra(q, pairs, pos, Lmax) + 1e-37
+
+
 def _check(hip, q, cache, pairs, pos, Lmax, y=None):
     """Every element within the bound; the whole, row by row, within a quarter of it (roundings are as often up as
     down)."""
@@ -55,9 +61,7 @@ def _check(hip, q, cache, pairs, pos, Lmax, y=None):
         assert torch.isfinite(out).all()
         assert torch.equal(out, hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax))
         y = out.cpu().numpy()
-    K, V = ((z.repeat(64, -1) + h.repeat(64, -1) * (2 * c - 15)) for c, z, h in zip(*pairs))
-    want = K4.attention(q, K, V, pos, Lmax)
-    bound = K4.attention_bound(q, *pairs, pos, Lmax) + _extra(q, pairs, pos, Lmax) + 1e-37
+    want, bound = _bounds(q, pairs, pos, Lmax)
     off = np.abs(y - want)
     assert np.isfinite(y).all()
     assert (off <= bound).all(), f"off by {np.max(off / bound):.3g} bounds"
@@ -175,7 +179,7 @@ def test_large_scores(hip, case, d):
 
 @pytest.mark.parametrize("d", [20, 40, 80])
 @pytest.mark.parametrize("which", ["v", "k", "both"])
-@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("case", FEW + MANY)
 def test_outlier(hip, case, which, d):
     """A key 2^d as large as the others that half of the rows see: it is nothing to the other half."""
     q, k, v, at = _parts(case)
@@ -198,14 +202,14 @@ def _little(case, nats, d):
 
 
 @pytest.mark.parametrize("d", [20, 40, 55])
-@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("case", FEW + MANY)
 def test_outlier_of_little_weight(hip, case, d):
     """Values 2^d as large as the others under weights of 2^-60."""
     _attend(hip, case, *_little(case, -42, d))
 
 
 @pytest.mark.parametrize("d", [-200, -40, -12])
-@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("case", FEW + MANY)
 def test_weight_on_a_key_of_little_value(hip, case, d):
     """One key has nearly all the weight and next to no value (or none): the rest of 2^-60 is the result."""
     _attend(hip, case, *_little(case, 42, d))
@@ -214,7 +218,7 @@ def test_weight_on_a_key_of_little_value(hip, case, d):
 @pytest.mark.parametrize("d", [8, 30, 60])
 @pytest.mark.parametrize("side", [0, 1])
 @pytest.mark.parametrize("which", ["v", "k", "q"])
-@pytest.mark.parametrize("case", [c for c in FEW if c[4] == 128])
+@pytest.mark.parametrize("case", [c for c in FEW + MANY if c[4] == 128])
 def test_halves_of_a_head_far_apart(hip, case, which, side, d):
     """One group of 64 dimensions is 2^d as large as the other (queries: 2^-d)."""
     q, k, v, _ = _parts(case)
@@ -243,14 +247,16 @@ def test_zero_queries(hip, case, kd):
     _attend(hip, case, 0 * q, np.ldexp(k, kd), v)
 
 
-@pytest.mark.parametrize("case", [c for c in FEW if c[1] > 1])
+@pytest.mark.parametrize("case", [c for c in FEW + MANY if c[1] > 1])
 def test_nan_next_to_an_outlier(hip, case):
     """A NaN that a row does not see leaves every bit of it also where the block holds an outlier."""
     B, M, H, Hkv, hd, Lmax, pos, n = case
     q, k, v, at = _parts(case)
     for b, p in at:
         v[b, p] = np.ldexp(v[b, p], 40)
-    y, _ = _attend(hip, case, q, k, v)
+    y, cache = _attend(hip, case, q, k, v)
+    pairs = [K4.quantise(x.transpose(0, 2, 1, 3)) for x in (k, v)]
+    want, bound = _bounds(q, list(zip(*pairs)), pos, Lmax)
     seen = np.zeros(y.shape, bool)
     for b, p in at:
         k[b, p, 0, 3], v[b, p, -1, 1] = np.nan, np.inf
@@ -260,10 +266,16 @@ def test_nan_next_to_an_outlier(hip, case):
         seen[b, rows, H - H // Hkv:, :64] = True
     cache, _ = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
     z = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax).cpu().numpy()
-    assert np.isnan(z[seen]).all() and np.array_equal(z[~seen], y[~seen])
+    assert np.isnan(z[seen]).all()
+    if hd == 64:  # (the last head's NaN takes the outlier's place, and with it the reason for other terms)
+        last = np.s_[:, :, H - H // Hkv:]
+        far = np.abs(z[last] - want[last]) <= bound[last]
+        assert (far | seen[last]).all()
+        z[last] = y[last]
+    assert np.array_equal(z[~seen], y[~seen])
 
 
-@pytest.mark.parametrize("case", [c for c in FEW if c[1] > 1])
+@pytest.mark.parametrize("case", [c for c in FEW + MANY if c[1] > 1])
 def test_in_place_with_an_outlier(hip, case):
     B, M, H, Hkv, hd, Lmax, pos, n = case
     q, k, v, at = _parts(case)
