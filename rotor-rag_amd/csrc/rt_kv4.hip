@@ -525,7 +525,8 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // then has 2 w h f >= 2^6, and the second fp16 term ends at 2^-25).  From the first block on where they do not,
 // or where they are below 2^-80, every column and group of 64 dimensions takes an f of its own, by the largest
 // w h that the column has seen (FAR below; a key that it does not see has w = 0): one product a weight and one
-// maximum more, and no loads ahead.
+// maximum more, and no loads ahead.  So do waves with a row whose queries' halves differ by more than 2^7: a half's
+// largest is then brought into [2^14, 2^15) for itself.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
@@ -611,24 +612,38 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
         load_v(j);
     }
     if constexpr (STEP && RT != 16) kv4_rotate_query<HD>(qx, cs, h);
-    float qs[NG], qi;
+    float qs[NG], qi, qr[NG];
     v8h qh[NG][2], ql[NG][2];
+    bool far = ANY;
     {
-        float big = 0.0f;
+        float big[NG], most = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g) {
+            big[g] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     qx[g][e][c] *= a.scale;
-                    big = fmaxf(big, fabsf(qx[g][e][c]));
+                    big[g] = fmaxf(big[g], fabsf(qx[g][e][c]));
                 }
-        const int qe = kv4_query_power(kv4_join16(big, Kv4Max()));
-        const float qf = kv4_pow2(qe);
+            big[g] = kv4_join16(big[g], Kv4Max());
+            most = fmaxf(most, big[g]);
+        }
+        const int qe = kv4_query_power(most);
         qi = kv4_pow2(1 - qe);
+        // a group that is far smaller than the other has a power of two of its own, which FAR takes off its products
+        int dq[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
+            dq[g] = NG == 1 || big[g] == 0.0f || most == INFINITY ? 0 : min(kv4_query_power(big[g]) - qe, 126);
+            far = far || __any(dq[g] > 6);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (!far) dq[g] = 0;
+            const float qf = kv4_pow2(qe + dq[g]);
+            qr[g] = kv4_pow2(-dq[g]);
             qs[g] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
@@ -644,7 +659,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
                     qs[g] += x[c];
                 }
             }
-            qs[g] = kv4_join16(qs[g], Kv4Sum()) * 0.5f;
+            qs[g] = kv4_join16(qs[g], Kv4Sum()) * (0.5f * qr[g]);
         }
     }
     float zs[NG];
@@ -653,7 +668,6 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
     unsigned vmax = 0u;                      // 2^e's number, as bits
     float vmin = INFINITY;                   // the smallest step that the lane has met
     int ve = -110, vn = ve;                  // e of the sums, and with the next block
-    bool far = ANY;
     int fe[NG];                              // FAR: the columns' f = 2^fe, and
     float seen[NG];                          // the largest 2 w h
     // block j's values' scales, which are loaded: h and z + h as numbers (what lies behind the newest key is not read as
@@ -673,7 +687,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
         }
         vmax = max(vmax, kv4_wave_max(__float_as_uint(big)));
         vn = max((int)(vmax >> 23) - 127, -110);
-        far = __any(vmin < kv4_pow2(max(vn - 8, -80)));
+        far = far || __any(vmin < kv4_pow2(max(vn - 8, -80)));
     };
     // the block's scales as numbers: h and z + h of the keys, 2 h f and z + h of the values, [64 keys] each, by group
     const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
@@ -728,6 +742,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const v4f kh = scale(0, g, q), kz = scale(1, g, q);
+                    if constexpr (FAR && NG > 1) own[g] *= qr[g];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[q][r] = fmaf(kh[r], own[g][r], fmaf(kz[r], qs[g], s[q][r]));
                 }
@@ -971,8 +986,9 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
 // the rows that see it afterwards: in a product it would reach every row.
 // A key's fp16 terms end at 2^-39 of the block's largest key, a value's at 2^-39 of the largest value so far, a weight's
 // at 2^-39 of 1.  That is below fp32's roundings where these (15 h + |z| of their groups, keys of 0 aside) lie within
-// 2^11 of each other.  A split whose keys or values do not, or are below 2^-97, whether its rows see them or not, goes
-// through the form for few rows, two tiles of 16 a wave, which scales by what a column sees.
+// 2^11 of each other, and the halves of a row's queries within 2^7.  A split whose keys or values do not, or are below
+// 2^-97, whether its rows see them or not, goes through the form for few rows, two tiles of 16 a wave, which scales by
+// what a column sees.
 // The largest of a wave's upper and lower halves (unsigned, each for itself), in an SGPR.
 __device__ __forceinline__ unsigned kv4_wave_max2(unsigned x) {
     typedef unsigned short v2s __attribute__((ext_vector_type(2)));
@@ -1192,7 +1208,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
             }
         }
     }
-    const v2u near = {kv4_wave_max2(__float_as_uint(kmax) >> 16 | (__float_as_uint(vmax) & 0xFFFF0000u)),
+    v2u near = {kv4_wave_max2(__float_as_uint(kmax) >> 16 | (__float_as_uint(vmax) & 0xFFFF0000u)),
                       kv4_wave_max2(~(__float_as_uint(kmin) >> 16 | (__float_as_uint(vmin) & 0xFFFF0000u)))};
     // A wave's rows pass through its part of LDS, queries here and results at the end, so that memory is read
     // and written in whole lines (lane by lane, 32 rows at once, the launch took some 1000 cycles more): 16-byte unit c
@@ -1216,7 +1232,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
                 const int r = n * RPI + lane / UPR;
                 *in_lds(r, lane % UPR) = *reinterpret_cast<const v4f*>(a.q + row_at(r) + lane % UPR * 4);
             }
-        float qx[OCT / 2][8], big = 0.0f;
+        float qx[OCT / 2][8], big[NG] = {};
 #pragma unroll
         for (int s = 0; s < OCT / 2; ++s)
 #pragma unroll
@@ -1225,10 +1241,14 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     qx[s][4 * e + c] = x[c] * a.scale;
-                    big = fmaxf(big, fabsf(qx[s][4 * e + c]));
+                    big[s / 4] = fmaxf(big[s / 4], fabsf(qx[s][4 * e + c]));
                 }
             }
-        const int qe = kv4_query_power(kv4_join32(big, Kv4Max()));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) big[g] = kv4_join32(big[g], Kv4Max());
+        const int qe = kv4_query_power(fmaxf(big[0], big[NG - 1]));
+        if constexpr (NG == 2)  // (a half that is far smaller: kv4_far_tile)
+            if (R0 < rows && __any(fminf(big[0], big[1]) > 0.0f && fmaxf(big[0], big[1]) < INFINITY && abs(kv4_exponent(big[0]) - kv4_exponent(big[1])) > 6)) near[0] |= 0x8000u;
         const float qf = kv4_pow2(qe);
         qi = kv4_pow2(-qe);
 #pragma unroll
@@ -1348,7 +1368,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
         const v2u x = span[lane & 7];
         const unsigned hi = kv4_wave_max2(x[0]), lo = ~kv4_wave_max2(x[1]);  // exponents of keys: bits 7.., of values: bits 23..
         const int kn = hi >> 7 & 255u, kl = lo >> 7 & 255u, vn = hi >> 23 & 255u, vl = lo >> 23 & 255u;
-        if (__builtin_expect(kl < max(kn - 10, 30) || (vn != 0 && vl < max(vn - 10, 30)), 0)) {
+        if (__builtin_expect((hi & 0x8000u) != 0u || kl < max(kn - 10, 30) || (vn != 0 && vl < max(vn - 10, 30)), 0)) {
             kv4_far_tile<HD>(a, (int)blockIdx.x, wave, lane, reinterpret_cast<float*>(own));
             return;
         }

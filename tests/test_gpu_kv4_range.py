@@ -217,7 +217,7 @@ def test_weight_on_a_key_of_little_value(hip, case, d):
 
 @pytest.mark.parametrize("d", [8, 30, 60])
 @pytest.mark.parametrize("side", [0, 1])
-@pytest.mark.parametrize("which", ["v", "k", "q"])
+@pytest.mark.parametrize("which", ["v", "k", "q", "qk"])
 @pytest.mark.parametrize("case", [c for c in FEW + MANY if c[4] == 128])
 def test_halves_of_a_head_far_apart(hip, case, which, side, d):
     """One group of 64 dimensions is 2^d as large as the other (queries: 2^-d)."""
@@ -285,3 +285,16 @@ def test_in_place_with_an_outlier(hip, case):
     (t,) = G._cuda(q)
     assert hip.kv4_attention(t, cache, G._pos(pos), max_len=Lmax, out=t) is t
     assert np.array_equal(t.cpu().numpy(), y)
+
+
+@pytest.mark.parametrize("x", [np.nan, np.inf])
+@pytest.mark.parametrize("case", [c for c in FEW + MANY if c[4] == 128 and c[2] > c[3]])
+def test_query_that_is_no_number(hip, case, x):
+    """Its row is NaN, every other row keeps every bit."""
+    B, M, H, Hkv, hd, Lmax, pos, n = case
+    q, k, v, _ = _parts(case)
+    y, cache = _attend(hip, case, q, k, v)
+    q[0, M - 1, 1, 77] = x
+    y[0, M - 1, 1] = np.nan
+    z = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax).cpu().numpy()
+    assert np.array_equal(z, y, equal_nan=True)
