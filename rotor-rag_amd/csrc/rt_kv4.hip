@@ -375,6 +375,13 @@ __device__ __forceinline__ unsigned kv4_wave_max(unsigned x) {
     const v2u w = __builtin_amdgcn_permlane32_swap(x, x, false, false);
     return __builtin_amdgcn_readfirstlane(max(w[0], w[1]));
 }
+// What a wave's lanes wrote to LDS is there for its other lanes: LDS takes a wave's accesses in order, so this is for the
+// compiler, and no instruction.
+__device__ __forceinline__ void kv4_wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
 struct Kv4Max {
     __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
@@ -715,6 +722,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
                 scales[64 * (4 * g + 2) + lane] = vh[g] * (two * (FAR ? 1.0f : kv4_pow2(13 - vn)));
                 scales[64 * (4 * g + 3) + lane] = vzh[g];
             }
+            kv4_wave_lds();
             if (!FAR && j + step < nb) load_s(j + step);
             float s[NQ][4];
 #pragma unroll
@@ -853,6 +861,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
                         }
             }
             if (!FAR && j + step < nb) load_v(j + step);
+            kv4_wave_lds();  // (before the next block's scales)
         }
     };
     if constexpr (!ANY) {
@@ -1232,6 +1241,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
                 const int r = n * RPI + lane / UPR;
                 *in_lds(r, lane % UPR) = *reinterpret_cast<const v4f*>(a.q + row_at(r) + lane % UPR * 4);
             }
+        kv4_wave_lds();
         float qx[OCT / 2][8], big[NG] = {};
 #pragma unroll
         for (int s = 0; s < OCT / 2; ++s)
@@ -1432,6 +1442,7 @@ __global__ void __launch_bounds__(512, 2) kv4_prefill_kernel(const Kv4AttnArgs a
             for (int e = 0; e < 4; ++e) x[e] = o[u][r + e] * inv * back;
             *in_lds(c32, 8 * u + r / 2 + hl) = x;
         }
+    kv4_wave_lds();
 #pragma unroll
     for (int n = 0; n < 32 / RPI; ++n) {
         const int r = n * RPI + lane / UPR;
