@@ -538,12 +538,13 @@ class HIPTernaryOps:
     def kv4_cache(self, n_kv_heads: int, head_dim: int, max_len: int, batch: int = 1):
         """One layer's 4-bit KV cache for `batch` sequences of up to max_len positions: a uint8
         device tensor [batch, n_kv_heads, ceil(max_len / 64), 72 * head_dim] (its bytes are
-        opaque and need no initialisation)."""
+        opaque).  Positions that nothing was written to read as NaN: a row that attends past what
+        was appended is NaN, not a number from old memory."""
         if not self.lib.rt_kv4_bytes(int(batch), int(n_kv_heads), int(head_dim), int(max_len)):
             raise ValueError("kv4_cache: needs head_dim 64 or 128, batch * n_kv_heads <= 2^24, 1 <= max_len <= 2^20")
         torch = _torch()
-        return torch.empty((int(batch), int(n_kv_heads), (int(max_len) + 63) // 64, 72 * int(head_dim)),
-                           dtype=torch.uint8, device=self.device)
+        return torch.full((int(batch), int(n_kv_heads), (int(max_len) + 63) // 64, 18 * int(head_dim)), 0x7FC00000,
+                          dtype=torch.int32, device=self.device).view(torch.uint8)  # (a scale's z = NaN, h = 0)
 
     # A step of decoding is a few microseconds of GPU work, so these calls look at each tensor once, touch
     # nothing that is already as the library takes it, and compare devices by their numbers.
@@ -620,8 +621,9 @@ class HIPTernaryOps:
         positions pos[b] + m (rt_kv4_append); rope float32 [>= max_len, hd / 2, 2].  Returns the
         rotated q (q_out, which may be q).  max_len: the cache's positions, where they are fewer
         than its blocks hold (None: as many as the blocks and rope hold; kv4_read and
-        kv4_attention do not see rope, and take what the blocks hold).  Rows outside [0, max_len)
-        are not written; their q is 0.  For inference: gradients do not pass."""
+        kv4_attention do not see rope, and take what the blocks hold: pass max_len to all of them
+        where it is no multiple of 64).  Rows outside [0, max_len) are not written; their q is 0.
+        For inference: gradients do not pass."""
         torch = _torch()
         B, Hkv, hd, Lmax = self._kv4_check("kv4_append", torch, cache, pos, max_len)
         q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))

@@ -1,0 +1,36 @@
+"""Calls of the 4-bit KV cache that its documentation allows and that once went wrong."""
+import numpy as np
+import pytest
+
+import test_gpu_kv4 as G
+from oracle import kv4_oracle as K4
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("M", [1, 4, 70])
+def test_rows_past_the_angles(hip, M):
+    """A cache of 100 positions (blocks for 128), angles for 100, and no max_len: rows from 100 on are not appended,
+    and attention, which does not see the angles, gives NaN for them; the rows before are as with max_len."""
+    import torch
+
+    B, H, Hkv, hd, Lmax = 2, 4, 2, 128, 100
+    q, k, v = G._inputs(M, B, Lmax, H, Hkv, hd)
+    table = G._rope(Lmax, hd)
+    old = torch.full((B, Hkv, 2, 72 * hd), 0x3C, dtype=torch.uint8, device="cuda")  # memory that was used before
+    del old
+    cache = hip.kv4_cache(Hkv, hd, Lmax, batch=B)
+    (rope,) = G._cuda(table)
+    hip.kv4_append(*G._cuda(q, k, v), cache, rope, G._pos([0, 0]))
+    pos = G._pos([Lmax - (M + 1) // 2, Lmax])
+    new = [x[:, :M] for x in G._inputs(M + 1, B, M, H, Hkv, hd)]
+    rows = hip.kv4_append(*G._cuda(*new), cache, rope, pos)
+    y = hip.kv4_attention(rows, cache, pos)
+    n = (M + 1) // 2
+    for b, first in enumerate((Lmax - n, Lmax)):  # positions 100..127 are in the blocks, those behind in no cache
+        at = first + torch.arange(M)
+        assert torch.isnan(y[b, (at >= Lmax) & (at < 128)]).all() and (y[b, at >= 128] == 0).all()
+    want = hip.kv4_attention(rows, cache, pos, max_len=Lmax)
+    assert torch.isfinite(want).all() and torch.equal(y[0, :n], want[0, :n]) and (want[1] == 0).all()
+    for x in hip.kv4_read(cache, G._pos([0, 0]), 128):
+        assert torch.isfinite(x[:, :, :Lmax]).all() and torch.isnan(x[:, :, Lmax:]).all()

@@ -212,3 +212,12 @@ def test_python_refusals(ops):
             call()
     with pytest.raises(TypeError):
         ops.kv4_read(cache, pos, 2.5)
+
+
+def test_python_cache_is_nan_until_written(ops):
+    """Every group of a new cache reads as NaN by the definition: z NaN, h 0."""
+    for hd in (64, 128):
+        words = ops.kv4_cache(3, hd, 130, batch=2).numpy().view(np.uint32)
+        scales = words[..., 16 * hd:]
+        z, h = ((x << np.uint32(16)).view(np.float32) for x in (scales >> np.uint32(16), scales & np.uint32(0xFFFF)))
+        assert scales.size == 2 * 3 * 3 * 2 * hd and np.isnan(z).all() and (h == 0).all()
