@@ -721,8 +721,11 @@ class _DeviceModel:
 
 
 def config_from_hf(cfg: Dict) -> Dict:
-    """HF config.json -> the model config dict (src/rotor/bitnet_model.py:368-375)."""
+    """HF config.json -> the model config dict (src/rotor/bitnet_model.py:368-375); kv_cache_bits is
+    this build's own key and goes through where the file has it."""
+    own = {"kv_cache_bits": cfg["kv_cache_bits"]} if "kv_cache_bits" in cfg else {}
     return {
+        **own,
         "vocab_size": cfg["vocab_size"],
         "d_model": cfg["hidden_size"],
         "n_layers": cfg["num_hidden_layers"],
@@ -735,12 +738,16 @@ def config_from_hf(cfg: Dict) -> Dict:
     }
 
 
-def load_bitnet_model(model_dir: str, use_gpu: bool = False, kv_cache_bits: int = 32) -> BitNetModel:
+def load_bitnet_model(model_dir: str, use_gpu: bool = False, kv_cache_bits: Optional[int] = None) -> BitNetModel:
     """src/rotor/bitnet_model.py:349-394: config.json + model.safetensors -> BitNetModel.
-    kv_cache_bits 4 keeps the KV cache in 4 bits (a 7.1th of the memory)."""
+    kv_cache_bits 4 keeps the KV cache in 4 bits (a 7.1th of the memory), 32 in fp32; None: as
+    config.json's "kv_cache_bits" says, else in fp32."""
     model_dir = Path(model_dir)
     with open(model_dir / "config.json") as f:
         cfg = json.load(f)
-    model = BitNetModel(dict(config_from_hf(cfg), kv_cache_bits=kv_cache_bits), use_gpu=use_gpu)
+    config = config_from_hf(cfg)
+    if kv_cache_bits is not None:
+        config["kv_cache_bits"] = kv_cache_bits
+    model = BitNetModel(config, use_gpu=use_gpu)
     model.load_weights_from_safetensors(str(model_dir / "model.safetensors"))
     return model

@@ -34,3 +34,28 @@ def test_rows_past_the_angles(hip, M):
     assert torch.isfinite(want).all() and torch.equal(y[0, :n], want[0, :n]) and (want[1] == 0).all()
     for x in hip.kv4_read(cache, G._pos([0, 0]), 128):
         assert torch.isfinite(x[:, :, :Lmax]).all() and torch.isnan(x[:, :, Lmax:]).all()
+
+
+def test_config_file_chooses_the_cache(hip, tmp_path):
+    """config.json's kv_cache_bits holds unless load_bitnet_model is told otherwise."""
+    import json
+
+    import test_gpu_model as T
+    from oracle import rotor_oracle as O
+    from rotor import gpu_layers
+    from rotor.bitnet_model import load_bitnet_model
+
+    T._write_checkpoint(tmp_path, O.make_bitnet_params(6, T.SMALL, 96), T.SMALL, 96)
+    file = tmp_path / "config.json"
+    cfg = json.loads(file.read_text())
+    gpu_layers._gpu_instance = hip
+    try:
+        assert load_bitnet_model(str(tmp_path), use_gpu=True).kv_cache_bits == 32
+        file.write_text(json.dumps(dict(cfg, kv_cache_bits=4)))
+        assert load_bitnet_model(str(tmp_path), use_gpu=True).kv_cache_bits == 4
+        assert load_bitnet_model(str(tmp_path), use_gpu=True, kv_cache_bits=32).kv_cache_bits == 32
+        file.write_text(json.dumps(dict(cfg, kv_cache_bits=8)))
+        with pytest.raises(ValueError, match="kv_cache_bits"):
+            load_bitnet_model(str(tmp_path), use_gpu=True)
+    finally:
+        gpu_layers._gpu_instance = None

@@ -221,3 +221,11 @@ def test_python_cache_is_nan_until_written(ops):
         scales = words[..., 16 * hd:]
         z, h = ((x << np.uint32(16)).view(np.float32) for x in (scales >> np.uint32(16), scales & np.uint32(0xFFFF)))
         assert scales.size == 2 * 3 * 3 * 2 * hd and np.isnan(z).all() and (h == 0).all()
+
+
+def test_config_file_keeps_the_cache_bits():
+    from rotor.bitnet_model import config_from_hf
+
+    cfg = dict(vocab_size=64, hidden_size=256, num_hidden_layers=1, num_attention_heads=2, intermediate_size=256)
+    assert "kv_cache_bits" not in config_from_hf(cfg)
+    assert config_from_hf(dict(cfg, kv_cache_bits=4))["kv_cache_bits"] == 4
