@@ -628,7 +628,7 @@ class HIPTernaryOps:
         B, Hkv, hd, Lmax = self._kv4_check("kv4_append", torch, cache, pos, max_len)
         q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
         Lmax, M, H = self._kv4_new("kv4_append", q, k, v, rope, B, Hkv, hd, Lmax, max_len)
-        out = self._kv4_out("kv4_append", torch, q_out, q, k, v, rope, cache)
+        out = self._kv4_out("kv4_append", torch, q_out, q, k, v, rope, cache, pos)
         self._kv4_run(torch, "rt_kv4_append", self.lib.rt_kv4_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
                       cache.data_ptr(), out.data_ptr(), B, M, H, Hkv, hd, Lmax, pos.data_ptr())
         return out
@@ -642,7 +642,7 @@ class HIPTernaryOps:
         Lmax, M, H = self._kv4_new("kv4_step", q, k, v, rope, B, Hkv, hd, Lmax, max_len)
         if M != 1 or H > 16 * Hkv:
             raise ValueError("kv4_step: takes one token a sequence, and H / Hkv <= 16")
-        out = self._kv4_out("kv4_step", torch, out, q, k, v, rope, cache)
+        out = self._kv4_out("kv4_step", torch, out, q, k, v, rope, cache, pos)
         need, ws = self._kv4_workspace(torch, B, 1, H, Hkv, hd, Lmax)
         self._kv4_run(torch, "rt_kv4_step", self.lib.rt_kv4_step, q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(),
                       cache.data_ptr(), out.data_ptr(), B, H, Hkv, hd, Lmax, pos.data_ptr(),
@@ -671,7 +671,7 @@ class HIPTernaryOps:
         B, Hkv, hd, Lmax = self._kv4_check("kv4_attention", torch, cache, pos, max_len)
         q = self._kv4_in(torch, q)
         M, H = self._kv4_rows("kv4_attention", q, B, Hkv, hd)
-        out = self._kv4_out("kv4_attention", torch, out, q, cache)
+        out = self._kv4_out("kv4_attention", torch, out, q, cache, pos)
         need, ws = self._kv4_workspace(torch, B, M, H, Hkv, hd, Lmax)
         self._kv4_run(torch, "rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
                       Hkv, hd, Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need)

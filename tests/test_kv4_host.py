@@ -229,3 +229,16 @@ def test_config_file_keeps_the_cache_bits():
     cfg = dict(vocab_size=64, hidden_size=256, num_hidden_layers=1, num_attention_heads=2, intermediate_size=256)
     assert "kv_cache_bits" not in config_from_hf(cfg)
     assert config_from_hf(dict(cfg, kv_cache_bits=4))["kv_cache_bits"] == 4
+
+
+def test_python_outputs_in_the_positions_memory(ops):
+    """An output over pos would move the rows of the workgroups that come later."""
+    import torch
+
+    out = torch.zeros(2, 1, 2, 64)
+    pos = out.view(torch.int32).view(-1)[64:66]
+    cache, rope, kv = ops.kv4_cache(2, 64, 64, batch=2), torch.zeros(64, 32, 2), torch.zeros(2, 1, 2, 64)
+    for call in (lambda: ops.kv4_append(kv, kv, kv, cache, rope, pos, q_out=out), lambda: ops.kv4_attention(kv, cache, pos, out=out),
+                 lambda: ops.kv4_step(kv, kv, kv, cache, rope, pos, out=out), lambda: ops.kv4_attention(out, cache, pos, out=out)):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
