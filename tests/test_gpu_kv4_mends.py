@@ -59,3 +59,34 @@ def test_config_file_chooses_the_cache(hip, tmp_path):
             load_bitnet_model(str(tmp_path), use_gpu=True)
     finally:
         gpu_layers._gpu_instance = None
+
+
+def test_model_past_65536_positions(hip):
+    """A sequence that runs past the 65536 positions of the fp32 cache: the last layer's attention over it, for nine
+    tokens and for one, against 64 bits over the values that the cache holds."""
+    import test_gpu_model as T
+    from oracle import rotor_oracle as O
+
+    cfg = T.SMALL
+    model = T._device_model(hip, O.make_bitnet_params(77, cfg, 192), dict(cfg, kv_cache_bits=4), 70000)
+    H, n, hd = cfg["n_heads"], cfg["n_layers"], cfg["d_model"] // cfg["n_heads"]
+    ids = np.random.default_rng(1).integers(0, cfg["vocab_size"], 65531).astype(np.int32)
+    cache = None
+    for at in range(0, len(ids), 512):
+        _, cache = model.forward(ids[at:at + 512], past_kv_cache=cache, use_cache=True, return_logits=False)
+    table = model._dev.rope.cpu().numpy().reshape(-1, hd // 2, 2)
+    for M in (9, 1):
+        model._dev.trace = {}
+        _, cache = model.forward(ids[:M], past_kv_cache=cache, use_cache=True)
+        trace, model._dev.trace = model._dev.trace, None
+        q = model._dev._state(M)["q"].cpu().numpy().reshape(1, M, H, hd)
+        if M == 1:  # (rotated in the attention's launch and not kept)
+            q = K4.rope(q, table, np.array([[cache.length - 1]]))
+            got = trace["steps"][0]["attn"][n - 1].cpu().numpy()
+        else:
+            got = trace["attn"][n - 1].cpu().numpy()
+        c = cache[n - 1]
+        want = K4.attention(q, c["k"], c["v"], [cache.length - M])
+        # (fp32 sums of 65540 numbers of random signs: below 2^-24 sqrt(2 x 65540) = 2.2e-5 of the result's own order)
+        assert np.linalg.norm(got.reshape(want.shape) - want) <= 2.2e-5 * np.linalg.norm(want)
+    assert cache.length == 65541
