@@ -56,7 +56,7 @@ __device__ __forceinline__ float kv4_h(unsigned s) { return __uint_as_float(s <<
 // z and h of a group from its extremes, as the cache's dword.  By definition in 64 bits up to the
 // roundings, so that nothing hangs on the order of fp32 operations.  z in fp32 is the same number; h
 // in fp32 is within 2^-22 of it, so its bf16 is the same unless it lies next to a border: those (one
-// group in 4000) and very small ones take the division.  A group with a value that is not finite, or
+// group in 2000) and very small ones take the division.  A group with a value that is not finite, or
 // whose z or h is not, reads as NaN.
 __device__ __forceinline__ unsigned kv4_scale(float lo, float hi, bool finite) {
     float fz = 0.5f * hi + 0.5f * lo, fh = (0.5f * hi - 0.5f * lo) * (1.0f / 15.0f);
