@@ -298,3 +298,30 @@ def test_query_that_is_no_number(hip, case, x):
     y[0, M - 1, 1] = np.nan
     z = hip.kv4_attention(*G._cuda(q), cache, G._pos(pos), max_len=Lmax).cpu().numpy()
     assert np.array_equal(z, y, equal_nan=True)
+
+
+@pytest.mark.parametrize("which", ["v", "k", "q"])
+def test_tiles_of_256_rows_without_splits(hip, which):
+    """A batch that fills the GPU: no join, results straight from the tiles, in place too; three sequences of 129
+    against the oracle."""
+    B, M, H, Hkv, hd, Lmax, n = 129, 64, 8, 2, 128, 600, 100
+    assert hip.lib.rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax) == 0
+    pos = [(b * 7) % 37 for b in range(B)]
+    case = (B, M, H, Hkv, hd, Lmax, pos, n)
+    q, k, v, at = _parts(case)
+    for b, p in at[::2]:
+        if which == "v":
+            v[b, p] = np.ldexp(v[b, p], 40)
+        elif which == "k":
+            k[b, p] = np.ldexp(k[b, p], 40)
+        else:
+            q[b, 5, :, 64:] = np.ldexp(q[b, 5, :, 64:], -30)
+            k[b, :, :, 64:] = np.ldexp(k[b, :, :, 64:], 30)
+    cache, pairs = G._filled(hip, 0, B, H, Hkv, hd, Lmax, n, k=k, v=v)
+    (t,) = G._cuda(q)
+    y = hip.kv4_attention(t, cache, G._pos(pos), max_len=Lmax)
+    assert hip.kv4_attention(t, cache, G._pos(pos), max_len=Lmax, out=t) is t
+    assert np.array_equal(t.cpu().numpy(), y.cpu().numpy())
+    for b in (0, 64, 65, 128):
+        sub = [tuple(x[b:b + 1] for x in p) for p in pairs]
+        _check(hip, q[b:b + 1], None, sub, pos[b:b + 1], Lmax, y=y[b:b + 1].cpu().numpy())
