@@ -362,9 +362,11 @@ int rt_rope_attention_decode(rt_ctx* ctx, const float* q, const float* k, const 
  *   c = clamp(rint(((x - z) / h + 15) / 2), 0, 15) in 64 bits; (x - z) / h is 0 where h = 0.
  * A group that holds a value that is not finite, or whose z or h is not, reads as NaN.
  * rt_kv4_attention and rt_kv4_step take keys and values up to 2^96 in magnitude (their
- * intermediate sums are fp32); append and read take every fp32 number.
+ * intermediate sums are fp32, and a weight below 2^-126 of its row's largest counts as none);
+ * append and read take every fp32 number.
  * The bytes are opaque; fresh memory needs no initialisation as long as a call reads or attends
- * to written positions only (a row at p to all of 0..p); dwords of 0x7FC00000 read as NaN.  Buffers are 16-byte aligned, pos 4-byte aligned.
+ * to written positions only (a row at p to all of 0..p); dwords of 0x7FC00000 read as NaN.
+ * Buffers are 16-byte aligned, pos 4-byte aligned.
  * B * Hkv <= 2^24, H / Hkv <= 1024, 1 <= M <= Lmax <= 2^20; the same Lmax goes to every call
  * on a cache. */
 

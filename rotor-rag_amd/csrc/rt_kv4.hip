@@ -532,13 +532,14 @@ __device__ __forceinline__ void kv4_rotate_query(v4f (&qx)[HD / 64][4], const v4
 // then has 2 w h f >= 2^6, and the second fp16 term ends at 2^-25).  From the first block on where they do not,
 // or where they are below 2^-80, every column and group of 64 dimensions takes an f of its own, by the largest
 // w h that the column has seen (FAR below; a key that it does not see has w = 0): one product a weight and one
-// maximum more, and no loads ahead.  So do waves with a row whose queries' halves differ by more than 2^7: a half's
+// maximum more, and no loads ahead (in every block: 131072 keys, 20 heads over 5, 30.2 us, so 31.5; 512 tokens from an
+// empty cache 18.1 / 19.2).  So do waves with a row whose queries' halves differ by more than 2^7: a half's
 // largest is then brought into [2^14, 2^15) for itself.
 // Every load is issued half a round before its use: the keys of the next block when those of this
 // one are multiplied, its values after this one's.  A block's scales are made numbers once, a key a lane,
 // and read from LDS by the lanes that use them (each for itself, tiles of 16 rows took 1000 vector
 // instructions a block and more registers than there are: 512 / 1024 tokens from an empty cache, 20 heads
-// over 5, 20.2 / 40.4 us, so 17.6 / 34.9; 64 sequences of 4 tokens at 500 17.3, so 13.8).
+// over 5, 20.2 / 40.4 us, so 17.6 / 34.9, with f as above 17.9 / 35; 64 sequences of 4 tokens at 500 17.3, so 13.8).
 
 // A wave's part of a tile of RT rows: blocks j, j + step, .. of head bh.  Column i = lane % 16 (its row, over its key
 // tiles) leaves its sums o (dimensions 32 u + 16 v + 4 h + r of o[2 u + v][r]), its largest score and its sum of
@@ -997,7 +998,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv4_attn_kernel(const Kv4AttnArgs 
 // at 2^-39 of 1.  That is below fp32's roundings where these (15 h + |z| of their groups, keys of 0 aside) lie within
 // 2^11 of each other, and the halves of a row's queries within 2^7.  A split whose keys or values do not, or are below
 // 2^-97, whether its rows see them or not, goes through the form for few rows, two tiles of 16 a wave, which scales by
-// what a column sees.
+// what a column sees (2048 of 8192 tokens 603 us instead of 400).
 // The largest of a wave's upper and lower halves (unsigned, each for itself), in an SGPR.
 __device__ __forceinline__ unsigned kv4_wave_max2(unsigned x) {
     typedef unsigned short v2s __attribute__((ext_vector_type(2)));
