@@ -620,56 +620,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
         load_v(j);
     }
     if constexpr (STEP && RT != 16) kv4_rotate_query<HD>(qx, cs, h);
-    float qs[NG], qi, qr[NG];
-    v8h qh[NG][2], ql[NG][2];
     bool far = ANY;
-    {
-        float big[NG], most = 0.0f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            big[g] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    qx[g][e][c] *= a.scale;
-                    big[g] = fmaxf(big[g], fabsf(qx[g][e][c]));
-                }
-            big[g] = kv4_join16(big[g], Kv4Max());
-            most = fmaxf(most, big[g]);
-        }
-        const int qe = kv4_query_power(most);
-        qi = kv4_pow2(1 - qe);
-        // a group that is far smaller than the other has a power of two of its own, which FAR takes off its products
-        int dq[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            dq[g] = NG == 1 || big[g] == 0.0f || most == INFINITY ? 0 : min(kv4_query_power(big[g]) - qe, 126);
-            far = far || __any(dq[g] > 6);
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (!far) dq[g] = 0;
-            const float qf = kv4_pow2(qe + dq[g]);
-            qr[g] = kv4_pow2(-dq[g]);
-            qs[g] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                // (every other pair meets codes that are 16 times as large)
-                const v2f x = {qx[g][e / 4][e % 4] * qf, qx[g][e / 4][e % 4 + 1] * qf};
-                const float part = e & 2 ? 0.0625f : 1.0f;
-                v2h hi, lo;
-                kv4_split(x * part, hi, lo);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    qh[g][e / 8][e % 8 + c] = hi[c];
-                    ql[g][e / 8][e % 8 + c] = lo[c];
-                    qs[g] += x[c];
-                }
-            }
-            qs[g] = kv4_join16(qs[g], Kv4Sum()) * (0.5f * qr[g]);
-        }
-    }
     float zs[NG];
     top = -INFINITY;
     lrow = 0.0f;
@@ -695,8 +646,60 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
         }
         vmax = max(vmax, kv4_wave_max(__float_as_uint(big)));
         vn = max((int)(vmax >> 23) - 127, -110);
-        far = far || __any(vmin < kv4_pow2(max(vn - 8, -80)));
+        far |= __any(vmin < kv4_pow2(max(vn - 8, -80))) != 0;
     };
+    if constexpr (!ANY) measure(j);
+    float qs[NG], qi, qr[NG];
+    v8h qh[NG][2], ql[NG][2];
+    {
+        float big[NG], most = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            big[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    qx[g][e][c] *= a.scale;
+                    big[g] = fmaxf(big[g], fabsf(qx[g][e][c]));
+                }
+            big[g] = kv4_join16(big[g], Kv4Max());
+            most = fmaxf(most, big[g]);
+        }
+        const int qe = kv4_query_power(most);
+        qi = kv4_pow2(1 - qe);
+        // a group that is far smaller than the other has a power of two of its own, which FAR takes off its products
+        int dq[NG];
+        bool apart = false;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            dq[g] = (int)(NG > 1) & (int)(big[g] > 0.0f) & (int)(most < INFINITY) ? min(kv4_query_power(big[g]) - qe, 126) : 0;
+            apart |= __any(dq[g] > 6) != 0;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            dq[g] = apart ? dq[g] : 0;
+            const float qf = kv4_pow2(qe + dq[g]);
+            qr[g] = kv4_pow2(-dq[g]);
+            qs[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                // (every other pair meets codes that are 16 times as large)
+                const v2f x = {qx[g][e / 4][e % 4] * qf, qx[g][e / 4][e % 4 + 1] * qf};
+                const float part = e & 2 ? 0.0625f : 1.0f;
+                v2h hi, lo;
+                kv4_split(x * part, hi, lo);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    qh[g][e / 8][e % 8 + c] = hi[c];
+                    ql[g][e / 8][e % 8 + c] = lo[c];
+                    qs[g] += x[c];
+                }
+            }
+            qs[g] = kv4_join16(qs[g], Kv4Sum()) * (0.5f * qr[g]);
+        }
+        far |= apart;
+    }
     // the block's scales as numbers: h and z + h of the keys, 2 h f and z + h of the values, [64 keys] each, by group
     const v4f* const own_scales = reinterpret_cast<const v4f*>(scales + tile_key(ca) + kl);
     auto scale = [&](int kind, int g, int q) { return own_scales[(64 * (4 * g + kind) + tile_key(NA * q)) / 4]; };
@@ -865,10 +868,7 @@ __device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int bh, int tile,
             kv4_wave_lds();  // (before the next block's scales)
         }
     };
-    if constexpr (!ANY) {
-        measure(j);
-        walk(std::false_type{});
-    }
+    if constexpr (!ANY) walk(std::false_type{});
 #pragma unroll
     for (int g = 0; g < NG; ++g) fe[g] = ANY ? 0 : 13 - ve;
     if (ANY || __builtin_expect(far && j < nb, 0)) {
