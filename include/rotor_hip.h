@@ -73,8 +73,8 @@ const char* rt_last_error(void);
  * 106 = 105 without rt_plan_set_row_stats and RT_SRC_RMSNORM_STATS (measured slower than each
  * decode prologue reducing its own row), + rt_attention_decode_combine,
  * rt_plan_attention_combine and rt_lm_head_argmax's next_h; 107 = 106 + rt_plan_set_output_ssq;
- * 108 = 107 + rt_plan_create_act_gate_up; the rt_kv4_* calls came to 108 later and change none
- * of its others. */
+ * 108 = 107 + rt_plan_create_act_gate_up; the rt_kv4_* and the rt_paged_* calls came to 108 later
+ * and change none of its others. */
 int rt_version(void);
 
 /* Number of visible HIP devices (0 when none); RT_OK even when 0. */
@@ -403,6 +403,73 @@ int rt_kv4_attention(rt_ctx* ctx, const float* q, const void* cache, float* out,
  * workspace: rt_kv4_attention_workspace(B, 1, ...) bytes. */
 int rt_kv4_step(rt_ctx* ctx, const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
                 int B, int H, int Hkv, int hd, int Lmax, const int* pos, void* workspace, size_t workspace_bytes);
+
+/* ---- KV cache in pages -------------------------------------------------------------
+ * One layer's keys and values for B sequences that take memory a page at a time (the reference's
+ * lists grow by copying, src/rotor/bitnet_model.py:223-228): [K, V][pages][Hkv][page][hd] in fp32, bf16
+ * or fp16; head_dim 64 or 128, page 16, 32, 64, 128 or 256 slots.  Slot t of sequence b is row t % page
+ * of page table[b][t / page]; sequence b holds lens[b] slots.  Sequences may share pages that no call writes
+ * to.  A table entry outside [0, pages) is a hole: its slots are not there (nothing is written to them, nothing is
+ * read or kept of them).  Table and lens are device memory that a call reads when it runs.
+ * cache is 16-byte aligned and so are both strides; a page's [Hkv][page][hd] is contiguous.
+ * fp16 keys and values past 65519 in magnitude become infinite.  Rows are for finite numbers: a query, or a
+ * key or value that is attended to, that is not finite leaves NaN or infinities in its heads' outputs.
+ * B * Hkv <= 2^24, H / Hkv <= 1024, P * page <= 2^20. */
+#define RT_PAGED_F32 0
+#define RT_PAGED_BF16 1
+#define RT_PAGED_F16 2
+typedef struct rt_pages {
+    void* cache;            /* the first page's keys                                        */
+    long long kv_stride;    /* elements from a page's keys to its values                    */
+    long long page_stride;  /* elements from a page to the next                             */
+    const int* table;       /* int32 [B][P] (device)                                        */
+    const int* lens;        /* int32 [B] (device): slots held, before the call's new tokens */
+    int type, pages, Hkv, page, hd, B, P;
+} rt_pages;
+/* New tokens: sequence b's token m stands at position pos[b] + m, its angles are row pos[b] + m of rope
+ * (fp32 [rope_rows][rotary / 2][2] = (cos, sin), which may be scaled for long contexts), and its place is slot
+ * lens[b] + m.  The first `rotary` dimensions of a head are rotated (a multiple of 8, up to hd), the others stay; pairs
+ * are (i, i + rotary / 2), or (2 i, 2 i + 1) where interleaved != 0.  A token with m >= counts[b] (counts NULL: none), or without
+ * an angle or a place, is not written, and its outputs are zeros.  Angles are applied in 64 bits, rounded once to
+ * fp32; keys and values are then rounded to the cache's type (nearest, ties to even). */
+typedef struct rt_paged_new {
+    const float* q;   /* fp32 [B][M][H][hd]   */
+    const float* k;   /* fp32 [B][M][Hkv][hd] */
+    const float* v;   /* fp32 [B][M][Hkv][hd] */
+    const float* rope;
+    const int* pos;     /* int32 [B] (device)                                  */
+    const int* counts;  /* int32 [B] (device) or NULL; rt_paged_step: NULL     */
+    int rope_rows, rotary, interleaved, M, H;
+} rt_paged_new;
+
+/* The rotated queries into q_out [B][M][H][hd] (which may be n->q), keys and values into the cache
+ * (src/rotor/transformer.py:250-252).  No place may be written by two tokens of a call. */
+int rt_paged_append(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float* q_out);
+
+/* Attention of one token a sequence: out [B][H][hd] of q [B][H][hd] (rotated, as rt_paged_append leaves them) over
+ * slots 0 .. lens[b] - 1, scale 1 / sqrt(hd), GQA (src/rotor/transformer.py:260-281); out may be q.  A sequence
+ * without slots gets zeros.  weights (may be NULL) fp32 [B][Hkv][weight_slots], weight_slots >= P * page:
+ * every slot's softmax weights of the KV head's query heads are added to it, in a fixed order (slots not attended to
+ * are left alone).  workspace: rt_paged_attention_workspace bytes of device memory, 16-byte aligned, possibly 0,
+ * no initialisation; calls that may run at the same time need workspaces of their own. */
+size_t rt_paged_attention_workspace(const rt_pages* c, int H, int weights);
+int rt_paged_attention(rt_ctx* ctx, const rt_pages* c, const float* q, int H, float* weights, int weight_slots, float* out,
+                       void* workspace, size_t workspace_bytes);
+
+/* rt_paged_append of one token a sequence (M = 1) and rt_paged_attention over the lens[b] + 1 slots that are then
+ * held, in one launch (one more where splits are joined or weights kept), with the same numbers in the cache; the rotated q is not
+ * kept.  A token without an angle or a place attends to nothing.  out may be n->q. */
+int rt_paged_step(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float* weights, int weight_slots, float* out,
+                  void* workspace, size_t workspace_bytes);
+
+/* Cuts every sequence to `keep` slots: for each KV head the last `recent` (<= keep) slots and, of those before
+ * them, the ones with the largest weights fp32 [B][Hkv][weight_slots] (ties: the lowest slot; NaN counts as the largest), in
+ * their order.  kept int32 [B][Hkv][keep]: the slots, -1 behind the last; new_lens int32 [B]: how many (all
+ * that are there where those are no more than keep; the same for every head); new_weights, shaped as weights: theirs, zeros
+ * behind them.  Their keys and values are copied to the pages of new_table int32 [B][new_P], new_P * page >= keep, none of
+ * which may be a page that `table` holds or another sequence's new one.  The old pages stay as they were. */
+int rt_paged_evict(rt_ctx* ctx, const rt_pages* c, const float* weights, int weight_slots, int keep, int recent,
+                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights);
 
 /* Final RMSNorm of x fp32 [D] with norm_w, tied bf16 LM head logits [V]
  * (src/rotor/bitnet_model.py:231-235) and greedy argmax (src/rotor/generation.py:42;

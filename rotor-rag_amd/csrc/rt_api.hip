@@ -8,6 +8,7 @@
 
 #include <cstdio>
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
@@ -91,6 +92,7 @@ struct Scratch {
 // the module load until the process ends.  In host code `scratch` is only a stand-in
 // symbol, not a device address: the address is resolved per device with
 // hipGetSymbolAddress (device current) and only that pointer is used.
+static_assert(kPagedF32 == RT_PAGED_F32 && kPagedBf16 == RT_PAGED_BF16 && kPagedF16 == RT_PAGED_F16, "types");
 static_assert(RT_NOALLOC_SCRATCH_BYTES % 256 == 0, "scratch size");
 static __device__ __align__(256) unsigned char scratch[RT_NOALLOC_SCRATCH_BYTES];
 
@@ -1291,6 +1293,133 @@ int rt_kv4_step(rt_ctx* ctx, const float* q, const float* k, const float* v, con
     DeviceGuard g(ctx->device);
     RT_HIP(launch_kv4_step(q, k, v, rope, cache, out, B, H, Hkv, hd, Lmax, pos, static_cast<float*>(workspace),
                            ctx->stream));
+    return RT_OK;
+}
+
+// --- KV cache in pages --------------------------------------------------------------------
+
+// A call's cache, checked; false with the message set otherwise.
+static bool paged_check(const rt_pages* p, int H, PagedCache& c, const char* who) {
+    auto no = [&](const char* what) {
+        fail(RT_EINVAL, std::string(who) + what);
+        return false;
+    };
+    if (!p || !p->cache || !p->table || !p->lens) return no(": NULL argument");
+    const int shift = p->page > 0 ? __builtin_ctz((unsigned)p->page) : 0;
+    if (p->type < RT_PAGED_F32 || p->type > RT_PAGED_F16 || (p->hd != 64 && p->hd != 128) || p->page < 16 || p->page > 256 ||
+        p->page != 1 << shift || p->pages <= 0 || p->B <= 0 || p->Hkv <= 0 || (long long)p->B * p->Hkv > (1 << 24) || p->P <= 0 ||
+        (long long)p->P * p->page > (1 << 20) || H <= 0 || H % p->Hkv || H / p->Hkv > 1024)
+        return no(": unsupported layout (fp32, bf16 or fp16; head_dim 64 or 128; page 16, 32, 64, 128 or 256; H % Hkv == 0, H / Hkv <= "
+                  "1024, B * Hkv <= 2^24, P * page <= 2^20)");
+    const long long size = p->type == RT_PAGED_F32 ? 4 : 2, rows = (long long)p->Hkv * p->page * p->hd;
+    const long long most = LLONG_MAX / 16 / ((long long)p->pages + 1);
+    if (p->page_stride < rows || p->page_stride > most || p->kv_stride < rows || p->kv_stride > LLONG_MAX / 16)
+        return no(": a page does not fit its stride");
+    // a page's keys and values must not lie in another's: values behind all keys, or each page's behind its keys
+    if (p->pages > 1 && p->kv_stride < (p->pages - 1) * p->page_stride + rows && p->page_stride < p->kv_stride + rows)
+        return no(": pages overlap");
+    if ((reinterpret_cast<uintptr_t>(p->cache) & 15u) || p->page_stride * size % 16 || p->kv_stride * size % 16)
+        return no(": buffers must be 16-byte aligned");
+    c = PagedCache{p->cache, p->kv_stride, p->page_stride, p->table, p->lens, p->B, p->P, p->Hkv, p->pages, shift};
+    return true;
+}
+
+static bool paged_check_new(const rt_paged_new* n, PagedNew& out, int hd, const char* who) {
+    auto no = [&](const char* what) {
+        fail(RT_EINVAL, std::string(who) + what);
+        return false;
+    };
+    if (!n || !n->q || !n->k || !n->v || !n->rope || !n->pos) return no(": NULL argument");
+    if (n->M <= 0 || n->M > (1 << 20)) return no(": M out of range");
+    if (n->rotary <= 0 || n->rotary > hd || n->rotary % 8 || n->rope_rows <= 0)
+        return no(": rotary must be a multiple of 8 up to head_dim, with angles");
+    for (const float* x : {n->q, n->k, n->v, n->rope})
+        if (reinterpret_cast<uintptr_t>(x) & 15u) return no(": buffers must be 16-byte aligned");
+    out = PagedNew{n->q, n->k, n->v, n->rope, n->pos, n->counts, n->rope_rows, n->rotary, n->interleaved != 0};
+    return true;
+}
+
+int rt_paged_append(rt_ctx* ctx, const rt_pages* p, const rt_paged_new* n, float* q_out) {
+    PagedCache c;
+    PagedNew in;
+    if (!ctx || !n || !q_out) return fail(RT_EINVAL, "rt_paged_append: NULL argument");
+    if (!paged_check(p, n->H, c, "rt_paged_append") || !paged_check_new(n, in, p->hd, "rt_paged_append")) return RT_EINVAL;
+    if (reinterpret_cast<uintptr_t>(q_out) & 15u) return fail(RT_EINVAL, "rt_paged_append: buffers must be 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_paged_append(c, in, q_out, n->M, n->H, p->type, p->hd, ctx->stream));
+    return RT_OK;
+}
+
+size_t rt_paged_attention_workspace(const rt_pages* p, int H, int weights) {
+    PagedCache c;
+    if (!paged_check(p, H, c, "rt_paged_attention_workspace")) return 0;
+    return paged_attention_workspace(c.B, H, c.Hkv, c.P << c.shift, p->type, p->hd, weights != 0);
+}
+
+static int paged_attend(rt_ctx* ctx, const rt_pages* p, PagedAttn& a, bool step, void* workspace, size_t bytes, const char* who) {
+    const PagedCache& c = a.c;
+    if (reinterpret_cast<uintptr_t>(a.q) & 15u || reinterpret_cast<uintptr_t>(a.out) & 15u)
+        return fail(RT_EINVAL, std::string(who) + ": buffers must be 16-byte aligned");
+    if (a.weights && a.slots < c.P << c.shift)
+        return fail(RT_EINVAL, std::string(who) + ": weights must have a place for each of P * page slots");
+    const size_t need = paged_attention_workspace(c.B, a.H, c.Hkv, c.P << c.shift, p->type, p->hd, a.weights != nullptr);
+    if (need && (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(RT_EINVAL, std::string(who) + ": workspace too small (rt_paged_attention_workspace) or not 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_paged_attention(a, step, p->type, p->hd, workspace, ctx->stream));
+    return RT_OK;
+}
+
+int rt_paged_attention(rt_ctx* ctx, const rt_pages* p, const float* q, int H, float* weights, int weight_slots, float* out,
+                       void* workspace, size_t workspace_bytes) {
+    PagedAttn a{};
+    if (!ctx || !q || !out) return fail(RT_EINVAL, "rt_paged_attention: NULL argument");
+    if (!paged_check(p, H, a.c, "rt_paged_attention")) return RT_EINVAL;
+    a.q = q;
+    a.out = out;
+    a.weights = weights;
+    a.slots = weight_slots;
+    a.H = H;
+    return paged_attend(ctx, p, a, false, workspace, workspace_bytes, "rt_paged_attention");
+}
+
+int rt_paged_step(rt_ctx* ctx, const rt_pages* p, const rt_paged_new* n, float* weights, int weight_slots, float* out,
+                  void* workspace, size_t workspace_bytes) {
+    PagedAttn a{};
+    if (!ctx || !n || !out) return fail(RT_EINVAL, "rt_paged_step: NULL argument");
+    if (!paged_check(p, n->H, a.c, "rt_paged_step") || !paged_check_new(n, a.n, p->hd, "rt_paged_step")) return RT_EINVAL;
+    if (n->M != 1 || n->counts) return fail(RT_EINVAL, "rt_paged_step: takes one token a sequence (M = 1, counts NULL)");
+    a.q = n->q;
+    a.out = out;
+    a.weights = weights;
+    a.slots = weight_slots;
+    a.H = n->H;
+    return paged_attend(ctx, p, a, true, workspace, workspace_bytes, "rt_paged_step");
+}
+
+int rt_paged_evict(rt_ctx* ctx, const rt_pages* p, const float* weights, int weight_slots, int keep, int recent,
+                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights) {
+    PagedEvict a{};
+    if (!ctx || !weights || !new_table || !kept || !new_lens || !new_weights) return fail(RT_EINVAL, "rt_paged_evict: NULL argument");
+    if (!paged_check(p, p ? p->Hkv : 0, a.c, "rt_paged_evict")) return RT_EINVAL;
+    if (keep <= 0 || recent < 0 || recent > keep || new_P <= 0 || (long long)new_P * p->page > (1 << 20) ||
+        keep > (long long)new_P * p->page)
+        return fail(RT_EINVAL, "rt_paged_evict: needs 0 <= recent <= keep, 0 < keep <= new_P * page <= 2^20");
+    if (weight_slots < a.c.P << a.c.shift)
+        return fail(RT_EINVAL, "rt_paged_evict: weights must have a place for each of P * page slots");
+    if (weights == new_weights || new_table == p->table || new_lens == p->lens)
+        return fail(RT_EINVAL, "rt_paged_evict: needs other memory for its outputs, and a table of other pages");
+    a.weights = weights;
+    a.new_weights = new_weights;
+    a.new_table = new_table;
+    a.kept = kept;
+    a.new_lens = new_lens;
+    a.new_P = new_P;
+    a.slots = weight_slots;
+    a.keep = keep;
+    a.recent = recent;
+    DeviceGuard g(ctx->device);
+    RT_HIP(launch_paged_evict(a, p->type, p->hd, ctx->stream));
     return RT_OK;
 }
 

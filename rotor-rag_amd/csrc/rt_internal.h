@@ -434,6 +434,42 @@ hipError_t launch_kv4_attention(const float* q, const void* cache, float* out, i
                                 int Lmax, const int* pos, float* work, hipStream_t s);
 hipError_t launch_kv4_step(const float* q, const float* k, const float* v, const float* rope, void* cache, float* out,
                            int B, int H, int Hkv, int hd, int Lmax, const int* pos, float* work, hipStream_t s);
+// KV cache in pages (rt_paged.hip).  RT_PAGED_*
+enum PagedType { kPagedF32 = 0, kPagedBf16 = 1, kPagedF16 = 2 };
+struct PagedCache {
+    void* cache;
+    long long kv_stride, page_stride;  // elements
+    const int *table, *lens;           // [B][P], [B]
+    int B, P, Hkv, pages, shift;       // slots of a page: 1 << shift
+};
+struct PagedNew {  // new tokens: q [B][M][H][hd], k and v [B][M][Hkv][hd]
+    const float *q, *k, *v, *rope;
+    const int *pos, *counts;  // counts may be null
+    int rope_rows, rotary;
+    bool interleaved;
+};
+struct PagedAttn {
+    PagedCache c;
+    PagedNew n;  // a step's
+    const float* q;
+    float *out, *weights, *part, *ml, *scores;  // weights, scores: null where they are not kept
+    int slots;                                  // a row of weights
+    int H, G, tiles, S, least;                  // G = H / Hkv, in tiles of 16; S splits of at least so many tiles of slots
+    float scale;                                // log2(e) / sqrt(hd)
+};
+struct PagedEvict {
+    PagedCache c;
+    const float* weights;
+    float* new_weights;
+    const int* new_table;
+    int *kept, *new_lens;
+    int new_P, slots, keep, recent;
+};
+hipError_t launch_paged_append(const PagedCache& c, const PagedNew& n, float* q_out, int M, int H, int type, int hd,
+                               hipStream_t s);
+size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int hd, bool weights);
+hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void* work, hipStream_t s);
+hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, hipStream_t s);
 hipError_t launch_lm_head(const uint16_t* E, const float* x, const float* norm_w, float eps, int V, int D,
                           float* logits, unsigned long long* best, int* token, int* pos, int advance,
                           int* next_ids, int* out_tokens, int pos_base, int out_cap, float* next_h, hipStream_t s);

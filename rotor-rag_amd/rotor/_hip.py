@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "librotor_hip.so"
@@ -22,6 +23,12 @@ class RtSrc(ctypes.Structure):
     _fields_ = [("mode", ctypes.c_int), ("x", ctypes.c_void_p), ("aux", ctypes.c_void_p), ("aux2", ctypes.c_void_p),
                 ("eps", ctypes.c_float), ("attn_head_dim", ctypes.c_int), ("attn_max_len", ctypes.c_int)]
 
+
+# rt_pages and rt_paged_new, as bytes in their layout (a call fills them at once, which costs less than a
+# ctypes structure's fields one by one)
+PAGES = struct.Struct("PqqPP7i4x")
+PAGED_NEW = struct.Struct("6P5i4x")
+PAGED_F32, PAGED_BF16, PAGED_F16 = 0, 1, 2
 
 SRC_QUANT, SRC_RMSNORM, SRC_RELU2MUL, SRC_RELU2MUL_NORM, SRC_ATTN_NORM, SRC_RMSNORM_SSQ = 0, 2, 3, 4, 5, 6
 LAUNCH_GEMV, LAUNCH_GEMV_FUSED, LAUNCH_SPLITK, LAUNCH_TILES = 0, 1, 2, 3
@@ -87,6 +94,11 @@ SIGNATURES = {
     "rt_kv4_attention_workspace": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I]),
     "rt_kv4_attention": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, ctypes.c_size_t]),
     "rt_kv4_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, ctypes.c_size_t]),
+    "rt_paged_append": (_I, [_P, _P, _P, _P]),
+    "rt_paged_attention_workspace": (ctypes.c_size_t, [_P, _I, _I]),
+    "rt_paged_attention": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, ctypes.c_size_t]),
+    "rt_paged_step": (_I, [_P, _P, _P, _P, _I, _P, _P, ctypes.c_size_t]),
+    "rt_paged_evict": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P]),
     "rt_lm_head_argmax": (_I, [_P, _P, _P, _P, _F, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P]),
 }
 

@@ -7,7 +7,7 @@ forward surface (src/rotor/bitnet_model.py):
 
 Checkpoint: ``model_dir/config.json`` (HF keys vocab_size, hidden_size,
 num_hidden_layers, num_attention_heads, num_key_value_heads, intermediate_size; optional
-rope_theta, rms_norm_eps, max_position_embeddings) and ``model_dir/model.safetensors`` with
+rope_theta, rope_scaling, rms_norm_eps, max_position_embeddings) and ``model_dir/model.safetensors`` with
 the tensor names the reference reads (src/rotor/bitnet_model.py:100-188): ternary weights
 as rotor/BitNet bytes ``[out, in/4]`` uint8 with a per-tensor ``weight_scale`` that
 multiplies (the reference's convention, :179-188), bf16/fp32 norms and a bf16 embedding
@@ -44,12 +44,42 @@ _SWITCHES = ("attn_in_prologue", "ffn_pair", "attn_in_qkv", "attn_combine_in_qkv
 _STAGE_BYTES = 8 << 20  # one of a model's two pinned staging buffers
 
 
-def rope_table(max_len: int, head_dim: int, theta: float) -> np.ndarray:
-    """(cos, sin) of pos * theta^(-2i/head_dim), [max_len, head_dim/2, 2] fp32 (computed in f64)."""
-    i = np.arange(head_dim // 2, dtype=np.float64)
-    inv = theta ** (-(2.0 * i) / head_dim)
+def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict] = None) -> np.ndarray:
+    """(cos, sin) of pos * theta^(-2i/head_dim), [max_len, head_dim/2, 2] fp32 (computed in f64); head_dim:
+    the dimensions that are rotated.  scaling, for contexts longer than the trained one, as in a config.json's
+    "rope_scaling": {"rope_type": ..., "factor": f, ...} with rope_type
+      linear  every frequency / f (position interpolation)
+      ntk     theta * f^(d / (d - 2)): the lowest frequency / f, the highest as it is
+      yarn    frequencies of more than beta_fast (32) turns in original_max_position_embeddings as they are, of fewer
+              than beta_slow (1) / f, between them mixed, and (cos, sin) times attention_factor (0.1 ln f + 1)"""
+    d = head_dim
+    i = np.arange(d // 2, dtype=np.float64)
+    inv, grow = theta ** (-(2.0 * i) / d), 1.0
+    if scaling:
+        kind, f = scaling.get("rope_type", scaling.get("type")), float(scaling.get("factor", 1.0))
+        if not (np.isfinite(f) and f > 0):
+            raise ValueError(f"rope_scaling: factor {f}")
+        if kind == "linear":
+            inv = inv / f
+        elif kind == "ntk":
+            if d <= 2:
+                raise ValueError("rope_scaling: ntk needs more than one pair")
+            inv = (theta * f ** (d / (d - 2.0))) ** (-(2.0 * i) / d)
+        elif kind == "yarn":
+            if "original_max_position_embeddings" not in scaling:
+                raise ValueError("rope_scaling: yarn needs original_max_position_embeddings")
+            n = float(scaling["original_max_position_embeddings"])
+            at = lambda turns: d * np.log(n / (turns * 2 * np.pi)) / (2 * np.log(theta))  # noqa: E731  (that pair's number)
+            first = max(np.floor(at(float(scaling.get("beta_fast", 32)))), 0)
+            last = min(np.ceil(at(float(scaling.get("beta_slow", 1)))), d - 1)
+            slow = np.clip((i - first) / max(last - first, 0.001), 0, 1)
+            inv = inv / f * slow + inv * (1 - slow)
+            grow = scaling.get("attention_factor")
+            grow = float(grow) if grow is not None else 0.1 * np.log(f) + 1 if f > 1 else 1.0
+        elif kind != "default":
+            raise ValueError(f"rope_scaling: rope_type {kind!r}: linear, ntk, yarn or default")
     ang = np.arange(max_len, dtype=np.float64)[:, None] * inv[None, :]
-    return np.stack([np.cos(ang), np.sin(ang)], axis=-1).astype(np.float32)
+    return (np.stack([np.cos(ang), np.sin(ang)], axis=-1) * grow).astype(np.float32)
 
 
 class KVCache:
@@ -104,6 +134,7 @@ class BitNetModel:
         self.d_ff = config.get("d_ff", 6912)
         self.head_dim = self.d_model // self.n_heads
         self.rope_theta = float(config.get("rope_theta", 500000.0))
+        self.rope_scaling = config.get("rope_scaling")  # None, or rope_table's scaling
         self.eps = float(config.get("rms_norm_eps", 1e-6))
         self.max_seq_len = int(config.get("max_seq_len", 2048))
         self.max_tokens = int(config.get("max_batch_tokens", 512))
@@ -257,7 +288,7 @@ class _DeviceModel:
             self.layers.append(d)
         self.emb = emb.to(dev)
         self.final_norm = final_norm.to(dev)
-        self.rope = torch.from_numpy(rope_table(self.Lmax, hd, model.rope_theta)).to(dev)
+        self.rope = torch.from_numpy(rope_table(self.Lmax, hd, model.rope_theta, model.rope_scaling)).to(dev)
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self.ids = torch.zeros(max(self.Lmax, 1), dtype=torch.int32, device=dev)
         self.token = torch.zeros(1, dtype=torch.int32, device=dev)
@@ -721,11 +752,13 @@ class _DeviceModel:
 
 
 def config_from_hf(cfg: Dict) -> Dict:
-    """HF config.json -> the model config dict (src/rotor/bitnet_model.py:368-375); kv_cache_bits is
-    this build's own key and goes through where the file has it."""
+    """HF config.json -> the model config dict (src/rotor/bitnet_model.py:368-375); kv_cache_bits (this build's
+    own key) and rope_scaling go through where the file has them."""
     own = {"kv_cache_bits": cfg["kv_cache_bits"]} if "kv_cache_bits" in cfg else {}
+    scaled = {"rope_scaling": cfg["rope_scaling"]} if cfg.get("rope_scaling") else {}
     return {
         **own,
+        **scaled,
         "vocab_size": cfg["vocab_size"],
         "d_model": cfg["hidden_size"],
         "n_layers": cfg["num_hidden_layers"],

@@ -38,6 +38,18 @@ def _kv4_workspace_bytes(B, M, H, Hkv, hd, Lmax):
     return _hip.load().rt_kv4_attention_workspace(B, M, H, Hkv, hd, Lmax)
 
 
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace_bytes(kind, Hkv, page, hd, B, P, H, weights):
+    rows = Hkv * page * hd
+    return _hip.load().rt_paged_attention_workspace(_hip.PAGES.pack(16, rows, rows, 16, 16, kind, 1, Hkv, page, hd, B, P), H, weights)
+
+
+@functools.lru_cache(maxsize=1)
+def _paged_types():
+    torch = _torch()
+    return {torch.float32: _hip.PAGED_F32, torch.bfloat16: _hip.PAGED_BF16, torch.float16: _hip.PAGED_F16}
+
+
 class DeviceTernaryWeights:
     """A device-resident ternary matrix (opaque ``rt_weights`` handle)."""
 
@@ -676,6 +688,165 @@ class HIPTernaryOps:
         self._kv4_run(torch, "rt_kv4_attention", self.lib.rt_kv4_attention, q.data_ptr(), cache.data_ptr(), out.data_ptr(), B, M, H,
                       Hkv, hd, Lmax, pos.data_ptr(), ws.data_ptr() if need else None, need)
         return out
+
+    # -- KV cache in pages (rt_paged_*) --------------------------------------------
+    def paged_cache(self, n_kv_heads: int, head_dim: int, n_pages: int, page: int = 64, dtype=None):
+        """One layer's paged KV cache: a tensor [2 (keys, values), n_pages, n_kv_heads, page, head_dim] of
+        torch.bfloat16 (default), float16 or float32.  Which sequence has which pages is the caller's: calls take a
+        table int32 [B, P] of page numbers and lens int32 [B], the slots that each sequence holds.  Slots
+        that nothing was written to read as NaN.  Any tensor of this form does (a layer of a
+        larger one too: the two outer dimensions may have any strides)."""
+        torch = _torch()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        if dtype not in _paged_types() or head_dim not in (64, 128) or page not in (16, 32, 64, 128, 256) or n_kv_heads < 1 or n_pages < 1:
+            raise ValueError("paged_cache: needs head_dim 64 or 128, page 16, 32, 64, 128 or 256, bfloat16, float16 or float32")
+        return torch.full((2, int(n_pages), int(n_kv_heads), page, head_dim), float("nan"), dtype=dtype, device=self.device)
+
+    def _paged_ints(self, who, torch, name, x, shape):
+        if x.dtype is not torch.int32 or x.shape != shape or x.get_device() != self.device_index or not x.is_contiguous():
+            raise ValueError(f"{who}: {name} must be a contiguous int32 {list(shape)} tensor on the backend's device")
+
+    def _paged_check(self, who, torch, cache, table, lens):
+        """(rt_pages, (type, Hkv, page, hd, B, P), bytes that the cache's pages span) of a cache, its table and lengths."""
+        shape, strides, kind = cache.shape, cache.stride(), _paged_types().get(cache.dtype)
+        if kind is None or len(shape) != 5 or shape[0] != 2 or cache.get_device() != self.device_index:
+            raise ValueError(f"{who}: cache must be a bfloat16, float16 or float32 [2, pages, Hkv, page, head_dim] tensor on the "
+                             "backend's device (paged_cache)")
+        _, pages, Hkv, page, hd = shape
+        rows = Hkv * page * hd
+        if strides[4] != 1 or strides[3] != hd or (strides[2] != page * hd and Hkv > 1):
+            raise ValueError(f"{who}: a page's [Hkv, page, head_dim] must be contiguous")
+        if len(table.shape) != 2:
+            raise ValueError(f"{who}: table must be int32 [B, P]")
+        B, P = table.shape
+        self._paged_ints(who, torch, "table", table, (B, P))
+        self._paged_ints(who, torch, "lens", lens, (B,))
+        step = strides[1] if pages > 1 else rows
+        span = (strides[0] + (pages - 1) * step + rows) * cache.element_size()
+        return (_hip.PAGES.pack(cache.data_ptr(), strides[0], step, table.data_ptr(), lens.data_ptr(), kind, pages, Hkv, page, hd, B, P),
+                (kind, Hkv, page, hd, B, P), span)
+
+    def _paged_new(self, who, torch, q, k, v, rope, pos, counts, interleaved, sizes):
+        """(rt_paged_new, the tensors it names) of new tokens."""
+        _, Hkv, _, hd, B, _ = sizes
+        q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
+        M, H = self._kv4_rows(who, q, B, Hkv, hd)
+        if k.shape != (B, M, Hkv, hd) or v.shape != (B, M, Hkv, hd):
+            raise ValueError(f"{who}: k and v must be {[B, M, Hkv, hd]}")
+        table = rope.shape
+        if len(table) != 3 or table[2] != 2 or table[1] % 4 or not 0 < 2 * table[1] <= hd or not table[0]:
+            raise ValueError(f"{who}: rope must be [positions, rotary / 2, 2], rotary a multiple of 8 up to head_dim")
+        self._paged_ints(who, torch, "pos", pos, (B,))
+        if counts is not None:
+            self._paged_ints(who, torch, "counts", counts, (B,))
+        new = _hip.PAGED_NEW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), pos.data_ptr(),
+                                  counts.data_ptr() if counts is not None else 0, table[0], 2 * table[1], bool(interleaved), M, H)
+        return new, (q, k, v, rope, pos, *(() if counts is None else (counts,)))
+
+    def _paged_apart(self, who, name, x, cache, span, *others):
+        """x, which the call writes, lies in none of the others."""
+        at = x.data_ptr()
+        end = at + x.numel() * x.element_size()
+        first = cache.data_ptr()
+        if first < end and at < first + span:
+            raise ValueError(f"{who}: {name} must not share memory with the cache")
+        for y in others:
+            first = y.data_ptr()
+            if first < end and at < first + y.numel() * y.element_size():
+                raise ValueError(f"{who}: {name} must not share memory with the other arguments")
+
+    def _paged_weights(self, who, torch, weights, sizes):
+        """The slots of a row of accumulated weights."""
+        _, Hkv, page, _, B, P = sizes
+        shape = weights.shape
+        if (weights.dtype is not torch.float32 or len(shape) != 3 or shape[0] != B or shape[1] != Hkv or shape[2] < P * page
+                or not weights.is_contiguous() or weights.get_device() != self.device_index):
+            raise ValueError(f"{who}: weights must be a contiguous float32 [{B}, {Hkv}, >= {P * page}] tensor on the backend's device")
+        return shape[2]
+
+    def paged_append(self, q, k, v, cache, table, lens, rope, pos, counts=None, interleaved: bool = False, q_out=None):
+        """RoPE of q [B, M, H, hd] and k [B, M, Hkv, hd], then k and v into the paged cache at slots lens[b] + m
+        (rt_paged_append).  Token m stands at position pos[b] + m (which runs ahead of the slots once a
+        cache was cut); rope float32 [positions, rotary / 2, 2] (rope_table) turns a head's first `rotary` dimensions: pairs (i,
+        i + rotary / 2), or (2 i, 2 i + 1) with interleaved.  counts int32 [B]: a sequence's tokens where they are
+        fewer than M.  Returns the rotated q (q_out, which may be q).  Tokens past counts, without a row of rope or without a
+        slot are not written; their q is 0.  lens is not changed.  For inference: gradients do not pass."""
+        torch = _torch()
+        pages, sizes, span = self._paged_check("paged_append", torch, cache, table, lens)
+        new, kept = self._paged_new("paged_append", torch, q, k, v, rope, pos, counts, interleaved, sizes)
+        out = self._kv4_out("paged_append", torch, q_out, *kept, table, lens)
+        if q_out is not None:
+            self._paged_apart("paged_append", "q_out", out, cache, span)
+        self._kv4_run(torch, "rt_paged_append", self.lib.rt_paged_append, pages, new, out.data_ptr())
+        return out
+
+    def paged_attention(self, q, cache, table, lens, weights=None, out=None):
+        """Attention of one token a sequence, q [B, 1, H, hd] (rotated, as paged_append returns it), over the lens[b] slots
+        of a paged cache (rt_paged_attention): float32 [B, 1, H, hd] (out, which may be q); zeros for a sequence
+        without slots.  weights float32 [B, Hkv, slots]: what every slot weighed (the softmax's weights, summed over a KV head's
+        query heads) is added to it, for paged_evict.  For inference: gradients do not pass."""
+        torch = _torch()
+        pages, sizes, span = self._paged_check("paged_attention", torch, cache, table, lens)
+        q = self._kv4_in(torch, q)
+        M, H = self._kv4_rows("paged_attention", q, sizes[4], sizes[1], sizes[3])
+        if M != 1:
+            raise ValueError("paged_attention: takes one token a sequence")
+        out = self._paged_attend("paged_attention", torch, out, q, cache, span, sizes, H, weights, (table, lens),
+                                 lambda *a: (self.lib.rt_paged_attention, pages, q.data_ptr(), H, *a))
+        return out
+
+    def paged_step(self, q, k, v, cache, table, lens, rope, pos, interleaved: bool = False, weights=None, out=None):
+        """A decoding step (q [B, 1, H, hd], k and v [B, 1, Hkv, hd]): paged_append, then paged_attention of its q over the
+        lens[b] + 1 slots there are then, in one call (rt_paged_step).  A token without a row of rope or without a slot
+        attends to nothing.  lens is not changed: the next step's is lens + 1."""
+        torch = _torch()
+        pages, sizes, span = self._paged_check("paged_step", torch, cache, table, lens)
+        new, kept = self._paged_new("paged_step", torch, q, k, v, rope, pos, None, interleaved, sizes)
+        H, M = kept[0].shape[2], kept[0].shape[1]
+        if M != 1:
+            raise ValueError("paged_step: takes one token a sequence")
+        return self._paged_attend("paged_step", torch, out, kept[0], cache, span, sizes, H, weights, (*kept[1:], table, lens),
+                                  lambda *a: (self.lib.rt_paged_step, pages, new, *a))
+
+    def _paged_attend(self, who, torch, out, q, cache, span, sizes, H, weights, others, call):
+        given = out is not None
+        out = self._kv4_out(who, torch, out, q, *others)
+        if given:
+            self._paged_apart(who, "out", out, cache, span)
+        slots = 0
+        if weights is not None:
+            slots = self._paged_weights(who, torch, weights, sizes)
+            self._paged_apart(who, "weights", weights, cache, span, q, out, *others)
+        need = _paged_workspace_bytes(*sizes, H, int(weights is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        fn, *args = call(weights.data_ptr() if slots else None, slots, out.data_ptr(), ws.data_ptr() if need else None, need)
+        self._kv4_run(torch, "rt_" + who, fn, *args)
+        return out
+
+    def paged_evict(self, cache, table, lens, weights, keep: int, recent: int, new_table):
+        """Cuts every sequence of a paged cache to `keep` slots (rt_paged_evict): for each KV head the last `recent` and, of
+        those before them, the ones with the largest weights (ties: the lowest slot), in their order.  Their keys and values
+        are copied to the pages of new_table int32 [B, new_P], which must be pages that no table of these sequences holds;
+        the old ones stay as they were and are free afterwards.  Returns (kept int32 [B, Hkv, keep]: the slots, -1 behind the
+        last; new_lens int32 [B]; new_weights, shaped as weights: the kept slots', then zeros).  Sequences of no
+        more than `keep` slots move as they are."""
+        torch = _torch()
+        pages, sizes, span = self._paged_check("paged_evict", torch, cache, table, lens)
+        _, Hkv, page, _, B, _ = sizes
+        slots = self._paged_weights("paged_evict", torch, weights, sizes)
+        keep, recent = operator.index(keep), operator.index(recent)
+        if len(new_table.shape) != 2:
+            raise ValueError("paged_evict: new_table must be int32 [B, new_P]")
+        self._paged_ints("paged_evict", torch, "new_table", new_table, (B, new_table.shape[1]))
+        if not (0 <= recent <= keep and 0 < keep <= new_table.shape[1] * page):
+            raise ValueError(f"paged_evict: keep {keep} and recent {recent}: needs 0 <= recent <= keep, and pages for keep >= 1 slots")
+        self._paged_apart("paged_evict", "new_table", new_table, cache, span, table)
+        self._paged_apart("paged_evict", "weights", weights, cache, span)
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=self.device)
+        new_lens, new_weights = torch.empty_like(lens), torch.empty_like(weights)
+        self._kv4_run(torch, "rt_paged_evict", self.lib.rt_paged_evict, pages, weights.data_ptr(), slots, keep, recent,
+                      new_table.data_ptr(), new_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr())
+        return kept, new_lens, new_weights
 
     def __del__(self):
         try:
