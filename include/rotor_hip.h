@@ -467,9 +467,12 @@ int rt_paged_step(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float* 
  * their order.  kept int32 [B][Hkv][keep]: the slots, -1 behind the last; new_lens int32 [B]: how many (all
  * that are there where those are no more than keep; the same for every head); new_weights, shaped as weights: theirs, zeros
  * behind them.  Their keys and values are copied to the pages of new_table int32 [B][new_P], new_P * page >= keep, none of
- * which may be a page that `table` holds or another sequence's new one.  The old pages stay as they were. */
+ * which may be a page that `table` holds or another sequence's new one.  The old pages stay as they were.  workspace:
+ * rt_paged_evict_workspace bytes of device memory (0 where P * page <= 32768), as for rt_paged_attention. */
+size_t rt_paged_evict_workspace(const rt_pages* c);
 int rt_paged_evict(rt_ctx* ctx, const rt_pages* c, const float* weights, int weight_slots, int keep, int recent,
-                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights);
+                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights, void* workspace,
+                   size_t workspace_bytes);
 
 /* Final RMSNorm of x fp32 [D] with norm_w, tied bf16 LM head logits [V]
  * (src/rotor/bitnet_model.py:231-235) and greedy argmax (src/rotor/generation.py:42;

@@ -1397,8 +1397,15 @@ int rt_paged_step(rt_ctx* ctx, const rt_pages* p, const rt_paged_new* n, float* 
     return paged_attend(ctx, p, a, true, workspace, workspace_bytes, "rt_paged_step");
 }
 
+size_t rt_paged_evict_workspace(const rt_pages* p) {
+    PagedCache c;
+    if (!paged_check(p, p ? p->Hkv : 0, c, "rt_paged_evict_workspace")) return 0;
+    return paged_evict_workspace(c.B, c.Hkv, c.P << c.shift);
+}
+
 int rt_paged_evict(rt_ctx* ctx, const rt_pages* p, const float* weights, int weight_slots, int keep, int recent,
-                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights) {
+                   const int* new_table, int new_P, int* kept, int* new_lens, float* new_weights, void* workspace,
+                   size_t workspace_bytes) {
     PagedEvict a{};
     if (!ctx || !weights || !new_table || !kept || !new_lens || !new_weights) return fail(RT_EINVAL, "rt_paged_evict: NULL argument");
     if (!paged_check(p, p ? p->Hkv : 0, a.c, "rt_paged_evict")) return RT_EINVAL;
@@ -1409,6 +1416,9 @@ int rt_paged_evict(rt_ctx* ctx, const rt_pages* p, const float* weights, int wei
         return fail(RT_EINVAL, "rt_paged_evict: weights must have a place for each of P * page slots");
     if (weights == new_weights || new_table == p->table || new_lens == p->lens)
         return fail(RT_EINVAL, "rt_paged_evict: needs other memory for its outputs, and a table of other pages");
+    const size_t need = paged_evict_workspace(a.c.B, a.c.Hkv, a.c.P << a.c.shift);
+    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(RT_EINVAL, "rt_paged_evict: workspace too small (rt_paged_evict_workspace) or not 16-byte aligned");
     a.weights = weights;
     a.new_weights = new_weights;
     a.new_table = new_table;
@@ -1419,7 +1429,7 @@ int rt_paged_evict(rt_ctx* ctx, const rt_pages* p, const float* weights, int wei
     a.keep = keep;
     a.recent = recent;
     DeviceGuard g(ctx->device);
-    RT_HIP(launch_paged_evict(a, p->type, p->hd, ctx->stream));
+    RT_HIP(launch_paged_evict(a, p->type, p->hd, workspace, ctx->stream));
     return RT_OK;
 }
 

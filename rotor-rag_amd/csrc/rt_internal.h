@@ -453,9 +453,10 @@ struct PagedAttn {
     PagedNew n;  // a step's
     const float* q;
     float *out, *weights, *part, *ml, *scores;  // weights, scores: null where they are not kept
-    int slots;                                  // a row of weights
-    int H, G, tiles, S, least;                  // G = H / Hkv, in tiles of 16; S splits of at least so many tiles of slots
-    float scale;                                // log2(e) / sqrt(hd)
+    int2* units;
+    int slots;                // a row of weights
+    int H, G, tiles, groups;  // G = H / Hkv, in tiles of 16; workgroups of the launch
+    float scale;              // log2(e) / sqrt(hd)
 };
 struct PagedEvict {
     PagedCache c;
@@ -469,7 +470,8 @@ hipError_t launch_paged_append(const PagedCache& c, const PagedNew& n, float* q_
                                hipStream_t s);
 size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int hd, bool weights);
 hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void* work, hipStream_t s);
-hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, hipStream_t s);
+size_t paged_evict_workspace(int B, int Hkv, int cap);
+hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, void* work, hipStream_t s);
 hipError_t launch_lm_head(const uint16_t* E, const float* x, const float* norm_w, float eps, int V, int D,
                           float* logits, unsigned long long* best, int* token, int* pos, int advance,
                           int* next_ids, int* out_tokens, int pos_base, int out_cap, float* next_h, hipStream_t s);

@@ -55,18 +55,11 @@ __device__ __forceinline__ typename Elem<T>::type paged_round(float x) {
     else if constexpr (T == kPagedBf16) return paged_bf16(x);
     else return __builtin_bit_cast(unsigned short, (_Float16)x);
 }
-// Eight numbers into a row of the cache (16-byte aligned).
+// Four numbers into a row of the cache.
 template <int T>
-__device__ __forceinline__ void paged_store8(typename Elem<T>::type* at, const float (&x)[8]) {
-    if constexpr (T == kPagedF32) {
-        *reinterpret_cast<v4f*>(at) = v4f{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<v4f*>(at + 4) = v4f{x[4], x[5], x[6], x[7]};
-    } else {
-        v4u w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (unsigned)paged_round<T>(x[2 * i]) | (unsigned)paged_round<T>(x[2 * i + 1]) << 16;
-        *reinterpret_cast<v4u*>(at) = w;
-    }
+__device__ __forceinline__ void paged_store4(typename Elem<T>::type* at, const v4f& x) {
+    if constexpr (T == kPagedF32) *reinterpret_cast<v4f*>(at) = x;
+    else *reinterpret_cast<v4s*>(at) = v4s{paged_round<T>(x[0]), paged_round<T>(x[1]), paged_round<T>(x[2]), paged_round<T>(x[3])};
 }
 
 // a b - c d of fp32 numbers: exact products and one rounding to 64 bits, one to fp32.  (A difference with one product's rounding
@@ -75,14 +68,14 @@ __device__ __forceinline__ void paged_store8(typename Elem<T>::type* at, const f
 __device__ __forceinline__ float paged_diff(float a, float b, float c, float d) { return (float)((double)a * b - (double)c * d); }
 // Dimensions d .. d + 3 (d % 4 == 0) of a row x, rotated over its first `rotary` (a multiple of 8); cs: (cos, sin) of the
 // row's position.  Half: pairs (i, i + rotary / 2); interleaved: (2 i, 2 i + 1).
+__device__ __forceinline__ v4f paged_turn_pairs(v4f y, v4f c) {  // (y0, y1), (y2, y3) by (c0, c1), (c2, c3)
+    return v4f{paged_diff(y[0], c[0], y[1], c[1]), paged_diff(y[1], c[0], -y[0], c[1]), paged_diff(y[2], c[2], y[3], c[3]),
+               paged_diff(y[3], c[2], -y[2], c[3])};
+}
 __device__ __forceinline__ v4f paged_rotate4(const float* x, const float* cs, int d, int rotary, bool interleaved) {
     v4f y = *reinterpret_cast<const v4f*>(x + d);
     if (d >= rotary) return y;
-    if (interleaved) {
-        const v4f c = *reinterpret_cast<const v4f*>(cs + d);  // pairs d / 2, d / 2 + 1
-        return v4f{paged_diff(y[0], c[0], y[1], c[1]), paged_diff(y[1], c[0], -y[0], c[1]), paged_diff(y[2], c[2], y[3], c[3]),
-                   paged_diff(y[3], c[2], -y[2], c[3])};
-    }
+    if (interleaved) return paged_turn_pairs(y, *reinterpret_cast<const v4f*>(cs + d));
     const bool up = d >= rotary / 2;
     const int i = up ? d - rotary / 2 : d;
     const v4f z = *reinterpret_cast<const v4f*>(x + (up ? i : i + rotary / 2));
@@ -93,6 +86,26 @@ __device__ __forceinline__ v4f paged_rotate4(const float* x, const float* cs, in
         y[e] = paged_diff(y[e], c, up ? -z[e] : z[e], s);
     }
     return y;
+}
+// Both fours of a row that item o of HD / 8 has: a pair's two halves where pairs lie apart, else eight in a row.
+__device__ __forceinline__ int2 paged_fours(int o, int rotary, bool interleaved) {
+    return !interleaved && 8 * o < rotary ? make_int2(4 * o, 4 * o + rotary / 2) : make_int2(8 * o, 8 * o + 4);
+}
+__device__ __forceinline__ void paged_rotate8(v4f& x, v4f& y, const float* cs, int o, int rotary, bool interleaved) {
+    if (8 * o >= rotary) return;
+    const v4f c0 = *reinterpret_cast<const v4f*>(cs + 8 * o), c1 = *reinterpret_cast<const v4f*>(cs + 8 * o + 4);
+    if (interleaved) {
+        x = paged_turn_pairs(x, c0);
+        y = paged_turn_pairs(y, c1);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // (the turn of paged_rotate4, pair by pair)
+        const float c = e < 2 ? c0[2 * e] : c1[2 * e - 4], s = e < 2 ? c0[2 * e + 1] : c1[2 * e - 3];
+        const float u = paged_diff(x[e], c, y[e], s);
+        y[e] = paged_diff(y[e], c, -x[e], s);
+        x[e] = u;
+    }
 }
 
 // Where slot t of sequence b lies (elements from the cache's start to the first head's row; kv head h is page * HD * h
@@ -105,12 +118,13 @@ __device__ __forceinline__ long long paged_slot(const PagedCache& c, int HD, int
 }
 
 // ---- append ------------------------------------------------------------------------------
-// A thread has 8 dimensions of one head of one row (q heads, then k, then v heads).  A head's threads are in one wave, whose
-// loads are all done before its stores, so q_out may be q.  Bound by memory: each number is read and written once (a pair's
-// other half comes from the same lines).
+// A thread has 8 dimensions of one head of one row (q heads, then k, then v heads), both halves of its pairs: each number is read
+// and written once, by one thread, so q_out may be q.  Bound by memory: 8 prompts of up to 2048 tokens (20 heads over 5 of
+// 128, bf16) 77 us, 5.3 TB/s.
 template <int T, int HD>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNew n, float* q_out, int M, int H) {
     constexpr int L = HD / 8;
+    typedef typename Elem<T>::type E;
     const unsigned units = H + 2 * c.Hkv, per = units * L;
     const unsigned long long first = (unsigned long long)blockIdx.x * 256u;
     const unsigned long long row0 = first / per;
@@ -118,44 +132,27 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNe
     const unsigned long long row = row0 + skip;
     if (row >= (unsigned long long)c.B * M) return;
     const unsigned item = local - skip * per;
-    const int unit = item / L, o = item % L * 8;
+    const int unit = item / L, o = item % L;
+    const bool is_q = unit < H, is_v = unit >= H + c.Hkv;
+    const int kh = unit - H - (is_v ? c.Hkv : 0);
+    const int2 d = is_v ? make_int2(8 * o, 8 * o + 4) : paged_fours(o, n.rotary, n.interleaved);
+    const float* const src = is_q ? n.q + ((size_t)row * H + unit) * HD : (is_v ? n.v : n.k) + ((size_t)row * c.Hkv + kh) * HD;
+    v4f x = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + d.x));
+    v4f y = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(src + d.y));
     const int b = (int)(row / (unsigned)M), m = (int)(row - (unsigned long long)b * M);
     const long long p = (long long)n.pos[b] + m, t = (long long)c.lens[b] + m;
     const int count = n.counts ? n.counts[b] : M;
     const long long at = m < count && p >= 0 && p < n.rope_rows && t >= 0 && t <= INT_MAX ? paged_slot(c, HD, b, (int)t) : -1;
-    const float* cs = n.rope + (size_t)(at >= 0 ? p : 0) * n.rotary;
-    float x[8];
-    if (unit < H) {
-        const size_t base = ((size_t)row * H + unit) * HD;
-        v4f y0{}, y1{};
-        if (at >= 0) {
-            y0 = paged_rotate4(n.q + base, cs, o, n.rotary, n.interleaved);
-            y1 = paged_rotate4(n.q + base, cs, o + 4, n.rotary, n.interleaved);
-        }
-        *reinterpret_cast<v4f*>(q_out + base + o) = y0;
-        *reinterpret_cast<v4f*>(q_out + base + o + 4) = y1;
-        return;
+    if (at >= 0 && !is_v) paged_rotate8(x, y, n.rope + (size_t)p * n.rotary, o, n.rotary, n.interleaved);
+    if (is_q) {
+        float* const to = q_out + ((size_t)row * H + unit) * HD;
+        *reinterpret_cast<v4f*>(to + d.x) = at >= 0 ? x : v4f{};
+        *reinterpret_cast<v4f*>(to + d.y) = at >= 0 ? y : v4f{};
+    } else if (at >= 0) {
+        E* const to = static_cast<E*>(c.cache) + (is_v ? c.kv_stride : 0) + at + ((long long)kh << c.shift) * HD;
+        paged_store4<T>(to + d.x, x);
+        paged_store4<T>(to + d.y, y);
     }
-    if (at < 0) return;
-    const bool is_v = unit >= H + c.Hkv;
-    const int kh = unit - H - (is_v ? c.Hkv : 0);
-    const size_t base = ((size_t)row * c.Hkv + kh) * HD;
-    v4f y0, y1;
-    if (is_v) {
-        y0 = *reinterpret_cast<const v4f*>(n.v + base + o);
-        y1 = *reinterpret_cast<const v4f*>(n.v + base + o + 4);
-    } else {
-        y0 = paged_rotate4(n.k + base, cs, o, n.rotary, n.interleaved);
-        y1 = paged_rotate4(n.k + base, cs, o + 4, n.rotary, n.interleaved);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[e] = y0[e];
-        x[4 + e] = y1[e];
-    }
-    typedef typename Elem<T>::type E;
-    E* const cache = static_cast<E*>(c.cache) + (is_v ? c.kv_stride : 0);
-    paged_store8<T>(cache + at + ((long long)kh << c.shift) * HD + o, x);
 }
 
 // ---- attention ---------------------------------------------------------------------------
@@ -180,12 +177,6 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNe
 // this one's.
 template <int T, int HD>
 struct AttnTile;
-
-// The head's row of q, rotated where the step asks for it, and times log2(e) / sqrt(HD): dimensions d .. d + 3.
-__device__ __forceinline__ v4f paged_query4(const PagedAttn& a, const float* q, const float* cs, int d) {
-    v4f x = cs ? paged_rotate4(q, cs, d, a.n.rotary, a.n.interleaved) : *reinterpret_cast<const v4f*>(q + d);
-    return x * a.scale;
-}
 
 // The largest of lanes l, l ^ 16, l ^ 32, l ^ 48; their sum.
 __device__ __forceinline__ float paged_max4(float x) {
@@ -231,6 +222,32 @@ __device__ __forceinline__ void paged_split(const float (&x)[8], v8h (&t)[3]) {
         t[1][e] = (_Float16)r;
         t[2][e] = (_Float16)((r - (float)t[1][e]) * kRest);
     }
+}
+
+__device__ __forceinline__ void paged_split_bf16(v4f x, v2u (&t)[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        t[k] = v2u{paged_high(__float_as_uint(x[0]), __float_as_uint(x[1])), paged_high(__float_as_uint(x[2]), __float_as_uint(x[3]))};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] -= __uint_as_float(__float_as_uint(x[e]) & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void paged_split(v4f x, v2u (&t)[3]) {
+    unsigned short h[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float u = x[e];
+        asm("" : "+v"(u));
+        const _Float16 a = (_Float16)u;
+        float r = u - (float)a;
+        asm("" : "+v"(r));
+        const _Float16 b = (_Float16)r;
+        h[0][e] = __builtin_bit_cast(unsigned short, a);
+        h[1][e] = __builtin_bit_cast(unsigned short, b);
+        h[2][e] = __builtin_bit_cast(unsigned short, (_Float16)((r - (float)b) * kRest));
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) t[k] = v2u{h[k][0] | (unsigned)h[k][1] << 16, h[k][2] | (unsigned)h[k][3] << 16};
 }
 
 // Tiles of 32 slots in 16 bits: two row tiles of 16.
@@ -286,42 +303,25 @@ struct AttnTile {
 #pragma unroll
         for (int w = 0; w < HD / 32; ++w) v[n][w] = 0u;
     }
-    __device__ __forceinline__ void set_query(const PagedAttn& a, const float* row, const float* cs, int g) {
-        float x[NC][8], big = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v4f y = paged_query4(a, row, cs, c * 32 + g * 8 + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[c][4 * h + e] = y[e];
-                    big = fmaxf(big, fabsf(y[e]));
-                }
-            }
-        if constexpr (F16) {  // the largest into [2^14, 2^15)
-            big = paged_max4(big);
-            const int n = min(max(14 + 127 - (int)(__float_as_uint(big) >> 23), -113), 126);
+    // Queries pass through LDS in the order that lanes take them, [term][c][g][i] of 16 bytes: put by the workgroup, four
+    // dimensions a thread (x: of head i, dimensions d .. d + 3, scaled by 2^n in fp16), taken by every wave.
+    static constexpr int QBYTES = 3 * NC * 64 * 16;
+    static __device__ __forceinline__ void stage(char* to, v4f x, int i, int d, int n) {
+        char* const at = to + ((d / 32 * 4 + d / 8 % 4) * 16 + i) * 16 + d % 8 * 2;
+        v2u t[3];
+        if constexpr (F16) {
             const float f = __uint_as_float((unsigned)(n + 127) << 23);
-            qi = __uint_as_float((unsigned)(127 - n) << 23);
+            paged_split(v4f{x[0] * f, x[1] * f, x[2] * f, x[3] * f}, t);
+        } else paged_split_bf16(x, t);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<v2u*>(at + p * NC * 1024) = t[p];
+    }
+    __device__ __forceinline__ void take(const char* from, int n, int i, int g) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e] *= f;
-                v8h t[3];
-                paged_split(x[c], t);
+        for (int p = 0; p < 3; ++p)
 #pragma unroll
-                for (int p = 0; p < 3; ++p) q[p][c] = __builtin_bit_cast(v4u, t[p]);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                v4u t[3];
-                paged_split(x[c], t);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) q[p][c] = t[p];
-            }
-        }
+            for (int c = 0; c < NC; ++c) q[p][c] = *reinterpret_cast<const v4u*>(from + (((p * NC + c) * 4 + g) * 16 + i) * 16);
+        qi = __uint_as_float((unsigned)(127 - n) << 23);
     }
     static __device__ __forceinline__ v4f mul(const v4u& x, const v4u& y, const v4f& z) {
         if constexpr (F16)
@@ -391,6 +391,7 @@ struct AttnTile {
 template <int HD>
 struct AttnTile<kPagedF32, HD> {
     static constexpr int TK = 16, NS = 4, NC = HD / 16, NU = HD / 64;
+    static constexpr bool F16 = false;
     typedef float E;
     v4f k[NC], v[4][NU], q[NC], o[NU][4];
 
@@ -419,9 +420,13 @@ struct AttnTile<kPagedF32, HD> {
 #pragma unroll
         for (int u = 0; u < NU; ++u) v[n][u] = v4f{};
     }
-    __device__ __forceinline__ void set_query(const PagedAttn& a, const float* row, const float* cs, int g) {
+    static constexpr int QBYTES = NC * 64 * 16;
+    static __device__ __forceinline__ void stage(char* to, v4f x, int i, int d, int) {
+        *reinterpret_cast<v4f*>(to + ((d / 16 * 4 + d / 4 % 4) * 16 + i) * 16) = x;
+    }
+    __device__ __forceinline__ void take(const char* from, int, int i, int g) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) q[c] = paged_query4(a, row, cs, c * 16 + g * 4);
+        for (int c = 0; c < NC; ++c) q[c] = *reinterpret_cast<const v4f*>(from + ((c * 4 + g) * 16 + i) * 16);
     }
     __device__ __forceinline__ void scores(float (&s)[NS]) {
         v4f d[2] = {};  // (two chains: a product waits for the one before it in its own)
@@ -457,44 +462,134 @@ struct AttnTile<kPagedF32, HD> {
     __device__ __forceinline__ float out(int r, int j) const { return o[r >> 2][j][r & 3]; }
 };
 
-// Slots that the token of sequence b attends to (STEP: its own, which is put there in this launch, among them).
+// Slots that a sequence of `len` attends to, the step's token among them: should that turn out to have no place or no angle, it
+// attends to none, but its share of the launch is as if it had.
 template <bool STEP>
-__device__ __forceinline__ int paged_len(const PagedAttn& a, int b) {
-    const int cap = a.c.P << a.c.shift, n = a.c.lens[b];
-    if constexpr (STEP) {
-        const int p = a.n.pos[b];
-        // (a token without a place or an angle is not there, and attends to nothing)
-        return p < 0 || p >= a.n.rope_rows || paged_slot(a.c, 0, b, n) < 0 ? 0 : n + 1;
-    }
-    return min(max(n, 0), cap);
+__device__ __forceinline__ int paged_span(const PagedAttn& a, int len) {
+    const int cap = a.c.P << a.c.shift;
+    if constexpr (STEP) return len < 0 || len >= cap ? 0 : len + 1;
+    return min(max(len, 0), cap);
 }
-// Tiles a split has, for a sequence of `tiles`: as many as fill S splits, but kPagedLeast at least.
-__device__ __forceinline__ int paged_piece(int tiles, int S, int least) { return max((tiles + S - 1) / S, least); }
+// The page of a step's token whose slot is the last of `span`, or -1 where it attends to nothing.
+__device__ __forceinline__ int paged_newest(const PagedAttn& a, int b, int span) {
+    const int p = a.n.pos[b], id = span > 0 ? a.c.table[(size_t)b * a.c.P + ((span - 1) >> a.c.shift)] : -1;
+    return p < 0 || p >= a.n.rope_rows || id >= a.c.pages ? -1 : id;
+}
+__device__ __forceinline__ int paged_scan(int x) {  // inclusive, over the lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
 
-constexpr int kWaves = 4;
+// The pieces of a launch.  A sequence of n tiles is cut, for each of its `per` units (a KV head's tile of heads), into pieces
+// of at most q tiles (one at least), q a multiple of the waves for which all pieces fit the launch's workgroups; workgroup w has
+// piece number w in the order (sequence, unit, piece).  Every wave works this out for itself, lane b for sequence b: the host
+// does not know the lengths, and with the same number of pieces for each the longest sequence decides the launch.
+constexpr int kWaves = 4, kPagedMapped = 4096;  // batches past kPagedMapped: a piece a unit
+struct PagedPiece {
+    int b, unit, piece, n, first, q;  // n pieces a unit of sequence b; first: the workgroup of this unit's first; n = 0: none
+    int span;                         // paged_span of sequence b
+};
+template <bool STEP, int TK>
+__device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int lane) {
+    const int B = a.c.B, per = a.c.Hkv * a.tiles;
+    PagedPiece p{};
+    if (B > kPagedMapped) {
+        p.b = w / per;
+        p.unit = w - p.b * per;
+        p.n = 1;
+        p.first = w;
+        p.q = INT_MAX / 2;
+        p.span = paged_span<STEP>(a, a.c.lens[p.b]);
+        return p;
+    }
+    int span = 0;
+    auto tiles = [&](int b) {
+        span = b < B ? paged_span<STEP>(a, a.c.lens[b]) : 0;
+        return (span + TK - 1) / TK;
+    };
+    // ceil(nb / q): nb <= 2^16, and 1 / q is good to 2^-23, so the quarter decides
+    auto pieces = [&](int nb, int b, int q) {
+        return b >= B ? 0 : nb <= q ? 1 : (int)(((float)(nb + q - 1) + 0.25f) * __builtin_amdgcn_rcpf((float)q));
+    };
+    const int mine = tiles(lane);
+    int q, n, incl;
+    if (B <= 64) {
+        const float all = (float)__builtin_amdgcn_readlane(paged_scan(mine), 63);
+        q = max(kWaves, ((int)(all * (float)per * __builtin_amdgcn_rcpf((float)a.groups)) + kWaves - 1) / kWaves * kWaves);
+        for (;; q += max(kWaves, q / 16 / kWaves * kWaves)) {  // (ends at the latest with a piece a unit: B per <= groups)
+            n = pieces(mine, lane, q);
+            incl = paged_scan(n);
+            if (__builtin_amdgcn_readlane(incl, 63) * per <= a.groups) break;
+        }
+        const unsigned long long here = __ballot(w < incl * per);
+        if (here == 0ull) return p;
+        p.b = (int)__builtin_ctzll(here);
+        p.n = __builtin_amdgcn_readlane(n, p.b);
+        p.first = (__builtin_amdgcn_readlane(incl, p.b) - p.n) * per;
+        p.span = __builtin_amdgcn_readlane(span, p.b);
+    } else {
+        // no more than B + all / q pieces a unit: q from that
+        int all = mine;
+        for (int b = 64; b < B; b += 64) all += tiles(b + lane);
+        all = __builtin_amdgcn_readlane(paged_scan(all), 63);
+        const float room = (float)(a.groups - B * per);
+        q = room > 0.0f ? (int)fminf((float)all * (float)per / room * 1.0001f, 1e6f) + 1 : 1 << 20;
+        q = max(kWaves, (q + kWaves - 1) / kWaves * kWaves);
+        int before = 0;
+        for (int b = 0;; b += 64) {
+            if (b >= B) return p;
+            n = pieces(tiles(b + lane), b + lane, q);
+            incl = paged_scan(n) + before;
+            const unsigned long long here = __ballot(w < incl * per);
+            if (here != 0ull) {
+                const int l = (int)__builtin_ctzll(here);
+                p.b = b + l;
+                p.n = __builtin_amdgcn_readlane(n, l);
+                p.first = (__builtin_amdgcn_readlane(incl, l) - p.n) * per;
+                p.span = __builtin_amdgcn_readlane(span, l);
+                break;
+            }
+            before = __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    p.q = q;
+    p.unit = (w - p.first) / p.n;
+    p.piece = w - p.first - p.unit * p.n;
+    p.first += p.unit * p.n;
+    return p;
+}
 
 template <int T, int HD, bool STEP>
 __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a) {
     typedef AttnTile<T, HD> Tile;
     typedef typename Tile::E E;
-    constexpr int TK = Tile::TK;
-    __shared__ float part[kWaves][16][HD + 4];
+    constexpr int TK = Tile::TK, L = HD / 4;
+    // the queries, and in their place, when all waves have taken them, the waves' sums
+    constexpr int kPart = kWaves * 16 * (HD + 4) * 4;
+    __shared__ __align__(16) char both[kPart > Tile::QBYTES ? kPart : Tile::QBYTES];
     __shared__ float ml[kWaves][16][2];
-    __shared__ __align__(16) E fresh[STEP ? 2 : 1][STEP ? HD : 16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x % a.S, unit = blockIdx.x / a.S;  // unit: (b, KV head, tile of heads)
-    const int ht = unit % a.tiles, bk = unit / a.tiles, kh = bk % a.c.Hkv, b = bk / a.c.Hkv;
-    const int len = paged_len<STEP>(a, b);
-    const int tiles = (len + TK - 1) / TK, piece = paged_piece(tiles, a.S, a.least);
-    const int first = split * piece, last = min(first + piece, tiles);
+    __shared__ int power[16];
+    __shared__ __align__(16) E fresh[2][STEP ? HD : 16];
+    float(*const part)[16][HD + 4] = reinterpret_cast<float(*)[16][HD + 4]>(both);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
+    const PagedPiece p = paged_piece<STEP, TK>(a, blockIdx.x, lane);
+    if (p.n == 0) return;
+    const int b = p.b, kh = p.unit / a.tiles, ht = p.unit - kh * a.tiles, bk = b * a.c.Hkv + kh;
+    const int len = p.span, tiles = (len + TK - 1) / TK, first = min(p.piece * p.q, tiles);
+    int last = min(first + p.q, tiles);
+    const int newest = STEP ? paged_newest(a, b, len) : 0;
     const int rows = min(a.G - 16 * ht, 16);
-    if (first >= last && (a.S > 1 || split > 0)) return;
     const int h0 = kh * a.G + 16 * ht;  // the tile's first head
     const int cap = a.c.P << a.c.shift;
     Tile x;
     float m = -INFINITY, l = 0.0f;
     x.clear();
-    if (first + wave < last) {
+    if (first < last) {
         // the pages of the wave's next 64 tiles, a tile a lane (two where a page is half a tile)
         int id0 = 0, id1 = 0;
         auto look = [&](int t) {
@@ -510,65 +605,71 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             there = id >= 0 && id < a.c.pages;
             return kbase + (long long)(there ? id : 0) * a.c.page_stride + ((t * TK + 16 * half) & in_page) * HD;
         };
-        look(first + wave);
-        int t = first + wave, n = 0;
-        bool there0, there1 = false, next0, next1 = false;
-        const E* b0 = base(n, t, 0, there0);
-        const E* b1 = TK == 32 ? base(n, t, 1, there1) : b0;
-        x.load_k(b0, b1, i, g);
-        x.load_v(b0 + a.c.kv_stride, b1 + a.c.kv_stride, i, g);
-        const int head = h0 + min(i, rows - 1);  // (columns past the last head repeat it)
-        const float* cs = STEP ? a.n.rope + (size_t)a.n.pos[b] * a.n.rotary : nullptr;
-        x.set_query(a, a.q + ((size_t)b * a.H + head) * HD, cs, g);
-        if constexpr (STEP) {
-            // the new row: rotated, rounded and written by the wave that has the last tile, which takes it from LDS
-            if (last == tiles && (tiles - 1 - first) % kWaves == wave && lane < HD / 4) {
-                const bool is_v = lane >= HD / 8;
-                const int o = lane % (HD / 8) * 8;
-                const float* src = (is_v ? a.n.v : a.n.k) + (size_t)bk * HD;
-                const v4f y0 = is_v ? *reinterpret_cast<const v4f*>(src + o) : paged_rotate4(src, cs, o, a.n.rotary, a.n.interleaved);
-                const v4f y1 =
-                    is_v ? *reinterpret_cast<const v4f*>(src + o + 4) : paged_rotate4(src, cs, o + 4, a.n.rotary, a.n.interleaved);
-                const float y[8] = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
-                paged_store8<T>(&fresh[is_v][o], y);
-                if (ht == 0) {
-                    E* const cache = static_cast<E*>(a.c.cache) + (is_v ? a.c.kv_stride : 0) + ((long long)kh << a.c.shift) * HD;
-                    paged_store8<T>(cache + paged_slot(a.c, HD, b, len - 1) + o, y);
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");  // (for the compiler: one wave's LDS accesses are in order)
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+        int at = first + wave, n = 0;
+        bool there0 = false, there1 = false, next0 = false, next1 = false;
+        const E *b0 = kbase, *b1 = kbase;
+        if (at < last) {
+            look(at);
+            b0 = base(n, at, 0, there0);
+            b1 = TK == 32 ? base(n, at, 1, there1) : b0;
+            x.load_k(b0, b1, i, g);
+            x.load_v(b0 + a.c.kv_stride, b1 + a.c.kv_stride, i, g);
         }
-        for (; t < last; t += kWaves, ++n, there0 = next0, there1 = next1) {
-            const bool more = t + kWaves < last;
+        // the queries, rotated where the step asks for it, times log2(e) / sqrt(HD), into LDS; a step's new row too, where
+        // this piece has the last tile
+        if (newest < 0) last = at = first;  // (a step without a place: nothing from here on)
+        const float* const cs = STEP && newest >= 0 ? a.n.rope + (size_t)a.n.pos[b] * a.n.rotary : nullptr;
+        const int items = newest < 0 ? 0 : rows * L, more = STEP && last == tiles ? 2 * L : 0;
+        for (int e = t; e < items + more; e += 64 * kWaves) {
+            const int d = e % L * 4, row = e / L;
+            if (row < rows) {
+                const float* const src = a.q + ((size_t)b * a.H + h0 + row) * HD;
+                v4f y = (STEP ? paged_rotate4(src, cs, d, a.n.rotary, a.n.interleaved) : *reinterpret_cast<const v4f*>(src + d)) * a.scale;
+                int pw = 0;
+                if constexpr (Tile::F16) {  // the head's largest into [2^14, 2^15): over the L lanes that have it
+                    float big = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+                    for (int w = 1; w < L; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
+                    pw = min(max(14 + 127 - (int)(__float_as_uint(big) >> 23), -113), 126);
+                    if (d == 0) power[row] = pw;
+                }
+                Tile::stage(both, y, row, d, pw);
+            } else if constexpr (STEP) {
+                const bool is_v = row > rows;
+                const float* const src = (is_v ? a.n.v : a.n.k) + (size_t)bk * HD;
+                const v4f y = is_v ? *reinterpret_cast<const v4f*>(src + d) : paged_rotate4(src, cs, d, a.n.rotary, a.n.interleaved);
+                paged_store4<T>(&fresh[is_v][d], y);
+                if (ht == 0)
+                    paged_store4<T>(const_cast<E*>(kbase) + (is_v ? a.c.kv_stride : 0) + (long long)newest * a.c.page_stride +
+                                        ((len - 1) & in_page) * HD + d, y);
+            }
+        }
+        __syncthreads();
+        x.take(both, Tile::F16 ? power[min(i, rows - 1)] : 0, min(i, rows - 1), g);  // (columns past the last head repeat it)
+        for (; at < last; at += kWaves, ++n, there0 = next0, there1 = next1) {
+            const bool more = at + kWaves < last;
             if constexpr (STEP)
-                if (t == tiles - 1) x.put(fresh[0], fresh[1], len - 1 - t * TK, i, g);
+                if (at == tiles - 1) x.put(fresh[0], fresh[1], len - 1 - at * TK, i, g);
             float s[Tile::NS];
             x.scores(s);
             if (more) {
-                if (((n + 1) & 63) == 0) look(t + kWaves);
-                b0 = base(n + 1, t + kWaves, 0, next0);
-                b1 = TK == 32 ? base(n + 1, t + kWaves, 1, next1) : b0;
+                if (((n + 1) & 63) == 0) look(at + kWaves);
+                b0 = base(n + 1, at + kWaves, 0, next0);
+                b1 = TK == 32 ? base(n + 1, at + kWaves, 1, next1) : b0;
                 x.load_k(b0, b1, i, g);
             }
-            if (t == tiles - 1 || !there0 || (TK == 32 && !there1)) {
+            if (at == tiles - 1 || !there0 || (TK == 32 && !there1)) {
 #pragma unroll
                 for (int e = 0; e < Tile::NS; ++e) {
-                    const int at = Tile::slot(e, g);
-                    if (t * TK + at >= len || !(TK == 32 && e >= 4 ? there1 : there0)) {
+                    if (at * TK + Tile::slot(e, g) >= len || !(TK == 32 && e >= 4 ? there1 : there0)) {
                         s[e] = -INFINITY;
                         x.hide(e);
                     }
                 }
             }
-            if (a.scores && i < rows) {
-                float* const to = a.scores + ((size_t)b * a.H + h0 + i) * cap + t * TK;
+            float raw[Tile::NS];
 #pragma unroll
-                for (int e = 0; e < Tile::NS; e += 4)
-                    if (TK == 16 || t * TK + 16 * (e >> 2) < cap)
-                        *reinterpret_cast<v4f*>(to + Tile::slot(e, g)) = v4f{s[e], s[e + 1], s[e + 2], s[e + 3]};
-            }
+            for (int e = 0; e < Tile::NS; ++e) raw[e] = s[e];
             float top = s[0];
 #pragma unroll
             for (int e = 1; e < Tile::NS; ++e) top = fmaxf(top, s[e]);
@@ -587,6 +688,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             }
             x.values(s);
             if (more) x.load_v(b0 + a.c.kv_stride, b1 + a.c.kv_stride, i, g);
+            if (a.scores && i < rows) {  // (behind the loads: a wave waits for its accesses in their order)
+                float* const to = a.scores + ((size_t)b * a.H + h0 + i) * cap + at * TK;
+#pragma unroll
+                for (int e = 0; e < Tile::NS; e += 4)
+                    if (TK == 16 || at * TK + 16 * (e >> 2) < cap)
+                        *reinterpret_cast<v4f*>(to + Tile::slot(e, g)) = v4f{raw[e], raw[e + 1], raw[e + 2], raw[e + 3]};
+            }
         }
     }
     // the waves' sums, joined
@@ -610,8 +718,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
                     v4f{x.out(r, j) * f, x.out(r, j + 1) * f, x.out(r, j + 2) * f, x.out(r, j + 3) * f};
     }
     __syncthreads();
-    for (int e = threadIdx.x * 4; e < rows * HD; e += 64 * kWaves * 4) {
-        const int row = e / HD, d = e % HD;
+    for (int e = t; e < rows * L; e += 64 * kWaves) {
+        const int row = e / L, d = e % L * 4;
         v4f y = *reinterpret_cast<const v4f*>(&part[0][row][d]);
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) y += *reinterpret_cast<const v4f*>(&part[w][row][d]);
@@ -621,64 +729,84 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         const float at = top > -INFINITY ? top : 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) sum += ml[w][row][1] * __builtin_amdgcn_exp2f(ml[w][row][0] - at);
-        if (a.S == 1) {
+        if (p.n == 1) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
             *reinterpret_cast<v4f*>(a.out + ((size_t)b * a.H + h0 + row) * HD + d) = y * inv;
-        } else *reinterpret_cast<v4f*>(a.part + (((size_t)unit * a.S + split) * 16 + row) * HD + d) = y;
-        if ((a.S > 1 || a.scores) && d == 0)
-            *reinterpret_cast<v2f*>(a.ml + (((size_t)unit * a.S + split) * 16 + row) * 2) = v2f{top, sum};
+        } else *reinterpret_cast<v4f*>(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d) = y;
+        if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)blockIdx.x * 16 + row) * 2) = v2f{top, sum};
     }
+    if (t == 0 && p.piece == 0 && a.ml) a.units[(size_t)b * a.c.Hkv * a.tiles + p.unit] = make_int2(p.first, p.n);
 }
 
-// The join: workgroups [0, B H): a head's partials into its output; the others: what 1024 slots of a KV head weighed
-// (every head's score against its reference and sum), added to the accumulated weights.
-template <int HD, bool STEP>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedAttn a, int TK, int joins, int chunks) {
-    __shared__ float sums[256 / (HD / 4)][HD];
-    const int t = threadIdx.x;
+// A head's reference (the largest of its pieces') and the reciprocal of its sum of weights, found by a wave: ml is the
+// head's (reference, sum) of its first piece, n pieces.
+__device__ __forceinline__ void paged_total(const float* ml, int n, int lane, float& ref, float& inv) {
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 64) top = fmaxf(top, ml[s * 32]);
+    top = lane63(wave_reduce63(top, -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
+    ref = top > -INFINITY ? top : 0.0f;
+    float sum = 0.0f;
+    for (int s = lane; s < n; s += 64) sum += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
+    sum = lane63(wave_reduce63(sum, 0.0f, [](float x, float y) { return x + y; }));
+    inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
+}
+
+// The join: workgroups [0, B H): a head's pieces into its output; the others: what 4 NT slots of a KV head weighed (every
+// head's score against its reference and sum), added to the accumulated weights.
+constexpr int kJoinHeads = 1024;  // H / Hkv at most
+
+template <int HD, bool STEP, int NT>
+__global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int joins, int chunks) {
+    constexpr int L = HD / 4;
+    __shared__ float sums[NT / L][HD];
+    __shared__ float total[kJoinHeads][2];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if ((int)blockIdx.x < joins) {
         const int head = blockIdx.x % a.H, b = blockIdx.x / a.H, kh = head / a.G, in = head % a.G;
-        const int tiles = (paged_len<STEP>(a, b) + TK - 1) / TK, piece = paged_piece(tiles, a.S, a.least);
-        const int n = (tiles + piece - 1) / piece;
-        const size_t first = ((size_t)(b * a.c.Hkv + kh) * a.tiles + in / 16) * a.S;
-        const float* ml = a.ml + (first * 16 + in % 16) * 2;
-        const float* part = a.part + (first * 16 + in % 16) * HD;
-        const int d = t % (HD / 4) * 4, grp = t / (HD / 4);
-        float top = -INFINITY;
-        for (int s = 0; s < n; ++s) top = fmaxf(top, ml[s * 32]);
-        const float ref = top > -INFINITY ? top : 0.0f;
-        float sum = 0.0f;
-        for (int s = 0; s < n; ++s) sum += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
+        const int2 unit = a.units[(size_t)(b * a.c.Hkv + kh) * a.tiles + in / 16];
+        const int n = unit.y;
+        if (n == 1) return;
+        const float* ml = a.ml + ((size_t)unit.x * 16 + in % 16) * 2;
+        const float* part = a.part + ((size_t)unit.x * 16 + in % 16) * HD;
+        const int d = t % L * 4, grp = t / L;
         v4f y{};
-        for (int s = grp; s < n; s += 256 / (HD / 4))
+        float own = -INFINITY, ref, inv;
+        if (grp < n) {  // (before the references are known, which takes as long as these loads)
+            y = *reinterpret_cast<const v4f*>(part + (size_t)grp * 16 * HD + d);
+            own = ml[grp * 32];
+        }
+        paged_total(ml, n, lane, ref, inv);
+        y *= __builtin_amdgcn_exp2f(own - ref);
+#pragma unroll 4
+        for (int s = grp + NT / L; s < n; s += NT / L)
             y += *reinterpret_cast<const v4f*>(part + (size_t)s * 16 * HD + d) * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
         *reinterpret_cast<v4f*>(&sums[grp][d]) = y;
         __syncthreads();
         if (grp) return;
 #pragma unroll
-        for (int w = 1; w < 256 / (HD / 4); ++w) y += *reinterpret_cast<const v4f*>(&sums[w][d]);
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        for (int w = 1; w < NT / L; ++w) y += *reinterpret_cast<const v4f*>(&sums[w][d]);
         *reinterpret_cast<v4f*>(a.out + ((size_t)b * a.H + head) * HD + d) = y * inv;
         return;
     }
     const int chunk = ((int)blockIdx.x - joins) % chunks, bk = ((int)blockIdx.x - joins) / chunks, b = bk / a.c.Hkv, kh = bk % a.c.Hkv;
-    const int len = paged_len<STEP>(a, b), cap = a.c.P << a.c.shift, s0 = chunk * 1024 + t * 4;
-    if (chunk * 1024 >= len) return;
-    const int tiles = (len + TK - 1) / TK, piece = paged_piece(tiles, a.S, a.least), n = (tiles + piece - 1) / piece;
+    const int len = paged_span<STEP>(a, a.c.lens[b]), cap = a.c.P << a.c.shift, s0 = (chunk * NT + t) * 4;
+    if (chunk * NT * 4 >= len || (STEP && paged_newest(a, b, len) < 0)) return;
+    for (int in = wave; in < a.G; in += NT / 64) {
+        float ref, inv;
+        const int2 unit = a.units[(size_t)bk * a.tiles + in / 16];
+        paged_total(a.ml + ((size_t)unit.x * 16 + in % 16) * 2, unit.y, lane, ref, inv);
+        total[in][0] = ref;
+        total[in][1] = inv;
+    }
+    __syncthreads();
+    if (s0 >= len) return;
     v4f add{};
+    const float* score = a.scores + ((size_t)b * a.H + kh * a.G) * cap + s0;
+#pragma unroll 4
     for (int in = 0; in < a.G; ++in) {
-        const float* ml = a.ml + (((size_t)bk * a.tiles + in / 16) * a.S * 16 + in % 16) * 2;
-        float top = -INFINITY;
-        for (int s = 0; s < n; ++s) top = fmaxf(top, ml[s * 32]);
-        const float ref = top > -INFINITY ? top : 0.0f;
-        float sum = 0.0f;
-        for (int s = 0; s < n; ++s) sum += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-        if (s0 < cap) {
-            const v4f s = *reinterpret_cast<const v4f*>(a.scores + ((size_t)b * a.H + kh * a.G + in) * cap + s0);
+        const v4f s = *reinterpret_cast<const v4f*>(score + (size_t)in * cap);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) add[e] += s0 + e < len ? __builtin_amdgcn_exp2f(s[e] - ref) * inv : 0.0f;
-        }
+        for (int e = 0; e < 4; ++e) add[e] += __builtin_amdgcn_exp2f(s[e] - total[in][0]) * total[in][1];
     }
     float* const w = a.weights + (size_t)bk * a.slots + s0;
 #pragma unroll
@@ -687,11 +815,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttn a, int TK, in
 }
 
 // ---- eviction ----------------------------------------------------------------------------
-// Which slots are kept: the last `recent`, and of those before them the largest weights, ties to the lowest slot; slots in
-// holes are not there.  One workgroup a KV head of a sequence.  Weights as whole numbers of the same order (NaN above all, -0 as
-// 0); the smallest that is kept is found bit by bit, eleven, eleven and ten at a time, from a histogram in LDS; then every
-// wave counts its own run of slots, and writes out those that are kept behind those of the waves before it.
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+// Which slots are kept: the last `recent`, and of those before them (the judged) the largest weights, ties to the lowest slot;
+// slots in holes are not there.  Weights are taken as whole numbers of the same order (NaN above all, -0 as 0; 0 for what is not
+// there).  The smallest that is kept is found from histograms of its upper 11 bits, of the next 11 among those that have these,
+// and of the last 10.  Then every wave counts the kept of its run of slots, and writes them out behind those of the waves before.
+// A workgroup of 1024 threads takes a KV head of a sequence, up to 32 slots a thread in registers; longer caches are shared among
+// workgroups of 8 slots a thread, in a launch for every histogram and two for the output.
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictBins = 2048;
+constexpr int kEvictAlone = 32 * kEvictThreads, kEvictChunk = 8 * kEvictThreads;
 
 __device__ __forceinline__ unsigned evict_key(float w) {  // 1 and up (0: not there)
     unsigned u = __float_as_uint(w);
@@ -699,137 +830,277 @@ __device__ __forceinline__ unsigned evict_key(float w) {  // 1 and up (0: not th
     if (u == 0x80000000u) u = 0u;
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ int evict_scan(int x) {  // inclusive, over the lanes
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-    return x;
-}
+__device__ __forceinline__ int evict_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ int evict_bins(int pass) { return pass == 2 ? 1024 : 2048; }
 
-__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict a) {
-    __shared__ int hist[2048];
-    __shared__ int totals[kEvictWaves][2], found[4];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int bk = blockIdx.x, b = bk / a.c.Hkv;
-    const int cap = a.c.P << a.c.shift, len = min(max(a.c.lens[b], 0), cap);
-    const int old = max(len - a.recent, 0);  // slots that are judged; [old, len) stay
-    const float* const w = a.weights + (size_t)bk * a.slots;
-    const int* const row = a.c.table + (size_t)b * a.c.P;
-    auto there = [&](int s) {
-        const int id = row[s >> a.c.shift];
-        return id >= 0 && id < a.c.pages;
-    };
-    auto key = [&](int s) { return there(s) ? evict_key(w[s]) : 0u; };
-    // the recent ones that are there, and the judged ones
-    if (t < 4) found[t] = 0;
-    __syncthreads();
-    {
-        int n = 0, r = 0;
-        for (int s = t; s < len; s += kEvictThreads) (s < old ? n : r) += there(s) ? 1 : 0;
-        n = evict_scan(n);
-        r = evict_scan(r);
-        if (lane == 63) {
-            atomicAdd(&found[0], n);
-            atomicAdd(&found[1], r);
+// A head's slots in a workgroup: `run` a wave from s0 on, thread by thread, R a thread at most.  key[j], mine and there of slot
+// s0 + 64 j + lane: keys of the judged, 0 for others; stay: bit j, a recent slot that is there.
+template <int R>
+struct EvictSlots {
+    unsigned key[R], stay;
+    int s0, n;
+    __device__ __forceinline__ void load(const PagedEvict& a, int bk, int from, int to, int len, int lane, int wave) {
+        n = (to - from + kEvictThreads - 1) / kEvictThreads;
+        s0 = from + wave * 64 * n;
+        const int b = bk / a.c.Hkv, old = max(len - a.recent, 0);
+        const int* const row = a.c.table + (size_t)b * a.c.P;
+        const float* const w = a.weights + (size_t)bk * a.slots;
+        stay = 0u;
+        int id[R];
+        float x[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int s = s0 + 64 * j + lane;
+            const bool in = j < n && s < to;
+            id[j] = in ? row[s >> a.c.shift] : -1;
+            x[j] = in && s < old ? w[s] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int s = s0 + 64 * j + lane;
+            const bool there = id[j] >= 0 && id[j] < a.c.pages;
+            key[j] = there && s < old ? evict_key(x[j]) : 0u;
+            if (there && s >= old) stay |= 1u << j;
         }
     }
+    // one histogram in LDS (bins cleared before; a barrier behind): of the keys with `prefix` under `mask`
+    __device__ __forceinline__ void count(int* hist, int pass, unsigned prefix, unsigned mask) const {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const unsigned k = key[j];
+            if (j < n && k && (k & mask) == prefix) atomicAdd(&hist[(k >> evict_shift(pass)) & (evict_bins(pass) - 1)], 1);
+        }
+    }
+    // how many lie above `prefix` (or stay), and how many are equal to it: of this wave, in every lane
+    __device__ __forceinline__ void sums(unsigned prefix, int& above, int& equal) const {
+        above = __popc(stay);
+        equal = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            above += key[j] > prefix ? 1 : 0;
+            equal += key[j] && key[j] == prefix ? 1 : 0;
+        }
+        above = __builtin_amdgcn_readlane(paged_scan(above), 63);
+        equal = __builtin_amdgcn_readlane(paged_scan(equal), 63);
+    }
+    // the kept ones, out: kept before this wave's; equal: equal ones before it, of which the first `want` are kept
+    __device__ __forceinline__ void write(const PagedEvict& a, int bk, unsigned prefix, int want, int out, int equal, int lane) const {
+        int* const kept = a.kept + (size_t)bk * a.keep;
+        float* const left = a.new_weights + (size_t)bk * a.slots;
+        const float* const w = a.weights + (size_t)bk * a.slots;
+        const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (j < n) {
+                const bool same = key[j] && key[j] == prefix;
+                const unsigned long long e = __ballot(same);
+                const bool keep = (stay >> j & 1u) || key[j] > prefix || (same && equal + __popcll(e & below) < want);
+                const unsigned long long k = __ballot(keep);
+                if (keep) {
+                    const int at = out + __popcll(k & below), s = s0 + 64 * j + lane;
+                    kept[at] = s;
+                    left[at] = w[s];
+                }
+                equal += __popcll(e);
+                out += __popcll(k);
+            }
+        }
+    }
+};
+
+// From a histogram: the bin that the key of number `want`, counted from the largest, is in, and its number there.
+__device__ __forceinline__ void evict_find(const int* hist, int pass, int (*totals)[2], int* found, unsigned& prefix, unsigned& mask,
+                                           int& want, int t, int lane, int wave) {
+    const int bins = evict_bins(pass), hi = bins - 1 - 2 * t;  // from the largest bin down, two a thread
+    const int n0 = hi >= 0 ? hist[hi] : 0, n1 = hi >= 1 ? hist[hi - 1] : 0, incl = paged_scan(n0 + n1);
+    if (lane == 63) totals[wave][0] = incl;
     __syncthreads();
-    const int judged = found[0], stay = found[1];
+    int before = incl - n0 - n1;
+#pragma unroll
+    for (int v = 0; v < kEvictWaves; ++v) before += v < wave ? totals[v][0] : 0;
+    if (n0 && before < want && before + n0 >= want) {
+        found[0] = hi;
+        found[1] = want - before;
+    } else if (n1 && before + n0 < want && before + n0 + n1 >= want) {
+        found[0] = hi - 1;
+        found[1] = want - before - n0;
+    }
+    __syncthreads();
+    prefix |= (unsigned)found[0] << evict_shift(pass);
+    mask |= (unsigned)(bins - 1) << evict_shift(pass);
+    want = found[1];
+}
+
+// What is left of a head's outputs behind its last kept slot, by `threads` threads.
+__device__ __forceinline__ void evict_rest(const PagedEvict& a, int bk, int total, int t, int threads) {
+    int* const kept = a.kept + (size_t)bk * a.keep;
+    float* const left = a.new_weights + (size_t)bk * a.slots;
+    for (int n = total + t; n < a.keep; n += threads) kept[n] = -1;
+    for (int n = total + t; n < a.slots; n += threads) left[n] = 0.0f;
+    if (bk % a.c.Hkv == 0 && t == 0) a.new_lens[bk / a.c.Hkv] = total;  // (the same for every head: holes are the sequence's)
+}
+
+template <int R>
+__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict a) {
+    __shared__ int hist[kEvictBins];
+    __shared__ int totals[kEvictWaves][2], found[2];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), bk = blockIdx.x;
+    const int len = min(max(a.c.lens[bk / a.c.Hkv], 0), a.c.P << a.c.shift);
+    EvictSlots<R> x;
+    x.load(a, bk, 0, len, len, lane, wave);
+    hist[t] = hist[t + kEvictThreads] = 0;
+    int stay, judged;
+    x.sums(0u, stay, judged);  // (every judged one lies above 0)
+    judged = stay - __builtin_amdgcn_readlane(paged_scan(__popc(x.stay)), 63);
+    if (lane == 0) {
+        totals[wave][0] = stay - judged;
+        totals[wave][1] = judged;
+    }
+    __syncthreads();
+    stay = judged = 0;
+#pragma unroll
+    for (int v = 0; v < kEvictWaves; ++v) {
+        stay += totals[v][0];
+        judged += totals[v][1];
+    }
     int want = min(judged, a.keep - stay);  // of the judged ones (recent <= keep)
-    // the key of number `want`, counted from the largest: `prefix`; `want` of those equal to it are kept
     unsigned prefix = 0u, mask = 0u;
     if (want > 0 && want < judged) {
         for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-            for (int n = t; n < 2048; n += kEvictThreads) hist[n] = 0;
-            __syncthreads();
-            for (int s = t; s < old; s += kEvictThreads) {
-                const unsigned k = key(s);
-                if (k && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            if (pass) {
+                hist[t] = hist[t + kEvictThreads] = 0;
+                __syncthreads();
             }
+            x.count(hist, pass, prefix, mask);
             __syncthreads();
-            // from the largest bin down: two bins a thread
-            const int hi = bins - 1 - 2 * t, n0 = hi >= 0 ? hist[hi] : 0, n1 = hi >= 1 ? hist[hi - 1] : 0;
-            const int incl = evict_scan(n0 + n1);
-            if (lane == 63) totals[wave][0] = incl;
-            __syncthreads();
-            int before = incl - n0 - n1;
-            for (int v = 0; v < wave; ++v) before += totals[v][0];
-            if (n0 && before < want && before + n0 >= want) {
-                found[2] = hi;
-                found[3] = want - before;
-            } else if (n1 && before + n0 < want && before + n0 + n1 >= want) {
-                found[2] = hi - 1;
-                found[3] = want - before - n0;
-            }
-            __syncthreads();
-            prefix |= (unsigned)found[2] << shift;
-            mask |= (unsigned)(bins - 1) << shift;
-            want = found[3];
-            __syncthreads();
+            evict_find(hist, pass, totals, found, prefix, mask, want, t, lane, wave);
         }
     } else {  // all of them, or none
         prefix = want > 0 ? 0u : 0xFFFFFFFFu;
         want = 0;
     }
-    // every wave has a run of slots
-    const int per = (len + kEvictThreads - 1) / kEvictThreads * 64, s0 = wave * per, s1 = min(s0 + per, len);
-    auto state = [&](int s, int& more, int& same) {
-        const bool in = s < s1;
-        const unsigned k = in && s < old ? key(s) : 0u;
-        more = (in && s >= old && there(s)) || k > prefix ? 1 : 0;
-        same = k && k == prefix ? 1 : 0;
-    };
-    int above = 0, equal = 0;
-    for (int s = s0 + lane; s - lane < s1; s += 64) {
-        int more, same;
-        state(s, more, same);
-        above += more;
-        equal += same;
-    }
-    above = evict_scan(above);
-    equal = evict_scan(equal);
-    if (lane == 63) {
+    int above, equal;
+    x.sums(prefix, above, equal);
+    __syncthreads();
+    if (lane == 0) {
         totals[wave][0] = above;
         totals[wave][1] = equal;
     }
     __syncthreads();
-    above = equal = 0;
-    int all = 0;
-    int equals = 0;
+    int before = 0, same = 0, all = 0, equals = 0;
+#pragma unroll
     for (int v = 0; v < kEvictWaves; ++v) {
-        if (v == wave) {
-            above = all;
-            equal = equals;
-        }
+        before += v < wave ? totals[v][0] : 0;
+        same += v < wave ? totals[v][1] : 0;
         all += totals[v][0];
         equals += totals[v][1];
     }
-    int out = above + min(equal, want);  // slots kept before this wave's
-    int* const kept = a.kept + (size_t)bk * a.keep;
-    float* const left = a.new_weights + (size_t)bk * a.slots;
-    for (int s = s0 + lane; s - lane < s1; s += 64) {
-        int more, same;
-        state(s, more, same);
-        const unsigned long long below = (1ull << lane) - 1, ge = __ballot(same);
-        const int rank = equal + __popcll(ge & below);  // of an equal one among the equal ones
-        const bool keep = more || (same && rank < want);
-        const unsigned long long gk = __ballot(keep);
-        if (keep) {
-            const int at = out + __popcll(gk & below);
-            kept[at] = s;
-            left[at] = w[s];
+    x.write(a, bk, prefix, want, before + min(same, want), same, lane);
+    evict_rest(a, bk, all + min(equals, want), t, kEvictThreads);
+}
+
+// The same in several launches (step 0 to 4), workgroup (head, chunk of kEvictChunk slots): histograms 0 to 2, the chunks' counts, the
+// output.  work, a head: [0] stay, [1] judged, [2 ..] histograms, then a word pair (prefix, want) a step, then (above, equal) a chunk.
+constexpr int kEvictState = 2 + 3 * kEvictBins, kEvictWords = kEvictState + 2 * 3;
+
+__global__ void __launch_bounds__(kEvictThreads) paged_clear_kernel(int* work, int words) {
+    for (int n = threadIdx.x; n < kEvictState; n += kEvictThreads) work[(size_t)blockIdx.x * words + n] = 0;
+}
+template <int STEP>
+__global__ void __launch_bounds__(kEvictThreads) paged_share_kernel(PagedEvict a, int* work, int words, int chunks) {
+    __shared__ int hist[STEP < 3 ? kEvictBins : 1];
+    __shared__ int totals[kEvictWaves][2], found[2];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int chunk = blockIdx.x % chunks, bk = blockIdx.x / chunks;
+    const int len = min(max(a.c.lens[bk / a.c.Hkv], 0), a.c.P << a.c.shift), from = chunk * kEvictChunk;
+    int* const own = work + (size_t)bk * words;
+    int* const counts = own + kEvictWords;
+    // (a chunk behind the slots still says that it has none, and step 4's clears)
+    EvictSlots<8> x;
+    x.load(a, bk, from, max(from, min(from + kEvictChunk, len)), len, lane, wave);
+    if constexpr (STEP == 0) {
+        hist[t] = hist[t + kEvictThreads] = 0;
+        __syncthreads();
+        x.count(hist, 0, 0u, 0u);
+        int above, equal;
+        x.sums(0u, above, equal);
+        const int stay = __builtin_amdgcn_readlane(paged_scan(__popc(x.stay)), 63);
+        if (lane == 0) {
+            if (stay) atomicAdd(&own[0], stay);
+            if (above - stay) atomicAdd(&own[1], above - stay);
         }
-        equal += __popcll(ge);
-        out += __popcll(gk);
+        __syncthreads();
+        for (int n = t; n < kEvictBins; n += kEvictThreads)
+            if (hist[n]) atomicAdd(&own[2 + n], hist[n]);
+        return;
     }
-    const int total = all + min(equals, want);
-    for (int n = total + t; n < a.keep; n += kEvictThreads) kept[n] = -1;
-    for (int n = total + t; n < a.slots; n += kEvictThreads) left[n] = 0.0f;
-    if (bk % a.c.Hkv == 0 && t == 0) a.new_lens[b] = total;  // (the same for every head: holes are the sequence's)
+    // what the step before has found
+    const int stay = own[0], judged = own[1];
+    unsigned prefix = 0u, mask = 0u;
+    int want = min(judged, a.keep - stay);
+    const bool search = want > 0 && want < judged;
+    if (!search) {
+        prefix = want > 0 ? 0u : 0xFFFFFFFFu;
+        want = 0;
+    } else if (STEP < 4) {
+        if (STEP > 1) {
+            prefix = (unsigned)own[kEvictState + 2 * (STEP - 2)];
+            want = own[kEvictState + 2 * (STEP - 2) + 1];
+            mask = STEP == 2 ? 0xFFE00000u : 0xFFFFFC00u;
+        }
+        evict_find(own + 2 + (STEP - 1) * kEvictBins, STEP - 1, totals, found, prefix, mask, want, t, lane, wave);
+        if (chunk == 0 && t == 0) {
+            own[kEvictState + 2 * (STEP - 1)] = (int)prefix;
+            own[kEvictState + 2 * (STEP - 1) + 1] = want;
+        }
+    } else {
+        prefix = (unsigned)own[kEvictState + 4];
+        want = own[kEvictState + 5];
+    }
+    if constexpr (STEP < 3) {
+        if (!search) return;
+        hist[t] = hist[t + kEvictThreads] = 0;
+        __syncthreads();
+        x.count(hist, STEP, prefix, mask);
+        __syncthreads();
+        for (int n = t; n < evict_bins(STEP); n += kEvictThreads)
+            if (hist[n]) atomicAdd(&own[2 + STEP * kEvictBins + n], hist[n]);
+        return;
+    }
+    int above, equal;
+    x.sums(prefix, above, equal);
+    __syncthreads();
+    if (lane == 0) {
+        totals[wave][0] = above;
+        totals[wave][1] = equal;
+    }
+    __syncthreads();
+    int before = 0, same = 0, all = 0, equals = 0;
+#pragma unroll
+    for (int v = 0; v < kEvictWaves; ++v) {
+        before += v < wave ? totals[v][0] : 0;
+        same += v < wave ? totals[v][1] : 0;
+        all += totals[v][0];
+        equals += totals[v][1];
+    }
+    if constexpr (STEP == 3) {
+        if (t == 0) {
+            counts[2 * chunk] = all;
+            counts[2 * chunk + 1] = equals;
+        }
+        return;
+    }
+    all = equals = 0;
+    for (int c = 0; c < chunks; ++c) {  // (at most 128)
+        if (c == chunk) {
+            before += all;
+            same += equals;
+        }
+        all += counts[2 * c];
+        equals += counts[2 * c + 1];
+    }
+    x.write(a, bk, prefix, want, before + min(same, want), same, lane);
+    evict_rest(a, bk, all + min(equals, want), chunk * kEvictThreads + t, chunks * kEvictThreads);
 }
 
 // The rows of the kept slots, in order, into the new table's pages: 16 bytes a thread of K and of V.
@@ -862,19 +1133,21 @@ void paged_by_type(int type, int hd, F go) {
                    : go(std::integral_constant<int, kPagedF16>(), std::integral_constant<int, 64>());
 }
 
-// Splits, and the tiles a split has at least.
+// The workgroups of the attention, and whether a unit may have several pieces.
 struct PagedShape {
-    long long units;
-    int tiles, S, least;
+    long long units, groups;
+    int tiles;
+    bool split;
 };
 PagedShape paged_shape(int B, int H, int Hkv, int cap, int type) {
     PagedShape p;
-    const int G = H / Hkv, tk = type == kPagedF32 ? 16 : 32;
+    const int G = H / Hkv, least = kWaves * (type == kPagedF32 ? 16 : 32);  // a piece's slots at least
     p.tiles = (G + 15) / 16;
     p.units = (long long)B * Hkv * p.tiles;
-    p.least = kWaves;
-    const int most = (cap + tk * p.least - 1) / (tk * p.least);
-    p.S = (int)std::max(1ll, std::min<long long>(most, 1024 / p.units));
+    const long long most = (cap + least - 1) / least;
+    p.split = most > 1 && B <= kPagedMapped;
+    // as many as run at once, two a CU; or more, for two pieces a unit
+    p.groups = p.split ? std::min(p.units * most, 512 * ((p.units + 255) / 256)) : p.units;
     return p;
 }
 
@@ -890,45 +1163,74 @@ hipError_t launch_paged_append(const PagedCache& c, const PagedNew& n, float* q_
     return hipGetLastError();
 }
 
-// The workspace: partials [unit][S][16][hd], (reference, sum) [unit][S][16][2], scores [B][H][cap], all fp32.
+// The workspace: sums [group][16][hd], (reference, sum of weights) [group][16][2], (first group, groups) [unit], scores
+// [B][H][cap].
 size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int hd, bool weights) {
     const PagedShape p = paged_shape(B, H, Hkv, cap, type);
-    const size_t parts = (size_t)p.units * p.S * 16;
-    return 4 * ((p.S > 1 ? parts * hd : 0) + (p.S > 1 || weights ? parts * 2 : 0) + (weights ? (size_t)B * H * cap : 0));
+    const size_t parts = (size_t)p.groups * 16;
+    return 4 * ((p.split ? parts * hd : 0) + (p.split || weights ? parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : 0) +
+                (weights ? (size_t)B * H * cap : 0));
 }
 
 hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void* work, hipStream_t s) {
-    const int cap = a.c.P << a.c.shift, TK = type == kPagedF32 ? 16 : 32;
+    const int cap = a.c.P << a.c.shift;
     const PagedShape p = paged_shape(a.c.B, a.H, a.c.Hkv, cap, type);
     a.G = a.H / a.c.Hkv;
     a.tiles = p.tiles;
-    a.S = p.S;
-    a.least = p.least;
     a.scale = 1.44269504088896341f / sqrtf((float)hd);
-    const size_t parts = (size_t)p.units * p.S * 16;
+    const size_t parts = (size_t)p.groups * 16;
     a.part = static_cast<float*>(work);
-    a.ml = a.part + (p.S > 1 ? parts * hd : 0);
-    a.scores = a.weights ? a.ml + parts * 2 : nullptr;
-    const long long groups = p.units * p.S, joins = p.S > 1 ? (long long)a.c.B * a.H : 0;
-    const int chunks = a.weights ? (cap + 1023) / 1024 : 0;
+    a.ml = p.split || a.weights ? a.part + (p.split ? parts * hd : 0) : nullptr;
+    a.units = reinterpret_cast<int2*>(a.ml + parts * 2);
+    a.scores = a.weights ? a.ml + parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : nullptr;
+    const long long groups = p.groups, joins = p.split ? (long long)a.c.B * a.H : 0;
+    if (groups > kPagedMaxGroups) return hipErrorInvalidValue;
+    a.groups = (int)groups;
+    const bool wide = p.groups > 16 * p.units;  // a head's pieces by 16 waves
+    const int nt = wide ? 1024 : 256, chunks = a.weights ? (cap + 4 * nt - 1) / (4 * nt) : 0;
     const long long second = joins + (long long)a.c.B * a.c.Hkv * chunks;
-    if (groups > kPagedMaxGroups || second > kPagedMaxGroups) return hipErrorInvalidValue;
+    if (second > kPagedMaxGroups) return hipErrorInvalidValue;
     paged_by_type(type, hd, [&](auto T, auto HD) {
         constexpr int t = decltype(T)::value, d = decltype(HD)::value;
         if (step) hipLaunchKernelGGL((paged_attn_kernel<t, d, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a);
         else hipLaunchKernelGGL((paged_attn_kernel<t, d, false>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a);
         if (!second) return;
-        if (step) hipLaunchKernelGGL((paged_join_kernel<d, true>), dim3((unsigned)second), dim3(256), 0, s, a, TK, (int)joins, chunks);
-        else hipLaunchKernelGGL((paged_join_kernel<d, false>), dim3((unsigned)second), dim3(256), 0, s, a, TK, (int)joins, chunks);
+        auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)second), dim3(nt), 0, s, a, (int)joins, chunks); };
+        if (step) wide ? join(paged_join_kernel<d, true, 1024>) : join(paged_join_kernel<d, true, 256>);
+        else wide ? join(paged_join_kernel<d, false, 1024>) : join(paged_join_kernel<d, false, 256>);
     });
     return hipGetLastError();
 }
 
-hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, hipStream_t s) {
-    const int esize = type == kPagedF32 ? 4 : 2, row = hd * esize, rows = 256 / (row / 16);
+// What an eviction from caches of more than kEvictAlone slots needs beside its outputs.
+size_t paged_evict_workspace(int B, int Hkv, int cap) {
+    const size_t chunks = (cap + kEvictChunk - 1) / kEvictChunk;
+    return cap <= kEvictAlone ? 0 : 4 * (size_t)B * Hkv * (kEvictWords + 2 * chunks);
+}
+
+hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, void* work, hipStream_t s) {
+    const int esize = type == kPagedF32 ? 4 : 2, row = hd * esize, rows = 256 / (row / 16), cap = a.c.P << a.c.shift;
+    const int chunks = (cap + kEvictChunk - 1) / kEvictChunk;
     const long long heads = (long long)a.c.B * a.c.Hkv, moves = heads * ((a.keep + rows - 1) / rows);
-    if (moves > kPagedMaxGroups) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)heads), dim3(kEvictThreads), 0, s, a);
+    if (moves > kPagedMaxGroups || heads * chunks > kPagedMaxGroups) return hipErrorInvalidValue;
+    const dim3 block(kEvictThreads);
+    if (cap <= kEvictAlone) {
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)heads), block, 0, s, a); };
+        if (cap <= 4 * kEvictThreads) go(paged_select_kernel<4>);
+        else if (cap <= 8 * kEvictThreads) go(paged_select_kernel<8>);
+        else if (cap <= 16 * kEvictThreads) go(paged_select_kernel<16>);
+        else go(paged_select_kernel<32>);
+    } else {
+        int* const w = static_cast<int*>(work);
+        const int words = kEvictWords + 2 * chunks;
+        hipLaunchKernelGGL(paged_clear_kernel, dim3((unsigned)heads), block, 0, s, w, words);
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * chunks)), block, 0, s, a, w, words, chunks); };
+        go(paged_share_kernel<0>);
+        go(paged_share_kernel<1>);
+        go(paged_share_kernel<2>);
+        go(paged_share_kernel<3>);
+        go(paged_share_kernel<4>);
+    }
     hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)moves), dim3(256), 0, s, a, row, esize);
     return hipGetLastError();
 }

@@ -98,7 +98,8 @@ SIGNATURES = {
     "rt_paged_attention_workspace": (ctypes.c_size_t, [_P, _I, _I]),
     "rt_paged_attention": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, ctypes.c_size_t]),
     "rt_paged_step": (_I, [_P, _P, _P, _P, _I, _P, _P, ctypes.c_size_t]),
-    "rt_paged_evict": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P]),
+    "rt_paged_evict_workspace": (ctypes.c_size_t, [_P]),
+    "rt_paged_evict": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, ctypes.c_size_t]),
     "rt_lm_head_argmax": (_I, [_P, _P, _P, _P, _F, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P]),
 }
 

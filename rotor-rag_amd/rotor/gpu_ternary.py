@@ -44,6 +44,12 @@ def _paged_workspace_bytes(kind, Hkv, page, hd, B, P, H, weights):
     return _hip.load().rt_paged_attention_workspace(_hip.PAGES.pack(16, rows, rows, 16, 16, kind, 1, Hkv, page, hd, B, P), H, weights)
 
 
+@functools.lru_cache(maxsize=1024)
+def _paged_evict_workspace_bytes(kind, Hkv, page, hd, B, P):
+    rows = Hkv * page * hd
+    return _hip.load().rt_paged_evict_workspace(_hip.PAGES.pack(16, rows, rows, 16, 16, kind, 1, Hkv, page, hd, B, P))
+
+
 @functools.lru_cache(maxsize=1)
 def _paged_types():
     torch = _torch()
@@ -844,8 +850,11 @@ class HIPTernaryOps:
         self._paged_apart("paged_evict", "weights", weights, cache, span)
         kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=self.device)
         new_lens, new_weights = torch.empty_like(lens), torch.empty_like(weights)
+        need = _paged_evict_workspace_bytes(*sizes)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._kv4_run(torch, "rt_paged_evict", self.lib.rt_paged_evict, pages, weights.data_ptr(), slots, keep, recent,
-                      new_table.data_ptr(), new_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr())
+                      new_table.data_ptr(), new_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
+                      ws.data_ptr() if need else None, need)
         return kept, new_lens, new_weights
 
     def __del__(self):

@@ -67,7 +67,8 @@ def call(lib, name, cache=CACHE, new=NEW, ctx=PTR, **kw):
         return lib.rt_paged_attention(ctx, c, a["q"], a["H"], a["weights"], a["slots"], a["out"], a["ws"], a["bytes"])
     if name == "step":
         return lib.rt_paged_step(ctx, c, n, a["weights"], a["slots"], a["out"], a["ws"], a["bytes"])
-    return lib.rt_paged_evict(ctx, c, a["weights"], a["slots"], a["keep"], a["recent"], a["table"], a["P"], a["kept"], a["lens"], a["left"])
+    return lib.rt_paged_evict(ctx, c, a["weights"], a["slots"], a["keep"], a["recent"], a["table"], a["P"], a["kept"], a["lens"], a["left"],
+                              a["ws"], a["bytes"])
 
 
 def refused(lib, name, match, **kw):
@@ -148,6 +149,17 @@ def test_refused_evictions(lib):
         refused(lib, "evict", "other memory", **bad)
 
 
+def test_refused_eviction_workspaces(lib):
+    from rotor import _hip
+
+    small, large = dict(CACHE, P=512), dict(CACHE, P=513)  # 32768 slots, and a page more
+    assert lib.rt_paged_evict_workspace(_hip.PAGES.pack(*small.values())) == 0
+    need = lib.rt_paged_evict_workspace(_hip.PAGES.pack(*large.values()))
+    assert need > 0 and lib.rt_paged_evict_workspace(_hip.PAGES.pack(*dict(large, hd=32).values())) == 0
+    for bad in (dict(bytes=need - 1), dict(ws=None), dict(ws=ODD)):
+        refused(lib, "evict", "workspace", cache=large, slots=1 << 20, **bad)
+
+
 def test_workspace_sizes(lib):
     from rotor import _hip
 
@@ -157,7 +169,7 @@ def test_workspace_sizes(lib):
     assert size(B=1, P=1) == 0                          # one split, and nothing to keep
     assert size(B=1, P=1, weights=1) >= 4 * 20 * 64     # the scores
     assert size(B=1, P=2048) > 0
-    assert size(B=512, P=2048) == 0                     # as many heads as fill the GPU
+    assert size(B=5000, P=2048) == 0                    # more heads than any launch has places for: a piece each
     assert size(B=256, P=16384, weights=1) >= 4 * 256 * 20 * (1 << 20)  # 64-bit
     for bad in [dict(H=21), dict(hd=32), dict(P=0), dict(pages=0)]:
         assert size(**bad) == 0
