@@ -454,6 +454,7 @@ struct PagedAttn {
     const float* q;
     float *out, *weights, *part, *ml, *scores;  // weights, scores: null where they are not kept
     int2* units;
+    unsigned long long *tickets, nonce;  // tickets: null where a second launch joins
     int slots;                // a row of weights
     int H, G, tiles, groups;  // G = H / Hkv, in tiles of 16; workgroups of the launch
     float scale;              // log2(e) / sqrt(hd)

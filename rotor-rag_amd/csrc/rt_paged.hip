@@ -11,7 +11,11 @@
 // Slot t of sequence b is row t % page of page table[b][t / page].  An entry outside [0, pages) is a
 // hole: its slots are not there.  Kernels look an entry up before they use it as an address, so no
 // table makes them read or write outside the cache.
+#include <time.h>
+#include <unistd.h>
+
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "rt_internal.h"
@@ -564,6 +568,93 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int
     return p;
 }
 
+// A unit's pieces are joined by the workgroup that ends last, where they are few (paged_shape).  Which one that is, its ticket
+// tells: a word of the launch's nonce and a count.  The workspace needs no clearing: the nonce is a number that none of the last
+// 2^44 launches of the process has had, a word of another is set to (nonce, 0) by whoever finds it so (if that fails, another has done it),
+// and the last leaves 0, so that the same launch can be replayed.  Sums go from one workgroup to the other past the caches of
+// their dies: stored and loaded coherent with the device, the stores done (s_waitcnt) before the count.
+constexpr int kTicketBits = 20;
+
+__device__ __forceinline__ void paged_put(float* at, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<unsigned long long*>(at),
+                       (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ v2f paged_get(const float* at) {
+    const unsigned long long w =
+        __hip_atomic_load(reinterpret_cast<const unsigned long long*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return v2f{__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32))};
+}
+// room: LDS for kLastMost floats and, behind them, a row's sums a group of threads; flag: a word of LDS.
+constexpr int kLastMost = 64;  // pieces times heads that the last workgroup joins
+template <int HD>
+__device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece& p, unsigned long long* ticket, float* out, int rows,
+                                           float* room, int* flag, int t, int lane, int wave) {
+    constexpr int L = HD / 4, NT = 64 * kWaves;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0) {
+        const unsigned long long c = __hip_atomic_fetch_add(ticket, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (int)(c & ((1u << kTicketBits) - 1)) + 1 == p.n;
+        if (last) __hip_atomic_store(ticket, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    const float* const part = a.part + (size_t)p.first * 16 * HD;
+    const float* const ml = a.ml + (size_t)p.first * 32;
+    const int n = p.n, cols = rows * L, groups = max(NT / cols, 1), grp = t / cols;
+    float* const factor = room;  // [rows][n]
+    v4f* const sums = reinterpret_cast<v4f*>(room + kLastMost);
+    constexpr int kAhead = 8;
+    v2f ahead[kAhead][2];
+    auto load = [&](int e) {  // of a group's first pieces
+        const float* const at = part + e * 4;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = grp + k * groups;
+            if (s < n) {
+                ahead[k][0] = paged_get(at + (size_t)s * 16 * HD);
+                ahead[k][1] = paged_get(at + (size_t)s * 16 * HD + 2);
+            }
+        }
+    };
+    int e = t - grp * cols;
+    const bool mine = grp < groups && e < cols;
+    if (mine) load(e);  // (while the references come)
+    for (int row = wave; row < rows; row += kWaves) {
+        const v2f x = lane < n ? paged_get(ml + lane * 32 + row * 2) : v2f{-INFINITY, 0.0f};
+        const float top = lane63(wave_reduce63(x[0], -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
+        const float f = __builtin_amdgcn_exp2f(x[0] - (top > -INFINITY ? top : 0.0f));
+        const float sum = lane63(wave_reduce63(x[1] * f, 0.0f, [](float x, float y) { return x + y; }));
+        if (lane < n) factor[row * n + lane] = sum != 0.0f ? f / sum : 0.0f;
+    }
+    __syncthreads();
+    for (; mine && e < cols; e += NT) {  // (one round where there are several groups)
+        const float* const weight = factor + e / L * n;
+        v4f y{};
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = grp + k * groups;
+            if (s < n) y += v4f{ahead[k][0][0], ahead[k][0][1], ahead[k][1][0], ahead[k][1][1]} * weight[s];
+        }
+        for (int s = grp + kAhead * groups; s < n; s += groups) {
+            const float* const at = part + e * 4 + (size_t)s * 16 * HD;
+            const v2f u = paged_get(at), v = paged_get(at + 2);
+            y += v4f{u[0], u[1], v[0], v[1]} * weight[s];
+        }
+        if (groups > 1) sums[t] = y;
+        else *reinterpret_cast<v4f*>(out + e * 4) = y;
+        if (e + NT < cols) load(e + NT);
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    if (t < cols) {
+        v4f y = sums[t];
+        for (int w = 1; w < groups; ++w) y += sums[w * cols + t];
+        *reinterpret_cast<v4f*>(out + t * 4) = y;
+    }
+}
+
 template <int T, int HD, bool STEP>
 __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a) {
     typedef AttnTile<T, HD> Tile;
@@ -586,10 +677,20 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     const int rows = min(a.G - 16 * ht, 16);
     const int h0 = kh * a.G + 16 * ht;  // the tile's first head
     const int cap = a.c.P << a.c.shift;
+    // the unit's ticket: whatever the memory held, the first to come makes it this launch's, with none counted
+    unsigned long long* const ticket = a.tickets ? a.tickets + (size_t)b * a.c.Hkv * a.tiles + p.unit : nullptr;
+    unsigned long long held = 0ull;
+    if (ticket && p.n > 1 && t == 0) held = __hip_atomic_load(ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto claim = [&] {
+        if (ticket && p.n > 1 && t == 0 && held >> kTicketBits != a.nonce)
+            __hip_atomic_compare_exchange_strong(ticket, &held, a.nonce << kTicketBits, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+    };
     Tile x;
     float m = -INFINITY, l = 0.0f;
     x.clear();
-    if (first < last) {
+    if (first >= last) claim();
+    else {
         // the pages of the wave's next 64 tiles, a tile a lane (two where a page is half a tile)
         int id0 = 0, id1 = 0;
         auto look = [&](int t) {
@@ -645,6 +746,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             }
         }
         __syncthreads();
+        claim();
         x.take(both, Tile::F16 ? power[min(i, rows - 1)] : 0, min(i, rows - 1), g);  // (columns past the last head repeat it)
         for (; at < last; at += kWaves, ++n, there0 = next0, there1 = next1) {
             const bool more = at + kWaves < last;
@@ -732,8 +834,17 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         if (p.n == 1) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
             *reinterpret_cast<v4f*>(a.out + ((size_t)b * a.H + h0 + row) * HD + d) = y * inv;
+        } else if (a.tickets) {
+            paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d, y[0], y[1]);
+            paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d + 2, y[2], y[3]);
+            if (d == 0) paged_put(a.ml + ((size_t)blockIdx.x * 16 + row) * 2, top, sum);
+            continue;
         } else *reinterpret_cast<v4f*>(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d) = y;
         if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)blockIdx.x * 16 + row) * 2) = v2f{top, sum};
+    }
+    if (a.tickets) {
+        if (p.n > 1) paged_last<HD>(a, p, ticket, a.out + ((size_t)b * a.H + h0) * HD, rows, reinterpret_cast<float*>(both), power, t, lane, wave);
+        return;
     }
     if (t == 0 && p.piece == 0 && a.ml) a.units[(size_t)b * a.c.Hkv * a.tiles + p.unit] = make_int2(p.first, p.n);
 }
@@ -1137,7 +1248,7 @@ void paged_by_type(int type, int hd, F go) {
 struct PagedShape {
     long long units, groups;
     int tiles;
-    bool split;
+    bool split, last;  // last: joined by a unit's last workgroup
 };
 PagedShape paged_shape(int B, int H, int Hkv, int cap, int type) {
     PagedShape p;
@@ -1148,6 +1259,12 @@ PagedShape paged_shape(int B, int H, int Hkv, int cap, int type) {
     p.split = most > 1 && B <= kPagedMapped;
     // as many as run at once, two a CU; or more, for two pieces a unit
     p.groups = p.split ? std::min(p.units * most, 512 * ((p.units + 255) / 256)) : p.units;
+    // The last workgroup joins where no unit has more than 32 pieces, or 64 heads of pieces: a launch less on the host (3.5 us),
+    // and on the GPU, us in two launches / one: 20 heads over 5, 1000 slots 6.4 + 3.2 / 8.6, 2000 6.3 + 3.8 / 9.0, 4000 (32 pieces of
+    // 4 heads) 6.9 + 4.4 / 12.5; 32 over 2, 500 6.8 + 3.4 / 10.6; 16 over 1, 1000 (8 of 16) 6.8 + 3.8 / 11.3; 5 over 5, 8000 (63 of 1)
+    // 9.8 + 4.2 / 15.7; one workgroup then reads what many would.
+    const long long pieces = std::min(most, p.groups / ((long long)Hkv * p.tiles));
+    p.last = p.split && pieces <= 32 && pieces * std::min(G, 16) <= kLastMost;
     return p;
 }
 
@@ -1165,9 +1282,21 @@ hipError_t launch_paged_append(const PagedCache& c, const PagedNew& n, float* q_
 
 // The workspace: sums [group][16][hd], (reference, sum of weights) [group][16][2], (first group, groups) [unit], scores
 // [B][H][cap].
+namespace {
+// Where the launches' numbers start: some 44 bits that memory does not hold by itself.
+unsigned long long paged_seed() {
+    timespec t{};
+    clock_gettime(CLOCK_REALTIME, &t);
+    unsigned long long z = (unsigned long long)t.tv_sec * 1000000000ull + (unsigned long long)t.tv_nsec + ((unsigned long long)getpid() << 40);
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;  // (SplitMix64's finaliser)
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+}  // namespace
 size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int hd, bool weights) {
     const PagedShape p = paged_shape(B, H, Hkv, cap, type);
     const size_t parts = (size_t)p.groups * 16;
+    // (first group, groups) or, in its place, the ticket of a unit
     return 4 * ((p.split ? parts * hd : 0) + (p.split || weights ? parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : 0) +
                 (weights ? (size_t)B * H * cap : 0));
 }
@@ -1183,7 +1312,15 @@ hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void
     a.ml = p.split || a.weights ? a.part + (p.split ? parts * hd : 0) : nullptr;
     a.units = reinterpret_cast<int2*>(a.ml + parts * 2);
     a.scores = a.weights ? a.ml + parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : nullptr;
-    const long long groups = p.groups, joins = p.split ? (long long)a.c.B * a.H : 0;
+    const bool last = p.last && !a.weights;
+    if (last) {
+        static std::atomic<unsigned long long> number{paged_seed()};
+        const unsigned long long most = ~0ull >> kTicketBits;
+        do a.nonce = number.fetch_add(1, std::memory_order_relaxed) & most;
+        while (a.nonce == 0);
+        a.tickets = reinterpret_cast<unsigned long long*>(a.units);
+    }
+    const long long groups = p.groups, joins = p.split && !last ? (long long)a.c.B * a.H : 0;
     if (groups > kPagedMaxGroups) return hipErrorInvalidValue;
     a.groups = (int)groups;
     const bool wide = p.groups > 16 * p.units;  // a head's pieces by 16 waves

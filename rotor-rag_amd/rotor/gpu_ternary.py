@@ -708,9 +708,18 @@ class HIPTernaryOps:
             raise ValueError("paged_cache: needs head_dim 64 or 128, page 16, 32, 64, 128 or 256, bfloat16, float16 or float32")
         return torch.full((2, int(n_pages), int(n_kv_heads), page, head_dim), float("nan"), dtype=dtype, device=self.device)
 
-    def _paged_ints(self, who, torch, name, x, shape):
-        if x.dtype is not torch.int32 or x.shape != shape or x.get_device() != self.device_index or not x.is_contiguous():
-            raise ValueError(f"{who}: {name} must be a contiguous int32 {list(shape)} tensor on the backend's device")
+    # (As with the calls above: each tensor is looked at once, and what is as the library takes it is not touched.)
+    def _paged_int(self, who, torch, name, x, B):
+        if (x.dtype is not torch.int32 or x.get_device() != self.device_index or not x.is_contiguous() or x.shape != (B,)):
+            raise ValueError(f"{who}: {name} must be a contiguous int32 [{B}] tensor on the backend's device")
+        return x.data_ptr()
+
+    def _paged_table(self, who, torch, name, x):
+        """[B, P] of a table."""
+        shape = x.shape
+        if x.dtype is not torch.int32 or x.get_device() != self.device_index or not x.is_contiguous() or len(shape) != 2:
+            raise ValueError(f"{who}: {name} must be a contiguous int32 [B, P] tensor on the backend's device")
+        return shape
 
     def _paged_check(self, who, torch, cache, table, lens):
         """(rt_pages, (type, Hkv, page, hd, B, P), bytes that the cache's pages span) of a cache, its table and lengths."""
@@ -722,32 +731,37 @@ class HIPTernaryOps:
         rows = Hkv * page * hd
         if strides[4] != 1 or strides[3] != hd or (strides[2] != page * hd and Hkv > 1):
             raise ValueError(f"{who}: a page's [Hkv, page, head_dim] must be contiguous")
-        if len(table.shape) != 2:
-            raise ValueError(f"{who}: table must be int32 [B, P]")
-        B, P = table.shape
-        self._paged_ints(who, torch, "table", table, (B, P))
-        self._paged_ints(who, torch, "lens", lens, (B,))
-        step = strides[1] if pages > 1 else rows
-        span = (strides[0] + (pages - 1) * step + rows) * cache.element_size()
-        return (_hip.PAGES.pack(cache.data_ptr(), strides[0], step, table.data_ptr(), lens.data_ptr(), kind, pages, Hkv, page, hd, B, P),
-                (kind, Hkv, page, hd, B, P), span)
+        B, P = self._paged_table(who, torch, "table", table)
+        apart, step = strides[0], strides[1] if pages > 1 else rows
+        return (_hip.PAGES.pack(cache.data_ptr(), apart, step, table.data_ptr(), self._paged_int(who, torch, "lens", lens, B), kind, pages,
+                                Hkv, page, hd, B, P),
+                (kind, Hkv, page, hd, B, P), (apart + (pages - 1) * step + rows) * (2 if kind else 4))
+
+    def _paged_in(self, torch, x):
+        """x as the library takes it: itself, or as _kv4_in copies it."""
+        if isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.get_device() == self.device_index and x.is_contiguous():
+            at = x.data_ptr()
+            if not at & 15:
+                return x, at
+        x = self._kv4_in(torch, x)
+        return x, x.data_ptr()
 
     def _paged_new(self, who, torch, q, k, v, rope, pos, counts, interleaved, sizes):
-        """(rt_paged_new, the tensors it names) of new tokens."""
+        """(rt_paged_new, q, (M, H), the other tensors that it names) of new tokens."""
         _, Hkv, _, hd, B, _ = sizes
-        q, k, v, rope = (self._kv4_in(torch, x) for x in (q, k, v, rope))
+        (q, at_q), (k, at_k), (v, at_v), (rope, at_rope) = (self._paged_in(torch, q), self._paged_in(torch, k),
+                                                            self._paged_in(torch, v), self._paged_in(torch, rope))
         M, H = self._kv4_rows(who, q, B, Hkv, hd)
-        if k.shape != (B, M, Hkv, hd) or v.shape != (B, M, Hkv, hd):
-            raise ValueError(f"{who}: k and v must be {[B, M, Hkv, hd]}")
+        rows = (B, M, Hkv, hd)
+        if k.shape != rows or v.shape != rows:
+            raise ValueError(f"{who}: k and v must be {list(rows)}")
         table = rope.shape
         if len(table) != 3 or table[2] != 2 or table[1] % 4 or not 0 < 2 * table[1] <= hd or not table[0]:
             raise ValueError(f"{who}: rope must be [positions, rotary / 2, 2], rotary a multiple of 8 up to head_dim")
-        self._paged_ints(who, torch, "pos", pos, (B,))
-        if counts is not None:
-            self._paged_ints(who, torch, "counts", counts, (B,))
-        new = _hip.PAGED_NEW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), pos.data_ptr(),
-                                  counts.data_ptr() if counts is not None else 0, table[0], 2 * table[1], bool(interleaved), M, H)
-        return new, (q, k, v, rope, pos, *(() if counts is None else (counts,)))
+        new = _hip.PAGED_NEW.pack(at_q, at_k, at_v, at_rope, self._paged_int(who, torch, "pos", pos, B),
+                                  self._paged_int(who, torch, "counts", counts, B) if counts is not None else 0, table[0], 2 * table[1],
+                                  bool(interleaved), M, H)
+        return new, q, (M, H), (k, v, rope, pos) if counts is None else (k, v, rope, pos, counts)
 
     def _paged_apart(self, who, name, x, cache, span, *others):
         """x, which the call writes, lies in none of the others."""
@@ -779,9 +793,11 @@ class HIPTernaryOps:
         slot are not written; their q is 0.  lens is not changed.  For inference: gradients do not pass."""
         torch = _torch()
         pages, sizes, span = self._paged_check("paged_append", torch, cache, table, lens)
-        new, kept = self._paged_new("paged_append", torch, q, k, v, rope, pos, counts, interleaved, sizes)
-        out = self._kv4_out("paged_append", torch, q_out, *kept, table, lens)
-        if q_out is not None:
+        new, q, _, others = self._paged_new("paged_append", torch, q, k, v, rope, pos, counts, interleaved, sizes)
+        if q_out is None:
+            out = torch.empty_like(q)
+        else:
+            out = self._kv4_out("paged_append", torch, q_out, q, *others, table, lens)
             self._paged_apart("paged_append", "q_out", out, cache, span)
         self._kv4_run(torch, "rt_paged_append", self.lib.rt_paged_append, pages, new, out.data_ptr())
         return out
@@ -793,12 +809,12 @@ class HIPTernaryOps:
         query heads) is added to it, for paged_evict.  For inference: gradients do not pass."""
         torch = _torch()
         pages, sizes, span = self._paged_check("paged_attention", torch, cache, table, lens)
-        q = self._kv4_in(torch, q)
+        q, at = self._paged_in(torch, q)
         M, H = self._kv4_rows("paged_attention", q, sizes[4], sizes[1], sizes[3])
         if M != 1:
             raise ValueError("paged_attention: takes one token a sequence")
-        out = self._paged_attend("paged_attention", torch, out, q, cache, span, sizes, H, weights, (table, lens),
-                                 lambda *a: (self.lib.rt_paged_attention, pages, q.data_ptr(), H, *a))
+        out, args = self._paged_attend("paged_attention", torch, out, q, cache, span, sizes, H, weights, (table, lens))
+        self._kv4_run(torch, "rt_paged_attention", self.lib.rt_paged_attention, pages, at, H, *args[1:])
         return out
 
     def paged_step(self, q, k, v, cache, table, lens, rope, pos, interleaved: bool = False, weights=None, out=None):
@@ -807,27 +823,29 @@ class HIPTernaryOps:
         attends to nothing.  lens is not changed: the next step's is lens + 1."""
         torch = _torch()
         pages, sizes, span = self._paged_check("paged_step", torch, cache, table, lens)
-        new, kept = self._paged_new("paged_step", torch, q, k, v, rope, pos, None, interleaved, sizes)
-        H, M = kept[0].shape[2], kept[0].shape[1]
+        new, q, (M, H), others = self._paged_new("paged_step", torch, q, k, v, rope, pos, None, interleaved, sizes)
         if M != 1:
             raise ValueError("paged_step: takes one token a sequence")
-        return self._paged_attend("paged_step", torch, out, kept[0], cache, span, sizes, H, weights, (*kept[1:], table, lens),
-                                  lambda *a: (self.lib.rt_paged_step, pages, new, *a))
-
-    def _paged_attend(self, who, torch, out, q, cache, span, sizes, H, weights, others, call):
-        given = out is not None
-        out = self._kv4_out(who, torch, out, q, *others)
-        if given:
-            self._paged_apart(who, "out", out, cache, span)
-        slots = 0
-        if weights is not None:
-            slots = self._paged_weights(who, torch, weights, sizes)
-            self._paged_apart(who, "weights", weights, cache, span, q, out, *others)
-        need = _paged_workspace_bytes(*sizes, H, int(weights is not None))
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        fn, *args = call(weights.data_ptr() if slots else None, slots, out.data_ptr(), ws.data_ptr() if need else None, need)
-        self._kv4_run(torch, "rt_" + who, fn, *args)
+        out, args = self._paged_attend("paged_step", torch, out, q, cache, span, sizes, H, weights, (*others, table, lens))
+        self._kv4_run(torch, "rt_paged_step", self.lib.rt_paged_step, pages, new, *args[1:])
         return out
+
+    def _paged_attend(self, who, torch, out, q, cache, span, sizes, H, weights, others):
+        """(out, (workspace, the arguments that follow the queries))."""
+        if out is None:
+            out = torch.empty_like(q)
+        else:
+            out = self._kv4_out(who, torch, out, q, *others)
+            self._paged_apart(who, "out", out, cache, span)
+        at, slots = None, 0
+        if weights is not None:
+            slots, at = self._paged_weights(who, torch, weights, sizes), weights.data_ptr()
+            self._paged_apart(who, "weights", weights, cache, span, q, out, *others)
+        need = _paged_workspace_bytes(*sizes, H, slots > 0)
+        if not need:
+            return out, (None, at, slots, out.data_ptr(), None, 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return out, (ws, at, slots, out.data_ptr(), ws.data_ptr(), need)
 
     def paged_evict(self, cache, table, lens, weights, keep: int, recent: int, new_table):
         """Cuts every sequence of a paged cache to `keep` slots (rt_paged_evict): for each KV head the last `recent` and, of
@@ -841,10 +859,10 @@ class HIPTernaryOps:
         _, Hkv, page, _, B, _ = sizes
         slots = self._paged_weights("paged_evict", torch, weights, sizes)
         keep, recent = operator.index(keep), operator.index(recent)
-        if len(new_table.shape) != 2:
-            raise ValueError("paged_evict: new_table must be int32 [B, new_P]")
-        self._paged_ints("paged_evict", torch, "new_table", new_table, (B, new_table.shape[1]))
-        if not (0 <= recent <= keep and 0 < keep <= new_table.shape[1] * page):
+        new_B, new_P = self._paged_table("paged_evict", torch, "new_table", new_table)
+        if new_B != B:
+            raise ValueError(f"paged_evict: new_table must be int32 [{B}, new_P]")
+        if not (0 <= recent <= keep and 0 < keep <= new_P * page):
             raise ValueError(f"paged_evict: keep {keep} and recent {recent}: needs 0 <= recent <= keep, and pages for keep >= 1 slots")
         self._paged_apart("paged_evict", "new_table", new_table, cache, span, table)
         self._paged_apart("paged_evict", "weights", weights, cache, span)
@@ -853,7 +871,7 @@ class HIPTernaryOps:
         need = _paged_evict_workspace_bytes(*sizes)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._kv4_run(torch, "rt_paged_evict", self.lib.rt_paged_evict, pages, weights.data_ptr(), slots, keep, recent,
-                      new_table.data_ptr(), new_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
+                      new_table.data_ptr(), new_P, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(),
                       ws.data_ptr() if need else None, need)
         return kept, new_lens, new_weights
 
