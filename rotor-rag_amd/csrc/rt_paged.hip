@@ -124,7 +124,8 @@ __device__ __forceinline__ long long paged_slot(const PagedCache& c, int HD, int
 // ---- append ------------------------------------------------------------------------------
 // A thread has 8 dimensions of one head of one row (q heads, then k, then v heads), both halves of its pairs: each number is read
 // and written once, by one thread, so q_out may be q.  Bound by memory: 8 prompts of up to 2048 tokens (20 heads over 5 of
-// 128, bf16) 77 us, 5.3 TB/s.
+// 128, bf16), one call after the other, 77.5 us, 5.25 TB/s; with the
+// queries' stores through the caches 88.
 template <int T, int HD>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNew n, float* q_out, int M, int H) {
     constexpr int L = HD / 8;
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNe
     if (at >= 0 && !is_v) paged_rotate8(x, y, n.rope + (size_t)p * n.rotary, o, n.rotary, n.interleaved);
     if (is_q) {
         float* const to = q_out + ((size_t)row * H + unit) * HD;
-        *reinterpret_cast<v4f*>(to + d.x) = at >= 0 ? x : v4f{};
-        *reinterpret_cast<v4f*>(to + d.y) = at >= 0 ? y : v4f{};
+        __builtin_nontemporal_store(at >= 0 ? x : v4f{}, reinterpret_cast<v4f*>(to + d.x));
+        __builtin_nontemporal_store(at >= 0 ? y : v4f{}, reinterpret_cast<v4f*>(to + d.y));
     } else if (at >= 0) {
         E* const to = static_cast<E*>(c.cache) + (is_v ? c.kv_stride : 0) + at + ((long long)kh << c.shift) * HD;
         paged_store4<T>(to + d.x, x);
@@ -179,8 +180,15 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNe
 //
 // Every load is issued half a round before its use: the next tile's keys when this one's are multiplied, its values after
 // this one's.
-template <int T, int HD>
+template <int T, int HD, bool ONCE>
 struct AttnTile;
+
+// A load of numbers that no other workgroup reads goes past the caches (launch_paged_attention has the measure).
+template <bool ONCE, typename V, typename E>
+__device__ __forceinline__ V paged_load(const E* at) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(at));
+    else return *reinterpret_cast<const V*>(at);
+}
 
 // The largest of lanes l, l ^ 16, l ^ 32, l ^ 48; their sum.
 __device__ __forceinline__ float paged_max4(float x) {
@@ -255,7 +263,7 @@ __device__ __forceinline__ void paged_split(v4f x, v2u (&t)[3]) {
 }
 
 // Tiles of 32 slots in 16 bits: two row tiles of 16.
-template <int T, int HD>
+template <int T, int HD, bool ONCE>
 struct AttnTile {
     static constexpr int TK = 32, NS = 8, NC = HD / 32, NO = HD / 16;  // NS scores a lane; NO sums (of 4 dimensions) a lane
     static constexpr bool F16 = T == kPagedF16;
@@ -271,18 +279,18 @@ struct AttnTile {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) k[tt][c] = *reinterpret_cast<const v4u*>((tt ? base1 : base0) + (i * HD + c * 32 + g * 8));
+            for (int c = 0; c < NC; ++c) k[tt][c] = paged_load<ONCE, v4u>((tt ? base1 : base0) + (i * HD + c * 32 + g * 8));
     }
     __device__ __forceinline__ void load_v(const E* base0, const E* base1, int i, int g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const E* at = (e < 4 ? base0 : base1) + ((4 * g + (e & 3)) * HD + i * (HD / 16));
             if constexpr (HD == 128) {
-                const v4u x = *reinterpret_cast<const v4u*>(at);
+                const v4u x = paged_load<ONCE, v4u>(at);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) v[e][w] = x[w];
             } else {
-                const v2u x = *reinterpret_cast<const v2u*>(at);
+                const v2u x = paged_load<ONCE, v2u>(at);
                 v[e][0] = x[0];
                 v[e][1] = x[1];
             }
@@ -392,8 +400,8 @@ struct AttnTile {
 };
 
 // Tiles of 16 slots in fp32.
-template <int HD>
-struct AttnTile<kPagedF32, HD> {
+template <int HD, bool ONCE>
+struct AttnTile<kPagedF32, HD, ONCE> {
     static constexpr int TK = 16, NS = 4, NC = HD / 16, NU = HD / 64;
     static constexpr bool F16 = false;
     typedef float E;
@@ -401,13 +409,13 @@ struct AttnTile<kPagedF32, HD> {
 
     __device__ __forceinline__ void load_k(const E* base0, const E*, int i, int g) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) k[c] = *reinterpret_cast<const v4f*>(base0 + (i * HD + c * 16 + g * 4));
+        for (int c = 0; c < NC; ++c) k[c] = paged_load<ONCE, v4f>(base0 + (i * HD + c * 16 + g * 4));
     }
     __device__ __forceinline__ void load_v(const E* base0, const E*, int i, int g) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int u = 0; u < NU; ++u) v[r][u] = *reinterpret_cast<const v4f*>(base0 + ((4 * g + r) * HD + u * 64 + i * 4));
+            for (int u = 0; u < NU; ++u) v[r][u] = paged_load<ONCE, v4f>(base0 + ((4 * g + r) * HD + u * 64 + i * 4));
     }
     static __device__ __forceinline__ int slot(int n, int g) { return 4 * g + n; }
     __device__ __forceinline__ void put(const E* nk, const E* nv, int at, int i, int g) {
@@ -655,9 +663,9 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
     }
 }
 
-template <int T, int HD, bool STEP>
+template <int T, int HD, bool STEP, bool ONCE>
 __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a) {
-    typedef AttnTile<T, HD> Tile;
+    typedef AttnTile<T, HD, ONCE> Tile;
     typedef typename Tile::E E;
     constexpr int TK = Tile::TK, L = HD / 4;
     // the queries, and in their place, when all waves have taken them, the waves' sums
@@ -1214,7 +1222,8 @@ __global__ void __launch_bounds__(kEvictThreads) paged_share_kernel(PagedEvict a
     evict_rest(a, bk, all + min(equals, want), chunk * kEvictThreads + t, chunks * kEvictThreads);
 }
 
-// The rows of the kept slots, in order, into the new table's pages: 16 bytes a thread of K and of V.
+// The rows of the kept slots, in order, into the new table's pages: 16 bytes a thread of K and of V, past the caches
+// (16 sequences of 1000 to 8191 cut to 4096: the whole eviction 63.4 us through them, so 59.8).
 __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvict a, int row_bytes, int esize) {
     const int lanes = row_bytes / 16, rows = 256 / lanes, t = threadIdx.x;
     const int chunks = (a.keep + rows - 1) / rows, chunk = blockIdx.x % chunks, bk = blockIdx.x / chunks;
@@ -1229,9 +1238,9 @@ __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvict a, int row_b
     const long long src = (long long)from * a.c.page_stride * esize + (long long)(s & in_page) * row_bytes;
     const long long dst = (long long)to * a.c.page_stride * esize + (long long)(n & in_page) * row_bytes;
     const long long v = a.c.kv_stride * esize;
-    const v4u x = *reinterpret_cast<const v4u*>(base + src), y = *reinterpret_cast<const v4u*>(base + src + v);
-    *reinterpret_cast<v4u*>(base + dst) = x;
-    *reinterpret_cast<v4u*>(base + dst + v) = y;
+    const v4u x = paged_load<true, v4u>(base + src), y = paged_load<true, v4u>(base + src + v);
+    __builtin_nontemporal_store(x, reinterpret_cast<v4u*>(base + dst));
+    __builtin_nontemporal_store(y, reinterpret_cast<v4u*>(base + dst + v));
 }
 
 template <typename F>
@@ -1329,8 +1338,14 @@ hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void
     if (second > kPagedMaxGroups) return hipErrorInvalidValue;
     paged_by_type(type, hd, [&](auto T, auto HD) {
         constexpr int t = decltype(T)::value, d = decltype(HD)::value;
-        if (step) hipLaunchKernelGGL((paged_attn_kernel<t, d, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a);
-        else hipLaunchKernelGGL((paged_attn_kernel<t, d, false>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a);
+        auto attend = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a); };
+        // Keys and values that one workgroup reads, once, go past the caches: 131072 slots (20 heads over 5 of 128, bf16) 61.0 us,
+        // so 54.8; 32 sequences of 100 to 4095 34.3 / 32.3 (a cache of 168 MB that is read again and again, as nothing between
+        // does in a model, 28.2 / 31.1).  Where tiles of heads share them, through the caches: 32 x 16000 slots,
+        // 32 heads over 1 58.1 / 69.9, 64 100 / 141 (16 50.4 / 44.8).
+        const bool once = p.tiles == 1;
+        if (step) once ? attend(paged_attn_kernel<t, d, true, true>) : attend(paged_attn_kernel<t, d, true, false>);
+        else once ? attend(paged_attn_kernel<t, d, false, true>) : attend(paged_attn_kernel<t, d, false, false>);
         if (!second) return;
         auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)second), dim3(nt), 0, s, a, (int)joins, chunks); };
         if (step) wide ? join(paged_join_kernel<d, true, 1024>) : join(paged_join_kernel<d, true, 256>);
