@@ -945,7 +945,10 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
 // there).  The smallest that is kept is found from histograms of its upper 11 bits, of the next 11 among those that have these,
 // and of the last 10.  Then every wave counts the kept of its run of slots, and writes them out behind those of the waves before.
 // A workgroup of 1024 threads takes a KV head of a sequence, up to 32 slots a thread in registers; longer caches are shared among
-// workgroups of 8 slots a thread, in a launch for every histogram and two for the output.
+// workgroups of 8 slots a thread, in a launch for every histogram and two for the output, all launches us, alone / shared: 5 heads
+// of 16000 slots 16 / 32, 32000 33 / 32 (and five launches more on the host), 80 heads 39 / 49, 300 heads 69 / 99; 10 heads of
+// 131072 slots by one workgroup each, the weights read again for every pass, 359 / 35.  Bound by the passes' latencies: 128 heads of up
+// to 8191 slots take 12 us for 12 MB.
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictBins = 2048;
 constexpr int kEvictAlone = 32 * kEvictThreads, kEvictChunk = 8 * kEvictThreads;
 
@@ -1014,27 +1017,35 @@ struct EvictSlots {
         float* const left = a.new_weights + (size_t)bk * a.slots;
         const float* const w = a.weights + (size_t)bk * a.slots;
         const unsigned long long below = (1ull << lane) - 1;
+        constexpr int N = R < 8 ? R : 8;
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if (j < n) {
-                const bool same = key[j] && key[j] == prefix;
+        for (int j0 = 0; j0 < R; j0 += N) {
+            if (j0 >= n) break;
+            float x[N];  // (asked for at once, not one by one behind each slot's decision)
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = key[j0 + j] || (stay >> (j0 + j) & 1u) ? w[s0 + 64 * (j0 + j) + lane] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const unsigned k = key[j0 + j];
+                const bool same = k && k == prefix;
                 const unsigned long long e = __ballot(same);
-                const bool keep = (stay >> j & 1u) || key[j] > prefix || (same && equal + __popcll(e & below) < want);
-                const unsigned long long k = __ballot(keep);
+                const bool keep = (stay >> (j0 + j) & 1u) || k > prefix || (same && equal + __popcll(e & below) < want);
+                const unsigned long long all = __ballot(keep);
                 if (keep) {
-                    const int at = out + __popcll(k & below), s = s0 + 64 * j + lane;
-                    kept[at] = s;
-                    left[at] = w[s];
+                    const int at = out + __popcll(all & below);
+                    kept[at] = s0 + 64 * (j0 + j) + lane;
+                    left[at] = x[j];
                 }
                 equal += __popcll(e);
-                out += __popcll(k);
+                out += __popcll(all);
             }
         }
     }
 };
 
-// From a histogram: the bin that the key of number `want`, counted from the largest, is in, and its number there.
-__device__ __forceinline__ void evict_find(const int* hist, int pass, int (*totals)[2], int* found, unsigned& prefix, unsigned& mask,
+// From a histogram: the bin that the key of number `want`, counted from the largest, is in, and its number there.  True where the
+// whole bin is kept.
+__device__ __forceinline__ bool evict_find(const int* hist, int pass, int (*totals)[2], int* found, unsigned& prefix, unsigned& mask,
                                            int& want, int t, int lane, int wave) {
     const int bins = evict_bins(pass), hi = bins - 1 - 2 * t;  // from the largest bin down, two a thread
     const int n0 = hi >= 0 ? hist[hi] : 0, n1 = hi >= 1 ? hist[hi - 1] : 0, incl = paged_scan(n0 + n1);
@@ -1046,14 +1057,17 @@ __device__ __forceinline__ void evict_find(const int* hist, int pass, int (*tota
     if (n0 && before < want && before + n0 >= want) {
         found[0] = hi;
         found[1] = want - before;
+        found[2] = n0;
     } else if (n1 && before + n0 < want && before + n0 + n1 >= want) {
         found[0] = hi - 1;
         found[1] = want - before - n0;
+        found[2] = n1;
     }
     __syncthreads();
     prefix |= (unsigned)found[0] << evict_shift(pass);
     mask |= (unsigned)(bins - 1) << evict_shift(pass);
     want = found[1];
+    return want == found[2];
 }
 
 // What is left of a head's outputs behind its last kept slot, by `threads` threads.
@@ -1068,7 +1082,7 @@ __device__ __forceinline__ void evict_rest(const PagedEvict& a, int bk, int tota
 template <int R>
 __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict a) {
     __shared__ int hist[kEvictBins];
-    __shared__ int totals[kEvictWaves][2], found[2];
+    __shared__ int totals[kEvictWaves][2], found[3];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), bk = blockIdx.x;
     const int len = min(max(a.c.lens[bk / a.c.Hkv], 0), a.c.P << a.c.shift);
     EvictSlots<R> x;
@@ -1098,7 +1112,11 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict 
             }
             x.count(hist, pass, prefix, mask);
             __syncthreads();
-            evict_find(hist, pass, totals, found, prefix, mask, want, t, lane, wave);
+            if (evict_find(hist, pass, totals, found, prefix, mask, want, t, lane, wave)) {
+                prefix = max(prefix, 1u) - 1u;  // right below the bin (keys are 1 and up), and none of those equal to it
+                want = 0;
+                break;
+            }
         }
     } else {  // all of them, or none
         prefix = want > 0 ? 0u : 0xFFFFFFFFu;
@@ -1134,7 +1152,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_clear_kernel(int* work, i
 template <int STEP>
 __global__ void __launch_bounds__(kEvictThreads) paged_share_kernel(PagedEvict a, int* work, int words, int chunks) {
     __shared__ int hist[STEP < 3 ? kEvictBins : 1];
-    __shared__ int totals[kEvictWaves][2], found[2];
+    __shared__ int totals[kEvictWaves][2], found[3];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int chunk = blockIdx.x % chunks, bk = blockIdx.x / chunks;
     const int len = min(max(a.c.lens[bk / a.c.Hkv], 0), a.c.P << a.c.shift), from = chunk * kEvictChunk;

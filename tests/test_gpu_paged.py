@@ -202,6 +202,81 @@ def test_attention_many_heads_long(hip):
     check_attention(hip, cache, table, n, queries(lens, 4, 64))
 
 
+def test_attention_large_batches(hip):
+    """More sequences than lanes, and than a launch has places to cut them for; more heads than a workgroup's tile."""
+    gen = torch.Generator().manual_seed(12)
+    lens = torch.randint(0, 600, (130,), generator=gen).tolist() + [3000]
+    cache, table, n = make(lens, 2, 64, 32, "bf16")
+    check_attention(hip, cache, table, n, queries(lens, 4, 64), weights=torch.zeros(131, 2, table.shape[1] * 32))
+    lens = torch.randint(0, 20, (4200,), generator=gen).tolist() + [300]
+    cache, table, n = make(lens, 1, 64, 16, "fp16")
+    check_attention(hip, cache, table, n, queries(lens, 1, 64))
+    check_attention(hip, cache, table, n, queries(lens, 1, 64), weights=torch.zeros(4201, 1, table.shape[1] * 16))
+    lens = [900, 40]
+    cache, table, n = make(lens, 1, 64, 16, "bf16")
+    check_attention(hip, cache, table, n, queries(lens, 1024, 64), weights=torch.zeros(2, 1, table.shape[1] * 16))
+
+
+def test_attention_table_much_longer_than_needed(hip):
+    """A table for 2^20 slots over sequences that hold a few."""
+    lens = [70, 0, 1300]
+    for dtype in TYPES:
+        cache, table, n = make(lens, 2, 64, 64, dtype)
+        wide = torch.full((3, 1 << 14), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        q = queries(lens, 8, 64)
+        got = check_attention(hip, cache, wide, n, q)
+        start = torch.zeros(3, 2, 1 << 20)
+        w = start.cuda()
+        o, sums, size, most = PO.attend(q, cache, table, n)
+        again = hip.paged_attention(q.cuda(), cache.cuda(), wide.cuda(), n.cuda(), weights=w)
+        assert ((again.cpu().double() - o).abs() <= attention_bound(o, size, most, n)).all() and (w[:, :, 1344:] == 0).all()
+        assert ((w[:, :, :1344].cpu().double() - sums).abs() <= 1e-5 * sums + 1e-30).all() and torch.allclose(got, again, atol=1e-5)
+
+
+def test_attention_workspace_holds_anything(hip):
+    """The same workspace, whatever is in it: noise, ones, the words of the calls before, other shapes'."""
+    from rotor import _hip
+
+    cases = []
+    for lens, H, Hkv, hd in (([1500], 20, 5, 128), ([900, 200], 8, 2, 64), ([300] * 7, 12, 12, 64)):
+        cache, table, n = make(lens, Hkv, hd, 64, "bf16")
+        q = queries(lens, H, hd)
+        o, _, size, most = PO.attend(q, cache, table, n)
+        bound = attention_bound(o, size, most, n)
+        c, t, m = cache.cuda(), table.cuda(), n.cuda()
+        rows = Hkv * 64 * hd
+        pages = _hip.PAGES.pack(c.data_ptr(), c.stride(0), rows, t.data_ptr(), m.data_ptr(), _hip.PAGED_BF16, c.shape[1], Hkv, 64, hd, len(lens), t.shape[1])
+        cases.append((pages, q.cuda(), H, o, bound, (c, t, m)))
+    need = max(hip.lib.rt_paged_attention_workspace(c[0], c[2], 0) for c in cases)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    fills = [lambda: ws.fill_(255), lambda: ws.random_(0, 256), lambda: ws.zero_()] + [lambda: None] * 6
+    hip._bind_stream()
+    for fill in fills:
+        fill()
+        for pages, q, H, o, bound, _ in cases:
+            outs = [torch.empty_like(q) for _ in range(2)]
+            for out in outs:  # (one behind the other, nothing waits)
+                _hip.check(hip.lib.rt_paged_attention(hip.ctx, pages, q.data_ptr(), H, None, 0, out.data_ptr(), ws.data_ptr(), need))
+            assert ((outs[0].cpu().double() - o).abs() <= bound).all() and torch.equal(outs[0], outs[1])
+
+
+def test_attention_on_two_streams(hip):
+    """Calls that run at the same time."""
+    cache, table, n = make([1500, 700], 5, 128, 64, "bf16")
+    q = queries([0] * 2, 20, 128).cuda()
+    c, t, m = cache.cuda(), table.cuda(), n.cuda()
+    want = hip.paged_attention(q, c, t, m)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(hip.paged_attention(q, c, t, m))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_attention_holes(hip):
     """Holes in the middle and at the end, whole sequences of them; lengths past the table and below 0."""
     lens = [200, 64, 90, 128, 40]
@@ -464,6 +539,20 @@ def test_evict_holes(hip):
     assert torch.equal(c[:, int(new[2, 1]), 0, :4].cpu(), cache[:, table[2].long()[t // 16], 0, t % 16])
 
 
+def test_evict_long_ties_and_holes(hip):
+    """Past 32768 slots: equal weights, odd ones, holes, everything kept and nothing but the recent."""
+    inf, nan = math.inf, math.nan
+    for values, keep, recent in (([0.0, 1.0], 20000, 0), ([nan, inf, -1.0, 0.0], 30000, 5000), ([1.0], 100, 100), ([2.0, 3.0], 34000, 33999)):
+        values = torch.tensor(values)
+        evict_case(hip, [33000, 40], keep, recent, 1, 64, 128,
+                   weights=lambda gen, S: values[torch.randint(len(values), (2, 1, S), generator=gen)])
+    cache, table, n = make([36000], 1, 64, 256, "bf16", spare=130)
+    free = torch.tensor(sorted(set(range(cache.shape[1])) - set(table.flatten().tolist())))
+    table[0, 5:20], table[0, 130:] = -1, cache.shape[1]
+    for keep, recent in ((32000, 4000), (33000, 0)):
+        check_evict(hip, cache, table, n, torch.rand(1, 1, table.shape[1] * 256), keep, recent, free)
+
+
 def test_evict_long(hip):
     evict_case(hip, [70000, 33000], 30000, 1000, 1, 64, 256)
     evict_case(hip, [40000], 1, 0, 1, 64, 256, weights=lambda gen, S: torch.ones(1, 1, S))
@@ -612,3 +701,31 @@ def test_the_same_twice(hip):
         runs.append((hip.paged_attention(q, c, t, m, weights=w), w))
     for o, w in runs[1:]:
         assert torch.equal(o, runs[0][0]) and torch.equal(w, runs[0][1])
+
+
+def test_model_with_scaled_angles(hip):
+    """rope_scaling in a model's config reaches its angles: linear by 2 at even positions is plain at half of them."""
+    import numpy as np
+
+    from rotor.bitnet_model import BitNetModel, rope_table
+
+    cfg = dict(vocab_size=512, d_model=512, n_layers=1, n_heads=4, n_kv_heads=2, d_ff=1024, max_seq_len=64, max_batch_tokens=32)
+    rng = np.random.default_rng(3)
+    p, state = "model.layers.0", {}
+    for name, out, inner in (("self_attn.q_proj", 512, 512), ("self_attn.k_proj", 256, 512), ("self_attn.v_proj", 256, 512),
+                             ("self_attn.o_proj", 512, 512), ("mlp.gate_proj", 1024, 512), ("mlp.up_proj", 1024, 512), ("mlp.down_proj", 512, 1024)):
+        state[f"{p}.{name}.weight"] = rng.choice(np.array([0, 1, 2], np.uint8), (out, inner // 4, 4)) @ np.array([1, 4, 16, 64], np.uint8)
+        state[f"{p}.{name}.weight_scale"] = np.array([0.02], np.float32)
+    for name, size in (("input_layernorm", 512), ("post_attention_layernorm", 512), ("self_attn.attn_sub_norm", 512), ("mlp.ffn_sub_norm", 1024)):
+        state[f"{p}.{name}.weight"] = np.ones(size, np.float32)
+    state["model.norm.weight"] = np.ones(512, np.float32)
+    state["model.embed_tokens.weight"] = torch.from_numpy(rng.standard_normal((512, 512)).astype(np.float32)).bfloat16()
+    scaling = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32}
+    ids = np.arange(20) * 7 % 512
+    outs = []
+    for s in (None, scaling):
+        model = BitNetModel(dict(cfg, rope_scaling=s), use_gpu=True)
+        model.load_state(state)
+        assert np.array_equal(model._dev.rope.cpu().numpy(), rope_table(64, 128, 500000.0, s))
+        outs.append(model.forward(ids)[0])
+    assert np.isfinite(outs[1]).all() and not np.array_equal(outs[0], outs[1])
