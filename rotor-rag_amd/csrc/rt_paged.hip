@@ -1011,8 +1011,10 @@ struct EvictSlots {
         above = __builtin_amdgcn_readlane(paged_scan(above), 63);
         equal = __builtin_amdgcn_readlane(paged_scan(equal), 63);
     }
-    // the kept ones, out: kept before this wave's; equal: equal ones before it, of which the first `want` are kept
-    __device__ __forceinline__ void write(const PagedEvict& a, int bk, unsigned prefix, int want, int out, int equal, int lane) const {
+    // the kept ones number lo .. hi - 1, out: kept before this wave's; equal: equal ones before it, of which the first `want` are
+    // kept; list: their slots in LDS too
+    __device__ __forceinline__ void write(const PagedEvict& a, int bk, unsigned prefix, int want, int out, int equal, int lane, int lo, int hi,
+                                          int* list) const {
         int* const kept = a.kept + (size_t)bk * a.keep;
         float* const left = a.new_weights + (size_t)bk * a.slots;
         const float* const w = a.weights + (size_t)bk * a.slots;
@@ -1031,10 +1033,11 @@ struct EvictSlots {
                 const unsigned long long e = __ballot(same);
                 const bool keep = (stay >> (j0 + j) & 1u) || k > prefix || (same && equal + __popcll(e & below) < want);
                 const unsigned long long all = __ballot(keep);
-                if (keep) {
-                    const int at = out + __popcll(all & below);
+                const int at = out + __popcll(all & below);
+                if (keep && at >= lo && at < hi) {
                     kept[at] = s0 + 64 * (j0 + j) + lane;
                     left[at] = x[j];
+                    if (list) list[at - lo] = s0 + 64 * (j0 + j) + lane;
                 }
                 equal += __popcll(e);
                 out += __popcll(all);
@@ -1079,11 +1082,32 @@ __device__ __forceinline__ void evict_rest(const PagedEvict& a, int bk, int tota
     if (bk % a.c.Hkv == 0 && t == 0) a.new_lens[bk / a.c.Hkv] = total;  // (the same for every head: holes are the sequence's)
 }
 
+// A kept slot's row of K and of V into the new table's page, 16 bytes a thread, past the caches (16 sequences of 1000 to 8191 cut
+// to 4096: the whole eviction 63.4 us through them, so 59.8).  n: its number; o: the thread's bytes of the row.
+__device__ __forceinline__ void evict_move(const PagedEvict& a, int b, int kh, int s, int n, int o, int row_bytes, int esize) {
+    const int in_page = (1 << a.c.shift) - 1;
+    const int from = a.c.table[(size_t)b * a.c.P + (s >> a.c.shift)], to = a.new_table[(size_t)b * a.new_P + (n >> a.c.shift)];
+    if (from < 0 || from >= a.c.pages || to < 0 || to >= a.c.pages) return;
+    char* const base = static_cast<char*>(a.c.cache) + ((long long)kh << a.c.shift) * row_bytes + o;
+    const long long src = (long long)from * a.c.page_stride * esize + (long long)(s & in_page) * row_bytes;
+    const long long dst = (long long)to * a.c.page_stride * esize + (long long)(n & in_page) * row_bytes;
+    const long long v = a.c.kv_stride * esize;
+    const v4u x = paged_load<true, v4u>(base + src), y = paged_load<true, v4u>(base + src + v);
+    __builtin_nontemporal_store(x, reinterpret_cast<v4u*>(base + dst));
+    __builtin_nontemporal_store(y, reinterpret_cast<v4u*>(base + dst + v));
+}
+
+// The whole of it, for a share of a head's kept slots: every workgroup of a head makes the same selection, and each moves
+// its own `share` rows, so that one launch does both: a chat's 2048 slots cut to 1024 15.0 us in two launches, so 12.6; 16
+// sequences of up to 8191 cut to 4096 58.4 / 58.5 on the GPU.
+constexpr int kEvictShare = 4096;
 template <int R>
-__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict a) {
+__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict a, int parts, int share, int row_bytes, int esize) {
     __shared__ int hist[kEvictBins];
     __shared__ int totals[kEvictWaves][2], found[3];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), bk = blockIdx.x;
+    __shared__ int list[kEvictShare];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int part = blockIdx.x % parts, bk = blockIdx.x / parts, b = bk / a.c.Hkv, lo = part * share;
     const int len = min(max(a.c.lens[bk / a.c.Hkv], 0), a.c.P << a.c.shift);
     EvictSlots<R> x;
     x.load(a, bk, 0, len, len, lane, wave);
@@ -1138,8 +1162,14 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict 
         all += totals[v][0];
         equals += totals[v][1];
     }
-    x.write(a, bk, prefix, want, before + min(same, want), same, lane);
-    evict_rest(a, bk, all + min(equals, want), t, kEvictThreads);
+    const int total = all + min(equals, want), hi = min(lo + share, total);
+    x.write(a, bk, prefix, want, before + min(same, want), same, lane, lo, hi, list);
+    evict_rest(a, bk, total, part * kEvictThreads + t, parts * kEvictThreads);
+    __syncthreads();
+    const int lanes = row_bytes / 16;
+#pragma unroll 4
+    for (int n = lo + t / lanes; n < hi; n += kEvictThreads / lanes)
+        evict_move(a, b, bk - b * a.c.Hkv, list[n - lo], n, t % lanes * 16, row_bytes, esize);
 }
 
 // The same in several launches (step 0 to 4), workgroup (head, chunk of kEvictChunk slots): histograms 0 to 2, the chunks' counts, the
@@ -1246,30 +1276,18 @@ __global__ void __launch_bounds__(kEvictThreads) paged_share_kernel(PagedEvict a
     same += wave_sum(equal);
     all = wave_sum(all);
     equals = wave_sum(equals);
-    x.write(a, bk, prefix, want, before + min(same, want), same, lane);
+    x.write(a, bk, prefix, want, before + min(same, want), same, lane, 0, INT_MAX, nullptr);
     evict_rest(a, bk, all + min(equals, want), chunk * kEvictThreads + t, chunks * kEvictThreads);
 }
 
-// The rows of the kept slots, in order, into the new table's pages: 16 bytes a thread of K and of V, past the caches
-// (16 sequences of 1000 to 8191 cut to 4096: the whole eviction 63.4 us through them, so 59.8).
+// The kept slots' rows, by 256 threads.
 __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvict a, int row_bytes, int esize) {
     const int lanes = row_bytes / 16, rows = 256 / lanes, t = threadIdx.x;
-    const int chunks = (a.keep + rows - 1) / rows, chunk = blockIdx.x % chunks, bk = blockIdx.x / chunks;
-    const int b = bk / a.c.Hkv, kh = bk % a.c.Hkv, n = chunk * rows + t / lanes, o = t % lanes * 16;
-    if (n >= a.keep) return;
-    const int s = a.kept[(size_t)bk * a.keep + n];
-    if (s < 0) return;
-    const int in_page = (1 << a.c.shift) - 1;
-    const int from = a.c.table[(size_t)b * a.c.P + (s >> a.c.shift)], to = a.new_table[(size_t)b * a.new_P + (n >> a.c.shift)];
-    if (from < 0 || from >= a.c.pages || to < 0 || to >= a.c.pages) return;
-    char* const base = static_cast<char*>(a.c.cache) + ((long long)kh << a.c.shift) * row_bytes + o;
-    const long long src = (long long)from * a.c.page_stride * esize + (long long)(s & in_page) * row_bytes;
-    const long long dst = (long long)to * a.c.page_stride * esize + (long long)(n & in_page) * row_bytes;
-    const long long v = a.c.kv_stride * esize;
-    const v4u x = paged_load<true, v4u>(base + src), y = paged_load<true, v4u>(base + src + v);
-    __builtin_nontemporal_store(x, reinterpret_cast<v4u*>(base + dst));
-    __builtin_nontemporal_store(y, reinterpret_cast<v4u*>(base + dst + v));
+    const int chunks = (a.keep + rows - 1) / rows, chunk = blockIdx.x % chunks, bk = blockIdx.x / chunks, b = bk / a.c.Hkv;
+    const int n = chunk * rows + t / lanes, s = n < a.keep ? a.kept[(size_t)bk * a.keep + n] : -1;
+    if (s >= 0) evict_move(a, b, bk - b * a.c.Hkv, s, n, t % lanes * 16, row_bytes, esize);
 }
+
 
 template <typename F>
 void paged_by_type(int type, int hd, F go) {
@@ -1396,22 +1414,27 @@ hipError_t launch_paged_evict(const PagedEvict& a, int type, int hd, void* work,
     if (moves > kPagedMaxGroups || heads * chunks > kPagedMaxGroups) return hipErrorInvalidValue;
     const dim3 block(kEvictThreads);
     if (cap <= kEvictAlone) {
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)heads), block, 0, s, a); };
+        // as many workgroups a head as there are CUs for, but 64 rows each at least
+        const int keep = std::min(a.keep, cap);
+        const int parts = std::max((keep + kEvictShare - 1) / kEvictShare, (int)std::min<long long>((keep + 63) / 64, 256 / heads));
+        const int share = (keep + parts - 1) / parts;
+        if (heads * parts > kPagedMaxGroups) return hipErrorInvalidValue;
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * parts)), block, 0, s, a, parts, share, row, esize); };
         if (cap <= 4 * kEvictThreads) go(paged_select_kernel<4>);
         else if (cap <= 8 * kEvictThreads) go(paged_select_kernel<8>);
         else if (cap <= 16 * kEvictThreads) go(paged_select_kernel<16>);
         else go(paged_select_kernel<32>);
-    } else {
-        int* const w = static_cast<int*>(work);
-        const int words = kEvictWords + 2 * chunks;
-        hipLaunchKernelGGL(paged_clear_kernel, dim3((unsigned)heads), block, 0, s, w, words);
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * chunks)), block, 0, s, a, w, words, chunks); };
-        go(paged_share_kernel<0>);
-        go(paged_share_kernel<1>);
-        go(paged_share_kernel<2>);
-        go(paged_share_kernel<3>);
-        go(paged_share_kernel<4>);
+        return hipGetLastError();
     }
+    int* const w = static_cast<int*>(work);
+    const int words = kEvictWords + 2 * chunks;
+    hipLaunchKernelGGL(paged_clear_kernel, dim3((unsigned)heads), block, 0, s, w, words);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * chunks)), block, 0, s, a, w, words, chunks); };
+    go(paged_share_kernel<0>);
+    go(paged_share_kernel<1>);
+    go(paged_share_kernel<2>);
+    go(paged_share_kernel<3>);
+    go(paged_share_kernel<4>);
     hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)moves), dim3(256), 0, s, a, row, esize);
     return hipGetLastError();
 }
