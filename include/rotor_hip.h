@@ -414,7 +414,7 @@ int rt_kv4_step(rt_ctx* ctx, const float* q, const float* k, const float* v, con
  * cache is 16-byte aligned and so are both strides; a page's [Hkv][page][hd] is contiguous.
  * fp16 keys and values past 65519 in magnitude become infinite.  Rows are for finite numbers: a query, or a
  * key or value that is attended to, that is not finite leaves NaN or infinities in its heads' outputs.
- * B * Hkv <= 2^24, H / Hkv <= 1024, P * page <= 2^20. */
+ * B * Hkv <= 2^24, H / Hkv <= 1024, H <= 2^20, P * page <= 2^20. */
 #define RT_PAGED_F32 0
 #define RT_PAGED_BF16 1
 #define RT_PAGED_F16 2

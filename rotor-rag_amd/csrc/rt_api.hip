@@ -1308,9 +1308,9 @@ static bool paged_check(const rt_pages* p, int H, PagedCache& c, const char* who
     const int shift = p->page > 0 ? __builtin_ctz((unsigned)p->page) : 0;
     if (p->type < RT_PAGED_F32 || p->type > RT_PAGED_F16 || (p->hd != 64 && p->hd != 128) || p->page < 16 || p->page > 256 ||
         p->page != 1 << shift || p->pages <= 0 || p->B <= 0 || p->Hkv <= 0 || (long long)p->B * p->Hkv > (1 << 24) || p->P <= 0 ||
-        (long long)p->P * p->page > (1 << 20) || H <= 0 || H % p->Hkv || H / p->Hkv > 1024)
+        (long long)p->P * p->page > (1 << 20) || H <= 0 || H % p->Hkv || H / p->Hkv > 1024 || H > (1 << 20))
         return no(": unsupported layout (fp32, bf16 or fp16; head_dim 64 or 128; page 16, 32, 64, 128 or 256; H % Hkv == 0, H / Hkv <= "
-                  "1024, B * Hkv <= 2^24, P * page <= 2^20)");
+                  "1024, H <= 2^20, B * Hkv <= 2^24, P * page <= 2^20)");
     const long long size = p->type == RT_PAGED_F32 ? 4 : 2, rows = (long long)p->Hkv * p->page * p->hd;
     const long long most = LLONG_MAX / 16 / ((long long)p->pages + 1);
     if (p->page_stride < rows || p->page_stride > most || p->kv_stride < rows || p->kv_stride > LLONG_MAX / 16)

@@ -501,23 +501,27 @@ __device__ __forceinline__ int paged_scan(int x) {  // inclusive, over the lanes
 __host__ __device__ __forceinline__ int paged_even(int cap) { return (cap + 31) & ~31; }
 
 // The pieces of a launch.  A sequence of n tiles is cut, for each of its `per` units (a KV head's tile of heads), into pieces
-// of at most q tiles (one at least), as equal as they can be, q about the least for which all fit the launch's workgroups; workgroup w
-// has piece number w in the order (sequence, unit, piece).  Every wave works this out for itself, lane b for sequence b: the host
-// does not know the lengths, and with the same number of pieces for each the longest sequence decides the launch.
-constexpr int kWaves = 4, kPagedMapped = 4096;  // batches past kPagedMapped: a piece a unit
+// of at most q tiles (one at least), as equal as they can be, q about the least for which all fit the launch's workgroups.  The first
+// B per workgroups have the units' first pieces; the others the further ones, in the order (sequence, unit, piece).  Every wave
+// works this out for itself, lane b for sequence b: the host does not know the lengths, and with the same number of
+// pieces for each the longest sequence decides the launch.
+constexpr int kWaves = 4;
 struct PagedPiece {
-    int b, unit, piece, n, first, q;  // n pieces of q tiles a unit of sequence b; first: the workgroup of this unit's first; n = 0: none
-    int span;                         // paged_span of sequence b
+    int b, unit, piece, n, q;  // piece number `piece` of n, q tiles each; n = 0: none
+    int more;                  // the workgroup of the unit's second piece (for a first piece: where B <= 64)
+    int span;                  // paged_span of sequence b
 };
+// The workgroup of piece s of unit u of the launch.
+__device__ __forceinline__ int paged_group(int s, int u, int more) { return s ? more + s - 1 : u; }
+
 template <bool STEP, int TK>
 __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int lane) {
-    const int B = a.c.B, per = a.c.Hkv * a.tiles;
+    const int B = a.c.B, per = a.c.Hkv * a.tiles, units = B * per, room = a.groups - units;
     PagedPiece p{};
-    if (B > kPagedMapped) {
+    if (room == 0) {
         p.b = w / per;
         p.unit = w - p.b * per;
         p.n = 1;
-        p.first = w;
         p.q = INT_MAX / 2;
         p.span = paged_span<STEP>(a, a.c.lens[p.b]);
         return p;
@@ -527,56 +531,66 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int
         span = b < B ? paged_span<STEP>(a, a.c.lens[b]) : 0;
         return (span + TK - 1) / TK;
     };
-    // ceil(nb / q): nb <= 2^16, and 1 / q is good to 2^-23, so the quarter decides
-    auto pieces = [&](int nb, int b, int q) {
-        return b >= B ? 0 : nb <= q ? 1 : (int)(((float)(nb + q - 1) + 0.25f) * __builtin_amdgcn_rcpf((float)q));
-    };
+    // ceil(nb / q), 1 at least: nb <= 2^16, and 1 / q is good to 2^-23, so the quarter decides
+    auto pieces = [&](int nb, int q) { return nb <= q ? 1 : (int)(((float)(nb + q - 1) + 0.25f) * __builtin_amdgcn_rcpf((float)q)); };
     const int mine = tiles(lane);
-    int q, n, incl;
+    int q, n = 1, incl = 0;  // incl: pieces past the first of this lane's sequence and those before it
     if (B <= 64) {
         const float all = (float)__builtin_amdgcn_readlane(paged_scan(mine), 63);
         // (the last pieces are half empty on the average)
-        q = max(kWaves, (int)(all * (float)per * __builtin_amdgcn_rcpf((float)a.groups - 0.4f * (float)(B * per))));
-        for (;; q += max(1, q / 32)) {  // (ends at the latest with a piece a unit: B per <= groups)
-            n = pieces(mine, lane, q);
-            incl = paged_scan(n);
-            if (__builtin_amdgcn_readlane(incl, 63) * per <= a.groups) break;
+        q = max(kWaves, (int)(all * (float)per * __builtin_amdgcn_rcpf((float)room + 0.6f * (float)units)));
+        for (;; q += max(1, q / 32)) {  // (ends at the latest when q tiles are the longest sequence)
+            n = pieces(mine, q);
+            incl = paged_scan(n - 1);
+            if (__builtin_amdgcn_readlane(incl, 63) * per <= room) break;
         }
-        const unsigned long long here = __ballot(w < incl * per);
-        if (here == 0ull) return p;
-        p.b = (int)__builtin_ctzll(here);
-        p.n = __builtin_amdgcn_readlane(n, p.b);
-        p.first = (__builtin_amdgcn_readlane(incl, p.b) - p.n) * per;
-        p.span = __builtin_amdgcn_readlane(span, p.b);
-    } else {
-        // no more than B + all / q pieces a unit: q from that
-        int all = mine;
-        for (int b = 64; b < B; b += 64) all += tiles(b + lane);
+    } else {  // all / q pieces past the first ones at most: q from that
+        int all = mine, most = mine;
+        for (int b = 64; b < B; b += 64) {
+            const int nb = tiles(b + lane);
+            all += nb;
+            most = max(most, nb);
+        }
         all = __builtin_amdgcn_readlane(paged_scan(all), 63);
-        const float room = (float)(a.groups - B * per);
-        q = room > 0.0f ? (int)fminf((float)all * (float)per / room * 1.0001f, 1e6f) + 1 : 1 << 20;
-        q = max(kWaves, q);
-        int before = 0;
-        for (int b = 0;; b += 64) {
-            if (b >= B) return p;
-            n = pieces(tiles(b + lane), b + lane, q);
-            incl = paged_scan(n) + before;
-            const unsigned long long here = __ballot(w < incl * per);
-            if (here != 0ull) {
-                const int l = (int)__builtin_ctzll(here);
-                p.b = b + l;
-                p.n = __builtin_amdgcn_readlane(n, l);
-                p.first = (__builtin_amdgcn_readlane(incl, l) - p.n) * per;
-                p.span = __builtin_amdgcn_readlane(span, l);
-                break;
-            }
-            before = __builtin_amdgcn_readlane(incl, 63);
+        most = lane63(wave_reduce63(most, 0, [](int x, int y) { return max(x, y); }));
+        q = max(kWaves, (int)fminf((float)all * (float)per / (float)room * 1.0001f, 1e6f) + 1);
+        if (w >= units && most <= q) return p;
+    }
+    if (w < units) {
+        p.b = w / per;
+        p.unit = w - p.b * per;
+        if (B <= 64) {
+            p.n = __builtin_amdgcn_readlane(n, p.b);
+            p.span = __builtin_amdgcn_readlane(span, p.b);
+            p.more = units + (__builtin_amdgcn_readlane(incl, p.b) - p.n + 1) * per + p.unit * (p.n - 1);
+        } else {
+            p.span = paged_span<STEP>(a, a.c.lens[p.b]);
+            p.n = pieces((p.span + TK - 1) / TK, q);
         }
+    } else {
+        const int e = w - units;
+        int at = 0, before = 0;
+        unsigned long long here = 0ull;
+        for (;; at += 64) {
+            if (at >= B) return p;
+            if (B > 64) {
+                n = pieces(tiles(at + lane), q);
+                incl = paged_scan(n - 1) + before;
+                before = __builtin_amdgcn_readlane(incl, 63);
+            }
+            here = __ballot(e < incl * per);
+            if (here != 0ull) break;
+        }
+        const int l = (int)__builtin_ctzll(here), others = __builtin_amdgcn_readlane(n, l) - 1;
+        const int start = (__builtin_amdgcn_readlane(incl, l) - others) * per;
+        p.b = at + l;
+        p.n = others + 1;
+        p.span = __builtin_amdgcn_readlane(span, l);
+        p.unit = (e - start) / others;
+        p.piece = 1 + e - start - p.unit * others;
+        p.more = units + start + p.unit * others;
     }
     p.q = ((p.span + TK - 1) / TK + p.n - 1) / p.n;
-    p.unit = (w - p.first) / p.n;
-    p.piece = w - p.first - p.unit * p.n;
-    p.first += p.unit * p.n;
     return p;
 }
 
@@ -599,7 +613,7 @@ __device__ __forceinline__ v2f paged_get(const float* at) {
 // room: LDS for kLastMost floats and, behind them, a row's sums a group of threads; flag: a word of LDS.
 constexpr int kLastMost = 64;  // pieces times heads that the last workgroup joins
 template <int HD>
-__device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece& p, unsigned long long* ticket, float* out, int rows,
+__device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece& p, int u, unsigned long long* ticket, float* out, int rows,
                                            float* room, int* flag, int t, int lane, int wave) {
     constexpr int L = HD / 4, NT = 64 * kWaves;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -612,21 +626,19 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
     }
     __syncthreads();
     if (!*flag) return;
-    const float* const part = a.part + (size_t)p.first * 16 * HD;
-    const float* const ml = a.ml + (size_t)p.first * 32;
+    auto part = [&](int s, int e) { return a.part + (size_t)paged_group(s, u, p.more) * 16 * HD + e * 4; };
     const int n = p.n, cols = rows * L, groups = max(NT / cols, 1), grp = t / cols;
     float* const factor = room;  // [rows][n]
     v4f* const sums = reinterpret_cast<v4f*>(room + kLastMost);
     constexpr int kAhead = 8;
     v2f ahead[kAhead][2];
     auto load = [&](int e) {  // of a group's first pieces
-        const float* const at = part + e * 4;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const int s = grp + k * groups;
             if (s < n) {
-                ahead[k][0] = paged_get(at + (size_t)s * 16 * HD);
-                ahead[k][1] = paged_get(at + (size_t)s * 16 * HD + 2);
+                ahead[k][0] = paged_get(part(s, e));
+                ahead[k][1] = paged_get(part(s, e) + 2);
             }
         }
     };
@@ -634,7 +646,7 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
     const bool mine = grp < groups && e < cols;
     if (mine) load(e);  // (while the references come)
     for (int row = wave; row < rows; row += kWaves) {
-        const v2f x = lane < n ? paged_get(ml + lane * 32 + row * 2) : v2f{-INFINITY, 0.0f};
+        const v2f x = lane < n ? paged_get(a.ml + (size_t)paged_group(lane, u, p.more) * 32 + row * 2) : v2f{-INFINITY, 0.0f};
         const float top = lane63(wave_reduce63(x[0], -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
         const float f = __builtin_amdgcn_exp2f(x[0] - (top > -INFINITY ? top : 0.0f));
         const float sum = lane63(wave_reduce63(x[1] * f, 0.0f, [](float x, float y) { return x + y; }));
@@ -650,9 +662,8 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
             if (s < n) y += v4f{ahead[k][0][0], ahead[k][0][1], ahead[k][1][0], ahead[k][1][1]} * weight[s];
         }
         for (int s = grp + kAhead * groups; s < n; s += groups) {
-            const float* const at = part + e * 4 + (size_t)s * 16 * HD;
-            const v2f u = paged_get(at), v = paged_get(at + 2);
-            y += v4f{u[0], u[1], v[0], v[1]} * weight[s];
+            const v2f lo = paged_get(part(s, e)), hi = paged_get(part(s, e) + 2);
+            y += v4f{lo[0], lo[1], hi[0], hi[1]} * weight[s];
         }
         if (groups > 1) sums[t] = y;
         else *reinterpret_cast<v4f*>(out + e * 4) = y;
@@ -682,7 +693,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
     const PagedPiece p = paged_piece<STEP, TK>(a, blockIdx.x, lane);
     if (p.n == 0) return;
-    const int b = p.b, kh = p.unit / a.tiles, ht = p.unit - kh * a.tiles, bk = b * a.c.Hkv + kh;
+    const int b = p.b, kh = p.unit / a.tiles, ht = p.unit - kh * a.tiles, bk = b * a.c.Hkv + kh, u = b * a.c.Hkv * a.tiles + p.unit;
     const int len = p.span, tiles = (len + TK - 1) / TK, first = min(p.piece * p.q, tiles);
     int last = min(first + p.q, tiles);
     const int newest = STEP ? paged_newest(a, b, len) : 0;
@@ -690,7 +701,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     const int h0 = kh * a.G + 16 * ht;  // the tile's first head
     const int cap = a.c.P << a.c.shift;
     // the unit's ticket: whatever the memory held, the first to come makes it this launch's, with none counted
-    unsigned long long* const ticket = a.tickets ? a.tickets + (size_t)b * a.c.Hkv * a.tiles + p.unit : nullptr;
+    unsigned long long* const ticket = a.tickets ? a.tickets + u : nullptr;
     unsigned long long held = 0ull;
     if (ticket && p.n > 1 && t == 0) held = __hip_atomic_load(ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     auto claim = [&] {
@@ -854,21 +865,23 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)blockIdx.x * 16 + row) * 2) = v2f{top, sum};
     }
     if (a.tickets) {
-        if (p.n > 1) paged_last<HD>(a, p, ticket, a.out + ((size_t)b * a.H + h0) * HD, rows, reinterpret_cast<float*>(both), power, t, lane, wave);
+        if (p.n > 1) paged_last<HD>(a, p, u, ticket, a.out + ((size_t)b * a.H + h0) * HD, rows, reinterpret_cast<float*>(both), power, t, lane, wave);
         return;
     }
-    if (t == 0 && p.piece == 0 && a.ml) a.units[(size_t)b * a.c.Hkv * a.tiles + p.unit] = make_int2(p.first, p.n);
+    if (t == 0 && a.ml && p.piece == (p.n > 1)) a.units[u] = make_int2(p.more, p.n);
 }
 
-// A head's reference (the largest of its pieces') and the reciprocal of its sum of weights, found by a wave: ml is the
-// head's (reference, sum) of its first piece, n pieces.
-__device__ __forceinline__ void paged_total(const float* ml, int n, int lane, float& ref, float& inv) {
+// Head number `row` of unit u: its reference (the largest of its pieces') and the reciprocal of its sum of weights, found by a
+// wave; unit: the workgroup of its second piece, and how many pieces there are.
+__device__ __forceinline__ void paged_total(const float* all, int u, int2 unit, int row, int lane, float& ref, float& inv) {
+    auto ml = [&](int s) { return all + (size_t)paged_group(s, u, unit.x) * 32 + row * 2; };
+    const int n = unit.y;
     float top = -INFINITY;
-    for (int s = lane; s < n; s += 64) top = fmaxf(top, ml[s * 32]);
+    for (int s = lane; s < n; s += 64) top = fmaxf(top, ml(s)[0]);
     top = lane63(wave_reduce63(top, -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
     ref = top > -INFINITY ? top : 0.0f;
     float sum = 0.0f;
-    for (int s = lane; s < n; s += 64) sum += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
+    for (int s = lane; s < n; s += 64) sum += ml(s)[1] * __builtin_amdgcn_exp2f(ml(s)[0] - ref);
     sum = lane63(wave_reduce63(sum, 0.0f, [](float x, float y) { return x + y; }));
     inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
 }
@@ -885,23 +898,23 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     if ((int)blockIdx.x < joins) {
         const int head = blockIdx.x % a.H, b = blockIdx.x / a.H, kh = head / a.G, in = head % a.G;
-        const int2 unit = a.units[(size_t)(b * a.c.Hkv + kh) * a.tiles + in / 16];
+        const int u = (b * a.c.Hkv + kh) * a.tiles + in / 16;
+        const int2 unit = a.units[u];
         const int n = unit.y;
         if (n == 1) return;
-        const float* ml = a.ml + ((size_t)unit.x * 16 + in % 16) * 2;
-        const float* part = a.part + ((size_t)unit.x * 16 + in % 16) * HD;
         const int d = t % L * 4, grp = t / L;
+        auto place = [&](int s) { return (size_t)paged_group(s, u, unit.x) * 16 + in % 16; };
+        auto part = [&](int s) { return *reinterpret_cast<const v4f*>(a.part + place(s) * HD + d); };
         v4f y{};
         float own = -INFINITY, ref, inv;
         if (grp < n) {  // (before the references are known, which takes as long as these loads)
-            y = *reinterpret_cast<const v4f*>(part + (size_t)grp * 16 * HD + d);
-            own = ml[grp * 32];
+            y = part(grp);
+            own = a.ml[place(grp) * 2];
         }
-        paged_total(ml, n, lane, ref, inv);
+        paged_total(a.ml, u, unit, in % 16, lane, ref, inv);
         y *= __builtin_amdgcn_exp2f(own - ref);
 #pragma unroll 4
-        for (int s = grp + NT / L; s < n; s += NT / L)
-            y += *reinterpret_cast<const v4f*>(part + (size_t)s * 16 * HD + d) * __builtin_amdgcn_exp2f(ml[s * 32] - ref);
+        for (int s = grp + NT / L; s < n; s += NT / L) y += part(s) * __builtin_amdgcn_exp2f(a.ml[place(s) * 2] - ref);
         *reinterpret_cast<v4f*>(&sums[grp][d]) = y;
         __syncthreads();
         if (grp) return;
@@ -915,8 +928,8 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
     if (chunk * NT * 4 >= len || (STEP && paged_newest(a, b, len) < 0)) return;
     for (int in = wave; in < a.G; in += NT / 64) {
         float ref, inv;
-        const int2 unit = a.units[(size_t)bk * a.tiles + in / 16];
-        paged_total(a.ml + ((size_t)unit.x * 16 + in % 16) * 2, unit.y, lane, ref, inv);
+        const int u = bk * a.tiles + in / 16;
+        paged_total(a.ml, u, a.units[u], in % 16, lane, ref, inv);
         total[in][0] = ref;
         total[in][1] = inv;
     }
@@ -1300,6 +1313,7 @@ void paged_by_type(int type, int hd, F go) {
 }
 
 // The workgroups of the attention, and whether a unit may have several pieces.
+constexpr int kPagedMapped = 1024;  // larger batches: a piece a unit
 struct PagedShape {
     long long units, groups;
     int tiles;
@@ -1312,14 +1326,17 @@ PagedShape paged_shape(int B, int H, int Hkv, int cap, int type) {
     p.units = (long long)B * Hkv * p.tiles;
     const long long most = (cap + least - 1) / least;
     p.split = most > 1 && B <= kPagedMapped;
-    // as many as run at once, two a CU; or more, for two pieces a unit
-    p.groups = p.split ? std::min(p.units * most, 512 * ((p.units + 255) / 256)) : p.units;
+    // As many as run at once, two a CU, or twice that for two pieces a unit; past 512 units, pieces for sequences that have
+    // more than a 512th of the work, no others.  Two pieces a unit / these / none, us: 128 sequences of 10 to 1500 slots (32 heads
+    // over 8) 83 / 77 / 76, 1000 of 700 (4 over 1; each workgroup looks at every length) 98 / 66 / 58; one of 30000 among 255 of 400
+    // 133 with these, 439 with none, one among 63 (64 over 16) 81 / 416.
+    p.groups = !p.split ? p.units : std::min(p.units * most, p.units <= 512 ? 512 * ((p.units + 255) / 256) : p.units + 512);
     // The last workgroup joins where no unit has more than 32 pieces, or 64 heads of pieces: a launch less on the host (3.5 us),
     // and on the GPU, us in two launches / one: 20 heads over 5, 1000 slots 6.4 + 3.2 / 8.6, 2000 6.3 + 3.8 / 9.0, 4000 (32 pieces of
     // 4 heads) 6.9 + 4.4 / 12.5; 32 over 2, 500 6.8 + 3.4 / 10.6; 16 over 1, 1000 (8 of 16) 6.8 + 3.8 / 11.3; 5 over 5, 8000 (63 of 1)
     // 9.8 + 4.2 / 15.7; one workgroup then reads what many would.
     const long long pieces = std::min(most, p.groups / ((long long)Hkv * p.tiles));
-    p.last = p.split && pieces <= 32 && pieces * std::min(G, 16) <= kLastMost;
+    p.last = p.split && B <= 64 && pieces <= 32 && pieces * std::min(G, 16) <= kLastMost;
     return p;
 }
 

@@ -212,6 +212,11 @@ def test_attention_large_batches(hip):
     cache, table, n = make(lens, 1, 64, 16, "fp16")
     check_attention(hip, cache, table, n, queries(lens, 1, 64))
     check_attention(hip, cache, table, n, queries(lens, 1, 64), weights=torch.zeros(4201, 1, table.shape[1] * 16))
+    for B, Hkv in ((60, 10), (300, 2)):  # (more heads than run at once, one sequence far longer than the others)
+        lens = torch.randint(0, 40, (B,), generator=gen).tolist()
+        lens[B // 3], lens[-1] = 6000, 1500
+        cache, table, n = make(lens, Hkv, 64, 32, "bf16")
+        check_attention(hip, cache, table, n, queries(lens, Hkv, 64), weights=torch.zeros(B, Hkv, table.shape[1] * 32))
     lens = [900, 40]
     cache, table, n = make(lens, 1, 64, 16, "bf16")
     check_attention(hip, cache, table, n, queries(lens, 1024, 64), weights=torch.zeros(2, 1, table.shape[1] * 16))

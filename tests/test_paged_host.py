@@ -110,8 +110,10 @@ def test_refused_tokens(lib, name):
         refused(lib, name, "M", new=dict(NEW, **bad))
     for bad in [dict(rotary=0), dict(rotary=4), dict(rotary=132), dict(rotary=136), dict(rotary=-8), dict(rope_rows=0), dict(rope_rows=-1)]:
         refused(lib, name, "rotary", new=dict(NEW, **bad))
-    for bad in [0, 21, -20, 5 * 1025]:
+    for bad in [0, 21, -20, 5 * 1025, 5 << 18]:
         refused(lib, name, "layout", new=dict(NEW, H=bad))
+    wide = dict(CACHE, Hkv=2048, page=16, hd=64, page_stride=1 << 30, kv_stride=1 << 38)
+    refused(lib, name, "layout", cache=wide, new=dict(NEW, H=2048 * 513, rotary=64))
     if name == "step":
         refused(lib, name, "one token", new=dict(NEW, M=2))
         refused(lib, name, "one token", new=dict(NEW, counts=PTR))
