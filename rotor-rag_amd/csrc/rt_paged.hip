@@ -272,7 +272,7 @@ struct AttnTile {
     unsigned v[8][HD / 32];
     v4u q[3][NC];
     v4f o[NO], rest[F16 ? NO : 1];
-    float qi;  // fp16: what the products of q are to be multiplied by
+    float qi;  // what a score's products are to be multiplied by: log2(e) / sqrt(HD) and, in fp16, the queries' power of two
 
     // base: the tile's two halves of 16 slots
     __device__ __forceinline__ void load_k(const E* base0, const E* base1, int i, int g) {
@@ -316,7 +316,7 @@ struct AttnTile {
         for (int w = 0; w < HD / 32; ++w) v[n][w] = 0u;
     }
     // Queries pass through LDS in the order that lanes take them, [term][c][g][i] of 16 bytes: put by the workgroup, four
-    // dimensions a thread (x: of head i, dimensions d .. d + 3, scaled by 2^n in fp16), taken by every wave.
+    // dimensions a thread (x: of head i, dimensions d .. d + 3; 2^n times that in fp16), taken by every wave.
     static constexpr int QBYTES = 3 * NC * 64 * 16;
     static __device__ __forceinline__ void stage(char* to, v4f x, int i, int d, int n) {
         char* const at = to + ((d / 32 * 4 + d / 8 % 4) * 16 + i) * 16 + d % 8 * 2;
@@ -328,12 +328,12 @@ struct AttnTile {
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<v2u*>(at + p * NC * 1024) = t[p];
     }
-    __device__ __forceinline__ void take(const char* from, int n, int i, int g) {
+    __device__ __forceinline__ void take(const char* from, int n, float scale, int i, int g) {
 #pragma unroll
         for (int p = 0; p < 3; ++p)
 #pragma unroll
             for (int c = 0; c < NC; ++c) q[p][c] = *reinterpret_cast<const v4u*>(from + (((p * NC + c) * 4 + g) * 16 + i) * 16);
-        qi = __uint_as_float((unsigned)(127 - n) << 23);
+        qi = scale * __uint_as_float((unsigned)(127 - n) << 23);
     }
     static __device__ __forceinline__ v4f mul(const v4u& x, const v4u& y, const v4f& z) {
         if constexpr (F16)
@@ -341,17 +341,20 @@ struct AttnTile {
         else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), z, 0, 0, 0);
     }
     __device__ __forceinline__ void scores(float (&s)[NS]) {
-        v4f d[2] = {}, r[2] = {};
+        v4f d[2] = {}, e[2] = {}, r[2] = {};  // (the small terms in sums of their own: fewer roundings of the large one)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
-                (F16 ? r : d)[tt] = mul(k[tt][c], q[2][c], (F16 ? r : d)[tt]);
-                d[tt] = mul(k[tt][c], q[1][c], d[tt]);
+                (F16 ? r : e)[tt] = mul(k[tt][c], q[2][c], (F16 ? r : e)[tt]);
+                e[tt] = mul(k[tt][c], q[1][c], e[tt]);
                 d[tt] = mul(k[tt][c], q[0][c], d[tt]);
             }
 #pragma unroll
-        for (int n = 0; n < 8; ++n) s[n] = F16 ? (d[n >> 2][n & 3] + r[n >> 2][n & 3] * (1.0f / kRest)) * qi : d[n >> 2][n & 3];
+        for (int n = 0; n < 8; ++n) {
+            const float small = e[n >> 2][n & 3];
+            s[n] = (d[n >> 2][n & 3] + (F16 ? small + r[n >> 2][n & 3] * (1.0f / kRest) : small)) * qi;
+        }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -406,6 +409,7 @@ struct AttnTile<kPagedF32, HD, ONCE> {
     static constexpr bool F16 = false;
     typedef float E;
     v4f k[NC], v[4][NU], q[NC], o[NU][4];
+    float qi;
 
     __device__ __forceinline__ void load_k(const E* base0, const E*, int i, int g) {
 #pragma unroll
@@ -436,18 +440,19 @@ struct AttnTile<kPagedF32, HD, ONCE> {
     static __device__ __forceinline__ void stage(char* to, v4f x, int i, int d, int) {
         *reinterpret_cast<v4f*>(to + ((d / 16 * 4 + d / 4 % 4) * 16 + i) * 16) = x;
     }
-    __device__ __forceinline__ void take(const char* from, int, int i, int g) {
+    __device__ __forceinline__ void take(const char* from, int, float scale, int i, int g) {
+        qi = scale;
 #pragma unroll
         for (int c = 0; c < NC; ++c) q[c] = *reinterpret_cast<const v4f*>(from + ((c * 4 + g) * 16 + i) * 16);
     }
     __device__ __forceinline__ void scores(float (&s)[NS]) {
-        v4f d[2] = {};  // (two chains: a product waits for the one before it in its own)
+        v4f d[4] = {};  // (four chains: a product waits for the one before it in its own, and long sums lose more)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) d[n & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][n], q[c][n], d[n & 1], 0, 0, 0);
+            for (int n = 0; n < 4; ++n) d[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][n], q[c][n], d[n], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) s[n] = d[0][n] + d[1][n];
+        for (int n = 0; n < 4; ++n) s[n] = ((d[0][n] + d[1][n]) + (d[2][n] + d[3][n])) * qi;
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -739,8 +744,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             x.load_k(b0, b1, i, g);
             x.load_v(b0 + a.c.kv_stride, b1 + a.c.kv_stride, i, g);
         }
-        // the queries, rotated where the step asks for it, times log2(e) / sqrt(HD), into LDS; a step's new row too, where
-        // this piece has the last tile
+        // the queries, rotated where the step asks for it, into LDS; a step's new row too, where this piece has the last tile
         if (newest < 0) last = at = first;  // (a step without a place: nothing from here on)
         const float* const cs = STEP && newest >= 0 ? a.n.rope + (size_t)a.n.pos[b] * a.n.rotary : nullptr;
         const int items = newest < 0 ? 0 : rows * L, more = STEP && last == tiles ? 2 * L : 0;
@@ -748,13 +752,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             const int d = e % L * 4, row = e / L;
             if (row < rows) {
                 const float* const src = a.q + ((size_t)b * a.H + h0 + row) * HD;
-                v4f y = (STEP ? paged_rotate4(src, cs, d, a.n.rotary, a.n.interleaved) : *reinterpret_cast<const v4f*>(src + d)) * a.scale;
+                const v4f y = STEP ? paged_rotate4(src, cs, d, a.n.rotary, a.n.interleaved) : *reinterpret_cast<const v4f*>(src + d);
                 int pw = 0;
                 if constexpr (Tile::F16) {  // the head's largest into [2^14, 2^15): over the L lanes that have it
                     float big = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
 #pragma unroll
                     for (int w = 1; w < L; w <<= 1) big = fmaxf(big, __shfl_xor(big, w, 64));
-                    pw = min(max(14 + 127 - (int)(__float_as_uint(big) >> 23), -113), 126);
+                    pw = min(max(14 + 127 - (int)(__float_as_uint(big) >> 23), -113), 120);
                     if (d == 0) power[row] = pw;
                 }
                 Tile::stage(both, y, row, d, pw);
@@ -770,7 +774,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         }
         __syncthreads();
         claim();
-        x.take(both, Tile::F16 ? power[min(i, rows - 1)] : 0, min(i, rows - 1), g);  // (columns past the last head repeat it)
+        x.take(both, Tile::F16 ? power[min(i, rows - 1)] : 0, a.scale, min(i, rows - 1), g);  // (columns past the last head repeat it)
         for (; at < last; at += kWaves, ++n, there0 = next0, there1 = next1) {
             const bool more = at + kWaves < last;
             if constexpr (STEP)
