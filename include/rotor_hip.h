@@ -457,7 +457,7 @@ int rt_paged_attention(rt_ctx* ctx, const rt_pages* c, const float* q, int H, fl
                        void* workspace, size_t workspace_bytes);
 
 /* rt_paged_append of one token a sequence (M = 1) and rt_paged_attention over the lens[b] + 1 slots that are then
- * held, in one launch (one more where splits are joined or weights kept), with the same numbers in the cache; the rotated q is not
+ * held, in one launch (one more where many splits are joined or many weights kept), with the same numbers in the cache; the rotated q is not
  * kept.  A token without an angle or a place attends to nothing.  out may be n->q. */
 int rt_paged_step(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float* weights, int weight_slots, float* out,
                   void* workspace, size_t workspace_bytes);

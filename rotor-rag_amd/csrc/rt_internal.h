@@ -454,7 +454,8 @@ struct PagedAttn {
     const float* q;
     float *out, *weights, *part, *ml, *scores;  // weights, scores: null where they are not kept
     int2* units;
-    unsigned long long *tickets, nonce;  // tickets: null where a second launch joins
+    unsigned long long *tickets, nonce;
+    bool whole;               // this launch joins (by tickets) and adds the weights itself
     int slots;                // a row of weights
     int H, G, tiles, groups;  // G = H / Hkv, in tiles of 16; workgroups of the launch
     float scale;              // log2(e) / sqrt(hd)

@@ -615,11 +615,32 @@ __device__ __forceinline__ v2f paged_get(const float* at) {
         __hip_atomic_load(reinterpret_cast<const unsigned long long*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return v2f{__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32))};
 }
-// room: LDS for kLastMost floats and, behind them, a row's sums a group of threads; flag: a word of LDS.
+// What the slots of unit u weighed, by the workgroup that has its heads' totals ((reference, 1 / sum of weights) a row): scores, as
+// all workgroups of the unit have stored them, to the KV head's accumulated weights.
+__device__ __forceinline__ void paged_weigh(const PagedAttn& a, const float* score, int bk, int len, int rows, int TK, const float (*total)[2],
+                                            int t) {
+    for (int s0 = t * 4; s0 < len; s0 += 256 * kWaves) {
+        const float* const at = score + s0 / TK * rows * TK + s0 % TK;
+        float* const w = a.weights + (size_t)bk * a.slots + s0;
+        v4f add{};
+#pragma unroll 8
+        for (int row = 0; row < rows; ++row) {
+            const v2f lo = paged_get(at + row * TK), hi = paged_get(at + row * TK + 2);
+            const float ref = total[row][0], inv = total[row][1];
+            add += v4f{__builtin_amdgcn_exp2f(lo[0] - ref), __builtin_amdgcn_exp2f(lo[1] - ref), __builtin_amdgcn_exp2f(hi[0] - ref),
+                       __builtin_amdgcn_exp2f(hi[1] - ref)} * inv;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (s0 + e < len) w[e] += add[e];
+    }
+}
+// True for the workgroup that joined.  room: LDS for kLastMost floats and, behind them, a row's sums a group of threads; flag: a word
+// of LDS; total: its rows'.
 constexpr int kLastMost = 64;  // pieces times heads that the last workgroup joins
 template <int HD>
-__device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece& p, int u, unsigned long long* ticket, float* out, int rows,
-                                           float* room, int* flag, int t, int lane, int wave) {
+__device__ __forceinline__ bool paged_last(const PagedAttn& a, const PagedPiece& p, int u, unsigned long long* ticket, float* out, int rows,
+                                           float* room, int* flag, float (*total)[2], int t, int lane, int wave) {
     constexpr int L = HD / 4, NT = 64 * kWaves;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -630,7 +651,7 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
         *flag = last;
     }
     __syncthreads();
-    if (!*flag) return;
+    if (!*flag) return false;
     auto part = [&](int s, int e) { return a.part + (size_t)paged_group(s, u, p.more) * 16 * HD + e * 4; };
     const int n = p.n, cols = rows * L, groups = max(NT / cols, 1), grp = t / cols;
     float* const factor = room;  // [rows][n]
@@ -653,9 +674,14 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
     for (int row = wave; row < rows; row += kWaves) {
         const v2f x = lane < n ? paged_get(a.ml + (size_t)paged_group(lane, u, p.more) * 32 + row * 2) : v2f{-INFINITY, 0.0f};
         const float top = lane63(wave_reduce63(x[0], -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
-        const float f = __builtin_amdgcn_exp2f(x[0] - (top > -INFINITY ? top : 0.0f));
+        const float ref = top > -INFINITY ? top : 0.0f, f = __builtin_amdgcn_exp2f(x[0] - ref);
         const float sum = lane63(wave_reduce63(x[1] * f, 0.0f, [](float x, float y) { return x + y; }));
-        if (lane < n) factor[row * n + lane] = sum != 0.0f ? f / sum : 0.0f;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
+        if (lane < n) factor[row * n + lane] = f * inv;
+        if (lane == 0) {
+            total[row][0] = ref;
+            total[row][1] = inv;
+        }
     }
     __syncthreads();
     for (; mine && e < cols; e += NT) {  // (one round where there are several groups)
@@ -674,13 +700,14 @@ __device__ __forceinline__ void paged_last(const PagedAttn& a, const PagedPiece&
         else *reinterpret_cast<v4f*>(out + e * 4) = y;
         if (e + NT < cols) load(e + NT);
     }
-    if (groups == 1) return;
+    if (groups == 1) return true;
     __syncthreads();
     if (t < cols) {
         v4f y = sums[t];
         for (int w = 1; w < groups; ++w) y += sums[w * cols + t];
         *reinterpret_cast<v4f*>(out + t * 4) = y;
     }
+    return true;
 }
 
 template <int T, int HD, bool STEP, bool ONCE>
@@ -693,6 +720,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     __shared__ __align__(16) char both[kPart > Tile::QBYTES ? kPart : Tile::QBYTES];
     __shared__ float ml[kWaves][16][2];
     __shared__ int power[16];
+    __shared__ float total[16][2];
     __shared__ __align__(16) E fresh[2][STEP ? HD : 16];
     float(*const part)[16][HD + 4] = reinterpret_cast<float(*)[16][HD + 4]>(both);
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
@@ -704,13 +732,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     const int newest = STEP ? paged_newest(a, b, len) : 0;
     const int rows = min(a.G - 16 * ht, 16);
     const int h0 = kh * a.G + 16 * ht;  // the tile's first head
-    const int cap = a.c.P << a.c.shift;
+    float* const score = a.scores ? a.scores + ((size_t)b * a.H + h0) * paged_even(a.c.P << a.c.shift) : nullptr;  // the unit's
     // the unit's ticket: whatever the memory held, the first to come makes it this launch's, with none counted
-    unsigned long long* const ticket = a.tickets ? a.tickets + u : nullptr;
+    unsigned long long* const ticket = a.whole && p.n > 1 ? a.tickets + u : nullptr;
     unsigned long long held = 0ull;
-    if (ticket && p.n > 1 && t == 0) held = __hip_atomic_load(ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (ticket && t == 0) held = __hip_atomic_load(ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     auto claim = [&] {
-        if (ticket && p.n > 1 && t == 0 && held >> kTicketBits != a.nonce)
+        if (ticket && t == 0 && held >> kTicketBits != a.nonce)
             __hip_atomic_compare_exchange_strong(ticket, &held, a.nonce << kTicketBits, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
                                                  __HIP_MEMORY_SCOPE_AGENT);
     };
@@ -817,11 +845,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
             }
             x.values(s);
             if (more) x.load_v(b0 + a.c.kv_stride, b1 + a.c.kv_stride, i, g);
-            if (a.scores && i < rows) {  // (behind the loads: a wave waits for its accesses in their order)
-                float* const to = a.scores + ((size_t)b * a.H + h0) * paged_even(cap) + (at * rows + i) * TK;
+            if (score && i < rows) {  // (behind the loads: a wave waits for its accesses in their order)
+                float* const to = score + (at * rows + i) * TK;
 #pragma unroll
-                for (int e = 0; e < Tile::NS; e += 4)
-                    *reinterpret_cast<v4f*>(to + Tile::slot(e, g)) = v4f{raw[e], raw[e + 1], raw[e + 2], raw[e + 3]};
+                for (int e = 0; e < Tile::NS; e += 4) {
+                    if (a.whole) {
+                        paged_put(to + Tile::slot(e, g), raw[e], raw[e + 1]);
+                        paged_put(to + Tile::slot(e, g) + 2, raw[e + 2], raw[e + 3]);
+                    } else *reinterpret_cast<v4f*>(to + Tile::slot(e, g)) = v4f{raw[e], raw[e + 1], raw[e + 2], raw[e + 3]};
+                }
             }
         }
     }
@@ -860,7 +892,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         if (p.n == 1) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // (no slot: zeros)
             *reinterpret_cast<v4f*>(a.out + ((size_t)b * a.H + h0 + row) * HD + d) = y * inv;
-        } else if (a.tickets) {
+            if (d == 0) {
+                total[row][0] = at;
+                total[row][1] = inv;
+            }
+        } else if (a.whole) {
             paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d, y[0], y[1]);
             paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d + 2, y[2], y[3]);
             if (d == 0) paged_put(a.ml + ((size_t)blockIdx.x * 16 + row) * 2, top, sum);
@@ -868,8 +904,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
         } else *reinterpret_cast<v4f*>(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d) = y;
         if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)blockIdx.x * 16 + row) * 2) = v2f{top, sum};
     }
-    if (a.tickets) {
-        if (p.n > 1) paged_last<HD>(a, p, u, ticket, a.out + ((size_t)b * a.H + h0) * HD, rows, reinterpret_cast<float*>(both), power, t, lane, wave);
+    if (a.whole) {
+        bool mine = true;
+        if (p.n > 1)
+            mine = paged_last<HD>(a, p, u, ticket, a.out + ((size_t)b * a.H + h0) * HD, rows, reinterpret_cast<float*>(both), power, total, t,
+                                  lane, wave);
+        if (!mine || !score || newest < 0) return;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        paged_weigh(a, score, bk, len, rows, TK, total, t);
         return;
     }
     if (t == 0 && a.ml && p.piece == (p.n > 1)) a.units[u] = make_int2(p.more, p.n);
@@ -1378,6 +1421,12 @@ size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int h
                 (weights ? (size_t)B * H * paged_even(cap) : 0));
 }
 
+// The weights are added by the workgroup that has a KV head's totals, a launch less, for up to 4096 scores a KV head and 2^18 in
+// all; a second launch otherwise.  Calls, us, by the one / the other: 20 heads over 5 of 128 in bf16, 1 sequence of 1000 slots
+// 12.4 / 15.1, 12 of up to 1000 15.1 / 15.3, 32 of 120 11.6 / 15.0; but 32 of up to 1000 22.3 / 21.1, 4 of 2000 18.0 / 15.2,
+// 1200 of up to 8000 (4 over 1 of 64) 422 / 400 and, within these limits, 8 of up to 2000 (12 over 12 of 64) 17.7 / 16.4.
+constexpr int kWeighHead = 1 << 12, kWeighAll = 1 << 18;
+
 hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void* work, hipStream_t s) {
     const int cap = a.c.P << a.c.shift;
     const PagedShape p = paged_shape(a.c.B, a.H, a.c.Hkv, cap, type);
@@ -1389,19 +1438,20 @@ hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void
     a.ml = p.split || a.weights ? a.part + (p.split ? parts * hd : 0) : nullptr;
     a.units = reinterpret_cast<int2*>(a.ml + parts * 2);
     a.scores = a.weights ? a.ml + parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : nullptr;
-    const bool last = p.last && !a.weights;
-    if (last) {
+    const bool few = p.tiles == 1 && (long long)cap * a.G <= kWeighHead && (long long)cap * a.G * p.units <= kWeighAll;
+    a.whole = (p.last || !p.split) && (!a.weights || few);
+    if (a.whole && p.split) {
         static std::atomic<unsigned long long> number{paged_seed()};
         const unsigned long long most = ~0ull >> kTicketBits;
         do a.nonce = number.fetch_add(1, std::memory_order_relaxed) & most;
         while (a.nonce == 0);
         a.tickets = reinterpret_cast<unsigned long long*>(a.units);
     }
-    const long long groups = p.groups, joins = p.split && !last ? (long long)a.c.B * a.H : 0;
+    const long long groups = p.groups, joins = p.split && !a.whole ? (long long)a.c.B * a.H : 0;
     if (groups > kPagedMaxGroups) return hipErrorInvalidValue;
     a.groups = (int)groups;
     const bool wide = p.groups > 16 * p.units;  // a head's pieces by 16 waves
-    const int nt = wide ? 1024 : 256, chunks = a.weights ? (cap + 4 * nt - 1) / (4 * nt) : 0;
+    const int nt = wide ? 1024 : 256, chunks = a.weights && !a.whole ? (cap + 4 * nt - 1) / (4 * nt) : 0;
     const long long second = joins + (long long)a.c.B * a.c.Hkv * chunks;
     if (second > kPagedMaxGroups) return hipErrorInvalidValue;
     paged_by_type(type, hd, [&](auto T, auto HD) {

@@ -282,6 +282,48 @@ def test_attention_on_two_streams(hip):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,H,Hkv,hd", [
+    ([1024], 4, 1, 64), ([1025], 4, 1, 64), ([1024, 0, 513, 1], 8, 2, 128), ([256, 256], 16, 1, 128), ([288], 16, 1, 64), ([32] * 70, 17, 1, 64),
+    ([500] * 16, 15, 3, 64), ([31 + b for b in range(90)], 6, 6, 64), ([576, 40], 14, 2, 64)])
+def test_attention_weights_of_short_caches(hip, dtype, lens, H, Hkv, hd):
+    """As long as one launch adds them up, and longer; three calls onto the same sums."""
+    cache, table, n = make(lens, Hkv, hd, 32, dtype, seed=H)
+    start = torch.rand((len(lens), Hkv, table.shape[1] * 32 + 3), generator=torch.Generator().manual_seed(4))
+    q = queries(lens, H, hd)
+    want = check_attention(hip, cache, table, n, q, weights=start)
+    w, c, t, m = start.cuda(), cache.cuda(), table.cuda(), n.cuda()
+    outs = [hip.paged_attention(q.cuda(), c, t, m, weights=w) for _ in range(3)]
+    assert all(torch.equal(o, want) for o in outs)
+    check_attention(hip, cache, table, n, q)  # (without weights pieces may be joined in another order: each within its bound)
+    sums = PO.attend(q, cache, table, n)[1]
+    S = sums.shape[2]
+    total = start[:, :, :S].double() + 3 * sums
+    # each time as near as one call's, and an addition's rounding
+    most = PO.attend(q, cache, table, n)[3].amax((1, 2, 3)).view(-1, 1, 1)
+    share = 2 * (16 + 2 * math.sqrt(3 * hd)) * most + 64 + 4 * n.clamp(min=1).double().sqrt().view(-1, 1, 1)
+    assert ((w[:, :, :S].cpu().double() - total).abs() <= 3 * U * (share * sums + total) + 2.0 ** -126).all()
+
+
+def test_attention_weights_on_streams(hip):
+    """Calls that run at the same time, each with sums of its own, in workspaces that hold anything."""
+    cache, table, n = make([900, 300], 5, 128, 64, "bf16")
+    q = queries([0] * 2, 20, 128).cuda()
+    c, t, m = cache.cuda(), table.cuda(), n.cuda()
+    want = torch.zeros(2, 5, t.shape[1] * 64, device="cuda")
+    out = hip.paged_attention(q, c, t, m, weights=want)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                torch.full((1 << 20,), -1 - i, dtype=torch.int32, device="cuda")  # (what the next workspace holds)
+                w = torch.zeros_like(want)
+                got.append((hip.paged_attention(q, c, t, m, weights=w), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) and torch.equal(w, want) for o, w in got)
+
+
 def test_attention_holes(hip):
     """Holes in the middle and at the end, whole sequences of them; lengths past the table and below 0."""
     lens = [200, 64, 90, 128, 40]
