@@ -753,9 +753,14 @@ class _DeviceModel:
 
 def config_from_hf(cfg: Dict) -> Dict:
     """HF config.json -> the model config dict (src/rotor/bitnet_model.py:368-375); kv_cache_bits (this build's
-    own key) and rope_scaling go through where the file has them."""
+    own key) and rope_scaling go through where the file has them (yarn's original context, where it is left out,
+    is the file's max_position_embeddings)."""
     own = {"kv_cache_bits": cfg["kv_cache_bits"]} if "kv_cache_bits" in cfg else {}
     scaled = {"rope_scaling": cfg["rope_scaling"]} if cfg.get("rope_scaling") else {}
+    r = scaled.get("rope_scaling")
+    if isinstance(r, dict) and r.get("rope_type", r.get("type")) == "yarn" and r.get("original_max_position_embeddings") is None:
+        if "max_position_embeddings" in cfg:
+            scaled["rope_scaling"] = {**r, "original_max_position_embeddings": cfg["max_position_embeddings"]}
     return {
         **own,
         **scaled,
