@@ -135,6 +135,8 @@ class BitNetModel:
         self.head_dim = self.d_model // self.n_heads
         self.rope_theta = float(config.get("rope_theta", 500000.0))
         self.rope_scaling = config.get("rope_scaling")  # None, or rope_table's scaling
+        if self.rope_scaling:
+            rope_table(1, self.head_dim, self.rope_theta, self.rope_scaling)  # (what it refuses, before anything is loaded)
         self.eps = float(config.get("rms_norm_eps", 1e-6))
         self.max_seq_len = int(config.get("max_seq_len", 2048))
         self.max_tokens = int(config.get("max_batch_tokens", 512))

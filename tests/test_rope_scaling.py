@@ -19,3 +19,15 @@ def test_yarn_takes_the_context_from_the_config():
     assert config_from_hf(dict(HF, rope_scaling=named))["rope_scaling"] == named
     linear = {"type": "linear", "factor": 2.0}
     assert config_from_hf(dict(HF, rope_scaling=linear))["rope_scaling"] == linear
+
+
+def model_config(**kw):
+    return dict(vocab_size=64, d_model=512, n_layers=1, n_heads=4, n_kv_heads=2, d_ff=256, max_seq_len=64, **kw)
+
+
+@pytest.mark.parametrize("bad", [{"rope_type": "llama3", "factor": 8.0}, {"type": "dynamic", "factor": 2.0}, {"rope_type": "longrope"},
+                                 {"rope_type": "linear", "factor": -1.0}, {"rope_type": "yarn", "factor": 2.0}, {"factor": 2.0}])
+def test_refused_with_the_config(bad):
+    """The constructor says so, with the config alone: no weight has been read and no device looked for."""
+    with pytest.raises(ValueError, match="rope_scaling"):
+        BitNetModel(model_config(rope_scaling=bad), use_gpu=True)
