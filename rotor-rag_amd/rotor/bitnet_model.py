@@ -44,6 +44,11 @@ _SWITCHES = ("attn_in_prologue", "ffn_pair", "attn_in_qkv", "attn_combine_in_qkv
 _STAGE_BYTES = 8 << 20  # one of a model's two pinned staging buffers
 
 
+# What a rope_scaling may say besides its type: a key that is not among these might change the angles, and is refused.
+_ROPE_KEYS = {"factor", "original_max_position_embeddings", "finetuned", "rope_type", "type"}
+_YARN_KEYS = {"beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"}
+
+
 def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict] = None) -> np.ndarray:
     """(cos, sin) of pos * theta^(-2i/head_dim), [max_len, head_dim/2, 2] fp32 (computed in f64); head_dim:
     the dimensions that are rotated.  scaling, for contexts longer than the trained one, as in a config.json's
@@ -51,12 +56,21 @@ def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict
       linear  every frequency / f (position interpolation)
       ntk     theta * f^(d / (d - 2)): the lowest frequency / f, the highest as it is
       yarn    frequencies of more than beta_fast (32) turns in original_max_position_embeddings as they are, of fewer
-              than beta_slow (1) / f, between them mixed, and (cos, sin) times attention_factor (0.1 ln f + 1)"""
+              than beta_slow (1) / f, between them mixed (truncate (True): from a whole pair to a whole pair), and
+              (cos, sin) times attention_factor (grow(mscale) / grow(mscale_all_dim), grow(1) where these are left out;
+              grow(m) = 0.1 m ln f + 1 for f > 1, else 1)
+      default as without scaling
+    Keys that a type does not take are refused (but for default, which takes none)."""
     d = head_dim
     i = np.arange(d // 2, dtype=np.float64)
     inv, grow = theta ** (-(2.0 * i) / d), 1.0
     if scaling:
         kind, f = scaling.get("rope_type", scaling.get("type")), float(scaling.get("factor", 1.0))
+        if kind not in ("linear", "ntk", "yarn", "default"):
+            raise ValueError(f"rope_scaling: rope_type {kind!r}: linear, ntk, yarn or default")
+        unknown = {k for k, v in scaling.items() if v is not None} - _ROPE_KEYS - (_YARN_KEYS if kind == "yarn" else set())
+        if unknown and kind != "default":
+            raise ValueError(f"rope_scaling: {kind} does not take {', '.join(map(str, sorted(unknown, key=str)))}")
         if not (np.isfinite(f) and f > 0):
             raise ValueError(f"rope_scaling: factor {f}")
         if kind == "linear":
@@ -70,14 +84,20 @@ def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict
                 raise ValueError("rope_scaling: yarn needs original_max_position_embeddings")
             n = float(scaling["original_max_position_embeddings"])
             at = lambda turns: d * np.log(n / (turns * 2 * np.pi)) / (2 * np.log(theta))  # noqa: E731  (that pair's number)
-            first = max(np.floor(at(float(scaling.get("beta_fast", 32)))), 0)
-            last = min(np.ceil(at(float(scaling.get("beta_slow", 1)))), d - 1)
+            first, last = at(float(scaling.get("beta_fast", 32))), at(float(scaling.get("beta_slow", 1)))
+            if scaling.get("truncate") is not False:
+                first, last = np.floor(first), np.ceil(last)
+            first, last = max(first, 0), min(last, d - 1)
             slow = np.clip((i - first) / max(last - first, 0.001), 0, 1)
             inv = inv / f * slow + inv * (1 - slow)
-            grow = scaling.get("attention_factor")
-            grow = float(grow) if grow is not None else 0.1 * np.log(f) + 1 if f > 1 else 1.0
-        elif kind != "default":
-            raise ValueError(f"rope_scaling: rope_type {kind!r}: linear, ntk, yarn or default")
+            grow, m, all_m = (scaling.get(k) for k in ("attention_factor", "mscale", "mscale_all_dim"))
+            if (m is None) != (all_m is None):
+                raise ValueError("rope_scaling: mscale and mscale_all_dim: both or neither")
+            size = lambda m: 0.1 * m * np.log(f) + 1 if f > 1 else 1.0  # noqa: E731
+            if grow is not None:
+                grow = float(grow)
+            else:
+                grow = size(float(m)) / size(float(all_m)) if m is not None else size(1)
     ang = np.arange(max_len, dtype=np.float64)[:, None] * inv[None, :]
     return (np.stack([np.cos(ang), np.sin(ang)], axis=-1) * grow).astype(np.float32)
 

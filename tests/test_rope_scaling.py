@@ -31,3 +31,62 @@ def test_refused_with_the_config(bad):
     """The constructor says so, with the config alone: no weight has been read and no device looked for."""
     with pytest.raises(ValueError, match="rope_scaling"):
         BitNetModel(model_config(rope_scaling=bad), use_gpu=True)
+
+
+def amplitude(**kw):
+    t = rope_table(4, 64, 1e4, {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096, **kw})
+    a = np.hypot(t[..., 0].astype(np.float64), t[..., 1])
+    assert np.ptp(a) < 1e-6
+    return a.mean()
+
+
+def test_yarn_amplitude():
+    """attention_factor, or the ratio of 0.1 m ln f + 1 for mscale and for mscale_all_dim, or that with 1 alone."""
+    ln = np.log(40.0)
+    for want, kw in ((0.1 * ln + 1, {}), (1.0, dict(mscale=1.0, mscale_all_dim=1.0)), (1.0, dict(mscale=0.707, mscale_all_dim=0.707)),
+                     ((0.1 * ln + 1) / (0.05 * ln + 1), dict(mscale=1.0, mscale_all_dim=0.5)), (0.1 * ln + 1, dict(mscale=1, mscale_all_dim=0)),
+                     (1.25, dict(attention_factor=1.25)), (1.25, dict(attention_factor=1.25, mscale=1.0, mscale_all_dim=0.5)),
+                     (0.1 * ln + 1, dict(attention_factor=None, mscale=None, mscale_all_dim=None, truncate=None))):
+        assert abs(amplitude(**kw) - want) < 1e-6, kw
+    for alone in (dict(mscale=0.707), dict(mscale_all_dim=1.0)):
+        with pytest.raises(ValueError, match="rope_scaling: .*mscale"):
+            amplitude(**alone)
+
+
+def frequencies(rotary, theta, **kw):
+    """Each pair's angle at position 1, over what it is without scaling."""
+    t = rope_table(2, rotary, theta, {"rope_type": "yarn", "attention_factor": 1.0, **kw})[1].astype(np.float64)
+    plain = theta ** (-np.arange(0, rotary, 2) / rotary)
+    return np.arctan2(t[:, 1], t[:, 0]) / plain
+
+
+@pytest.mark.parametrize("truncate", [True, False])
+def test_yarn_mixed_frequencies(truncate):
+    """The ramp worked out by hand.  rotary 16, theta 2^16: pair i turns n 2^(-2 i) / (2 pi) times in n positions.  With n = 2^13 pi
+    it is 2^(12 - 2 i): beta_fast 2^7 turns is pair 2.5, beta_slow 2 is pair 5.5."""
+    got = frequencies(16, 65536.0, factor=8.0, original_max_position_embeddings=2.0 ** 13 * np.pi, beta_fast=128, beta_slow=2, truncate=truncate)
+    ramp = [0, 0, 0, 1 / 4, 2 / 4, 3 / 4, 1, 1] if truncate else [0, 0, 0, 1 / 6, 3 / 6, 5 / 6, 1, 1]  # from 2 to 6, or 2.5 to 5.5
+    want = np.array([1 - r + r / 8 for r in ramp])
+    assert np.allclose(got, want, rtol=1e-6, atol=0)
+
+
+@pytest.mark.parametrize("bad", [{"rope_type": "linear", "factor": 2.0, "attention_factor": 2.0}, {"rope_type": "linear", "factor": 2.0, "rope_theta": 5e5},
+                                 {"rope_type": "ntk", "factor": 2.0, "alpha": 3.0}, {"rope_type": "ntk", "factor": 2.0, "beta_fast": 32},
+                                 {**YARN, "original_max_position_embeddings": 4096, "short_factor": [1.0]},
+                                 {**YARN, "original_max_position_embeddings": 4096, "high_freq_factor": 4.0}])
+def test_keys_that_a_type_does_not_take(bad):
+    """... and might change the angles are refused, not dropped."""
+    with pytest.raises(ValueError, match="rope_scaling: .*" + list(bad)[-1]):
+        rope_table(4, 64, 1e4, bad)
+
+
+def test_keys_that_change_nothing():
+    """Null, a type under both names, what another program noted; the context that a type does not go by; plain angles by name."""
+    plain = rope_table(50, 64, 1e4)
+    for kind in ("linear", "ntk"):
+        want = rope_table(50, 64, 1e4, {"type": kind, "factor": 2.0})
+        assert not np.array_equal(want, plain)
+        assert np.array_equal(want, rope_table(50, 64, 1e4, {"rope_type": kind, "type": kind, "factor": 2, "finetuned": True, "alpha": None,
+                                                             "original_max_position_embeddings": 4096}))
+    assert np.array_equal(plain, rope_table(50, 64, 1e4, {"rope_type": "default", "mrope_section": [16, 8, 8]}))
+    assert np.array_equal(plain, rope_table(50, 64, 1e4, {}))
