@@ -57,22 +57,34 @@ def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict
       ntk     theta * f^(d / (d - 2)): the lowest frequency / f, the highest as it is
       yarn    frequencies of more than beta_fast (32) turns in original_max_position_embeddings as they are, of fewer
               than beta_slow (1) / f, between them mixed (truncate (True): from a whole pair to a whole pair), and
-              (cos, sin) times attention_factor (grow(mscale) / grow(mscale_all_dim), grow(1) where these are left out;
-              grow(m) = 0.1 m ln f + 1 for f > 1, else 1)
+              (cos, sin) times attention_factor (size(mscale) / size(mscale_all_dim), size(1) where these are left out;
+              size(m) = 0.1 m ln f + 1 for f > 1, else 1)
       default as without scaling
     Keys that a type does not take are refused (but for default, which takes none)."""
     d = head_dim
     i = np.arange(d // 2, dtype=np.float64)
     inv, grow = theta ** (-(2.0 * i) / d), 1.0
     if scaling:
-        kind, f = scaling.get("rope_type", scaling.get("type")), float(scaling.get("factor", 1.0))
+        if not isinstance(scaling, dict):
+            raise ValueError(f"rope_scaling: {scaling!r}: a dict")
+        kind = scaling.get("rope_type", scaling.get("type"))
         if kind not in ("linear", "ntk", "yarn", "default"):
             raise ValueError(f"rope_scaling: rope_type {kind!r}: linear, ntk, yarn or default")
         unknown = {k for k, v in scaling.items() if v is not None} - _ROPE_KEYS - (_YARN_KEYS if kind == "yarn" else set())
         if unknown and kind != "default":
             raise ValueError(f"rope_scaling: {kind} does not take {', '.join(map(str, sorted(unknown, key=str)))}")
-        if not (np.isfinite(f) and f > 0):
-            raise ValueError(f"rope_scaling: factor {f}")
+
+        def number(name, default=None, zero=False):
+            v = scaling.get(name)
+            try:
+                x = float(default if v is None else v)
+            except (TypeError, ValueError):
+                x = np.nan
+            if not (0 < x < np.inf or zero and x == 0):
+                raise ValueError(f"rope_scaling: {name} {v!r}: needs a number {'>= 0' if zero else '> 0'}")
+            return x
+
+        f = number("factor") if kind != "default" else 1.0
         if kind == "linear":
             inv = inv / f
         elif kind == "ntk":
@@ -80,24 +92,24 @@ def rope_table(max_len: int, head_dim: int, theta: float, scaling: Optional[Dict
                 raise ValueError("rope_scaling: ntk needs more than one pair")
             inv = (theta * f ** (d / (d - 2.0))) ** (-(2.0 * i) / d)
         elif kind == "yarn":
-            if "original_max_position_embeddings" not in scaling:
-                raise ValueError("rope_scaling: yarn needs original_max_position_embeddings")
-            n = float(scaling["original_max_position_embeddings"])
+            n, fast, slow = number("original_max_position_embeddings"), number("beta_fast", 32), number("beta_slow", 1)
+            if fast < slow:
+                raise ValueError(f"rope_scaling: beta_fast {fast} and beta_slow {slow}: needs beta_fast >= beta_slow")
+            if not theta > 1:
+                raise ValueError(f"rope_scaling: yarn needs theta > 1, not {theta}")
+            if not isinstance(scaling.get("truncate"), (bool, type(None))):
+                raise ValueError(f"rope_scaling: truncate {scaling['truncate']!r}: true or false")
             at = lambda turns: d * np.log(n / (turns * 2 * np.pi)) / (2 * np.log(theta))  # noqa: E731  (that pair's number)
-            first, last = at(float(scaling.get("beta_fast", 32))), at(float(scaling.get("beta_slow", 1)))
+            first, last = at(fast), at(slow)
             if scaling.get("truncate") is not False:
                 first, last = np.floor(first), np.ceil(last)
             first, last = max(first, 0), min(last, d - 1)
-            slow = np.clip((i - first) / max(last - first, 0.001), 0, 1)
-            inv = inv / f * slow + inv * (1 - slow)
-            grow, m, all_m = (scaling.get(k) for k in ("attention_factor", "mscale", "mscale_all_dim"))
-            if (m is None) != (all_m is None):
+            mixed = np.clip((i - first) / max(last - first, 0.001), 0, 1)
+            inv = inv / f * mixed + inv * (1 - mixed)
+            if (scaling.get("mscale") is None) != (scaling.get("mscale_all_dim") is None):
                 raise ValueError("rope_scaling: mscale and mscale_all_dim: both or neither")
             size = lambda m: 0.1 * m * np.log(f) + 1 if f > 1 else 1.0  # noqa: E731
-            if grow is not None:
-                grow = float(grow)
-            else:
-                grow = size(float(m)) / size(float(all_m)) if m is not None else size(1)
+            grow = number("attention_factor", size(number("mscale", 1, True)) / size(number("mscale_all_dim", 0, True)))
     ang = np.arange(max_len, dtype=np.float64)[:, None] * inv[None, :]
     return (np.stack([np.cos(ang), np.sin(ang)], axis=-1) * grow).astype(np.float32)
 

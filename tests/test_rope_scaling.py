@@ -90,3 +90,41 @@ def test_keys_that_change_nothing():
                                                              "original_max_position_embeddings": 4096}))
     assert np.array_equal(plain, rope_table(50, 64, 1e4, {"rope_type": "default", "mrope_section": [16, 8, 8]}))
     assert np.array_equal(plain, rope_table(50, 64, 1e4, {}))
+
+
+@pytest.mark.parametrize("kind", ["linear", "ntk", "yarn"])
+@pytest.mark.parametrize("name,values", [
+    ("factor", [0, -2.0, float("inf"), float("nan"), "two", [2.0]]), ("original_max_position_embeddings", [0, -5, float("inf"), float("nan"), "long"]),
+    ("beta_fast", [0, -1, 0.5, float("nan"), "x"]), ("beta_slow", [0, -1, 33, float("inf")]), ("attention_factor", [0, -1, float("nan"), "x"]),
+    ("mscale", [-1, float("nan"), "x"]), ("mscale_all_dim", [-1, float("inf")]), ("truncate", [0, "no"])])
+def test_values_out_of_range(kind, name, values):
+    """A ValueError that names the key, and neither a table of NaN nor another error."""
+    whole = dict(rope_type=kind, factor=4.0)
+    if kind == "yarn":
+        whole.update(original_max_position_embeddings=4096, mscale=1.0, mscale_all_dim=1.0)
+    elif name != "factor":
+        return
+    rope_table(4, 64, 1e4, whole)
+    for v in values:
+        with np.errstate(all="raise"), pytest.raises(ValueError, match="rope_scaling: .*" + name):
+            rope_table(4, 64, 1e4, {**whole, name: v})
+
+
+def test_a_factor_is_needed():
+    for kind in ("linear", "ntk", "yarn"):
+        for missing in ({}, {"factor": None}):
+            with pytest.raises(ValueError, match="rope_scaling: factor"):
+                rope_table(4, 64, 1e4, {"rope_type": kind, "original_max_position_embeddings": 4096, **missing})
+    assert np.array_equal(rope_table(4, 64, 1e4, {"rope_type": "default", "factor": None}), rope_table(4, 64, 1e4))
+
+
+def test_odd_forms():
+    for bad in ("linear", ["linear", 2.0], 4):
+        with pytest.raises(ValueError, match="rope_scaling"):
+            rope_table(4, 64, 1e4, bad)
+        with pytest.raises(ValueError, match="rope_scaling"):
+            BitNetModel(model_config(rope_scaling=bad), use_gpu=True)
+    for theta in (1.0, 0.5):  # (the pair that turns so often: no such number)
+        with np.errstate(all="raise"), pytest.raises(ValueError, match="rope_scaling: .*theta"):
+            rope_table(4, 64, theta, {**YARN, "original_max_position_embeddings": 4096})
+    assert np.isfinite(rope_table(4, 64, 1.0, {"rope_type": "linear", "factor": 2.0})).all()
