@@ -615,6 +615,12 @@ __device__ __forceinline__ v2f paged_get(const float* at) {
         __hip_atomic_load(reinterpret_cast<const unsigned long long*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return v2f{__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32))};
 }
+// Whether slots s .. s + 3 (s % 4 == 0, so of one page) are there: weights of those in a hole are left alone, where a head
+// whose sum is NaN would leave a NaN.
+__device__ __forceinline__ bool paged_there(const PagedCache& c, int b, int s) {
+    const int id = c.table[(size_t)b * c.P + (s >> c.shift)];
+    return id >= 0 && id < c.pages;
+}
 // What the slots of unit u weighed, by the workgroup that has its heads' totals ((reference, 1 / sum of weights) a row): scores, as
 // all workgroups of the unit have stored them, to the KV head's accumulated weights.
 __device__ __forceinline__ void paged_weigh(const PagedAttn& a, const float* score, int bk, int len, int rows, int TK, const float (*total)[2],
@@ -622,6 +628,7 @@ __device__ __forceinline__ void paged_weigh(const PagedAttn& a, const float* sco
     for (int s0 = t * 4; s0 < len; s0 += 256 * kWaves) {
         const float* const at = score + s0 / TK * rows * TK + s0 % TK;
         float* const w = a.weights + (size_t)bk * a.slots + s0;
+        const bool there = paged_there(a.c, bk / a.c.Hkv, s0);
         v4f add{};
 #pragma unroll 8
         for (int row = 0; row < rows; ++row) {
@@ -632,7 +639,7 @@ __device__ __forceinline__ void paged_weigh(const PagedAttn& a, const float* sco
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (s0 + e < len) w[e] += add[e];
+            if (there && s0 + e < len) w[e] += add[e];
     }
 }
 // True for the workgroup that joined.  room: LDS for kLastMost floats and, behind them, a row's sums a group of threads; flag: a word
@@ -982,6 +989,7 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
     }
     __syncthreads();
     if (s0 >= len) return;
+    const bool there = paged_there(a.c, b, s0);
     v4f add{};
     for (int h = 0; h < a.G; h += 16) {
         const int rows = min(a.G - h, 16);
@@ -996,7 +1004,7 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
     float* const w = a.weights + (size_t)bk * a.slots + s0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (s0 + e < len) w[e] += add[e];
+        if (there && s0 + e < len) w[e] += add[e];
 }
 
 // ---- eviction ----------------------------------------------------------------------------
