@@ -10,6 +10,14 @@ import test_gpu_paged as P
 pytestmark = pytest.mark.gpu
 
 
+def workspace(H, cache, table, weights):
+    """Bytes that a call's pieces need: above 0 where it may cut a sequence."""
+    from rotor.gpu_ternary import _paged_types, _paged_workspace_bytes
+
+    Hkv, page, hd = cache.shape[2:]
+    return _paged_workspace_bytes(_paged_types()[cache.dtype], Hkv, page, hd, *table.shape, H, weights)
+
+
 # ---- weights -----------------------------------------------------------------------------
 
 
@@ -37,3 +45,110 @@ def test_weights_of_holes(hip, dtype, slots, bad):
         for h in range(2):
             nan = bad and b == 0 and h == 0
             assert w[b, h, there].isnan().all() if nan else (w[b, h, there] > 0).all()
+
+
+# ---- together with torch's graphs ----------------------------------------------------------
+
+
+STEPS = {  # lens, H, Hkv, hd, page, dtype, weights, slots of the table beyond the lengths
+    "last workgroup, weights in the launch": ([900], 20, 5, 128, 64, "bf16", True, 20),
+    "last workgroup": ([900, 350, 0], 20, 5, 128, 64, "bf16", False, 20),
+    "second launch, weights": ([4000, 30], 20, 5, 128, 64, "bf16", True, 20),
+    "second launch": ([9000], 8, 2, 64, 128, "fp16", False, 20),
+    "second launch, 1024 threads": ([1800, 3, 700], 14, 2, 64, 32, "fp32", True, 20),
+    "more sequences than lanes": ([10 * b for b in range(70)], 4, 2, 64, 32, "bf16", True, 300),
+}
+
+
+@pytest.mark.parametrize("name", STEPS)
+def test_replayed_steps_that_are_joined(hip, name):
+    """Two captured steps that advance by themselves, in one workspace of the caller's that holds anything between the replays;
+    every replay equal to the eager call on the same state, and that to the definition."""
+    from rotor import _hip
+
+    lens, H, Hkv, hd, page, dtype, weighted, extra = STEPS[name]
+    cache, table, n = P.make(lens, Hkv, hd, page, dtype, extra=extra)
+    B, t, need = len(lens), table.cuda(), workspace(H, cache, table, weighted)
+    assert need > 0
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn((B, 1, m, hd), generator=gen).cuda() for m in (H, Hkv, Hkv))
+    rope = P.rope_angles(max(lens) + extra, hd).cuda()
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+
+    class State:
+        def __init__(self):
+            self.cache, self.lens = cache.cuda(), n.cuda()
+            self.w = torch.zeros((B, Hkv, t.shape[1] * page), device="cuda") if weighted else None
+            self.out = torch.zeros_like(q)
+
+        def call(self):
+            c = self.cache
+            pages = _hip.PAGES.pack(c.data_ptr(), c.stride(0), c.stride(1), t.data_ptr(), self.lens.data_ptr(), {"fp32": 0, "bf16": 1, "fp16": 2}[dtype],
+                                    c.shape[1], Hkv, page, hd, B, t.shape[1])
+            new = _hip.PAGED_NEW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), rope.data_ptr(), self.lens.data_ptr(), 0, rope.shape[0], hd, 0, 1, H)
+            hip._bind_stream()
+            _hip.check(hip.lib.rt_paged_step(hip.ctx, pages, new, self.w.data_ptr() if weighted else None, t.shape[1] * page,
+                                             self.out.data_ptr(), ws.data_ptr(), need))
+            self.lens += 1
+
+    a, b, e = State(), State(), State()
+    side, graphs = torch.cuda.Stream(), []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in (a, b):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                s.call()
+    torch.cuda.current_stream().wait_stream(side)
+    bits = torch.int32 if dtype == "fp32" else torch.int16
+    for i, fill in enumerate([lambda: ws.fill_(255), lambda: ws.random_(0, 256), lambda: ws.zero_(), lambda: None, lambda: ws.fill_(1), lambda: None]):
+        old = (e.w.cpu() if weighted else None, e.lens.cpu())
+        e.call()
+        for g in graphs:
+            fill()
+            g.replay()
+        for s in (a, b):
+            assert torch.equal(s.out, e.out) and torch.equal(s.lens, e.lens) and torch.equal(s.cache.view(bits), e.cache.view(bits)), i
+            assert not weighted or torch.equal(s.w, e.w), i
+        torch.cuda.synchronize()
+        if i in (0, 5):  # (the queries as paged_append turns them)
+            turned = hip.paged_append(q, k, v, e.cache.clone(), t, old[1].cuda(), rope, old[1].cuda())
+
+            def once(w):
+                if weighted:
+                    w.copy_(e.w)
+                return e.out
+
+            P.check_attention(hip, e.cache.cpu(), table, e.lens.cpu(), turned.cpu(), weights=old[0], call=once)
+
+
+def test_replayed_steps_whose_memory_is_used_again(hip):
+    """Through the Python entry point: within a graph, the step's workspace is memory that other tensors of the graph have next."""
+    cache, table, n = P.make([1500, 900], 5, 128, 64, "bf16", extra=10)
+    need = workspace(20, cache, table, True)
+    assert need > 0
+    q, k = P.queries([0] * 2, 20, 128).cuda(), torch.randn(2, 1, 5, 128, device="cuda")
+    rope, t = P.rope_angles(1600, 128).cuda(), table.cuda()
+
+    def state():
+        return [cache.cuda(), n.cuda(), torch.zeros(2, 5, t.shape[1] * 64, device="cuda")]
+
+    def step(s, value):
+        outs = [hip.paged_step(q, k, k, s[0], t, s[1], rope, s[1], weights=s[2])]
+        torch.full((need,), value, dtype=torch.uint8, device="cuda")
+        s[1] += 1
+        outs.append(hip.paged_attention(q, s[0], t, s[1]))
+        torch.full((need,), 255 - value, dtype=torch.uint8, device="cuda")
+        return outs
+
+    a, e = state(), state()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        got = step(a, 3)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(6):
+        want = step(e, i)
+        g.replay()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a[2], e[2]), i
+        torch.cuda.synchronize()
