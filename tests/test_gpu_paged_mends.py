@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import test_gpu_paged as P
+from oracle import paged_oracle as PO
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +153,40 @@ def test_replayed_steps_whose_memory_is_used_again(hip):
         g.replay()
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a[2], e[2]), i
         torch.cuda.synchronize()
+
+
+# ---- tokens without a place ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("held,heads", [(1500, 4), (1500, 16), (9000, 4)])
+def test_step_without_a_place_that_is_joined(hip, weights, held, heads):
+    """No page, no slot, no angle, over caches that are cut into pieces: nothing written, zeros, weights left, and the others as they
+    would be."""
+    page, hd = 64, 64
+    cache, table, _ = P.make([held] * 6, 1, hd, page, "bf16", extra=page)
+    cap = table.shape[1] * page
+    assert workspace(heads, cache, table, weights) > 0
+    table[1, held // page] = -1
+    lens = torch.tensor([held, held, cap, -1, held, held], dtype=torch.int32)
+    pos = torch.tensor([40, 40, 40, 40, 50, -1], dtype=torch.int32)
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn((6, 1, n, hd), generator=gen) for n in (heads, 1, 1))
+    rope = P.rope_angles(50, hd)
+    start = torch.rand((6, 1, cap), generator=gen)
+    c, w = cache.cuda(), start.cuda() if weights else None
+    out = hip.paged_step(*(x.cuda() for x in (q, k, v)), c, table.cuda(), lens.cuda(), rope.cuda(), pos.cuda(), weights=w).cpu()
+    assert (out[1:] == 0).all()
+    if weights:
+        assert torch.equal(w[1:].cpu(), start[1:])
+    changed = (c.cpu().float().nan_to_num(7.0) != cache.float().nan_to_num(7.0)).any(-1).nonzero()
+    assert {(int(p), int(r)) for _, p, _, r in changed} == {(int(table[0, held // page]), held % page)}
+    turned, _ = PO.append(q[:1], k[:1], v[:1], cache, table[:1], lens[:1], rope, pos[:1])
+    n = torch.tensor([held + 1], dtype=torch.int32)
+
+    def first(wd):
+        if weights:
+            wd.copy_(w[:1])
+        return out[:1]
+
+    P.check_attention(hip, c.cpu(), table[:1], n, turned.float(), weights=start[:1] if weights else None, call=first)
