@@ -190,3 +190,36 @@ def test_step_without_a_place_that_is_joined(hip, weights, held, heads):
         return out[:1]
 
     P.check_attention(hip, c.cpu(), table[:1], n, turned.float(), weights=start[:1] if weights else None, call=first)
+
+
+# ---- layouts -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", P.TYPES)
+def test_layers_of_one_tensor(hip, dtype):
+    """Append, step and eviction on a layer whose pages hold keys next to values, between other layers: as on a cache of its own, and
+    nothing else is touched."""
+    B, H, Hkv, hd, page, keep = 2, 8, 2, 64, 32, 40
+    cache, table, n = P.make([90, 40], Hkv, hd, page, dtype, extra=12, spare=6)
+    free = torch.tensor(sorted(set(range(cache.shape[1])) - set(table.flatten().tolist())))[:4].view(2, 2).int().cuda()
+    gen = torch.Generator().manual_seed(6)
+    bits = torch.int32 if dtype == "fp32" else torch.int16
+    layers = torch.randn((cache.shape[1], 3, 2, *cache.shape[2:]), generator=gen).to(cache.dtype).cuda()
+    layers[:, 1] = cache.cuda().transpose(0, 1)
+    others = layers[:, ::2].clone()
+    near, apart = layers[:, 1].transpose(0, 1), cache.cuda()
+    assert not near.is_contiguous()
+    new = lambda M: [torch.randn((B, M, m, hd), generator=gen).cuda() for m in (H, Hkv, Hkv)]  # noqa: E731
+    rope, t, lens = P.rope_angles(200, 32).cuda(), table.cuda(), n.cuda()
+    prompt, one, w = new(9), new(1), torch.rand((B, Hkv, table.shape[1] * page), generator=gen).cuda()
+    runs = []
+    for c in (near, apart):
+        weights = w.clone()
+        outs = [hip.paged_append(*prompt, c, t, lens, rope, lens), c.clone()]
+        outs += [hip.paged_step(*one, c, t, lens + 9, rope, lens + 9, weights=weights), c.clone(), weights]
+        outs += [*hip.paged_evict(c, t, lens + 10, weights, keep, 7, free), c.clone()]
+        runs.append(outs)
+    for x, y in zip(*runs):
+        assert torch.equal(x.contiguous().view(bits if x.dtype == cache.dtype else torch.int32),
+                           y.contiguous().view(bits if x.dtype == cache.dtype else torch.int32))
+    assert torch.equal(layers[:, ::2].view(bits), others.view(bits))
