@@ -9,6 +9,7 @@ import test_gpu_paged as P
 from oracle import paged_oracle as PO
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
 
 
 def workspace(H, cache, table, weights):
@@ -223,3 +224,32 @@ def test_layers_of_one_tensor(hip, dtype):
         assert torch.equal(x.contiguous().view(bits if x.dtype == cache.dtype else torch.int32),
                            y.contiguous().view(bits if x.dtype == cache.dtype else torch.int32))
     assert torch.equal(layers[:, ::2].view(bits), others.view(bits))
+
+
+# ---- accuracy ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", P.TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_every_bit_of_queries_and_weights(hip, dtype, hd):
+    """Two slots, keys e_d and 0, values 1 and 0: the output is 1 / (1 + exp(-x / sqrt(hd))) for a query x e_d whose 24 bits all count.
+    With s = x log2(e) / sqrt(hd): products and their sums are exact; the scale's constant, root and quotient and the product with it are
+    off by 4 u |s|, which is no more than 4 ln 2 u |s| of a weight; exp2 by an ulp (2 u), sum, reciprocal and product by u each, and
+    the splits of the weights by nothing: (4 |s| + 8) u of the output.  Queries, or weights, of two bf16 are off by up to 2^-15 of
+    themselves, 512 u.  Another dimension of the query, where the keys are 0, is 2^20 times as large and must not cost it bits."""
+    H, gen = 64, torch.Generator().manual_seed(hd)
+    x = (torch.rand(H, generator=gen) * 8 - 4) * math.sqrt(hd) / math.log2(math.e)
+    table, n = torch.tensor([[1]], dtype=torch.int32), torch.tensor([2], dtype=torch.int32)
+    for d, big in ((5, None), (hd - 1, 3), (33, 60)):
+        cache = torch.full((2, 3, 1, 16, hd), math.nan, dtype=P.TYPES[dtype])
+        cache[:, 1, :, :2] = 0
+        cache[0, 1, 0, 0, d], cache[1, 1, 0, 0] = 1, 1
+        q = torch.zeros(1, 1, H, hd)
+        q[0, 0, :, d] = x
+        if big is not None:
+            q[..., big] = x.abs().max() * 2.0 ** 20
+        s = x.double() * math.log2(math.e) / math.sqrt(hd)
+        want = (1 / (1 + torch.exp2(-s)))[None, None, :, None]
+        got = hip.paged_attention(q.cuda(), cache.cuda(), table.cuda(), n.cuda()).cpu().double()
+        bound = (4 * s.abs() + 8)[None, None, :, None] * U * want
+        assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max().item()
