@@ -253,3 +253,30 @@ def test_every_bit_of_queries_and_weights(hip, dtype, hd):
         got = hip.paged_attention(q.cuda(), cache.cuda(), table.cuda(), n.cuda()).cpu().double()
         bound = (4 * s.abs() + 8)[None, None, :, None] * U * want
         assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max().item()
+
+
+# ---- a model's angles ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+def test_model_with_angles_scaled_by_two(hip, bits):
+    """The first layer's keys at position 2 p under linear scaling by 2 are those of the same token at p without it, bit for bit: in a
+    prompt and in single steps."""
+    import numpy as np
+
+    import test_gpu_model as T
+    from oracle import rotor_oracle as O
+
+    params = O.make_bitnet_params(77, T.SMALL, 96)
+    ids = np.random.default_rng(2).integers(0, T.SMALL["vocab_size"], 21).astype(np.int32)
+    twice = np.repeat(ids, 2)
+    keys = []
+    for scaling, seq in ((None, ids), ({"rope_type": "linear", "factor": 2.0}, twice)):
+        model = T._device_model(hip, params, dict(T.SMALL, kv_cache_bits=bits, rope_scaling=scaling), 96)
+        first = len(seq) // 3 * 2 // 2 * 2
+        _, cache = model.forward(seq[:first], use_cache=True)
+        for token in seq[first:]:
+            _, cache = model.forward(np.array([token], np.int32), past_kv_cache=cache, use_cache=True)
+        keys.append(np.asarray(cache[0]["k"]))
+    assert keys[0].shape[2] == 21 and keys[1].shape[2] == 42
+    assert np.array_equal(keys[0], keys[1][:, :, ::2]) and not np.array_equal(keys[0], keys[1][:, :, :21])
