@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedCache c, PagedNe
 //
 // fp32 numbers times 16-bit ones, in fp32: x is cut into three bf16 that sum up to x exactly (for a cache in
 // bf16), or two fp16 and what is left times 2^20 as a third in sums of its own (fp16, x scaled into [0, 2^15]): every product
-// is then exact, and all sums are fp32.  Two terms would leave 2^-17 (bf16), or 2^-40 of the row's largest (fp16), which
-// numbers 2^16 apart would show.  A cache in fp32 takes fp32 products.
+// is then exact, and all sums are fp32.  Two terms would leave up to 2^-15 of x (bf16, cut off and not rounded), or 2^-40 of the row's
+// largest (fp16).  A cache in fp32 takes fp32 products.
 //
 // Every load is issued half a round before its use: the next tile's keys when this one's are multiplied, its values after
 // this one's.
@@ -1429,11 +1429,14 @@ size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int h
                 (weights ? (size_t)B * H * paged_even(cap) : 0));
 }
 
-// The weights are added by the workgroup that has a KV head's totals, a launch less, for up to 4096 scores a KV head and 2^18 in
-// all; a second launch otherwise.  Calls, us, by the one / the other: 20 heads over 5 of 128 in bf16, 1 sequence of 1000 slots
-// 12.4 / 15.1, 12 of up to 1000 15.1 / 15.3, 32 of 120 11.6 / 15.0; but 32 of up to 1000 22.3 / 21.1, 4 of 2000 18.0 / 15.2,
-// 1200 of up to 8000 (4 over 1 of 64) 422 / 400 and, within these limits, 8 of up to 2000 (12 over 12 of 64) 17.7 / 16.4.
-constexpr int kWeighHead = 1 << 12, kWeighAll = 1 << 18;
+// The weights are added by the workgroup that has a KV head's totals, a launch less, for up to 4096 scores a KV head and 2^17 in
+// all (of the table's slots: the host does not know the lengths); a second launch otherwise.  us of a call in a row, and in a replayed
+// graph, by the one | the other: 20 heads over 5 of 128 in bf16, 1 sequence of 1000 slots 11.7, 11.5 | 14.3, 10.0, 6 of up to 1000
+// 12.0, 11.6 | 13.7, 10.5, 32 of 120 11.6, 8.7 | 14.0, 10.2; 12 heads over 12 of 64, 8 of up to 1000 12.1, 12.0 | 13.7, 11.1, 4 of up
+// to 2000 14.2, 14.3 | 13.9, 11.1; past the limits 12 of up to 1000 15.2, 15.1 | 14.1, 13.4, 8 of up to 2000 (12 over 12) 16.0, 16.1 |
+// 13.8, 13.5, 32 of up to 1000 18.8, 19.0 | 17.7, 17.6, 4 of 2000 18.8, 19.0 | 14.1, 13.9.  (Eager calls, whose launch costs the
+// host more, decide.)
+constexpr int kWeighHead = 1 << 12, kWeighAll = 1 << 17;
 
 hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void* work, hipStream_t s) {
     const int cap = a.c.P << a.c.shift;
