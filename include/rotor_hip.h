@@ -450,8 +450,14 @@ int rt_paged_append(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float
  * slots 0 .. lens[b] - 1, scale 1 / sqrt(hd), GQA (src/rotor/transformer.py:260-281); out may be q.  A sequence
  * without slots gets zeros.  weights (may be NULL) fp32 [B][Hkv][weight_slots], weight_slots >= P * page:
  * every slot's softmax weights of the KV head's query heads are added to it, in a fixed order (slots not attended to
- * are left alone).  workspace: rt_paged_attention_workspace bytes of device memory, 16-byte aligned, possibly 0,
- * no initialisation; calls that may run at the same time need workspaces of their own. */
+ * are left alone).  A call with weights may join a sequence's pieces in another order than one without: the outputs agree to
+ * fp32 rounding, not always bit for bit (the same call gives the same bits).
+ * workspace: rt_paged_attention_workspace bytes of device memory, 16-byte aligned, possibly 0, no
+ * initialisation; calls that may run at the same time need workspaces of their own.  With weights it holds a score for every head
+ * and slot of the table, 4 * B * H * P * page bytes whatever the lengths, and a second launch passes over as many: a table no wider
+ * than the longest sequence needs keeps both small.
+ * Up to 1024 sequences a call, long ones are cut into pieces for several workgroups; in larger batches a KV head of a sequence (16 query
+ * heads of it) is one workgroup's, and the longest sequence decides the call. */
 size_t rt_paged_attention_workspace(const rt_pages* c, int H, int weights);
 int rt_paged_attention(rt_ctx* ctx, const rt_pages* c, const float* q, int H, float* weights, int weight_slots, float* out,
                        void* workspace, size_t workspace_bytes);
@@ -466,7 +472,7 @@ int rt_paged_step(rt_ctx* ctx, const rt_pages* c, const rt_paged_new* n, float* 
  * them, the ones with the largest weights fp32 [B][Hkv][weight_slots] (ties: the lowest slot; NaN counts as the largest), in
  * their order.  kept int32 [B][Hkv][keep]: the slots, -1 behind the last; new_lens int32 [B]: how many (all
  * that are there where those are no more than keep; the same for every head); new_weights, shaped as weights: theirs, zeros
- * behind them.  Their keys and values are copied to the pages of new_table int32 [B][new_P], new_P * page >= keep, none of
+ * behind them (weights that are to go on over a new table of more slots need rows for it: weight_slots >= new_P * page).  Their keys and values are copied to the pages of new_table int32 [B][new_P], new_P * page >= keep, none of
  * which may be a page that `table` holds or another sequence's new one.  The old pages stay as they were.  workspace:
  * rt_paged_evict_workspace bytes of device memory (0 where P * page <= 32768), as for rt_paged_attention. */
 size_t rt_paged_evict_workspace(const rt_pages* c);

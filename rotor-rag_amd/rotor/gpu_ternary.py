@@ -806,7 +806,10 @@ class HIPTernaryOps:
         """Attention of one token a sequence, q [B, 1, H, hd] (rotated, as paged_append returns it), over the lens[b] slots
         of a paged cache (rt_paged_attention): float32 [B, 1, H, hd] (out, which may be q); zeros for a sequence
         without slots.  weights float32 [B, Hkv, slots]: what every slot weighed (the softmax's weights, summed over a KV head's
-        query heads) is added to it, for paged_evict.  For inference: gradients do not pass."""
+        query heads) is added to it, for paged_evict.  (With weights the output may differ in its last bits: another order of
+        additions; and memory of 4 bytes for every head and slot of the table, so give a table no wider than the longest sequence
+        needs.  Up to 1024 sequences are cut into pieces that run side by side; in a larger batch the longest decides.)  For
+        inference: gradients do not pass."""
         torch = _torch()
         pages, sizes, span = self._paged_check("paged_attention", torch, cache, table, lens)
         q, at = self._paged_in(torch, q)
@@ -852,8 +855,8 @@ class HIPTernaryOps:
         those before them, the ones with the largest weights (ties: the lowest slot), in their order.  Their keys and values
         are copied to the pages of new_table int32 [B, new_P], which must be pages that no table of these sequences holds;
         the old ones stay as they were and are free afterwards.  Returns (kept int32 [B, Hkv, keep]: the slots, -1 behind the
-        last; new_lens int32 [B]; new_weights, shaped as weights: the kept slots', then zeros).  Sequences of no
-        more than `keep` slots move as they are."""
+        last; new_lens int32 [B]; new_weights, shaped as weights: the kept slots', then zeros; to go on with them over a new_table of
+        more slots, give weights with rows for new_P * page).  Sequences of no more than `keep` slots move as they are."""
         torch = _torch()
         pages, sizes, span = self._paged_check("paged_evict", torch, cache, table, lens)
         _, Hkv, page, _, B, _ = sizes

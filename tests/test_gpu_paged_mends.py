@@ -49,6 +49,27 @@ def test_weights_of_holes(hip, dtype, slots, bad):
             assert w[b, h, there].isnan().all() if nan else (w[b, h, there] > 0).all()
 
 
+def test_weights_over_a_wider_table(hip):
+    """An eviction to more pages than there were: weights whose rows have the room go on, others are refused by the next step."""
+    cache, table, n = P.make([90, 40], 2, 64, 16, "bf16", spare=22)
+    free = torch.tensor(sorted(set(range(cache.shape[1])) - set(table.flatten().tolist())))[:20].view(2, 10).int().cuda()
+    k, rope = torch.randn(2, 1, 2, 64, device="cuda"), P.rope_angles(200, 64).cuda()
+    for slots in (6 * 16, 10 * 16):
+        w = torch.rand(2, 2, slots, device="cuda")
+        c, pos = cache.cuda(), n.cuda()
+        kept, lens, left = hip.paged_evict(c, table.cuda(), n.cuda(), w, 120, 5, free)
+        assert lens.tolist() == [90, 40] and left.shape == w.shape and torch.equal(left[0, :, :90], w[0, :, :90])
+        args = (P.queries([0] * 2, 8, 64).cuda(), k, k, c, free, lens, rope, pos)
+        if slots < 160:
+            with pytest.raises(ValueError, match="weights"):
+                hip.paged_step(*args, weights=left)
+        else:
+            before = left.clone()
+            hip.paged_step(*args, weights=left)
+            assert (left[0, :, :91] > before[0, :, :91]).all() and (left[1, :, :41] > before[1, :, :41]).all()
+            assert (left[0, :, 91:] == 0).all() and (left[1, :, 41:] == 0).all()
+
+
 # ---- together with torch's graphs ----------------------------------------------------------
 
 
