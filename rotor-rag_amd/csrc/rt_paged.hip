@@ -1012,7 +1012,8 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
 // slots in holes are not there.  Weights are taken as whole numbers of the same order (NaN above all, -0 as 0; 0 for what is not
 // there).  The smallest that is kept is found from histograms of its upper 11 bits, of the next 11 among those that have these,
 // and of the last 10.  Then every wave counts the kept of its run of slots, and writes them out behind those of the waves before.
-// A workgroup of 1024 threads takes a KV head of a sequence, up to 32 slots a thread in registers; longer caches are shared among
+// A workgroup of 1024 threads takes a KV head of a sequence, up to 32 slots a thread, in registers (of 17 to 32 a part spills: 28
+// registers, 116 bytes a lane; 16000 slots cut to half, 5 heads of 128, 25 us, 24000 41); longer caches are shared among
 // workgroups of 8 slots a thread, in a launch for every histogram and two for the output, all launches us, alone / shared: 5 heads
 // of 16000 slots 16 / 32, 32000 33 / 32 (and five launches more on the host), 80 heads 39 / 49, 300 heads 69 / 99; 10 heads of
 // 131072 slots by one workgroup each, the weights read again for every pass, 359 / 35.  Bound by the passes' latencies: 128 heads of up
@@ -1368,7 +1369,9 @@ void paged_by_type(int type, int hd, F go) {
 }
 
 // The workgroups of the attention, and whether a unit may have several pieces.
-constexpr int kPagedMapped = 1024;  // larger batches: a piece a unit
+// Larger batches: a piece a unit, as every workgroup reads all lengths to find its own.  One sequence of 30000 slots behind others of
+// 400, us: 1024 sequences 67 (4 heads over 1 of 128), 303 (20 over 5), 1025 400, 485.
+constexpr int kPagedMapped = 1024;
 struct PagedShape {
     long long units, groups;
     int tiles;
@@ -1383,8 +1386,8 @@ PagedShape paged_shape(int B, int H, int Hkv, int cap, int type) {
     p.split = most > 1 && B <= kPagedMapped;
     // As many as run at once, two a CU, or twice that for two pieces a unit; past 512 units, pieces for sequences that have
     // more than a 512th of the work, no others.  Two pieces a unit / these / none, us: 128 sequences of 10 to 1500 slots (32 heads
-    // over 8) 83 / 77 / 76, 1000 of 700 (4 over 1; each workgroup looks at every length) 98 / 66 / 58; one of 30000 among 255 of 400
-    // 133 with these, 439 with none, one among 63 (64 over 16) 81 / 416.
+    // over 8) 83 / 80 / 77, 1000 of 700 (4 over 1; each workgroup looks at every length) 98 / 69 / 59; one of 30000 among 255 of 400
+    // (32 over 8) 127 with these, 428 with none, one among 63 (64 over 16) 87 / 416.
     p.groups = !p.split ? p.units : std::min(p.units * most, p.units <= 512 ? 512 * ((p.units + 255) / 256) : p.units + 512);
     // The last workgroup joins where no unit has more than 32 pieces, or 64 heads of pieces: a launch less on the host (3.5 us),
     // and on the GPU, us in two launches / one: 20 heads over 5, 1000 slots 6.4 + 3.2 / 8.6, 2000 6.3 + 3.8 / 9.0, 4000 (32 pieces of
@@ -1468,10 +1471,11 @@ hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void
     paged_by_type(type, hd, [&](auto T, auto HD) {
         constexpr int t = decltype(T)::value, d = decltype(HD)::value;
         auto attend = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a); };
-        // Keys and values that one workgroup reads, once, go past the caches: 131072 slots (20 heads over 5 of 128, bf16) 61.0 us,
-        // so 54.8; 32 sequences of 100 to 4095 34.3 / 32.3 (a cache of 168 MB that is read again and again, as nothing between
-        // does in a model, 28.2 / 31.1).  Where tiles of heads share them, through the caches: 32 x 16000 slots,
-        // 32 heads over 1 58.1 / 69.9, 64 100 / 141 (16 50.4 / 44.8).
+        // Keys and values that one workgroup reads, once, go past the caches.  us through them / past them (20 heads over 5 of 128,
+        // bf16, three caches in turn): 131072 slots 67.5 / 59.5, 32 sequences of 100 to 4095 37.8 / 34.7; 32 of 16000, 16 heads over 1
+        // 54.0 / 48.3.  Where tiles of heads share them, through the caches: 32 over 1 82.3 / 87.9, 64 156 / 169.  Pages that sequences
+        // share are read past the caches too, as the host does not know the tables: 32 sequences over the same 4000 slots 32.7 / 49.6
+        // (of their own 64.1 / 56.7), 500 11.5 / 12.4 (14.3 / 15.0).
         const bool once = p.tiles == 1;
         if (step) once ? attend(paged_attn_kernel<t, d, true, true>) : attend(paged_attn_kernel<t, d, true, false>);
         else once ? attend(paged_attn_kernel<t, d, false, true>) : attend(paged_attn_kernel<t, d, false, false>);
