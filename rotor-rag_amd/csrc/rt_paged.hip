@@ -507,17 +507,26 @@ __host__ __device__ __forceinline__ int paged_even(int cap) { return (cap + 31) 
 
 // The pieces of a launch.  A sequence of n tiles is cut, for each of its `per` units (a KV head's tile of heads), into pieces
 // of at most q tiles (one at least), as equal as they can be, q about the least for which all fit the launch's workgroups.  The first
-// B per workgroups have the units' first pieces; the others the further ones, in the order (sequence, unit, piece).  Every wave
-// works this out for itself, lane b for sequence b: the host does not know the lengths, and with the same number of
+// B per places have the units' first pieces; the others the further ones, in the order (sequence, KV head, piece, tile of heads).
+// Every wave works this out for itself, lane b for sequence b: the host does not know the lengths, and with the same number of
 // pieces for each the longest sequence decides the launch.
+// Tiles of heads that read the same keys, which stand next to each other in that order, go to one of the 8 dies (workgroup
+// number mod 8), whose L2 then reads them once: 32 sequences of 16000 slots (262 MB), 64 heads over 1, 260 MB and 96 us, by
+// the order alone, on four dies, 1026 MB and 153; 32 over 1 61 and 81.
 constexpr int kWaves = 4;
 struct PagedPiece {
     int b, unit, piece, n, q;  // piece number `piece` of n, q tiles each; n = 0: none
-    int more;                  // the workgroup of the unit's second piece (for a first piece: where B <= 64)
+    int more;                  // the place of the unit's second piece (for a first piece: where B <= 64)
     int span;                  // paged_span of sequence b
 };
-// The workgroup of piece s of unit u of the launch.
-__device__ __forceinline__ int paged_group(int s, int u, int more) { return s ? more + s - 1 : u; }
+// The place of workgroup w: of 8 `tiles` places in a row, number 8 t + x takes the one of tile t of the x-th keys.
+__device__ __forceinline__ int paged_place(const PagedAttn& a, int w) {
+    if (a.tiles == 1) return w;
+    const int run = 8 * a.tiles, in = w % run;
+    return w - in + run > a.groups ? w : w - in + in % 8 * a.tiles + in / 8;
+}
+// The place of piece s of unit u of the launch.
+__device__ __forceinline__ int paged_group(int s, int u, int more, int tiles) { return s ? more + (s - 1) * tiles : u; }
 
 template <bool STEP, int TK>
 __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int lane) {
@@ -567,7 +576,8 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int
         if (B <= 64) {
             p.n = __builtin_amdgcn_readlane(n, p.b);
             p.span = __builtin_amdgcn_readlane(span, p.b);
-            p.more = units + (__builtin_amdgcn_readlane(incl, p.b) - p.n + 1) * per + p.unit * (p.n - 1);
+            const int ht = a.tiles == 1 ? 0 : p.unit % a.tiles;
+            p.more = units + (__builtin_amdgcn_readlane(incl, p.b) - p.n + 1) * per + (p.unit - ht) * (p.n - 1) + ht;
         } else {
             p.span = paged_span<STEP>(a, a.c.lens[p.b]);
             p.n = pieces((p.span + TK - 1) / TK, q);
@@ -591,9 +601,11 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttn& a, int w, int
         p.b = at + l;
         p.n = others + 1;
         p.span = __builtin_amdgcn_readlane(span, l);
-        p.unit = (e - start) / others;
-        p.piece = 1 + e - start - p.unit * others;
-        p.more = units + start + p.unit * others;
+        const int kh = (e - start) / (others * a.tiles), in = e - start - kh * others * a.tiles, s = a.tiles == 1 ? in : in / a.tiles;
+        const int ht = in - s * a.tiles;
+        p.unit = kh * a.tiles + ht;
+        p.piece = 1 + s;
+        p.more = units + start + kh * others * a.tiles + ht;
     }
     p.q = ((p.span + TK - 1) / TK + p.n - 1) / p.n;
     return p;
@@ -659,7 +671,7 @@ __device__ __forceinline__ bool paged_last(const PagedAttn& a, const PagedPiece&
     }
     __syncthreads();
     if (!*flag) return false;
-    auto part = [&](int s, int e) { return a.part + (size_t)paged_group(s, u, p.more) * 16 * HD + e * 4; };
+    auto part = [&](int s, int e) { return a.part + (size_t)paged_group(s, u, p.more, a.tiles) * 16 * HD + e * 4; };
     const int n = p.n, cols = rows * L, groups = max(NT / cols, 1), grp = t / cols;
     float* const factor = room;  // [rows][n]
     v4f* const sums = reinterpret_cast<v4f*>(room + kLastMost);
@@ -679,7 +691,7 @@ __device__ __forceinline__ bool paged_last(const PagedAttn& a, const PagedPiece&
     const bool mine = grp < groups && e < cols;
     if (mine) load(e);  // (while the references come)
     for (int row = wave; row < rows; row += kWaves) {
-        const v2f x = lane < n ? paged_get(a.ml + (size_t)paged_group(lane, u, p.more) * 32 + row * 2) : v2f{-INFINITY, 0.0f};
+        const v2f x = lane < n ? paged_get(a.ml + (size_t)paged_group(lane, u, p.more, a.tiles) * 32 + row * 2) : v2f{-INFINITY, 0.0f};
         const float top = lane63(wave_reduce63(x[0], -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
         const float ref = top > -INFINITY ? top : 0.0f, f = __builtin_amdgcn_exp2f(x[0] - ref);
         const float sum = lane63(wave_reduce63(x[1] * f, 0.0f, [](float x, float y) { return x + y; }));
@@ -731,7 +743,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
     __shared__ __align__(16) E fresh[2][STEP ? HD : 16];
     float(*const part)[16][HD + 4] = reinterpret_cast<float(*)[16][HD + 4]>(both);
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
-    const PagedPiece p = paged_piece<STEP, TK>(a, blockIdx.x, lane);
+    const int place = paged_place(a, blockIdx.x);
+    const PagedPiece p = paged_piece<STEP, TK>(a, place, lane);
     if (p.n == 0) return;
     const int b = p.b, kh = p.unit / a.tiles, ht = p.unit - kh * a.tiles, bk = b * a.c.Hkv + kh, u = b * a.c.Hkv * a.tiles + p.unit;
     const int len = p.span, tiles = (len + TK - 1) / TK, first = min(p.piece * p.q, tiles);
@@ -904,12 +917,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
                 total[row][1] = inv;
             }
         } else if (a.whole) {
-            paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d, y[0], y[1]);
-            paged_put(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d + 2, y[2], y[3]);
-            if (d == 0) paged_put(a.ml + ((size_t)blockIdx.x * 16 + row) * 2, top, sum);
+            paged_put(a.part + ((size_t)place * 16 + row) * HD + d, y[0], y[1]);
+            paged_put(a.part + ((size_t)place * 16 + row) * HD + d + 2, y[2], y[3]);
+            if (d == 0) paged_put(a.ml + ((size_t)place * 16 + row) * 2, top, sum);
             continue;
-        } else *reinterpret_cast<v4f*>(a.part + ((size_t)blockIdx.x * 16 + row) * HD + d) = y;
-        if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)blockIdx.x * 16 + row) * 2) = v2f{top, sum};
+        } else *reinterpret_cast<v4f*>(a.part + ((size_t)place * 16 + row) * HD + d) = y;
+        if (d == 0 && a.ml) *reinterpret_cast<v2f*>(a.ml + ((size_t)place * 16 + row) * 2) = v2f{top, sum};
     }
     if (a.whole) {
         bool mine = true;
@@ -926,9 +939,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedAttn a)
 }
 
 // Head number `row` of unit u: its reference (the largest of its pieces') and the reciprocal of its sum of weights, found by a
-// wave; unit: the workgroup of its second piece, and how many pieces there are.
-__device__ __forceinline__ void paged_total(const float* all, int u, int2 unit, int row, int lane, float& ref, float& inv) {
-    auto ml = [&](int s) { return all + (size_t)paged_group(s, u, unit.x) * 32 + row * 2; };
+// wave; unit: the place of its second piece, and how many pieces there are.
+__device__ __forceinline__ void paged_total(const PagedAttn& a, int u, int2 unit, int row, int lane, float& ref, float& inv) {
+    auto ml = [&](int s) { return a.ml + (size_t)paged_group(s, u, unit.x, a.tiles) * 32 + row * 2; };
     const int n = unit.y;
     float top = -INFINITY;
     for (int s = lane; s < n; s += 64) top = fmaxf(top, ml(s)[0]);
@@ -957,7 +970,7 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
         const int n = unit.y;
         if (n == 1) return;
         const int d = t % L * 4, grp = t / L;
-        auto place = [&](int s) { return (size_t)paged_group(s, u, unit.x) * 16 + in % 16; };
+        auto place = [&](int s) { return (size_t)paged_group(s, u, unit.x, a.tiles) * 16 + in % 16; };
         auto part = [&](int s) { return *reinterpret_cast<const v4f*>(a.part + place(s) * HD + d); };
         v4f y{};
         float own = -INFINITY, ref, inv;
@@ -965,7 +978,7 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
             y = part(grp);
             own = a.ml[place(grp) * 2];
         }
-        paged_total(a.ml, u, unit, in % 16, lane, ref, inv);
+        paged_total(a, u, unit, in % 16, lane, ref, inv);
         y *= __builtin_amdgcn_exp2f(own - ref);
 #pragma unroll 4
         for (int s = grp + NT / L; s < n; s += NT / L) y += part(s) * __builtin_amdgcn_exp2f(a.ml[place(s) * 2] - ref);
@@ -983,7 +996,7 @@ __global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttn a, int TK, int
     for (int in = wave; in < a.G; in += NT / 64) {
         float ref, inv;
         const int u = bk * a.tiles + in / 16;
-        paged_total(a.ml, u, a.units[u], in % 16, lane, ref, inv);
+        paged_total(a, u, a.units[u], in % 16, lane, ref, inv);
         total[in][0] = ref;
         total[in][1] = inv;
     }
@@ -1410,7 +1423,7 @@ hipError_t launch_paged_append(const PagedCache& c, const PagedNew& n, float* q_
     return hipGetLastError();
 }
 
-// The workspace: sums [group][16][hd], (reference, sum of weights) [group][16][2], (first group, groups) [unit], scores
+// The workspace: sums [place][16][hd], (reference, sum of weights) [place][16][2], (place of the second piece, pieces) [unit], scores
 // [B][KV head and tile of heads][tile of slots][head][slot] (a tile's in one piece: with a head's in one, writing them took
 // 20 sequences of 3025 slots, 32 heads over 8, 47.5 us, so 46.7).
 namespace {
@@ -1427,7 +1440,7 @@ unsigned long long paged_seed() {
 size_t paged_attention_workspace(int B, int H, int Hkv, int cap, int type, int hd, bool weights) {
     const PagedShape p = paged_shape(B, H, Hkv, cap, type);
     const size_t parts = (size_t)p.groups * 16;
-    // (first group, groups) or, in its place, the ticket of a unit
+    // (place of the second piece, pieces) or, instead, the ticket of a unit
     return 4 * ((p.split ? parts * hd : 0) + (p.split || weights ? parts * 2 + ((size_t)p.units * 2 + 3) / 4 * 4 : 0) +
                 (weights ? (size_t)B * H * paged_even(cap) : 0));
 }
@@ -1473,7 +1486,7 @@ hipError_t launch_paged_attention(PagedAttn a, bool step, int type, int hd, void
         auto attend = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * kWaves), 0, s, a); };
         // Keys and values that one workgroup reads, once, go past the caches.  us through them / past them (20 heads over 5 of 128,
         // bf16, three caches in turn): 131072 slots 67.5 / 59.5, 32 sequences of 100 to 4095 37.8 / 34.7; 32 of 16000, 16 heads over 1
-        // 54.0 / 48.3.  Where tiles of heads share them, through the caches: 32 over 1 82.3 / 87.9, 64 156 / 169.  Pages that sequences
+        // 54.0 / 48.3.  Where tiles of heads share them, through the caches: 32 over 1 61.1 / 73.0, 64 95.6 / 126.  Pages that sequences
         // share are read past the caches too, as the host does not know the tables: 32 sequences over the same 4000 slots 32.7 / 49.6
         // (of their own 64.1 / 56.7), 500 11.5 / 12.4 (14.3 / 15.0).
         const bool once = p.tiles == 1;
