@@ -79,6 +79,8 @@ STEPS = {  # lens, H, Hkv, hd, page, dtype, weights, slots of the table beyond t
     "second launch, weights": ([4000, 30], 20, 5, 128, 64, "bf16", True, 20),
     "second launch": ([9000], 8, 2, 64, 128, "fp16", False, 20),
     "second launch, 1024 threads": ([1800, 3, 700], 14, 2, 64, 32, "fp32", True, 20),
+    "last workgroup, tiles of heads": ([480, 300, 0], 40, 2, 64, 32, "bf16", False, 20),
+    "second launch, tiles of heads": ([2900, 100], 50, 1, 128, 64, "fp16", True, 20),
     "more sequences than lanes": ([10 * b for b in range(70)], 4, 2, 64, 32, "bf16", True, 300),
 }
 
@@ -175,6 +177,21 @@ def test_replayed_steps_whose_memory_is_used_again(hip):
         g.replay()
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a[2], e[2]), i
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", P.TYPES)
+@pytest.mark.parametrize("lens,H,Hkv", [
+    ([500, 300, 7], 20, 1), ([500] * 5 + [1], 40, 2), ([250, 100], 33, 1), ([130] * 30, 64, 2), ([6000, 0, 50], 130, 2), ([20000], 64, 1),
+    ([700 + 9 * b for b in range(40)], 48, 1), ([300] * 66 + [5000], 34, 2)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_tiles_of_heads_in_pieces(hip, dtype, lens, H, Hkv, weights):
+    """Two to five tiles of heads a KV head, joined in both ways, in numbers of workgroups that 8 dies divide and that they do not."""
+    cache, table, n = P.make(lens, Hkv, 64, 32, dtype, seed=H)
+    start = torch.rand((len(lens), Hkv, table.shape[1] * 32), generator=torch.Generator().manual_seed(3)) if weights else None
+    assert workspace(H, cache, table, weights) > 0
+    check = P.check_attention(hip, cache, table, n, P.queries(lens, H, 64), weights=start)
+    assert torch.equal(check, hip.paged_attention(P.queries(lens, H, 64).cuda(), cache.cuda(), table.cuda(), n.cuda(),
+                                                  weights=start.cuda() if weights else None))
 
 
 # ---- tokens without a place ----------------------------------------------------------------
